@@ -280,6 +280,55 @@ int vt_rope_qkv(cudaStream_t stream, const uint16_t* qkv, long long ld, int n, i
 int vt_attn_causal(cudaStream_t stream, const uint16_t* q, const uint16_t* kc, const uint16_t* vc, int n, int H,
                    int pos0, int ctx, float scale, uint16_t* out, long long ldo);
 
+/* ---- 8-bit key / value cache.  One layer's cache: int8 codes kc, vc [B][H][C][D] and one fp32 scale per block of
+ * 64 slots and head ks, vs [B][H][C / 64] (contiguous; C % 64 == 0, D 64 or 128, codes 16-byte aligned); a value is
+ * code * scale.  lens[b] (int, device memory) is the number of tokens that sequence b holds before the call, counts[b]
+ * (int, device memory, NULL: n for all) the number of its new tokens, 0 .. n; rows past counts[b] are padding: never
+ * read into a result, and left as they were in every output.  Lengths on the device cannot be refused by the host: a
+ * negative one, a count outside 0 .. n, tokens past C and positions past the rotary table are clamped and set bit 9
+ * of the status word (vt_device_status).  Query head hq reads head hq / (Hq / H).  The reference has a bf16 cache only
+ * (moondream/gpu/md2fast.py:186-191); these stand beside vt_rope_qkv and vt_attn_causal. */
+
+/* Rotary embedding (vt_rope_qkv's: the first 32 dims of each q / k head) and quantised cache write of n new tokens for
+ * each of B sequences: qkv bf16, row (b, i) at qkv + b*sx_b + i*sx_t = q [Hq][D] | k [H][D] | v [H][D]; cos_t / sin_t
+ * fp32 [tab][16], row pos[b] + i (pos NULL: lens[b] + i); q rows to q + b*sq_b + i*sq_t + hq*sq_h; k (rounded to bf16) and v
+ * into slots lens[b] + i.  Strides multiples of 8 elements.  A block without tokens, or with zeros only (scale 0),
+ * takes the scale max|x| / 127 of its new ones; a block that holds tokens keeps its scale, doubled as often as the
+ * new ones need, its codes halved as often (rint): a value is then at most one step off however it arrived, half a
+ * step when its block was written in one call.  A NaN or an infinity makes its block's scale NaN.  A call may be
+ * repeated from the same lens (a question asked again over the same prefix). */
+int vt_rope_kv8(cudaStream_t stream, const uint16_t* qkv, long long sx_b, long long sx_t, int B, int n, int Hq, int H,
+                int D, const float* cos_t, const float* sin_t, int tab, const int* lens, const int* pos,
+                const int* counts, uint16_t* q, long long sq_b, long long sq_t, long long sq_h, int8_t* kc, int8_t* vc,
+                float* ks, float* vs, int C);
+
+/* Bytes of the workspace of vt_attn_kv8 (0 for an empty problem); contents need no initialisation. */
+long long vt_attn_kv8_ws_bytes(int B, int n, int Hq, int H, int D, int C, int weights);
+
+/* Attention of the n new rows of each sequence over its cache, their own tokens already in it: row i of sequence b
+ * sees slots 0 .. lens[b] + i (causal != 0) or 0 .. lens[b] + counts[b] - 1; softmax(scale q k^T) v, sums in fp32, out
+ * bf16 at out + b*so_b + i*so_t + hq*so_h.  weights fp32 [B][H][C] (NULL: none) receives the attention weight of each
+ * slot j < lens[b] + counts[b]: its probabilities summed over the sequence's rows and the group's query heads, plus
+ * weights_in[b][h][j] (NULL: none; may be weights) for j < lens[b].  ws: vt_attn_kv8_ws_bytes bytes, 16-byte
+ * aligned, one call at a time.  Results do not depend on the other sequences of the batch beyond the rounding of
+ * how the keys are split, and are the same every time.
+ * Replaces: nothing in the reference; the 8-bit form of the question's attention (md2fast.py:192-193). */
+int vt_attn_kv8(cudaStream_t stream, const uint16_t* q, long long sq_b, long long sq_t, long long sq_h, const int8_t* kc,
+                const int8_t* vc, const float* ks, const float* vs, int C, const int* lens, const int* counts, int B,
+                int n, int Hq, int H, int D, int causal, float scale, uint16_t* out, long long so_b, long long so_t,
+                long long so_h, float* weights, const float* weights_in, void* ws, long long ws_bytes);
+
+/* Eviction by accumulated attention weight into another cache of dst_C >= keep slots.  A sequence with lens[b] <= keep is
+ * copied.  Of one with more, each head keeps its last `recent` tokens and the keep - recent of the others with the
+ * largest weights [B][H][C] (of equal ones the lowest slots; NaN counts as largest), in order, with new block scales
+ * max|value| / 127 and codes rint(value / scale).  keep % 64 == 0, 0 <= recent <= keep.  dst_lens[b] =
+ * min(lens[b], keep); index [B][H][keep] the slots kept and dst_weights [B][H][dst_C] their weights, both written up
+ * to dst_lens[b].  The destination must not overlap the source.  New tokens go on at position lens[b] (vt_rope_kv8's
+ * pos) and slot dst_lens[b]. */
+int vt_kv8_evict(cudaStream_t stream, const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, int C,
+                 const float* weights, const int* lens, int B, int H, int D, int keep, int recent, int8_t* dst_kc,
+                 int8_t* dst_vc, float* dst_ks, float* dst_vs, int dst_C, float* dst_weights, int* dst_lens, int* index);
+
 /* One pass of the LANCZOS frame squash on 3-channel uint8 images: out[o, j, c] = clip(2^21 + sum_k
  * in[x0(o) + k, j, c] * w[o][k] >> 22) for o < n_out positions on the resampled axis and j < n_other along
  * the other, with bounds int32 [n_out][2] = (x0, count) and fixed-point weights int32 [n_out][ksize]

@@ -49,6 +49,10 @@ SIGNATURES = {
     "vt_gelu_erf": (I, [P, P, LL, I, I]),
     "vt_rope_qkv": (I, [P, P, LL, I, I, I, P, P, P, P, P, I]),
     "vt_attn_causal": (I, [P, P, P, P, I, I, I, I, F, P, LL]),
+    "vt_rope_kv8": (I, [P, P, LL, LL, I, I, I, I, I, P, P, I, P, P, P, P, LL, LL, LL, P, P, P, P, I]),
+    "vt_attn_kv8_ws_bytes": (LL, [I, I, I, I, I, I, I]),
+    "vt_attn_kv8": (I, [P, P, LL, LL, LL, P, P, P, P, I, P, P, I, I, I, I, I, I, F, P, LL, LL, LL, P, P, P, LL]),
+    "vt_kv8_evict": (I, [P, P, P, P, P, I, P, P, I, I, I, I, I, P, P, P, P, I, P, P, P]),
     "vt_resize_pass_u8": (I, [P, P, LL, LL, LL, P, LL, LL, LL, I, I, P, P, I]),
 }
 

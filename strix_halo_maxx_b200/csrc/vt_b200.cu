@@ -8,5 +8,6 @@
 #include "elementwise.cu"
 #include "ssm.cu"
 #include "text.cu"
+#include "kv8.cu"
 #include "resize.cu"
 #include "heads.cu"

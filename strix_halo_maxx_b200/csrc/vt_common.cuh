@@ -23,6 +23,8 @@ enum : unsigned int {
   ST_ATTN_SOFTMAX = 1u << 6,
   ST_SSM_MMA = 1u << 7,
   ST_SELFTEST = 1u << 8,  // vt_wait_selftest
+  ST_KV8_RANGE = 1u << 9,  // a length or position on the device beyond the 8-bit cache or the rotary table
+  ST_KV8_WAIT = 1u << 10,
 };
 // A wait gives up after this many SM clock cycles (~2 s at 1.9 GHz); legitimate waits are microseconds.
 constexpr long long kSpinCycles = 4000000000LL;

@@ -7,11 +7,13 @@
 * I8Lin  -- the `tlin_cls` of the reference's int8 text model, hgemm.HI8Lin (hgemm.py:95-137): W8A8 with
   quant(x) -> (q, s) and __call__(x, gelu=False, res=None, pre=None); quant_rows / layer_norm_quant / gemm_i8
   are its kernels.
+* Kv8 / kv8_cache -- the 8-bit KV cache, with rope_kv8 (rotary + quantised write), attn_kv8 and kv8_evict.
 * layer_norm / im2col / crop_combine / rglru -- thin wrappers of the remaining kernels.
 
 Every call launches on torch's current stream and raises VtError on a non-zero return code.
 """
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -428,6 +430,143 @@ def attn_causal(q, kc, vc, pos0, out, scale=None):
                               out.data_ptr(), out.stride(0))
     check(rc, "vt_attn_causal")
     return out
+
+
+# ---------------------------------------------------------------- 8-bit KV cache
+KV8_BLOCK = 64  # slots that share a scale
+
+
+class Kv8(NamedTuple):
+    """One layer's 8-bit KV cache: codes k, v int8 [B, H, C, D] (C a multiple of 64, D 64 or 128) and one scale per 64
+    slots and head ks, vs fp32 [B, H, C / 64]; a value is code * scale.  Lengths are kept beside it, int32 on the device."""
+    k: torch.Tensor
+    v: torch.Tensor
+    ks: torch.Tensor
+    vs: torch.Tensor
+
+    def values(self):
+        """(k, v) fp32 [B, H, C, D]: what the codes stand for."""
+        B, H, C, D = self.k.shape
+        return tuple((c.view(B, H, C // KV8_BLOCK, KV8_BLOCK, D) * s[..., None, None]).view(B, H, C, D)
+                     for c, s in ((self.k, self.ks), (self.v, self.vs)))
+
+
+def kv8_cache(B, H, C, D, device):
+    """A zero-filled Kv8 of at least C slots (rounded up to a multiple of 64)."""
+    C = (C + KV8_BLOCK - 1) // KV8_BLOCK * KV8_BLOCK
+    return Kv8(*(torch.zeros(B, H, C, D, dtype=torch.int8, device=device) for _ in range(2)),
+               *(torch.zeros(B, H, C // KV8_BLOCK, dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _kv8_fail(what, why):
+    raise ValueError(f"{what}: {why}")
+
+
+def _kv8_dims(what, cache, dev):
+    """B, H, C, D of a cache whose four tensors have the right types and shapes, contiguous on device dev."""
+    k, v, ks, vs = cache
+    B, H, C, D = k.shape
+    if k.dtype != torch.int8 or v.dtype != torch.int8 or ks.dtype != torch.float32 or vs.dtype != torch.float32:
+        _kv8_fail(what, "codes are int8, scales float32")
+    if v.shape != k.shape or ks.shape != (B, H, C // KV8_BLOCK) or vs.shape != ks.shape or C % KV8_BLOCK:
+        _kv8_fail(what, f"cache shapes {tuple(k.shape)} {tuple(v.shape)} {tuple(ks.shape)} {tuple(vs.shape)}")
+    for t in cache:
+        if t.device != dev or not t.is_contiguous():
+            _kv8_fail(what, f"cache tensors must be contiguous on {dev}")
+    return B, H, C, D
+
+
+def _kv8_vec(what, name, t, shape, dtype, dev):
+    if t.shape != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous():
+        _kv8_fail(what, f"{name} must be a contiguous {dtype} {tuple(shape)} on {dev}")
+    return t.data_ptr()
+
+
+def _kv8_call(fn, what, dev, *args):
+    """The call on torch's current stream of the tensors' device."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(_stream(), *args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(_stream(), *args)
+    check(rc, what)
+
+
+def rope_kv8(qkv, cache, lens, cos_t, sin_t, q, pos=None, counts=None):
+    """vt_rope_kv8: qkv [B, n, (Hq + 2 H) D] bf16 (q | k | v, head-major) -> q [B, n, Hq, D] rotated, k and v quantised
+    into slots lens[b] .. of the cache.  lens, pos (default lens: the rotary positions) and counts (default n: each
+    sequence's number of new tokens) int32 [B] on the device; cos_t / sin_t fp32 [positions, 16]."""
+    what, dev = "rope_kv8", q.device
+    B, H, C, D = _kv8_dims(what, cache, dev)
+    n, Hq = q.shape[1], q.shape[2]
+    if q.shape != (B, n, Hq, D) or qkv.shape != (B, n, (Hq + 2 * H) * D) or q.dtype != BF16 or qkv.dtype != BF16 or \
+            qkv.device != dev or (q.numel() and (q.stride(3) != 1 or qkv.stride(2) != 1)):
+        _kv8_fail(what, f"qkv {tuple(qkv.shape)}, q {tuple(q.shape)} for a cache of B={B} H={H} D={D} (bf16, contiguous rows)")
+    tab = cos_t.shape[0]
+    _kv8_call(lib().vt_rope_kv8, "vt_rope_kv8", dev, qkv.data_ptr(), qkv.stride(0), qkv.stride(1), B, n, Hq, H, D,
+              _kv8_vec(what, "cos_t", cos_t, (tab, 16), torch.float32, dev),
+              _kv8_vec(what, "sin_t", sin_t, (tab, 16), torch.float32, dev), tab,
+              _kv8_vec(what, "lens", lens, (B,), torch.int32, dev),
+              None if pos is None else _kv8_vec(what, "pos", pos, (B,), torch.int32, dev),
+              None if counts is None else _kv8_vec(what, "counts", counts, (B,), torch.int32, dev),
+              q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), cache.k.data_ptr(), cache.v.data_ptr(),
+              cache.ks.data_ptr(), cache.vs.data_ptr(), C)
+    return q
+
+
+def attn_kv8_workspace(B, n, Hq, H, D, C, device, weights=False):
+    """A workspace for attn_kv8 calls of these sizes, one call at a time (vt_attn_kv8_ws_bytes)."""
+    return torch.empty(max(lib().vt_attn_kv8_ws_bytes(B, n, Hq, H, D, C, int(weights)), 16), dtype=torch.uint8, device=device)
+
+
+def attn_kv8(q, cache, lens, out=None, counts=None, causal=True, scale=None, weights=None, weights_in=None, ws=None):
+    """vt_attn_kv8: q [B, n, Hq, D] bf16, the sequences' new rows (already in the cache by rope_kv8 with the same lens and
+    counts) -> out [B, n, Hq D] bf16; row i sees slots 0 .. lens[b] + i (causal) or all lens[b] + counts[b].  weights fp32
+    [B, H, C]: each slot's attention weight, summed over the rows and the group's query heads, plus weights_in for slots
+    before lens[b] (weights_in=weights accumulates in place).  ws: attn_kv8_workspace, else one is allocated."""
+    what, dev = "attn_kv8", q.device
+    B, H, C, D = _kv8_dims(what, cache, dev)
+    n, Hq = q.shape[1], q.shape[2]
+    if out is None:
+        out = torch.empty(B, n, Hq * D, dtype=BF16, device=dev)
+    if q.shape != (B, n, Hq, D) or out.shape != (B, n, Hq * D) or q.dtype != BF16 or out.dtype != BF16 or out.device != dev or \
+            (q.numel() and (q.stride(3) != 1 or out.stride(2) != 1)):
+        _kv8_fail(what, f"q {tuple(q.shape)}, out {tuple(out.shape)} for a cache of B={B} H={H} D={D} (bf16, contiguous rows)")
+    if ws is None:
+        ws = attn_kv8_workspace(B, n, Hq, H, D, C, dev, weights is not None)
+    elif ws.device != dev:
+        _kv8_fail(what, f"the workspace must be on {dev}")
+    _kv8_call(lib().vt_attn_kv8, "vt_attn_kv8", dev, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
+              cache.k.data_ptr(), cache.v.data_ptr(), cache.ks.data_ptr(), cache.vs.data_ptr(), C,
+              _kv8_vec(what, "lens", lens, (B,), torch.int32, dev),
+              None if counts is None else _kv8_vec(what, "counts", counts, (B,), torch.int32, dev), B, n, Hq, H, D,
+              int(bool(causal)), float(D ** -0.5 if scale is None else scale), out.data_ptr(), out.stride(0), out.stride(1), D,
+              None if weights is None else _kv8_vec(what, "weights", weights, (B, H, C), torch.float32, dev),
+              None if weights_in is None else _kv8_vec(what, "weights_in", weights_in, (B, H, C), torch.float32, dev),
+              ws.data_ptr(), ws.numel() * ws.element_size())
+    return out
+
+
+def kv8_evict(cache, weights, lens, keep, recent, dst, dst_weights, dst_lens, index=None):
+    """vt_kv8_evict: of each sequence with more than `keep` tokens (a multiple of 64) every head keeps its last `recent`
+    tokens and the keep - recent others with the largest weights [B, H, C], in order, in the cache dst; shorter
+    sequences are copied.  dst_weights fp32 [B, H, dst C] and dst_lens int32 [B] receive the kept weights and the new lengths,
+    index int32 [B, H, keep] (allocated when None, and returned) the slots they had.  dst must be another cache."""
+    what, dev = "kv8_evict", cache.k.device
+    B, H, C, D = _kv8_dims(what, cache, dev)
+    Bd, Hd, Cd, Dd = _kv8_dims(what, dst, dev)
+    if (Bd, Hd, Dd) != (B, H, D):
+        _kv8_fail(what, f"dst {tuple(dst.k.shape)} for a cache of {tuple(cache.k.shape)}")
+    if index is None:
+        index = torch.empty(B, H, keep, dtype=torch.int32, device=dev)
+    _kv8_call(lib().vt_kv8_evict, "vt_kv8_evict", dev, cache.k.data_ptr(), cache.v.data_ptr(), cache.ks.data_ptr(),
+              cache.vs.data_ptr(), C, _kv8_vec(what, "weights", weights, (B, H, C), torch.float32, dev),
+              _kv8_vec(what, "lens", lens, (B,), torch.int32, dev), B, H, D, int(keep), int(recent), dst.k.data_ptr(),
+              dst.v.data_ptr(), dst.ks.data_ptr(), dst.vs.data_ptr(), Cd,
+              _kv8_vec(what, "dst_weights", dst_weights, (B, H, Cd), torch.float32, dev),
+              _kv8_vec(what, "dst_lens", dst_lens, (B,), torch.int32, dev),
+              _kv8_vec(what, "index", index, (B, H, keep), torch.int32, dev))
+    return index
 
 
 def head_linear(x2, wt, bias, out):
