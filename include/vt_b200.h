@@ -302,7 +302,8 @@ int vt_rope_kv8(cudaStream_t stream, const uint16_t* qkv, long long sx_b, long l
                 const int* counts, uint16_t* q, long long sq_b, long long sq_t, long long sq_h, int8_t* kc, int8_t* vc,
                 float* ks, float* vs, int C);
 
-/* Bytes of the workspace of vt_attn_kv8 (0 for an empty problem); contents need no initialisation. */
+/* Bytes of the workspace of vt_attn_kv8 (0 for an empty problem), enough for fewer tokens, slots and sequences too;
+ * its contents need no initialisation. */
 long long vt_attn_kv8_ws_bytes(int B, int n, int Hq, int H, int D, int C, int weights);
 
 /* Attention of the n new rows of each sequence over its cache, their own tokens already in it: row i of sequence b
