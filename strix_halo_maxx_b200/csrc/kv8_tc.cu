@@ -1,0 +1,674 @@
+// Attention of many rows over the 8-bit cache (a prompt, a chunk of one) on tcgen05, and the weights its slots receive.
+//
+// A kv head's rows r = i * G + g (token i, query head h G + g of its group) go 256 to an item, two M = 128 tiles that share
+// every converted key tile.  The items' tiles of 64 keys (a cache block, so each tile has one K and one V scale) form
+// one list that is cut into equal runs, one for each SM, whatever the sequences' lengths and the causal limits; an item
+// that spans CTAs leaves its parts (unnormalised O, row max, row sum) for attn_kv8_tc_join_kernel.
+//
+// CTA = 13 warps:
+//   warps 0-3, 4-7   softmax of M tile 0 / 1, thread = row (TMEM lane): P = 2^(s - m) as bf16 over the scores;
+//   warps 8-11       codes -> bf16 operands in shared memory (ST stages), one tile's codes ahead in registers; q once an item;
+//   warp 12          tcgen05.mma: S_(j+1) of both M tiles, then O += P_j V_j of both (P from TMEM, V as an MN-major B operand).
+// Codes are exact in bf16: byte b -> 0x4300 | b, and (that & ~0x80) - (that & 0x80 | 0x4300) = 128 + low bits - (128 or 256).
+// K and V tiles have the same layout (no-swizzle core matrices, [D/8][64][8]), so both take the same conversion.
+// Scales cost nothing per score: K's joins the softmax scale of the tile; V's shifts the exponent, P' = vs P = 2^(s - (m - log2
+// vs)), and the row sum takes sum(P') / vs.  So P' is rounded to bf16 with its scale in the exponent, whatever its size
+// (scales of 2^-100 .. 2^100; V blocks with a smaller one are zeros).
+// Bound: MUFU (one ex2 a score, 16 a clock and SM) for D = 64, the tensor pipe nearly as much for D = 128.
+#include "vt_common.cuh"
+#include "vt_host.h"
+
+namespace vt {
+namespace kv8 {
+namespace tc {
+
+constexpr int ROWS = 256, KEYS = 64, THREADS = 13 * 32, ST = 3, MAXB = 2048;
+constexpr uint32_t TMEM_COLS = 512;  // S of M tile t, buffer f: columns 128 t + 64 f; O of tile t: 256 + 128 t
+constexpr long long kDrainCycles = 200000000LL;
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr float kTinyScale = 0x1p-100f;
+constexpr int WHOLE_TILES = 24;  // items of up to so many tiles stay whole when there are fewer of them than SMs
+
+template <int D>
+struct Smem {
+  static constexpr int QT = 128 * D * 2;   // bytes of one M tile of q
+  static constexpr int KT = KEYS * D * 2;  // of a converted K or V tile
+  static constexpr int K = 2 * QT, V = K + ST * KT, BYTES = V + ST * KT;
+};
+
+struct Args {
+  const uint16_t* q;
+  long long sq_b, sq_t, sq_h;
+  const int8_t *kc, *vc;
+  const float *ks, *vs;
+  const int *lens, *counts;
+  int B, n, G, H, C, causal, rows, ctas;
+  float scale_log2;
+  uint16_t* out;
+  long long so_b, so_t, so_h;
+  float* part_o;     // [2 ctas][ROWS][D]
+  float2* part_ml;   // [2 ctas][ROWS]
+  float* lse;        // [B][H][rows], or null
+  float* w;
+  const float* w_in;
+};
+
+struct Plan {
+  int rows, ctas;
+  long long ml_off, lse_off, bytes;
+};
+static Plan make_plan(int B, int n, int Hq, int H, int D, bool weights, int sms) {
+  Plan p;
+  p.rows = n * (Hq / H);
+  p.ctas = sms;
+  auto up = [](long long x) { return (x + 255) / 256 * 256; };
+  p.ml_off = up(2LL * sms * ROWS * D * 4);
+  p.lse_off = p.ml_off + up(2LL * sms * ROWS * 8);
+  p.bytes = p.lse_off + (weights ? up((long long)B * H * p.rows * 4) : 0);
+  return p;
+}
+
+// Key tiles of rows [ROWS qt, ROWS qt + ROWS) of one head: up to the last key that the last of them sees.
+__device__ __forceinline__ int item_tiles(const Args& a, const Seq& s, int qt) {
+  const int last = min((qt * ROWS + ROWS - 1) / a.G, s.cnt - 1);
+  return ((a.causal ? s.len + last + 1 : s.len + s.cnt) + KEYS - 1) / KEYS;
+}
+__device__ __forceinline__ int seq_items(const Args& a, const Seq& s) { return (s.cnt * a.G + ROWS - 1) / ROWS; }
+
+// The list of all tiles, sequence by sequence, head by head, item by item: pre[b] first tile of sequence b; and the run.
+__device__ __forceinline__ int tile_list(const Args& a, int* pre, int* scratch) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x / 32;
+  if (tid == 0) scratch[nw] = 0;
+  __syncthreads();
+  const int per = (a.B + (int)blockDim.x - 1) / (int)blockDim.x, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
+  int sum = 0, most = 0;
+  for (int b = b0; b < b1; b++) {
+    Seq s;
+    s.len = min(max(a.lens[b], 0), a.C);
+    s.cnt = min(min(max(a.counts ? a.counts[b] : a.n, 0), a.n), a.C - s.len);
+    int t = 0;
+    const int items = seq_items(a, s);
+    if (a.causal)
+      for (int q = 0; q < items; q++) t += item_tiles(a, s, q);
+    else if (items)
+      t = items * item_tiles(a, s, 0);
+    if (items) most = max(most, item_tiles(a, s, items - 1));
+    pre[b] = t * a.H;
+    sum += t * a.H;
+  }
+  int inc = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += y;
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 31) scratch[warp] = inc;
+  if (lane == 0) atomicMax(&scratch[nw], most);
+  __syncthreads();
+  int at = inc - sum;
+  for (int i = 0; i < warp; i++) at += scratch[i];
+  for (int b = b0; b < b1; b++) {
+    const int t = pre[b];
+    pre[b] = at;
+    at += t;
+  }
+  if (tid == (int)blockDim.x - 1) pre[a.B] = at;
+  __syncthreads();
+  const int run = max((pre[a.B] + a.ctas - 1) / a.ctas, 1);
+  // fewer tiles for each CTA than the largest item has, and not many: whole items, no parts to join
+  return run < scratch[nw] && scratch[nw] <= WHOLE_TILES ? scratch[nw] : run;
+}
+
+// A CTA's share of one item: rows r0 .. of (b, h), key tiles [ta, tb) of `tiles`.
+struct Seg {
+  int b, h, r0, ta, tb, tiles;
+  Seq s;
+};
+__device__ __forceinline__ Seg segment(const Args& a, const int* pre, int u, int u_end) {
+  Seg g;
+  g.b = split::find_seq(pre, a.B, u);
+  g.s = seq_of(a.lens, a.counts, g.b, a.n, a.C);
+  const int head = (pre[g.b + 1] - pre[g.b]) / a.H;  // tiles of one head
+  g.h = (u - pre[g.b]) / head;
+  int at = (u - pre[g.b]) % head, qt = 0;
+  for (g.tiles = item_tiles(a, g.s, 0); at >= g.tiles; g.tiles = item_tiles(a, g.s, ++qt)) at -= g.tiles;
+  g.r0 = qt * ROWS, g.ta = at, g.tb = min(g.tiles, at + (u_end - u));
+  return g;
+}
+
+__device__ __forceinline__ uint32_t sub_bf2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Two codes (bytes lo, lo + 1 of x) as bf16.
+template <int SEL>
+__device__ __forceinline__ uint32_t bf_of_codes(uint32_t x) {
+  const uint32_t w = __byte_perm(x, 0x43434343u, SEL);
+  return sub_bf2(w & 0xff7fff7fu, w & 0xff80ff80u);
+}
+// 16 codes of a row: dims 16 p .. of row `row` into operand chunks 2p, 2p + 1 (CR rows each).
+template <int CR>
+__device__ __forceinline__ void store_codes(uint8_t* tile, int row, int p, uint4 c) {
+  uint8_t* at = tile + (2 * p * CR + row) * 16;
+  *reinterpret_cast<uint4*>(at) = make_uint4(bf_of_codes<0x4140>(c.x), bf_of_codes<0x4342>(c.x), bf_of_codes<0x4140>(c.y), bf_of_codes<0x4342>(c.y));
+  *reinterpret_cast<uint4*>(at + CR * 16) = make_uint4(bf_of_codes<0x4140>(c.z), bf_of_codes<0x4342>(c.z), bf_of_codes<0x4140>(c.w), bf_of_codes<0x4342>(c.w));
+}
+// The address of q row r of (b, h).
+__device__ __forceinline__ const uint16_t* q_row(const Args& a, int b, int h, int r) {
+  return a.q + b * a.sq_b + r / a.G * a.sq_t + (size_t)(h * a.G + r % a.G) * a.sq_h;
+}
+
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
+  using L = Smem<D>;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  __shared__ int pre[MAXB + 1], scratch[THREADS / 32 + 1];
+  __shared__ __align__(8) uint64_t bars[2 + 2 * ST + 4 + 4 + 4 + 1];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int sh_abort;
+  volatile int* abort_flag = &sh_abort;
+  uint64_t *q_full = bars, *q_empty = bars + 1, *kv_full = bars + 2, *kv_empty = kv_full + ST;
+  uint64_t *s_full = kv_empty + ST, *p_full = s_full + 4, *o_full = p_full + 4, *o_empty = o_full + 2, *drain = o_empty + 2;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    mbar_init(q_full, 4);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < ST; i++) mbar_init(&kv_full[i], 4), mbar_init(&kv_empty[i], 1);
+    for (int i = 0; i < 4; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4);
+    for (int i = 0; i < 2; i++) mbar_init(&o_full[i], 1), mbar_init(&o_empty[i], 4);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(&tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  griddep_wait();  // programmatic dependent launch: the previous kernel has completed
+  griddep_launch();
+  const int run = tile_list(a, pre, scratch), total = pre[a.B];
+  const int u_begin = (int)min((long long)blockIdx.x * run, (long long)total);
+  const int u_end = (int)min((long long)u_begin + run, (long long)total);
+
+  if (warp == 12) {
+    if (lane == 0) {
+      // ---------------- MMA issuer.  j: key tiles of all segments; js: of those in which M tile t had rows
+      constexpr uint32_t IDESC_S = idesc_bf16(128, KEYS), IDESC_O = idesc_bf16(128, D) | (1u << 16);  // V MN-major
+      const uint32_t sq = smem_u32(sm), sk = smem_u32(sm + L::K), sv = smem_u32(sm + L::V);
+      bool ok = true;
+      int j = 0, seg = 0, js[2] = {0, 0}, so[2] = {0, 0};
+      for (int u = u_begin; u < u_end && ok; seg++) {
+        const Seg g = segment(a, pre, u, u_end);
+        const int nt = g.tb - g.ta, mt = g.s.cnt * a.G - g.r0 > 128 ? 2 : 1;
+        u += nt;
+        auto issue_s = [&](int i) -> bool {  // tile i of the segment
+          const int st = (j + i) % ST;
+          if (!mbar_wait(&kv_full[st], ((j + i) / ST) & 1, abort_flag, ST_KV8_WAIT)) return false;
+          tc_fence_after();
+          for (int t = 0; t < mt; t++) {
+            const int f = (js[t] + i) & 1;
+#pragma unroll
+            for (int k = 0; k < D / 16; k++)
+              umma_f16(tmem + 128 * t + 64 * f, sdesc_noswz(sq + t * L::QT + k * 4096, 2048, 128),
+                       sdesc_noswz(sk + st * L::KT + k * 2048, 1024, 128), IDESC_S, k > 0 ? 1u : 0u);
+            umma_commit(&s_full[2 * t + f]);
+          }
+          if (i == nt - 1) umma_commit(q_empty);
+          return true;
+        };
+        ok = mbar_wait(q_full, seg & 1, abort_flag, ST_KV8_WAIT) && issue_s(0);
+        for (int i = 0; i < nt && ok; i++) {
+          if (i + 1 < nt && !issue_s(i + 1)) { ok = false; break; }
+          const int st = (j + i) % ST;
+          for (int t = 0; t < mt && ok; t++) {
+            const int f = (js[t] + i) & 1;
+            if (i == 0 && so[t] > 0 && !mbar_wait(&o_empty[t], (so[t] - 1) & 1, abort_flag, ST_KV8_WAIT)) { ok = false; break; }
+            if (!mbar_wait(&p_full[2 * t + f], ((js[t] + i) >> 1) & 1, abort_flag, ST_KV8_WAIT)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < KEYS / 16; k++)
+              umma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 64 * f + k * 8,
+                          sdesc_noswz(sv + st * L::KT + k * 256, 128, 1024), IDESC_O, i > 0 || k > 0 ? 1u : 0u);
+            if (i == nt - 1) umma_commit(&o_full[t]);
+          }
+          if (ok) umma_commit(&kv_empty[st]);
+        }
+        j += nt;
+        for (int t = 0; t < mt; t++) js[t] += nt, so[t]++;
+      }
+      umma_commit(drain);
+      mbar_wait_drain(drain, 0, kDrainCycles);
+    }
+  } else if (warp >= 8) {
+    // ---------------- converters: warp w rows 16 w .. of a tile, 8 lanes = 8 rows of one 16-byte piece
+    constexpr int PC = D / 64;  // pieces a lane takes of a row
+    const int w = warp - 8, ct = tid - 256;
+    bool ok = true;
+    int j = 0, seg = 0;
+    for (int u = u_begin; u < u_end && ok; seg++) {
+      const Seg g = segment(a, pre, u, u_end);
+      const int nt = g.tb - g.ta;
+      u += nt;
+      const size_t bh = (size_t)g.b * a.H + g.h;
+      const int8_t *kp = a.kc + bh * a.C * D, *vp = a.vc + bh * a.C * D;
+      const float* vsp = a.vs + bh * (a.C / BLK) + g.ta;
+      uint4 kr[2 * PC], vr[2 * PC];
+      float sr;
+      auto fetch = [&](int i) {
+        sr = vsp[i];
+#pragma unroll
+        for (int x = 0; x < 2 * PC; x++) {
+          const int row = 16 * w + 8 * (x & 1) + (lane & 7), p = (lane >> 3) + 4 * (x >> 1);
+          const size_t off = ((size_t)(g.ta + i) * KEYS + row) * D + 16 * p;
+          kr[x] = *reinterpret_cast<const uint4*>(kp + off);
+          vr[x] = *reinterpret_cast<const uint4*>(vp + off);
+        }
+      };
+      fetch(0);
+      if (seg > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1) & 1, abort_flag, ST_KV8_WAIT));
+      if (!ok) break;
+      for (int e = ct; e < ROWS * D / 8; e += 128) {
+        const int r = e % ROWS, c = e / ROWS;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (g.r0 + r < g.s.cnt * a.G) v = *reinterpret_cast<const uint4*>(q_row(a, g.b, g.h, g.r0 + r) + 8 * c);
+        *reinterpret_cast<uint4*>(sm + (r >> 7) * L::QT + (c * 128 + (r & 127)) * 16) = v;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      for (int i = 0; i < nt; i++, j++) {
+        const int st = j % ST;
+        uint4 kn[2 * PC], vn[2 * PC];
+#pragma unroll
+        for (int x = 0; x < 2 * PC; x++) kn[x] = kr[x], vn[x] = sr < kTinyScale ? make_uint4(0, 0, 0, 0) : vr[x];
+        if (i + 1 < nt) fetch(i + 1);
+        if (j >= ST) ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[st], (j / ST - 1) & 1, abort_flag, ST_KV8_WAIT));
+        if (!ok) break;
+#pragma unroll
+        for (int x = 0; x < 2 * PC; x++) {
+          const int row = 16 * w + 8 * (x & 1) + (lane & 7), p = (lane >> 3) + 4 * (x >> 1);
+          store_codes<KEYS>(sm + L::K + st * L::KT, row, p, kn[x]);
+          store_codes<KEYS>(sm + L::V + st * L::KT, row, p, vn[x]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kv_full[st]);
+      }
+    }
+  } else {
+    // ---------------- softmax of M tile t: thread = row
+    const int t = warp >> 2;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16, t_o = tmem + 256 + 128 * t + lane_off;
+    bool ok = true;
+    int j = 0, js = 0, so = 0;
+    for (int u = u_begin; u < u_end && ok;) {
+      const Seg g = segment(a, pre, u, u_end);
+      const int nt = g.tb - g.ta, row = g.r0 + 128 * t + (warp & 3) * 32 + lane, valid = g.s.cnt * a.G;
+      const bool first = u == u_begin;
+      u += nt;
+      if (g.r0 + 128 * t >= valid) {  // no rows: the MMA issuer skips this M tile too
+        j += nt;
+        continue;
+      }
+      const size_t bh = (size_t)g.b * a.H + g.h;
+      const float *ksp = a.ks + bh * (a.C / BLK) + g.ta, *vsp = a.vs + bh * (a.C / BLK) + g.ta;
+      const int lim = a.causal ? g.s.len + min(row / a.G, g.s.cnt - 1) + 1 : g.s.len + g.s.cnt;
+      // the fewest keys that a row of this warp sees: tiles up to there need no mask
+      const int lim_min = __reduce_min_sync(0xffffffffu, lim);
+      float m = -INFINITY, l = 0.f;
+      float ks_next = ksp[0], vs_next = vsp[0];
+      for (int i = 0; i < nt; i++) {
+        const int f = (js + i) & 1, key0 = (g.ta + i) * KEYS;
+        const float c = ks_next * a.scale_log2;
+        const float vs = vs_next < kTinyScale ? 1.f : vs_next;  // the converters made V zero
+        if (i + 1 < nt) ks_next = ksp[i + 1], vs_next = vsp[i + 1];
+        const float lvs = log2f(vs), ivs = 1.f / vs;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * t + f], ((js + i) >> 1) & 1, abort_flag, ST_KV8_WAIT));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t t_s = tmem + 128 * t + 64 * f + lane_off;
+        const bool edge = key0 + KEYS > lim_min;
+        uint32_t r0[32], r1[32];
+        tmem_ld32(t_s, r0);
+        tmem_ld32(t_s + 32, r1);
+        tmem_ld_wait();
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 32; e++) {
+            if (key0 + e >= lim) r0[e] = 0xff800000u;
+            if (key0 + 32 + e >= lim) r1[e] = 0xff800000u;
+          }
+        }
+        float x[22];
+#pragma unroll
+        for (int e = 0; e < 10; e++) {
+          x[e] = max3f(__uint_as_float(r0[3 * e]), __uint_as_float(r0[3 * e + 1]), __uint_as_float(r0[3 * e + 2]));
+          x[10 + e] = max3f(__uint_as_float(r1[3 * e]), __uint_as_float(r1[3 * e + 1]), __uint_as_float(r1[3 * e + 2]));
+        }
+        x[20] = fmaxf(__uint_as_float(r0[30]), __uint_as_float(r0[31]));
+        x[21] = fmaxf(__uint_as_float(r1[30]), __uint_as_float(r1[31]));
+#pragma unroll
+        for (int e = 0; e < 7; e++) x[e] = max3f(x[3 * e], x[3 * e + 1], x[3 * e + 2]);
+        float mx = fmaxf(max3f(max3f(x[0], x[1], x[2]), max3f(x[3], x[4], x[5]), x[6]), x[21]);
+        mx = mx == -INFINITY ? mx : mx * c;
+        if (i == 0) {
+          m = mx;
+        } else {
+          const bool need = mx > m + kRescaleThreshold;
+          if (__any_sync(0xffffffffu, need)) {  // O through registers (warp-collective), rare
+            // O must hold every product up to tile i - 1; the barrier's next arrival, ST tiles on, needs P of this row
+            ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[(j + i - 1) % ST], ((j + i - 1) / ST) & 1, abort_flag, ST_KV8_WAIT));
+            if (!ok) break;
+            tc_fence_after();
+            const float mn = need ? mx : m, alpha = need ? ex2_approx(m - mn) : 1.f;
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int x16 = 0; x16 < D / 16; x16++) {
+              uint32_t r[16];
+              tmem_ld16(t_o + x16 * 16, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
+              tmem_st16(t_o + x16 * 16, r);
+            }
+            tmem_st_wait();
+          }
+        }
+        // P' = 2^(s c - (m - log2 vs)), its sum / vs; a row that sees nothing of the tile takes no part in its scales
+        const float sh = (m == -INFINITY ? 0.f : m) - lvs;
+        const unsigned long long c2 = f2_pack(c, c), sh2 = f2_pack(-sh, -sh);
+        unsigned long long sum2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++) {
+          const uint32_t* r = hf ? r1 : r0;
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), c2, sh2), x0, x1);
+            float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+            if (edge) {
+              if (key0 + 32 * hf + 2 * e >= lim) p0 = 0.f;
+              if (key0 + 32 * hf + 2 * e + 1 >= lim) p1 = 0.f;
+            }
+            sum2[e & 3] = f2_add(sum2[e & 3], f2_pack(p0, p1));
+            pk[e] = pack_bf2(p0, p1);
+          }
+          tmem_st16(t_s + hf * 16, pk);
+        }
+        float lo, hi;
+        f2_unpack(f2_add(f2_add(sum2[0], sum2[1]), f2_add(sum2[2], sum2[3])), lo, hi);
+        if (key0 < lim) l += (lo + hi) * ivs;
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * t + f]);
+      }
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(&o_full[t], so & 1, abort_flag, ST_KV8_WAIT));
+      if (!ok) break;
+      tc_fence_after();
+      const bool whole = g.ta == 0 && g.tb == g.tiles;
+      const float inv = 1.f / l;
+      const int at = row - g.r0;
+      const size_t slot = (2 * (size_t)blockIdx.x + (first ? 0 : 1)) * ROWS + at;
+      uint16_t* op = a.out + g.b * a.so_b + row / a.G * a.so_t + (size_t)(g.h * a.G + row % a.G) * a.so_h;
+#pragma unroll
+      for (int x16 = 0; x16 < D / 16; x16++) {
+        uint32_t r[16];
+        tmem_ld16(t_o + x16 * 16, r);
+        tmem_ld_wait();
+        if (row < valid) {
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 8)
+              *reinterpret_cast<uint4*>(op + 16 * x16 + e) =
+                  make_uint4(pack_bf2(__uint_as_float(r[e]) * inv, __uint_as_float(r[e + 1]) * inv),
+                             pack_bf2(__uint_as_float(r[e + 2]) * inv, __uint_as_float(r[e + 3]) * inv),
+                             pack_bf2(__uint_as_float(r[e + 4]) * inv, __uint_as_float(r[e + 5]) * inv),
+                             pack_bf2(__uint_as_float(r[e + 6]) * inv, __uint_as_float(r[e + 7]) * inv));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<uint4*>(a.part_o + slot * D + 16 * x16 + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
+          }
+        }
+      }
+      if (row < valid) {
+        if (!whole) a.part_ml[slot] = make_float2(m, l);
+        else if (a.lse) a.lse[bh * a.rows + row] = m + log2f(l);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_empty[t]);
+      j += nt, js += nt, so++;
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// Merges the parts of an item, in the CTAs' order.  blockIdx.x = c: the item that CTA c left unfinished, if its first part is
+// in c's run; blockIdx.y: 16 of its rows; thread = 4 dims of a row.
+template <int D>
+__global__ void __launch_bounds__(128) attn_kv8_tc_join_kernel(Args a) {
+  __shared__ int pre[MAXB + 1], scratch[5];
+  constexpr int PER = 128 * 4 / D;
+  griddep_wait();
+  griddep_launch();
+  const int run = tile_list(a, pre, scratch), total = pre[a.B];
+  const long long bound = ((long long)blockIdx.x + 1) * run;  // first tile of the next CTA's run
+  if (bound >= total) return;
+  const Seg g = segment(a, pre, (int)bound, total);
+  const int u0 = (int)bound - g.ta, c0 = u0 / run, c1 = (u0 + g.tiles - 1) / run;
+  if (g.ta == 0 || c0 != (int)blockIdx.x) return;
+  const size_t first = 2 * (size_t)c0 + (u0 == c0 * run ? 0 : 1);
+  const int d = threadIdx.x % (D / 4) * 4;
+  const size_t bh = (size_t)g.b * a.H + g.h;
+  for (int x = threadIdx.x / (D / 4); x < 16; x += PER) {
+    const int at = blockIdx.y * 16 + x, row = g.r0 + at;
+    if (row >= g.s.cnt * a.G) break;
+    float mx = -INFINITY;
+    for (int c = c0; c <= c1; c++) mx = fmaxf(mx, a.part_ml[(c == c0 ? first : 2 * (size_t)c) * ROWS + at].x);
+    float sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+    for (int c = c0; c <= c1; c++) {
+      const size_t p = (c == c0 ? first : 2 * (size_t)c) * ROWS + at;
+      const float2 ml = a.part_ml[p];
+      const float4 o = *reinterpret_cast<const float4*>(a.part_o + p * D + d);
+      const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - mx);
+      sum += ml.y * f, v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
+    }
+    const float inv = 1.f / sum;
+    uint16_t* op = a.out + g.b * a.so_b + row / a.G * a.so_t + (size_t)(g.h * a.G + row % a.G) * a.so_h + d;
+    *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
+    if (d == 0 && a.lse) a.lse[bh * a.rows + row] = mx + log2f(sum);
+  }
+}
+
+// ---------------------------------------------------------------- weights
+// weights[b][h][j] = (j < len ? weights_in : 0) + sum over rows of 2^(s - lse): S^T = K Q^T with keys as the M dimension, so
+// a thread owns a key and adds up along its TMEM lane: no atomics, one order.  CTA = 128 keys of one (sequence, head);
+// rows 128 at a time:
+//   warps 0-3, 4-7   rows 0-63 / 64-127 of the row tile, thread = key;
+//   warps 8-11       K's codes -> the A operand once; q rows and lse of each row tile (2 stages);
+//   warp 12          tcgen05.mma into two S buffers.
+// Bound: MUFU, one ex2 a score.
+constexpr int WK = 128, WR = 128;
+template <int D>
+struct WSmem {
+  static constexpr int K = 0, Q = WK * D * 2, QT = WR * D * 2, BYTES = Q + 2 * QT;
+};
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1) kv8_weights_tc_kernel(Args a) {
+  using L = WSmem<D>;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  __shared__ __align__(16) float sh_lse[2][WR], half_sum[WK];
+  __shared__ __align__(8) uint64_t bars[2 + 2 + 2 + 2 + 1];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int sh_abort;
+  volatile int* abort_flag = &sh_abort;
+  uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *s_empty = bars + 6, *drain = bars + 8;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kt = (a.C + WK - 1) / WK, key0 = blockIdx.x % kt * WK;
+  const size_t bh = blockIdx.x / kt;
+  const int h = (int)(bh % a.H), b = (int)(bh / a.H);
+  griddep_wait();
+  const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C);
+  const int T = s.len + s.cnt, rows = s.cnt * a.G;
+  if (key0 >= T) return;
+  // the first row that sees a key of this CTA, down to a whole tile
+  const int first = a.causal ? max(key0 - s.len, 0) * a.G / WR : 0, nt = (rows + WR - 1) / WR - first;
+  if (tid == 0) {
+    for (int i = 0; i < 2; i++) mbar_init(&q_full[i], 4), mbar_init(&q_empty[i], 8), mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], 8);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(&tmem_slot, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  griddep_launch();  // not before the tensor memory is allocated: the next kernel's CTAs may take theirs while they wait
+  const uint32_t tmem = tmem_slot;
+  float acc = 0.f;
+  bool ok = true;
+  if (warp == 12) {
+    if (lane == 0) {
+      const uint32_t sk = smem_u32(sm + L::K), sq = smem_u32(sm + L::Q);
+      for (int i = 0; i < nt && ok; i++) {
+        const int f = i & 1;
+        ok = mbar_wait(&q_full[f], (i >> 1) & 1, abort_flag, ST_KV8_WAIT) &&
+             (i < 2 || mbar_wait(&s_empty[f], ((i >> 1) - 1) & 1, abort_flag, ST_KV8_WAIT));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < D / 16; k++)
+          umma_f16(tmem + 128 * f, sdesc_noswz(sk + k * 4096, 2048, 128), sdesc_noswz(sq + f * L::QT + k * 4096, 2048, 128),
+                   idesc_bf16(WK, WR), k > 0 ? 1u : 0u);
+        umma_commit(&s_full[f]);
+      }
+      umma_commit(drain);
+      mbar_wait_drain(drain, 0, kDrainCycles);
+    }
+  } else if (warp >= 8) {
+    const int w = warp - 8, ct = tid - 256;
+    const int8_t* kp = a.kc + bh * a.C * D;
+    for (int x = 0; x < 4 * (D / 64); x++) {  // warp w rows 32 w ..; slots behind the cache's last one are zero
+      const int row = 32 * w + 8 * (x & 3) + (lane & 7), p = (lane >> 3) + 4 * (x >> 2);
+      uint4 c = make_uint4(0, 0, 0, 0);
+      if (key0 + row < a.C) c = *reinterpret_cast<const uint4*>(kp + (size_t)(key0 + row) * D + 16 * p);
+      store_codes<WK>(sm + L::K, row, p, c);
+    }
+    for (int i = 0; i < nt; i++) {
+      const int f = i & 1, r0 = (first + i) * WR;
+      // the stage is free when both halves have read its lse, which comes after its products
+      if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[f], ((i >> 1) - 1) & 1, abort_flag, ST_KV8_WAIT));
+      if (!ok) break;
+      for (int e = ct; e < WR * D / 8; e += 128) {
+        const int r = e % WR, c = e / WR;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r0 + r < rows) v = *reinterpret_cast<const uint4*>(q_row(a, b, h, r0 + r) + 8 * c);
+        *reinterpret_cast<uint4*>(sm + L::Q + f * L::QT + (c * WR + r) * 16) = v;
+      }
+      sh_lse[f][ct] = r0 + ct < rows ? a.lse[bh * a.rows + r0 + ct] : INFINITY;  // rows past the last add 2^-inf
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[f]);
+    }
+  } else {
+    const int half = warp >> 2, key = key0 + (warp & 3) * 32 + lane;
+    const uint32_t t_s = tmem + 64 * half + ((uint32_t)((warp & 3) * 32) << 16);
+    const float c = key < T ? a.ks[bh * (a.C / BLK) + key / BLK] * a.scale_log2 : 0.f;
+    const int r_min = a.causal ? (key - s.len) * a.G : 0;  // rows before it do not see this key
+    const int warp_max = __reduce_max_sync(0xffffffffu, r_min);
+    unsigned long long acc2[2] = {0ull, 0ull};
+    for (int i = 0; i < nt; i++) {
+      const int f = i & 1, r0 = (first + i) * WR + 64 * half;
+      ok = __all_sync(0xffffffffu, mbar_wait(&q_full[f], (i >> 1) & 1, abort_flag, ST_KV8_WAIT) &&  // lse
+                                       mbar_wait(&s_full[f], (i >> 1) & 1, abort_flag, ST_KV8_WAIT));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t x0[32], x1[32];
+      tmem_ld32(t_s + 128 * f, x0);
+      tmem_ld32(t_s + 128 * f + 32, x1);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_empty[f]);
+      const bool edge = r0 < warp_max;
+      const unsigned long long c2 = f2_pack(c, c), minus = f2_pack(-1.f, -1.f);
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++) {
+        const uint32_t* x = hf ? x1 : x0;
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 z = *reinterpret_cast<const float4*>(&sh_lse[f][64 * half + 32 * hf + e]);
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            const unsigned long long lz = k ? f2_pack(z.z, z.w) : f2_pack(z.x, z.y);
+            const unsigned long long y = f2_fma(f2_pack(__uint_as_float(x[e + 2 * k]), __uint_as_float(x[e + 2 * k + 1])), c2, f2_mul(lz, minus));
+            float y0, y1;
+            f2_unpack(y, y0, y1);
+            y0 = ex2_approx(y0), y1 = ex2_approx(y1);
+            if (edge) {
+              if (r0 + 32 * hf + e + 2 * k < r_min) y0 = 0.f;
+              if (r0 + 32 * hf + e + 2 * k + 1 < r_min) y1 = 0.f;
+            }
+            acc2[k] = f2_add(acc2[k], f2_pack(y0, y1));
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_empty[f]);
+    }
+    float lo, hi;
+    f2_unpack(f2_add(acc2[0], acc2[1]), lo, hi);
+    acc = lo + hi;
+    if (half == 1) half_sum[key - key0] = acc;
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp < 4) {
+    const int key = key0 + tid;
+    if (key < T) {
+      const size_t at = bh * a.C + key;
+      a.w[at] = (a.w_in && key < s.len ? a.w_in[at] : 0.f) + (acc + half_sum[tid]);
+    }
+  }
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+template <int D>
+static int launch(cudaStream_t st, const Args& a) {
+  int rc = smem_attr_once((const void*)attn_kv8_tc_kernel<D>, Smem<D>::BYTES, "vt_attn_kv8");
+  if (!rc) rc = smem_attr_once((const void*)kv8_weights_tc_kernel<D>, WSmem<D>::BYTES, "vt_attn_kv8");
+  if (rc) return rc;
+  launch_k(attn_kv8_tc_kernel<D>, a.ctas, THREADS, Smem<D>::BYTES, st, a);
+  launch_k(attn_kv8_tc_join_kernel<D>, dim3(a.ctas, ROWS / 16), 128, 0, st, a);
+  if (a.w) launch_k(kv8_weights_tc_kernel<D>, (unsigned)(a.B * a.H * ((a.C + WK - 1) / WK)), THREADS, WSmem<D>::BYTES, st, a);
+  return check_launch("vt_attn_kv8");
+}
+
+}  // namespace tc
+}  // namespace kv8
+}  // namespace vt
