@@ -5,16 +5,18 @@
 // one list that is cut into equal runs, one for each SM, whatever the sequences' lengths and the causal limits; an item
 // that spans CTAs leaves its parts (unnormalised O, row max, row sum) for attn_kv8_tc_join_kernel.
 //
-// CTA = 13 warps:
+// CTA = 14 warps:
 //   warps 0-3, 4-7   softmax of M tile 0 / 1, thread = row (TMEM lane): P = 2^(s - m) as bf16 over the scores;
 //   warps 8-11       codes -> bf16 operands in shared memory (ST stages), one tile's codes ahead in registers; q once an item;
-//   warp 12          tcgen05.mma: S_(j+1) of both M tiles, then O += P_j V_j of both (P from TMEM, V as an MN-major B operand).
+//   warps 12, 13     tcgen05.mma of M tile 0 / 1: S_(j+1), then O += P_j V_j (P from TMEM, V as an MN-major B operand).
 // Codes are exact in bf16: byte b -> 0x4300 | b, and (that & ~0x80) - (that & 0x80 | 0x4300) = 128 + low bits - (128 or 256).
 // K and V tiles have the same layout (no-swizzle core matrices, [D/8][64][8]), so both take the same conversion.
 // Scales cost nothing per score: K's joins the softmax scale of the tile; V's shifts the exponent, P' = vs P = 2^(s - (m - log2
 // vs)), and the row sum takes sum(P') / vs.  So P' is rounded to bf16 with its scale in the exponent, whatever its size
 // (scales of 2^-100 .. 2^100; V blocks with a smaller one are zeros).
 // Bound: MUFU (one ex2 a score, 16 a clock and SM) for D = 64, the tensor pipe nearly as much for D = 128.
+#include <type_traits>
+
 #include "vt_common.cuh"
 #include "vt_host.h"
 
@@ -22,7 +24,7 @@ namespace vt {
 namespace kv8 {
 namespace tc {
 
-constexpr int ROWS = 256, KEYS = 64, THREADS = 13 * 32, ST = 3, MAXB = 2048;
+constexpr int ROWS = 256, KEYS = 64, THREADS = 14 * 32, ST = 3, MAXB = 2048;
 constexpr uint32_t TMEM_COLS = 512;  // S of M tile t, buffer f: columns 128 t + 64 f; O of tile t: 256 + 128 t
 constexpr long long kDrainCycles = 200000000LL;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
@@ -165,20 +167,21 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
   using L = Smem<D>;
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ int pre[MAXB + 1], scratch[THREADS / 32 + 1];
-  __shared__ __align__(8) uint64_t bars[2 + 2 * ST + 4 + 4 + 4 + 1];
+  __shared__ __align__(8) uint64_t bars[2 + 2 * ST + 4 + 4 + 4 + 2];
   __shared__ uint32_t tmem_slot;
   __shared__ int sh_abort;
   volatile int* abort_flag = &sh_abort;
-  uint64_t *q_full = bars, *q_empty = bars + 1, *kv_full = bars + 2, *kv_empty = kv_full + ST;
+  uint64_t *q_full = bars, *kv_full = bars + 2, *kv_empty = kv_full + ST;
   uint64_t *s_full = kv_empty + ST, *p_full = s_full + 4, *o_full = p_full + 4, *o_empty = o_full + 2, *drain = o_empty + 2;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    mbar_init(q_full, 4);
-    mbar_init(q_empty, 1);
-    for (int i = 0; i < ST; i++) mbar_init(&kv_full[i], 4), mbar_init(&kv_empty[i], 1);
+    mbar_init(&q_full[0], 4);
+    mbar_init(&q_full[1], 4);
+    for (int i = 0; i < ST; i++) mbar_init(&kv_full[i], 4), mbar_init(&kv_empty[i], 2);
     for (int i = 0; i < 4; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4);
     for (int i = 0; i < 2; i++) mbar_init(&o_full[i], 1), mbar_init(&o_empty[i], 4);
-    mbar_init(drain, 1);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -195,125 +198,147 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
   const int run = tile_list(a, pre, scratch), total = pre[a.B];
   const int u_begin = (int)min((long long)blockIdx.x * run, (long long)total);
   const int u_end = (int)min((long long)u_begin + run, (long long)total);
+  // a wait of the whole warp: every lane gives up when one does
+  auto wait = [&](uint64_t* bar, int parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, ST_KV8_WAIT)) != 0;
+  };
 
-  if (warp == 12) {
-    if (lane == 0) {
-      // ---------------- MMA issuer.  j: key tiles of all segments; js: of those in which M tile t had rows
-      constexpr uint32_t IDESC_S = idesc_bf16(128, KEYS), IDESC_O = idesc_bf16(128, D) | (1u << 16);  // V MN-major
-      const uint32_t sq = smem_u32(sm), sk = smem_u32(sm + L::K), sv = smem_u32(sm + L::V);
-      bool ok = true;
-      int j = 0, seg = 0, js[2] = {0, 0}, so[2] = {0, 0};
-      for (int u = u_begin; u < u_end && ok; seg++) {
-        const Seg g = segment(a, pre, u, u_end);
-        const int nt = g.tb - g.ta, mt = g.s.cnt * a.G - g.r0 > 128 ? 2 : 1;
-        u += nt;
-        auto issue_s = [&](int i) -> bool {  // tile i of the segment
-          const int st = (j + i) % ST;
-          if (!mbar_wait(&kv_full[st], ((j + i) / ST) & 1, abort_flag, ST_KV8_WAIT)) return false;
-          tc_fence_after();
-          for (int t = 0; t < mt; t++) {
-            const int f = (js[t] + i) & 1;
-#pragma unroll
-            for (int k = 0; k < D / 16; k++)
-              umma_f16(tmem + 128 * t + 64 * f, sdesc_noswz(sq + t * L::QT + k * 4096, 2048, 128),
-                       sdesc_noswz(sk + st * L::KT + k * 2048, 1024, 128), IDESC_S, k > 0 ? 1u : 0u);
-            umma_commit(&s_full[2 * t + f]);
-          }
-          if (i == nt - 1) umma_commit(q_empty);
-          return true;
-        };
-        ok = mbar_wait(q_full, seg & 1, abort_flag, ST_KV8_WAIT) && issue_s(0);
-        for (int i = 0; i < nt && ok; i++) {
-          if (i + 1 < nt && !issue_s(i + 1)) { ok = false; break; }
-          const int st = (j + i) % ST;
-          for (int t = 0; t < mt && ok; t++) {
-            const int f = (js[t] + i) & 1;
-            if (i == 0 && so[t] > 0 && !mbar_wait(&o_empty[t], (so[t] - 1) & 1, abort_flag, ST_KV8_WAIT)) { ok = false; break; }
-            if (!mbar_wait(&p_full[2 * t + f], ((js[t] + i) >> 1) & 1, abort_flag, ST_KV8_WAIT)) { ok = false; break; }
-            tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < KEYS / 16; k++)
-              umma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 64 * f + k * 8,
-                          sdesc_noswz(sv + st * L::KT + k * 256, 128, 1024), IDESC_O, i > 0 || k > 0 ? 1u : 0u);
-            if (i == nt - 1) umma_commit(&o_full[t]);
-          }
-          if (ok) umma_commit(&kv_empty[st]);
+  if (warp >= 12) {
+    // ---------------- MMA issuer of M tile t (one warp each: issuing is what a tile's time is made of otherwise).  The
+    // whole warp walks the loop, one lane issues.  j: key tiles of all segments; js: of those in which t had rows
+    const int t = warp - 12;
+    const uint32_t leader = elect_one();
+    constexpr uint32_t IDESC_S = idesc_bf16(128, KEYS), IDESC_O = idesc_bf16(128, D) | (1u << 16);  // V MN-major
+    const uint64_t dq = sdesc_noswz(smem_u32(sm) + t * L::QT, 2048, 128), dk = sdesc_noswz(smem_u32(sm + L::K), 1024, 128);
+    const uint64_t dv = sdesc_noswz(smem_u32(sm + L::V), 128, 1024);
+    const uint32_t t_s = tmem + 128 * t, t_o = tmem + 256 + 128 * t;
+    bool ok = true;
+    int st = 0, ph = 0, js = 0, so = 0;  // stage and phase of the next tile's operands; tiles, segments in which t had rows
+    auto next = [](int& x, int& y) { if (++x == ST) x = 0, y ^= 1; };
+    for (int u = u_begin; u < u_end && ok;) {
+      const Seg g = segment(a, pre, u, u_end);
+      const int nt = g.tb - g.ta;
+      u += nt;
+      if (g.r0 + 128 * t >= g.s.cnt * a.G) {  // no rows in this M tile: only the barriers
+        for (int i = 0; i < nt && ok; i++, next(st, ph)) {
+          ok = wait(&kv_full[st], ph);
+          if (leader) mbar_arrive(&kv_empty[st]);
         }
-        j += nt;
-        for (int t = 0; t < mt; t++) js[t] += nt, so[t]++;
+        continue;
       }
-      umma_commit(drain);
-      mbar_wait_drain(drain, 0, kDrainCycles);
+      auto issue_s = [&](int i) {  // S_i of the segment; its operands' stage is st
+        if (!wait(&kv_full[st], ph)) return false;
+        tc_fence_after();
+        const int f = (js + i) & 1;
+        if (leader) {
+          const uint64_t b = dk + st * (L::KT >> 4);
+#pragma unroll
+          for (int k = 0; k < D / 16; k++) umma_f16(t_s + 64 * f, dq + k * (4096 >> 4), b + k * (2048 >> 4), IDESC_S, k > 0 ? 1u : 0u);
+          umma_commit(&s_full[2 * t + f]);
+        }
+        __syncwarp();
+        next(st, ph);
+        return true;
+      };
+      int sv = st;  // stage of tile i
+      ok = wait(&q_full[t], so & 1) && issue_s(0);
+      for (int i = 0; i < nt && ok; i++, sv = sv + 1 == ST ? 0 : sv + 1) {
+        const int f = (js + i) & 1;
+        ok = (i + 1 == nt || issue_s(i + 1)) && (i > 0 || so == 0 || wait(&o_empty[t], (so - 1) & 1)) &&
+             wait(&p_full[2 * t + f], ((js + i) >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+          const uint64_t b = dv + sv * (L::KT >> 4);
+#pragma unroll
+          for (int k = 0; k < KEYS / 16; k++) umma_f16_ts(t_o, t_s + 64 * f + k * 8, b + k * (256 >> 4), IDESC_O, i > 0 || k > 0 ? 1u : 0u);
+          umma_commit(&kv_empty[sv]);
+          if (i == nt - 1) umma_commit(&o_full[t]);
+        }
+        __syncwarp();
+      }
+      js += nt, so++;
+    }
+    if (leader) {
+      umma_commit(&drain[t]);
+      mbar_wait_drain(&drain[t], 0, kDrainCycles);
     }
   } else if (warp >= 8) {
-    // ---------------- converters: warp w rows 16 w .. of a tile, 8 lanes = 8 rows of one 16-byte piece
-    constexpr int PC = D / 64;  // pieces a lane takes of a row
-    const int w = warp - 8, ct = tid - 256;
+    // ---------------- converters: warp w rows 16 w .. of a block, 8 lanes = 8 rows of one 16-byte piece.  K's and V's codes of
+    // the next tile are fetched as soon as this tile's are out of the registers
+    constexpr int PER = D / 32;  // pieces of a K or V block that a lane takes
+    const int w = warp - 8;
     bool ok = true;
-    int j = 0, seg = 0;
-    for (int u = u_begin; u < u_end && ok; seg++) {
+    int j = 0;
+    for (int u = u_begin; u < u_end && ok;) {
       const Seg g = segment(a, pre, u, u_end);
       const int nt = g.tb - g.ta;
       u += nt;
       const size_t bh = (size_t)g.b * a.H + g.h;
-      const int8_t *kp = a.kc + bh * a.C * D, *vp = a.vc + bh * a.C * D;
+      const int8_t *kp = a.kc + (bh * a.C + (size_t)g.ta * KEYS) * D, *vp = a.vc + (bh * a.C + (size_t)g.ta * KEYS) * D;
       const float* vsp = a.vs + bh * (a.C / BLK) + g.ta;
-      uint4 kr[2 * PC], vr[2 * PC];
-      float sr;
-      auto fetch = [&](int i) {
-        sr = vsp[i];
+      const int row = 16 * w + (lane & 7), piece = lane >> 3;
+      uint4 kr[PER], vr[PER];
+      float vs;
+      auto fetch = [&](uint4 (&to)[PER], const int8_t* from) {
 #pragma unroll
-        for (int x = 0; x < 2 * PC; x++) {
-          const int row = 16 * w + 8 * (x & 1) + (lane & 7), p = (lane >> 3) + 4 * (x >> 1);
-          const size_t off = ((size_t)(g.ta + i) * KEYS + row) * D + 16 * p;
-          kr[x] = *reinterpret_cast<const uint4*>(kp + off);
-          vr[x] = *reinterpret_cast<const uint4*>(vp + off);
-        }
+        for (int x = 0; x < PER; x++)
+          to[x] = *reinterpret_cast<const uint4*>(from + (row + 8 * (x & 1)) * D + 16 * (piece + 4 * (x >> 1)));
       };
-      fetch(0);
-      if (seg > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1) & 1, abort_flag, ST_KV8_WAIT));
-      if (!ok) break;
-      for (int e = ct; e < ROWS * D / 8; e += 128) {
-        const int r = e % ROWS, c = e / ROWS;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (g.r0 + r < g.s.cnt * a.G) v = *reinterpret_cast<const uint4*>(q_row(a, g.b, g.h, g.r0 + r) + 8 * c);
-        *reinterpret_cast<uint4*>(sm + (r >> 7) * L::QT + (c * 128 + (r & 127)) * 16) = v;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
+      auto convert = [&](uint8_t* tile, const uint4 (&from)[PER], bool zero) {
+#pragma unroll
+        for (int x = 0; x < PER; x++)
+          store_codes<KEYS>(tile, row + 8 * (x & 1), piece + 4 * (x >> 1), zero ? make_uint4(0, 0, 0, 0) : from[x]);
+      };
+      fetch(kr, kp);
+      fetch(vr, vp);
+      vs = vsp[0];
       for (int i = 0; i < nt; i++, j++) {
         const int st = j % ST;
-        uint4 kn[2 * PC], vn[2 * PC];
-#pragma unroll
-        for (int x = 0; x < 2 * PC; x++) kn[x] = kr[x], vn[x] = sr < kTinyScale ? make_uint4(0, 0, 0, 0) : vr[x];
-        if (i + 1 < nt) fetch(i + 1);
-        if (j >= ST) ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[st], (j / ST - 1) & 1, abort_flag, ST_KV8_WAIT));
+        if (j >= ST) ok = wait(&kv_empty[st], (j / ST - 1) & 1);
         if (!ok) break;
-#pragma unroll
-        for (int x = 0; x < 2 * PC; x++) {
-          const int row = 16 * w + 8 * (x & 1) + (lane & 7), p = (lane >> 3) + 4 * (x >> 1);
-          store_codes<KEYS>(sm + L::K + st * L::KT, row, p, kn[x]);
-          store_codes<KEYS>(sm + L::V + st * L::KT, row, p, vn[x]);
-        }
+        kp += KEYS * D, vp += KEYS * D;
+        convert(sm + L::K + st * L::KT, kr, false);
+        if (i + 1 < nt) fetch(kr, kp);
+        convert(sm + L::V + st * L::KT, vr, vs < kTinyScale);
+        if (i + 1 < nt) fetch(vr, vp), vs = vsp[i + 1];
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&kv_full[st]);
       }
     }
   } else {
-    // ---------------- softmax of M tile t: thread = row
+    // ---------------- softmax of M tile t: thread = row.  It brings in its row of q itself
     const int t = warp >> 2;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16, t_o = tmem + 256 + 128 * t + lane_off;
     bool ok = true;
     int j = 0, js = 0, so = 0;
+    auto load_q = [&](const Seg& g) {  // every product with the q before it is done: its last scores have been read
+      const int r = (warp & 3) * 32 + lane, row = g.r0 + 128 * t + r;
+      if (g.r0 + 128 * t >= g.s.cnt * a.G) return;
+      const uint16_t* src = q_row(a, g.b, g.h, min(row, g.s.cnt * a.G - 1));  // rows past the last are copies of it
+      uint8_t* dst = sm + t * L::QT + r * 16;
+#pragma unroll
+      for (int c0 = 0; c0 < D / 8; c0 += 8) {
+        uint4 v[8];
+#pragma unroll
+        for (int c = 0; c < 8; c++) v[c] = *reinterpret_cast<const uint4*>(src + 8 * (c0 + c));
+#pragma unroll
+        for (int c = 0; c < 8; c++) *reinterpret_cast<uint4*>(dst + (c0 + c) * 2048) = v[c];
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[t]);
+    };
+    Seg g;
+    if (u_begin < u_end) load_q(g = segment(a, pre, u_begin, u_end));
     for (int u = u_begin; u < u_end && ok;) {
-      const Seg g = segment(a, pre, u, u_end);
       const int nt = g.tb - g.ta, row = g.r0 + 128 * t + (warp & 3) * 32 + lane, valid = g.s.cnt * a.G;
       const bool first = u == u_begin;
       u += nt;
       if (g.r0 + 128 * t >= valid) {  // no rows: the MMA issuer skips this M tile too
         j += nt;
+        if (u < u_end) load_q(g = segment(a, pre, u, u_end));
         continue;
       }
       const size_t bh = (size_t)g.b * a.H + g.h;
@@ -322,103 +347,127 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       // the fewest keys that a row of this warp sees: tiles up to there need no mask
       const int lim_min = __reduce_min_sync(0xffffffffu, lim);
       float m = -INFINITY, l = 0.f;
+      float c, lvs, ivs;  // of the tile: K's scale times the softmax scale, log2 and inverse of V's scale
       float ks_next = ksp[0], vs_next = vsp[0];
       for (int i = 0; i < nt; i++) {
         const int f = (js + i) & 1, key0 = (g.ta + i) * KEYS;
-        const float c = ks_next * a.scale_log2;
-        const float vs = vs_next < kTinyScale ? 1.f : vs_next;  // the converters made V zero
-        if (i + 1 < nt) ks_next = ksp[i + 1], vs_next = vsp[i + 1];
-        const float lvs = log2f(vs), ivs = 1.f / vs;
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * t + f], ((js + i) >> 1) & 1, abort_flag, ST_KV8_WAIT));
-        if (!ok) break;
-        tc_fence_after();
         const uint32_t t_s = tmem + 128 * t + 64 * f + lane_off;
-        const bool edge = key0 + KEYS > lim_min;
+        {
+          const float v = vs_next < kTinyScale ? 1.f : vs_next;  // the converters made V zero
+          c = ks_next * a.scale_log2, lvs = log2f(v), ivs = 1.f / v;
+          if (i + 1 < nt) ks_next = ksp[i + 1], vs_next = vsp[i + 1];
+        }
         uint32_t r0[32], r1[32];
-        tmem_ld32(t_s, r0);
-        tmem_ld32(t_s + 32, r1);
-        tmem_ld_wait();
-        if (edge) {
+        float mx, sum;
+        auto top32 = [&](const uint32_t (&r)[32]) {
+          float x[11];
 #pragma unroll
-          for (int e = 0; e < 32; e++) {
-            if (key0 + e >= lim) r0[e] = 0xff800000u;
-            if (key0 + 32 + e >= lim) r1[e] = 0xff800000u;
-          }
-        }
-        float x[22];
+          for (int e = 0; e < 10; e++) x[e] = max3f(__uint_as_float(r[3 * e]), __uint_as_float(r[3 * e + 1]), __uint_as_float(r[3 * e + 2]));
+          x[10] = fmaxf(__uint_as_float(r[30]), __uint_as_float(r[31]));
 #pragma unroll
-        for (int e = 0; e < 10; e++) {
-          x[e] = max3f(__uint_as_float(r0[3 * e]), __uint_as_float(r0[3 * e + 1]), __uint_as_float(r0[3 * e + 2]));
-          x[10 + e] = max3f(__uint_as_float(r1[3 * e]), __uint_as_float(r1[3 * e + 1]), __uint_as_float(r1[3 * e + 2]));
-        }
-        x[20] = fmaxf(__uint_as_float(r0[30]), __uint_as_float(r0[31]));
-        x[21] = fmaxf(__uint_as_float(r1[30]), __uint_as_float(r1[31]));
-#pragma unroll
-        for (int e = 0; e < 7; e++) x[e] = max3f(x[3 * e], x[3 * e + 1], x[3 * e + 2]);
-        float mx = fmaxf(max3f(max3f(x[0], x[1], x[2]), max3f(x[3], x[4], x[5]), x[6]), x[21]);
-        mx = mx == -INFINITY ? mx : mx * c;
-        if (i == 0) {
-          m = mx;
-        } else {
-          const bool need = mx > m + kRescaleThreshold;
-          if (__any_sync(0xffffffffu, need)) {  // O through registers (warp-collective), rare
-            // O must hold every product up to tile i - 1; the barrier's next arrival, ST tiles on, needs P of this row
-            ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[(j + i - 1) % ST], ((j + i - 1) / ST) & 1, abort_flag, ST_KV8_WAIT));
-            if (!ok) break;
-            tc_fence_after();
-            const float mn = need ? mx : m, alpha = need ? ex2_approx(m - mn) : 1.f;
-            m = mn;
-            l *= alpha;
-#pragma unroll
-            for (int x16 = 0; x16 < D / 16; x16++) {
-              uint32_t r[16];
-              tmem_ld16(t_o + x16 * 16, r);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 16; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
-              tmem_st16(t_o + x16 * 16, r);
-            }
-            tmem_st_wait();
-          }
-        }
-        // P' = 2^(s c - (m - log2 vs)), its sum / vs; a row that sees nothing of the tile takes no part in its scales
-        const float sh = (m == -INFINITY ? 0.f : m) - lvs;
-        const unsigned long long c2 = f2_pack(c, c), sh2 = f2_pack(-sh, -sh);
-        unsigned long long sum2[4] = {0ull, 0ull, 0ull, 0ull};
-#pragma unroll
-        for (int hf = 0; hf < 2; hf++) {
-          const uint32_t* r = hf ? r1 : r0;
+          for (int e = 0; e < 3; e++) x[e] = max3f(x[3 * e], x[3 * e + 1], x[3 * e + 2]);
+          return max3f(max3f(x[0], x[1], x[2]), x[9], x[10]);
+        };
+        // P' = 2^(s c - (m - log2 vs)) of 32 scores into columns `at` of P; returns their sum
+        auto exps = [&](const uint32_t (&r)[32], uint32_t at, float mu) {
+          const unsigned long long c2 = f2_pack(c, c), sh2 = f2_pack(lvs - mu, lvs - mu);
+          unsigned long long sum2[2] = {0ull, 0ull};
           uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 16; e++) {
             float x0, x1;
             f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), c2, sh2), x0, x1);
-            float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-            if (edge) {
-              if (key0 + 32 * hf + 2 * e >= lim) p0 = 0.f;
-              if (key0 + 32 * hf + 2 * e + 1 >= lim) p1 = 0.f;
-            }
-            sum2[e & 3] = f2_add(sum2[e & 3], f2_pack(p0, p1));
+            const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+            sum2[e & 1] = f2_add(sum2[e & 1], f2_pack(p0, p1));
             pk[e] = pack_bf2(p0, p1);
           }
-          tmem_st16(t_s + hf * 16, pk);
+          tmem_st16(t_s + at, pk);
+          float lo, hi;
+          f2_unpack(f2_add(sum2[0], sum2[1]), lo, hi);
+          return lo + hi;
+        };
+        ok = wait(&s_full[2 * t + f], ((js + i) >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        tmem_ld32(t_s, r0);
+        tmem_ld_wait();
+        tmem_ld32(t_s + 32, r1);
+        // a tile that every row sees whole, once a row has a maximum: P with the maximum so far, while the second half of
+        // the scores arrives and the new maximum is found beside the exponentials; they stand unless it grew by 2^8
+        const bool edge = key0 + KEYS > lim_min;
+        bool again = i == 0 || edge;
+        if (!again) {
+          sum = exps(r0, 0, m);
+          const float ma = top32(r0);
+          tmem_ld_wait();
+          sum += exps(r1, 16, m);
+          mx = fmaxf(ma, top32(r1)) * c;
+          again = __any_sync(0xffffffffu, mx > m + kRescaleThreshold);
         }
-        float lo, hi;
-        f2_unpack(f2_add(f2_add(sum2[0], sum2[1]), f2_add(sum2[2], sum2[3])), lo, hi);
-        if (key0 < lim) l += (lo + hi) * ivs;
+        if (again) {
+          tmem_ld_wait();
+          const int left = lim - key0;  // keys of the tile that the row sees
+          if (edge) {
+#pragma unroll
+            for (int e = 0; e < 32; e++) {
+              if (e >= left) r0[e] = 0xff800000u;
+              if (32 + e >= left) r1[e] = 0xff800000u;
+            }
+          }
+          mx = left > 0 ? fmaxf(top32(r0), top32(r1)) * c : -INFINITY;
+          const bool need = mx > m + kRescaleThreshold;
+          const float mn = i == 0 || need ? mx : m;
+          if (i > 0 && __any_sync(0xffffffffu, need)) {  // O through registers (warp-collective)
+            // O must hold every product up to tile i - 1; the barrier's next arrival, ST tiles on, needs P of this row
+            ok = wait(&kv_empty[(j + i - 1) % ST], ((j + i - 1) / ST) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            const float alpha = need ? ex2_approx(m - mn) : 1.f;
+            l *= alpha;
+#pragma unroll
+            for (int x = 0; x < D / 16; x++) {
+              uint32_t r[16];
+              tmem_ld16(t_o + x * 16, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
+              tmem_st16(t_o + x * 16, r);
+            }
+          }
+          m = mn;
+          // a row that sees nothing of the tile takes no part in its scales, which may be NaN; scores out of sight are -inf,
+          // and -inf * 0 of a zero scale must not be NaN
+          const float mu = m == -INFINITY ? 0.f : m;
+          if (edge) {
+            if (left <= 0) c = 1.f, lvs = 0.f, ivs = 1.f;
+            if (c == 0.f) {
+#pragma unroll
+              for (int e = 0; e < 32; e++) {
+                r0[e] = e < left ? 0u : r0[e];
+                r1[e] = 32 + e < left ? 0u : r1[e];
+              }
+              c = 1.f;
+            }
+          }
+          sum = exps(r0, 0, mu) + exps(r1, 16, mu);
+        }
+        l += sum * ivs;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * t + f]);
       }
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&o_full[t], so & 1, abort_flag, ST_KV8_WAIT));
+      if (!ok) break;
+      const Seg done = g;
+      if (u < u_end) load_q(g = segment(a, pre, u, u_end));  // the next item's products start before this one's O is stored
+      ok = wait(&o_full[t], so & 1);
       if (!ok) break;
       tc_fence_after();
-      const bool whole = g.ta == 0 && g.tb == g.tiles;
+      const bool whole = done.ta == 0 && done.tb == done.tiles;
       const float inv = 1.f / l;
-      const int at = row - g.r0;
+      const int at = row - done.r0;
       const size_t slot = (2 * (size_t)blockIdx.x + (first ? 0 : 1)) * ROWS + at;
-      uint16_t* op = a.out + g.b * a.so_b + row / a.G * a.so_t + (size_t)(g.h * a.G + row % a.G) * a.so_h;
+      uint16_t* op = a.out + done.b * a.so_b + row / a.G * a.so_t + (size_t)(done.h * a.G + row % a.G) * a.so_h;
 #pragma unroll
       for (int x16 = 0; x16 < D / 16; x16++) {
         uint32_t r[16];
@@ -506,13 +555,13 @@ __global__ void __launch_bounds__(128) attn_kv8_tc_join_kernel(Args a) {
 //   warps 8-11       K's codes -> the A operand once; q rows and lse of each row tile (2 stages);
 //   warp 12          tcgen05.mma into two S buffers.
 // Bound: MUFU, one ex2 a score.
-constexpr int WK = 128, WR = 128;
+constexpr int WK = 128, WR = 128, WTHREADS = 13 * 32;
 template <int D>
 struct WSmem {
   static constexpr int K = 0, Q = WK * D * 2, QT = WR * D * 2, BYTES = Q + 2 * QT;
 };
 template <int D>
-__global__ void __launch_bounds__(THREADS, 1) kv8_weights_tc_kernel(Args a) {
+__global__ void __launch_bounds__(WTHREADS, 1) kv8_weights_tc_kernel(Args a) {
   using L = WSmem<D>;
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ __align__(16) float sh_lse[2][WR], half_sum[WK];
@@ -665,7 +714,7 @@ static int launch(cudaStream_t st, const Args& a) {
   if (rc) return rc;
   launch_k(attn_kv8_tc_kernel<D>, a.ctas, THREADS, Smem<D>::BYTES, st, a);
   launch_k(attn_kv8_tc_join_kernel<D>, dim3(a.ctas, ROWS / 16), 128, 0, st, a);
-  if (a.w) launch_k(kv8_weights_tc_kernel<D>, (unsigned)(a.B * a.H * ((a.C + WK - 1) / WK)), THREADS, WSmem<D>::BYTES, st, a);
+  if (a.w) launch_k(kv8_weights_tc_kernel<D>, (unsigned)(a.B * a.H * ((a.C + WK - 1) / WK)), WTHREADS, WSmem<D>::BYTES, st, a);
   return check_launch("vt_attn_kv8");
 }
 

@@ -345,6 +345,13 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
                : "r"(taddr));
 }
 
+// One lane of a converged warp: 1 on it, 0 on the others.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+  return r;
+}
+
 // Non-tensor bulk copy global -> shared (16-byte aligned addresses, size a multiple of 16), completion
 // counted on the mbarrier; it fills only the issuing CTA.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
