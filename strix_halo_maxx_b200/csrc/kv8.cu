@@ -193,6 +193,8 @@ struct EvictArgs {
   int *dlens, *index;
 };
 
+constexpr int MAX_EVICT = 8 * 1024 * 32;  // slots of a head that a cluster of 8 CTAs holds in registers
+
 // Order of weights as unsigned numbers: -inf .. +inf, NaN above all, -0 equal to 0.
 __device__ __forceinline__ uint32_t order_of(float f) {
   if (isnan(f)) return 0xffffffffu;
@@ -200,160 +202,245 @@ __device__ __forceinline__ uint32_t order_of(float f) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// CTA = one head: the (keep - recent) largest of the slots before the recent ones, by radix selection on 8 bits a
-// pass, then their slots in order (ties: the lowest slots), the recent ones behind them.
-constexpr int SEL = 1024;
-__global__ void __launch_bounds__(SEL) kv8_select_kernel(EvictArgs a) {
-  __shared__ unsigned int hist[256], warp_cnt[32];
-  __shared__ unsigned int sh_prefix, sh_left;
+// Which slots of a head stay: the (keep - recent) largest weights before the recent ones, and the recent ones.  A head is one
+// CTA's, or a cluster's of CS CTAs (each a contiguous range of slots), and every weight is read once: a thread keeps the
+// order keys of up to KPT slots in registers (warp w of a CTA has 32 kpt consecutive slots, key i of lane l is slot 32 i + l).
+// The threshold is found two bits at a time from the top: three counts of keys above a candidate, added up over warps,
+// CTAs and the cluster; a candidate with exactly the wanted count ends the search (after about 11 of 16 rounds for
+// weights that differ).  Counting by comparison needs no atomics, whose same-address conflicts made histograms of
+// these skewed weights (most share an exponent) eight times slower: 397 us for 8 heads of 131k slots, 98 us for 256 heads
+// of 16k.  Then positions by ballots and prefix sums: kept slots are written in order, ties to the lowest slots.
+// Latency bound: rounds of compare, reduce and barrier.
+template <int THREADS, int KPT, int CS>
+__global__ void __launch_bounds__(THREADS) kv8_select_kernel(EvictArgs a) {
+  constexpr int W = THREADS / 32;
+  __shared__ unsigned int sh_warp[2][W];
+  __shared__ unsigned int sh_cta[2][CS][3];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int h = blockIdx.x, b = blockIdx.y;
+  const int rank = CS > 1 ? (int)cluster_ctarank() : 0;
+  const long long bh = blockIdx.x / CS;
+  const int h = (int)(bh % a.H), b = (int)(bh / a.H);
   griddep_wait();
   griddep_launch();
   int len = a.lens[b];
   if ((len < 0 || len > a.C) && tid == 0) atomicOr(&g_status, (unsigned int)ST_KV8_RANGE);
   len = min(max(len, 0), a.C);
-  const size_t bh = (size_t)b * a.H + h;
   const float* w = a.w + bh * a.C;
   float* dw = a.dw + bh * a.Cd;
   int* idx = a.index + bh * a.keep;
-  if (h == 0 && tid == 0) a.dlens[b] = min(len, a.keep);
-  if (len <= a.keep) {
-    for (int j = tid; j < len; j += SEL) {
+  if (h == 0 && rank == 0 && tid == 0) a.dlens[b] = min(len, a.keep);
+  if (len <= a.keep) {  // the whole cluster
+    for (int j = rank * THREADS + tid; j < len; j += CS * THREADS) {
       idx[j] = j;
       dw[j] = w[j];
     }
     return;
   }
-  const int N = len - a.recent, want = a.keep - a.recent;
-  unsigned int prefix = 0, left = want;  // the want-th largest key's leading bits, and its rank among those that share them
-  for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+  const int N = len - a.recent, kpt = (len + CS * THREADS - 1) / (CS * THREADS);
+  const unsigned int want = a.keep - a.recent;
+  const int j0 = (rank * W + warp) * 32 * kpt + lane;  // slot of key i: j0 + 32 i
+  uint32_t key[KPT];  // 0: not a candidate (the key of -inf is 0x007fffff)
+#pragma unroll
+  for (int i = 0; i < KPT; i++) key[i] = i < kpt && j0 + 32 * i < N ? order_of(w[j0 + 32 * i]) : 0u;
+  // sums over the head of three counts (at most 1024 in a warp: two to a register)
+  int round = 0;
+  auto total3 = [&](unsigned int c1, unsigned int c2, unsigned int c3, unsigned int (&sum)[3]) {
+    const int f = round++ & 1;
+    const unsigned int p12 = __reduce_add_sync(0xffffffffu, c1 | (c2 << 16));
+    const unsigned int p3 = __reduce_add_sync(0xffffffffu, c3);
+    __shared__ unsigned int sh3[2][W];
+    if (lane == 0) sh_warp[f][warp] = p12, sh3[f][warp] = p3;
     __syncthreads();
-    for (int j = tid; j < N; j += SEL) {
-      const uint32_t u = order_of(w[j]);
-      if (shift == 24 || (u >> (shift + 8)) == prefix) atomicAdd(&hist[(u >> shift) & 255u], 1u);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      unsigned int acc = 0;
-      int d = 255;
-      for (; d > 0 && acc + hist[d] < left; d--) acc += hist[d];
-      sh_prefix = (prefix << 8) | (unsigned int)d;
-      sh_left = left - acc;
-    }
-    __syncthreads();
-    prefix = sh_prefix;
-    left = sh_left;
-  }
-  unsigned int base = 0, ties = 0;  // slots kept and ties seen so far
-  for (int j0 = 0; j0 < N && want > 0; j0 += SEL) {
-    const int j = j0 + tid;
-    const uint32_t u = j < N ? order_of(w[j]) : 0u;
-    const bool gt = j < N && u > prefix, eq = j < N && u == prefix;
-    const unsigned int bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-    const unsigned int below = (1u << lane) - 1u;
-    if (lane == 0) warp_cnt[warp] = __popc(bg) | (__popc(be) << 16);
-    __syncthreads();
-    unsigned int cg = 0, ce = 0, tg = 0, te = 0;
-    for (int i = 0; i < 32; i++) {
-      const unsigned int c = warp_cnt[i];
-      if (i < warp) {
-        cg += c & 0xffffu;
-        ce += c >> 16;
+    const unsigned int x = lane < W ? sh_warp[f][lane] : 0u, y = lane < W ? sh3[f][lane] : 0u;
+    sum[0] = __reduce_add_sync(0xffffffffu, x & 0xffffu);
+    sum[1] = __reduce_add_sync(0xffffffffu, x >> 16);
+    sum[2] = __reduce_add_sync(0xffffffffu, y);
+    if constexpr (CS > 1) {
+      if (tid < CS * 3) {  // this CTA's sums to every CTA of the cluster
+        const uint32_t to = mapa_shared(smem_u32(&sh_cta[f][rank][tid % 3]), tid / 3);
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(sum[tid % 3]) : "memory");
       }
-      tg += c & 0xffffu;
-      te += c >> 16;
+      cluster_sync();
+#pragma unroll
+      for (int k = 0; k < 3; k++) sum[k] = __reduce_add_sync(0xffffffffu, lane < CS ? sh_cta[f][lane][k] : 0u);
     }
-    cg += __popc(bg & below);
-    ce += __popc(be & below);
-    const unsigned int eq_before = min(ties + ce, left);  // ties kept before this slot
-    if (gt || (eq && ties + ce < left)) {
-      const unsigned int at = base + cg + (eq_before - min(ties, left));
-      idx[at] = j;
-      dw[at] = w[j];
+  };
+  // T: the largest key with at least `want` keys >= T; above: how many are > T
+  unsigned int T = 0, above = 0;
+  if (want == 0) T = 0xffffffffu;
+  for (int shift = 30; shift >= 0 && want > 0; shift -= 2) {
+    unsigned int c1 = 0, c2 = 0, c3 = 0, sum[3];
+    const uint32_t t1 = T + (1u << shift), t2 = T + (2u << shift), t3 = T + (3u << shift);
+#pragma unroll
+    for (int i = 0; i < KPT; i++)
+      if (i < kpt) c1 += key[i] >= t1, c2 += key[i] >= t2, c3 += key[i] >= t3;
+    total3(c1, c2, c3, sum);
+    const int d = sum[2] >= want ? 3 : sum[1] >= want ? 2 : sum[0] >= want ? 1 : 0;
+    if (d < 3) above = sum[d];
+    T += (unsigned int)d << shift;
+    if (d > 0 && sum[d - 1] == want) {  // exactly the keys >= T
+      T--, above = want;
+      break;
     }
-    base += tg + (min(ties + te, left) - min(ties, left));
-    ties += te;
-    __syncthreads();
   }
-  for (int r = tid; r < a.recent; r += SEL) {
-    idx[want + r] = len - a.recent + r;
-    dw[want + r] = w[len - a.recent + r];
+  const unsigned int ties = want - above;  // of the keys equal to T
+  // positions: kept (key > T, or recent) and equal keys before each slot, over CTAs, warps, rows of 32 and lanes
+  unsigned int gt = 0, eq = 0;
+#pragma unroll
+  for (int i = 0; i < KPT; i++)
+    if (i < kpt) {
+      const int j = j0 + 32 * i;
+      gt += __popc(__ballot_sync(0xffffffffu, key[i] > T || (j >= N && j < len)));
+      eq += __popc(__ballot_sync(0xffffffffu, key[i] == T && key[i] != 0u));
+    }
+  __shared__ unsigned int sh_gt[W], sh_eq[W];
+  __shared__ unsigned int sh_before[CS][2];
+  if (lane == 0) sh_gt[warp] = gt, sh_eq[warp] = eq;
+  __syncthreads();
+  const unsigned int xg = lane < W ? sh_gt[lane] : 0u, xe = lane < W ? sh_eq[lane] : 0u;
+  unsigned int bg = __reduce_add_sync(0xffffffffu, lane < warp ? xg : 0u), be = __reduce_add_sync(0xffffffffu, lane < warp ? xe : 0u);
+  if constexpr (CS > 1) {
+    const unsigned int tg = __reduce_add_sync(0xffffffffu, xg), te = __reduce_add_sync(0xffffffffu, xe);
+    if (tid < CS * 2) {
+      const uint32_t to = mapa_shared(smem_u32(&sh_before[rank][tid & 1]), tid / 2);
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(tid & 1 ? te : tg) : "memory");
+    }
+    cluster_sync();  // the last access to another CTA's shared memory is before it
+    for (int r = 0; r < rank; r++) bg += sh_before[r][0], be += sh_before[r][1];
+  }
+  const unsigned int below = (1u << lane) - 1u;
+#pragma unroll
+  for (int i = 0; i < KPT; i++)
+    if (i < kpt) {
+      const int j = j0 + 32 * i;
+      const bool sure = key[i] > T || (j >= N && j < len), even = key[i] == T && key[i] != 0u;
+      const unsigned int mg = __ballot_sync(0xffffffffu, sure), me = __ballot_sync(0xffffffffu, even);
+      const unsigned int e = be + __popc(me & below);
+      if (sure || (even && e < ties)) {
+        const unsigned int at = bg + __popc(mg & below) + min(e, ties);
+        idx[at] = j;
+        dw[at] = w[j];
+      }
+      bg += __popc(mg), be += __popc(me);
+    }
+}
+
+// Largest |code| of 16, as a number.
+__device__ __forceinline__ int top_code(uint4 c) {
+
+  uint32_t m = __vmaxu4(__vmaxu4(__vabsdiffs4(c.x, 0), __vabsdiffs4(c.y, 0)), __vmaxu4(__vabsdiffs4(c.z, 0), __vabsdiffs4(c.w, 0)));
+  m = __vmaxu2(m & 0x00ff00ffu, (m >> 8) & 0x00ff00ffu);
+  return (int)max(m & 0xffffu, m >> 16);
+}
+// Four codes times `s` (rounded), each divided by `d` (1 / d rounded: rd) and rounded half to even: codes again.
+__device__ __forceinline__ uint32_t recode4(uint32_t c, float s, float d, float rd, bool fast) {
+  uint32_t o = 0;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    // byte ^ 0x80 into the mantissa of 2^23: 2^23 + 128 + code
+    const float x = __fmul_rn(__uint_as_float(__byte_perm(c ^ 0x80808080u, 0x4b000000u, 0x7440 + e)) - 8388736.f, s);
+    if (fast) {
+      // + 1.5 * 2^23 rounds to an integer, which is then in the low bits
+      const uint32_t r = __float_as_uint(__fadd_rn(div_rn_by(x, d, rd), 12582912.f));
+      o |= (r & 0xffu) << (8 * e);
+    } else {
+      o |= code_of(x, d) << (8 * e);
+    }
+  }
+  return o;
+}
+
+// CTA = one block of 64 kept tokens of one (sequence, head), K and V: values code * scale (rounded to fp32), the block's
+// scale max |value| / 127 and codes rint(value / scale).  All of a thread's rows are on their way at once.  The
+// quotient is the IEEE one in five operations (div_rn_by) wherever that is exact; a division each made this
+// kernel compute bound (246 us for 285 MB).  Sequences that lost nothing are copied.
+template <int D>
+__global__ void __launch_bounds__(128) kv8_gather_kernel(EvictArgs a) {
+  constexpr int PC = D / 16, PER = BLK * PC / 128;  // 16-byte pieces of a row, pieces a thread takes of K and of V
+  __shared__ float red[2][4];
+  const int tid = threadIdx.x;
+  griddep_wait();
+  griddep_launch();
+  const int nb = a.keep / BLK, blk = (int)(blockIdx.x % nb);
+  const size_t bh = blockIdx.x / nb;
+  const int len = min(max(a.lens[bh / a.H], 0), a.C);
+  const int rows = min(len, a.keep) - blk * BLK;
+  if (rows <= 0) return;
+  const int* idx = a.index + bh * a.keep + blk * BLK;
+  const bool copy = len <= a.keep;
+  uint4 c[2][PER];
+  float sc[2][PER];
+#pragma unroll
+  for (int k = 0; k < PER; k++) {
+    const int row = (tid + 128 * k) / PC, p = (tid + 128 * k) % PC;
+#pragma unroll
+    for (int v = 0; v < 2; v++) c[v][k] = make_uint4(0, 0, 0, 0), sc[v][k] = 0.f;
+    if (row >= rows) continue;
+    const int j = copy ? blk * BLK + row : idx[row];
+    const size_t at = (bh * a.C + j) * D + 16 * p, sat = bh * (a.C / BLK) + j / BLK;
+    c[0][k] = *reinterpret_cast<const uint4*>(a.kc + at);
+    c[1][k] = *reinterpret_cast<const uint4*>(a.vc + at);
+    sc[0][k] = a.ks[sat], sc[1][k] = a.vs[sat];
+  }
+  float s[2];
+  if (copy) {
+    s[0] = sc[0][0], s[1] = sc[1][0];  // thread 0's first row is in this block
+  } else {
+#pragma unroll
+    for (int v = 0; v < 2; v++) {
+      float top = 0.f;  // rounding is monotonic: the largest rounded product is that of the largest code
+#pragma unroll
+      for (int k = 0; k < PER; k++) {
+        const float x = __fmul_rn((float)top_code(c[v][k]), fabsf(sc[v][k]));
+        top = isnan(sc[v][k]) ? INFINITY : fmaxf(top, x);
+      }
+      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+      if ((tid & 31) == 0) red[v][tid >> 5] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < 2; v++) {
+      const float top = fmaxf(fmaxf(red[v][0], red[v][1]), fmaxf(red[v][2], red[v][3]));
+      s[v] = isinf(top) ? __uint_as_float(0x7fc00000u) : __fdiv_rn(top, 127.f);
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < 2; v++) {
+    int8_t* dst = (v ? a.dvc : a.dkc) + (bh * a.Cd + (size_t)blk * BLK) * D;
+    const bool fast = s[v] > 0x1p-80f && s[v] < 0x1p100f;
+    const float rd = fast ? __frcp_rn(s[v]) : 0.f;
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const int row = (tid + 128 * k) / PC, p = (tid + 128 * k) % PC;
+      if (row >= rows) continue;
+      uint4 o = c[v][k];
+      if (!copy) {
+        if (s[v] > 0.f)
+          o = make_uint4(recode4(o.x, sc[v][k], s[v], rd, fast), recode4(o.y, sc[v][k], s[v], rd, fast),
+                         recode4(o.z, sc[v][k], s[v], rd, fast), recode4(o.w, sc[v][k], s[v], rd, fast));
+        else
+          o = make_uint4(0, 0, 0, 0);
+      }
+      *reinterpret_cast<uint4*>(dst + (size_t)row * D + 16 * p) = o;
+    }
+    if (tid == 0) (v ? a.dvs : a.dks)[bh * (a.Cd / BLK) + blk] = s[v];
   }
 }
 
-// CTA = one block of 64 kept tokens of one (sequence, head, K or V): their values code * scale (rounded to fp32), the
-// scale max |value| / 127 and the codes rint(value / scale).  Sequences that lost nothing are copied.
-template <int D>
-__global__ void __launch_bounds__(128) kv8_gather_kernel(EvictArgs a) {
-  constexpr int CH = D / 8, PER = BLK * CH / 128;
-  __shared__ float red[4];
-  const int tid = threadIdx.x, w = blockIdx.x & 1;
-  griddep_wait();
-  griddep_launch();
-  long long u = blockIdx.x >> 1;
-  const int nb = a.keep / BLK, blk = (int)(u % nb);
-  u /= nb;
-  const int h = (int)(u % a.H), b = (int)(u / a.H);
-  const int len = min(max(a.lens[b], 0), a.C);
-  const int rows = min(len, a.keep) - blk * BLK;
-  if (rows <= 0) return;
-  const size_t bh = (size_t)b * a.H + h;
-  const int8_t* src = (w ? a.vc : a.kc) + bh * a.C * D;
-  const float* ss = (w ? a.vs : a.ks) + bh * (a.C / BLK);
-  int8_t* dst = (w ? a.dvc : a.dkc) + (bh * a.Cd + (size_t)blk * BLK) * D;
-  float* ds = (w ? a.dvs : a.dks) + bh * (a.Cd / BLK) + blk;
-  const int* idx = a.index + bh * a.keep + blk * BLK;
-  const bool copy = len <= a.keep;
-  uint2 c[PER];
-  float sc[PER], top = 0.f;
-  bool odd = false;
-#pragma unroll
-  for (int k = 0; k < PER; k++) {
-    const int t = tid + 128 * k, row = t / CH;
-    c[k] = make_uint2(0, 0);
-    sc[k] = 0.f;
-    if (row >= rows) continue;
-    const int j = copy ? blk * BLK + row : idx[row];
-    c[k] = *reinterpret_cast<const uint2*>(src + (size_t)j * D + 8 * (t % CH));
-    sc[k] = ss[j / BLK];
-    odd |= isnan(sc[k]);
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const int x = (int8_t)((e < 4 ? c[k].x : c[k].y) >> (8 * (e & 3)));
-      top = fmaxf(top, fabsf(__fmul_rn((float)x, sc[k])));
-    }
-  }
-  if (copy) {
-#pragma unroll
-    for (int k = 0; k < PER; k++) {
-      const int t = tid + 128 * k, row = t / CH;
-      if (row < rows) *reinterpret_cast<uint2*>(dst + (size_t)row * D + 8 * (t % CH)) = c[k];
-    }
-    if (tid == 0) *ds = ss[blk];
-    return;
-  }
-  top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(odd ? INFINITY : top)));
-  if ((tid & 31) == 0) red[tid >> 5] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float s = isinf(top) ? __uint_as_float(0x7fc00000u) : __fdiv_rn(top, 127.f);
-#pragma unroll
-  for (int k = 0; k < PER; k++) {
-    const int t = tid + 128 * k, row = t / CH;
-    if (row >= rows) continue;
-    uint2 o = make_uint2(0, 0);
-    if (s > 0.f) {
-      float f[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        f[e] = __fmul_rn((float)(int8_t)((e < 4 ? c[k].x : c[k].y) >> (8 * (e & 3))), sc[k]);
-      o = codes8(f, s);
-    }
-    *reinterpret_cast<uint2*>(dst + (size_t)row * D + 8 * (t % CH)) = o;
-  }
-  if (tid == 0) *ds = s;
+template <int THREADS, int KPT, int CS>
+static void launch_select(cudaStream_t st, const EvictArgs& a) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.B * a.H * CS));
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CS, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kv8_select_kernel<THREADS, KPT, CS>, a);
 }
 
 static bool overlap(const void* p, long long n, const void* q, long long m) {
@@ -414,6 +501,7 @@ int vt_kv8_evict(cudaStream_t st, const int8_t* kc, const int8_t* vc, const floa
   if (keep <= 0 || keep % kv8::BLK || keep > dst_C || recent < 0 || recent > keep)
     return set_error(E_SHAPE, "vt_kv8_evict: keep=%d (a multiple of %d, at most the destination's %d slots), recent=%d", keep,
                      kv8::BLK, dst_C, recent);
+  if (C > kv8::MAX_EVICT) return set_error(E_SHAPE, "vt_kv8_evict: C=%d (at most %d)", C, kv8::MAX_EVICT);
   if (B == 0) return OK;
   if (!weights || !lens || !dst_weights || !dst_lens || !index) return set_error(E_SHAPE, "vt_kv8_evict: null pointer");
   const long long n = (long long)B * H, nc = n * C * D, nd = n * dst_C * D;
@@ -422,10 +510,18 @@ int vt_kv8_evict(cudaStream_t st, const int8_t* kc, const int8_t* vc, const floa
   for (const auto& s : src)
     for (const auto& d : dst)
       if (kv8::overlap(s.p, s.n, d.p, d.n)) return set_error(E_SHAPE, "vt_kv8_evict: the destination overlaps the source");
-  const long long units = 2LL * B * H * (keep / kv8::BLK);
-  if (B > 65535 || units > 0x7fffffffLL) return set_error(E_SHAPE, "vt_kv8_evict: grid too large (B=%d H=%d keep=%d)", B, H, keep);
+  const long long units = n * (keep / kv8::BLK);
+  if (units > 0x7fffffffLL || n > 0x0fffffffLL)
+    return set_error(E_SHAPE, "vt_kv8_evict: grid too large (B=%d H=%d keep=%d)", B, H, keep);
   kv8::EvictArgs a{kc, vc, ks, vs, weights, lens, B, H, C, keep, recent, dst_C, dst_kc, dst_vc, dst_ks, dst_vs, dst_weights, dst_lens, index};
-  launch_k(kv8::kv8_select_kernel, dim3(H, B), kv8::SEL, 0, st, a);
+  // 256 threads for up to 2048 slots, else 1024; as many CTAs a head as leave each thread at most 16 slots when there
+  // are fewer heads than SMs, 32 otherwise (one CTA then has a head of up to 32k slots; 256 heads fill the GPU)
+  const int most = n < sm_count() ? 16 : 32;
+  if (C <= 2048) kv8::launch_select<256, 8, 1>(st, a);
+  else if (C <= most * 1024) kv8::launch_select<1024, 32, 1>(st, a);
+  else if (C <= most * 2048) kv8::launch_select<1024, 32, 2>(st, a);
+  else if (C <= most * 4096) kv8::launch_select<1024, 32, 4>(st, a);
+  else kv8::launch_select<1024, 32, 8>(st, a);
   if (D == 64) launch_k(kv8::kv8_gather_kernel<64>, (unsigned)units, 128, 0, st, a);
   else launch_k(kv8::kv8_gather_kernel<128>, (unsigned)units, 128, 0, st, a);
   return check_launch("vt_kv8_evict");

@@ -463,32 +463,36 @@ def _kv8_fail(what, why):
 
 
 def _kv8_dims(what, cache, dev):
-    """B, H, C, D of a cache whose four tensors have the right types and shapes, contiguous on device dev."""
+    """B, H, C, D of a cache whose four tensors have the right types and shapes, contiguous on CUDA device number dev."""
     k, v, ks, vs = cache
-    B, H, C, D = k.shape
-    if k.dtype != torch.int8 or v.dtype != torch.int8 or ks.dtype != torch.float32 or vs.dtype != torch.float32:
+    shape = k.shape
+    B, H, C, D = shape
+    blocks = (B, H, C // KV8_BLOCK)
+    if k.dtype is not torch.int8 or v.dtype is not torch.int8 or ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
         _kv8_fail(what, "codes are int8, scales float32")
-    if v.shape != k.shape or ks.shape != (B, H, C // KV8_BLOCK) or vs.shape != ks.shape or C % KV8_BLOCK:
+    if v.shape != shape or ks.shape != blocks or vs.shape != blocks or C % KV8_BLOCK:
         _kv8_fail(what, f"cache shapes {tuple(k.shape)} {tuple(v.shape)} {tuple(ks.shape)} {tuple(vs.shape)}")
     for t in cache:
-        if t.device != dev or not t.is_contiguous():
-            _kv8_fail(what, f"cache tensors must be contiguous on {dev}")
+        if t.get_device() != dev or not t.is_contiguous():
+            _kv8_fail(what, "cache tensors must be contiguous on one device")
     return B, H, C, D
 
 
 def _kv8_vec(what, name, t, shape, dtype, dev):
-    if t.shape != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous():
-        _kv8_fail(what, f"{name} must be a contiguous {dtype} {tuple(shape)} on {dev}")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        _kv8_fail(what, f"{name} must be a contiguous {dtype} {tuple(shape)} on device {dev}")
     return t.data_ptr()
 
 
 def _kv8_call(fn, what, dev, *args):
     """The call on torch's current stream of the tensors' device."""
-    if dev.index == torch.cuda.current_device():
-        rc = fn(_stream(), *args)
+    if dev < 0:
+        _kv8_fail(what, "the tensors must be on a CUDA device")
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(torch._C._cuda_getCurrentRawStream(dev), *args)
     else:
         with torch.cuda.device(dev):
-            rc = fn(_stream(), *args)
+            rc = fn(torch._C._cuda_getCurrentRawStream(dev), *args)
     check(rc, what)
 
 
@@ -496,20 +500,21 @@ def rope_kv8(qkv, cache, lens, cos_t, sin_t, q, pos=None, counts=None):
     """vt_rope_kv8: qkv [B, n, (Hq + 2 H) D] bf16 (q | k | v, head-major) -> q [B, n, Hq, D] rotated, k and v quantised
     into slots lens[b] .. of the cache.  lens, pos (default lens: the rotary positions) and counts (default n: each
     sequence's number of new tokens) int32 [B] on the device; cos_t / sin_t fp32 [positions, 16]."""
-    what, dev = "rope_kv8", q.device
+    what, dev = "rope_kv8", q.get_device()
     B, H, C, D = _kv8_dims(what, cache, dev)
-    n, Hq = q.shape[1], q.shape[2]
-    if q.shape != (B, n, Hq, D) or qkv.shape != (B, n, (Hq + 2 * H) * D) or q.dtype != BF16 or qkv.dtype != BF16 or \
-            qkv.device != dev or (q.numel() and (q.stride(3) != 1 or qkv.stride(2) != 1)):
+    Bq, n, Hq, Dq = q.shape
+    sq, sx, i32 = q.stride(), qkv.stride(), torch.int32
+    if (Bq, Dq) != (B, D) or qkv.shape != (B, n, (Hq + 2 * H) * D) or q.dtype is not BF16 or qkv.dtype is not BF16 or \
+            qkv.get_device() != dev or sq[3] != 1 or sx[2] != 1:
         _kv8_fail(what, f"qkv {tuple(qkv.shape)}, q {tuple(q.shape)} for a cache of B={B} H={H} D={D} (bf16, contiguous rows)")
     tab = cos_t.shape[0]
-    _kv8_call(lib().vt_rope_kv8, "vt_rope_kv8", dev, qkv.data_ptr(), qkv.stride(0), qkv.stride(1), B, n, Hq, H, D,
+    _kv8_call(lib().vt_rope_kv8, "vt_rope_kv8", dev, qkv.data_ptr(), sx[0], sx[1], B, n, Hq, H, D,
               _kv8_vec(what, "cos_t", cos_t, (tab, 16), torch.float32, dev),
               _kv8_vec(what, "sin_t", sin_t, (tab, 16), torch.float32, dev), tab,
-              _kv8_vec(what, "lens", lens, (B,), torch.int32, dev),
-              None if pos is None else _kv8_vec(what, "pos", pos, (B,), torch.int32, dev),
-              None if counts is None else _kv8_vec(what, "counts", counts, (B,), torch.int32, dev),
-              q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), cache.k.data_ptr(), cache.v.data_ptr(),
+              _kv8_vec(what, "lens", lens, (B,), i32, dev),
+              None if pos is None else _kv8_vec(what, "pos", pos, (B,), i32, dev),
+              None if counts is None else _kv8_vec(what, "counts", counts, (B,), i32, dev),
+              q.data_ptr(), sq[0], sq[1], sq[2], cache.k.data_ptr(), cache.v.data_ptr(),
               cache.ks.data_ptr(), cache.vs.data_ptr(), C)
     return q
 
@@ -524,26 +529,27 @@ def attn_kv8(q, cache, lens, out=None, counts=None, causal=True, scale=None, wei
     counts) -> out [B, n, Hq D] bf16; row i sees slots 0 .. lens[b] + i (causal) or all lens[b] + counts[b].  weights fp32
     [B, H, C]: each slot's attention weight, summed over the rows and the group's query heads, plus weights_in for slots
     before lens[b] (weights_in=weights accumulates in place).  ws: attn_kv8_workspace, else one is allocated."""
-    what, dev = "attn_kv8", q.device
+    what, dev = "attn_kv8", q.get_device()
     B, H, C, D = _kv8_dims(what, cache, dev)
-    n, Hq = q.shape[1], q.shape[2]
+    Bq, n, Hq, Dq = q.shape
     if out is None:
-        out = torch.empty(B, n, Hq * D, dtype=BF16, device=dev)
-    if q.shape != (B, n, Hq, D) or out.shape != (B, n, Hq * D) or q.dtype != BF16 or out.dtype != BF16 or out.device != dev or \
-            (q.numel() and (q.stride(3) != 1 or out.stride(2) != 1)):
+        out = torch.empty(B, n, Hq * D, dtype=BF16, device=q.device)
+    sq, so = q.stride(), out.stride()
+    if (Bq, Dq) != (B, D) or out.shape != (B, n, Hq * D) or q.dtype is not BF16 or out.dtype is not BF16 or \
+            out.get_device() != dev or sq[3] != 1 or so[2] != 1:
         _kv8_fail(what, f"q {tuple(q.shape)}, out {tuple(out.shape)} for a cache of B={B} H={H} D={D} (bf16, contiguous rows)")
     if ws is None:
-        ws = attn_kv8_workspace(B, n, Hq, H, D, C, dev, weights is not None)
-    elif ws.device != dev:
-        _kv8_fail(what, f"the workspace must be on {dev}")
-    _kv8_call(lib().vt_attn_kv8, "vt_attn_kv8", dev, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
+        ws = attn_kv8_workspace(B, n, Hq, H, D, C, q.device, weights is not None)
+    elif ws.get_device() != dev or not ws.is_contiguous():
+        _kv8_fail(what, "the workspace must be contiguous on the tensors' device")
+    _kv8_call(lib().vt_attn_kv8, "vt_attn_kv8", dev, q.data_ptr(), sq[0], sq[1], sq[2],
               cache.k.data_ptr(), cache.v.data_ptr(), cache.ks.data_ptr(), cache.vs.data_ptr(), C,
               _kv8_vec(what, "lens", lens, (B,), torch.int32, dev),
               None if counts is None else _kv8_vec(what, "counts", counts, (B,), torch.int32, dev), B, n, Hq, H, D,
-              int(bool(causal)), float(D ** -0.5 if scale is None else scale), out.data_ptr(), out.stride(0), out.stride(1), D,
+              int(bool(causal)), D ** -0.5 if scale is None else float(scale), out.data_ptr(), so[0], so[1], D,
               None if weights is None else _kv8_vec(what, "weights", weights, (B, H, C), torch.float32, dev),
               None if weights_in is None else _kv8_vec(what, "weights_in", weights_in, (B, H, C), torch.float32, dev),
-              ws.data_ptr(), ws.numel() * ws.element_size())
+              ws.data_ptr(), ws.nbytes)
     return out
 
 
@@ -552,13 +558,13 @@ def kv8_evict(cache, weights, lens, keep, recent, dst, dst_weights, dst_lens, in
     tokens and the keep - recent others with the largest weights [B, H, C], in order, in the cache dst; shorter
     sequences are copied.  dst_weights fp32 [B, H, dst C] and dst_lens int32 [B] receive the kept weights and the new lengths,
     index int32 [B, H, keep] (allocated when None, and returned) the slots they had.  dst must be another cache."""
-    what, dev = "kv8_evict", cache.k.device
+    what, dev = "kv8_evict", cache.k.get_device()
     B, H, C, D = _kv8_dims(what, cache, dev)
     Bd, Hd, Cd, Dd = _kv8_dims(what, dst, dev)
     if (Bd, Hd, Dd) != (B, H, D):
         _kv8_fail(what, f"dst {tuple(dst.k.shape)} for a cache of {tuple(cache.k.shape)}")
     if index is None:
-        index = torch.empty(B, H, keep, dtype=torch.int32, device=dev)
+        index = torch.empty(B, H, keep, dtype=torch.int32, device=cache.k.device)
     _kv8_call(lib().vt_kv8_evict, "vt_kv8_evict", dev, cache.k.data_ptr(), cache.v.data_ptr(), cache.ks.data_ptr(),
               cache.vs.data_ptr(), C, _kv8_vec(what, "weights", weights, (B, H, C), torch.float32, dev),
               _kv8_vec(what, "lens", lens, (B,), torch.int32, dev), B, H, D, int(keep), int(recent), dst.k.data_ptr(),
