@@ -61,16 +61,25 @@ __device__ __forceinline__ uint4 head_chunk(const uint16_t* x, int c, bool rotat
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// rint(x / s) clamped to +-127 (s > 0), as a byte.
-__device__ __forceinline__ uint32_t code_of(float x, float s) {
-  const float r = fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.f), 127.f);
-  return (uint32_t)(int)r & 0xffu;
+// rint(x / s) as a byte, s > 0 a block's scale.  The IEEE quotient in five operations (div_rn_by) where that is exact, which
+// is for every scale that is not extreme; adding 1.5 * 2^23 rounds it half to even and leaves the integer in the low bits.
+// The division itself, with its clamp for subnormal scales, stays out of line: inlined once for each value of a thread it
+// filled the instruction cache (eviction's gather 188 us for 268 MB, half of its stalls for want of instructions).
+__noinline__ __device__ uint32_t code_div(float x, float s) {
+  return (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.f), 127.f);
 }
-__device__ __forceinline__ uint2 codes8(const float* x, float s) {
-  uint32_t w[2] = {0, 0};
-#pragma unroll
-  for (int e = 0; e < 8; e++) w[e >> 2] |= code_of(x[e], s) << (8 * (e & 3));
-  return make_uint2(w[0], w[1]);
+struct Divisor {
+  float s, rs;
+  bool fast;
+  __device__ explicit Divisor(float scale) : s(scale), rs(0.f), fast(scale > 0x1p-80f && scale < 0x1p100f) {
+    if (fast) rs = __frcp_rn(s);
+  }
+};
+__device__ __forceinline__ uint32_t code_of(float x, const Divisor& d) {  // in the low byte
+  return d.fast ? __float_as_uint(__fadd_rn(div_rn_by(x, d.s, d.rs), 12582912.f)) : code_div(x, d.s);
+}
+__device__ __forceinline__ uint32_t codes4(float x0, float x1, float x2, float x3, const Divisor& d) {
+  return __byte_perm(__byte_perm(code_of(x0, d), code_of(x1, d), 0x0040), __byte_perm(code_of(x2, d), code_of(x3, d), 0x0040), 0x5410);
 }
 
 // CTA = one block of 64 slots of one (sequence, head, K or V) that gets new tokens, or a run of q chunks.
@@ -162,20 +171,17 @@ __global__ void __launch_bounds__(128) rope_kv8_kernel(AppendArgs a) {
       }
     }
   }
+  const Divisor div(sc);
 #pragma unroll
   for (int k = 0; k < PER; k++) {
     const int t = tid + 128 * k, row = t / CH, c = t % CH;
     if (row >= m) continue;
     uint2 o = make_uint2(0, 0);
     if (sc > 0.f) {  // neither zero nor NaN
-      const uint32_t x[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-      float f[8];
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        f[2 * e] = __uint_as_float(x[e] << 16);
-        f[2 * e + 1] = __uint_as_float(x[e] & 0xffff0000u);
-      }
-      o = codes8(f, sc);
+      auto lo = [](uint32_t x) { return __uint_as_float(x << 16); };
+      auto hi = [](uint32_t x) { return __uint_as_float(x & 0xffff0000u); };
+      o.x = codes4(lo(v[k].x), hi(v[k].x), lo(v[k].y), hi(v[k].y), div);
+      o.y = codes4(lo(v[k].z), hi(v[k].z), lo(v[k].w), hi(v[k].w), div);
     }
     *reinterpret_cast<uint2*>(codes + (size_t)(held + row) * D + 8 * c) = o;
   }
@@ -268,6 +274,7 @@ __global__ void __launch_bounds__(THREADS) kv8_select_kernel(EvictArgs a) {
   // T: the largest key with at least `want` keys >= T; above: how many are > T
   unsigned int T = 0, above = 0;
   if (want == 0) T = 0xffffffffu;
+#pragma unroll 1
   for (int shift = 30; shift >= 0 && want > 0; shift -= 2) {
     unsigned int c1 = 0, c2 = 0, c3 = 0, sum[3];
     const uint32_t t1 = T + (1u << shift), t2 = T + (2u << shift), t3 = T + (3u << shift);
@@ -332,28 +339,17 @@ __device__ __forceinline__ int top_code(uint4 c) {
   m = __vmaxu2(m & 0x00ff00ffu, (m >> 8) & 0x00ff00ffu);
   return (int)max(m & 0xffffu, m >> 16);
 }
-// Four codes times `s` (rounded), each divided by `d` (1 / d rounded: rd) and rounded half to even: codes again.
-__device__ __forceinline__ uint32_t recode4(uint32_t c, float s, float d, float rd, bool fast) {
-  uint32_t o = 0;
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    // byte ^ 0x80 into the mantissa of 2^23: 2^23 + 128 + code
-    const float x = __fmul_rn(__uint_as_float(__byte_perm(c ^ 0x80808080u, 0x4b000000u, 0x7440 + e)) - 8388736.f, s);
-    if (fast) {
-      // + 1.5 * 2^23 rounds to an integer, which is then in the low bits
-      const uint32_t r = __float_as_uint(__fadd_rn(div_rn_by(x, d, rd), 12582912.f));
-      o |= (r & 0xffu) << (8 * e);
-    } else {
-      o |= code_of(x, d) << (8 * e);
-    }
-  }
-  return o;
+// Four codes times `s` (rounded), each divided by the new scale and rounded half to even: codes again.
+__device__ __forceinline__ uint32_t recode4(uint32_t c, float s, const Divisor& d) {
+  c ^= 0x80808080u;
+  // byte into the mantissa of 2^23: 2^23 + 128 + code
+  auto value = [&](uint32_t sel) { return __fmul_rn(__uint_as_float(__byte_perm(c, 0x4b000000u, sel)) - 8388736.f, s); };
+  return codes4(value(0x7440), value(0x7441), value(0x7442), value(0x7443), d);
 }
 
 // CTA = one block of 64 kept tokens of one (sequence, head), K and V: values code * scale (rounded to fp32), the block's
 // scale max |value| / 127 and codes rint(value / scale).  All of a thread's rows are on their way at once.  The
-// quotient is the IEEE one in five operations (div_rn_by) wherever that is exact; a division each made this
-// kernel compute bound (246 us for 285 MB).  Sequences that lost nothing are copied.
+// quotient is code_of's.  Sequences that lost nothing are copied.
 template <int D>
 __global__ void __launch_bounds__(128) kv8_gather_kernel(EvictArgs a) {
   constexpr int PC = D / 16, PER = BLK * PC / 128;  // 16-byte pieces of a row, pieces a thread takes of K and of V
@@ -407,8 +403,7 @@ __global__ void __launch_bounds__(128) kv8_gather_kernel(EvictArgs a) {
 #pragma unroll
   for (int v = 0; v < 2; v++) {
     int8_t* dst = (v ? a.dvc : a.dkc) + (bh * a.Cd + (size_t)blk * BLK) * D;
-    const bool fast = s[v] > 0x1p-80f && s[v] < 0x1p100f;
-    const float rd = fast ? __frcp_rn(s[v]) : 0.f;
+    const Divisor d(s[v]);
 #pragma unroll
     for (int k = 0; k < PER; k++) {
       const int row = (tid + 128 * k) / PC, p = (tid + 128 * k) % PC;
@@ -416,8 +411,7 @@ __global__ void __launch_bounds__(128) kv8_gather_kernel(EvictArgs a) {
       uint4 o = c[v][k];
       if (!copy) {
         if (s[v] > 0.f)
-          o = make_uint4(recode4(o.x, sc[v][k], s[v], rd, fast), recode4(o.y, sc[v][k], s[v], rd, fast),
-                         recode4(o.z, sc[v][k], s[v], rd, fast), recode4(o.w, sc[v][k], s[v], rd, fast));
+          o = make_uint4(recode4(o.x, sc[v][k], d), recode4(o.y, sc[v][k], d), recode4(o.z, sc[v][k], d), recode4(o.w, sc[v][k], d));
         else
           o = make_uint4(0, 0, 0, 0);
       }
