@@ -202,10 +202,15 @@ struct EvictArgs {
 constexpr int MAX_EVICT = 8 * 1024 * 32;  // slots of a head that a cluster of 8 CTAs holds in registers
 
 // Order of weights as unsigned numbers: -inf .. +inf, NaN above all, -0 equal to 0.
-__device__ __forceinline__ uint32_t order_of(float f) {
-  if (isnan(f)) return 0xffffffffu;
-  const uint32_t u = __float_as_uint(f == 0.f ? 0.f : f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+__device__ __forceinline__ uint32_t order_of(uint32_t u) {
+  const uint32_t mag = u & 0x7fffffffu;
+  const uint32_t k = u & 0x80000000u && mag ? ~u : mag | 0x80000000u;
+  return mag > 0x7f800000u ? 0xffffffffu : k;
+}
+
+// The weight with that key (+0 for -0).
+__device__ __forceinline__ float weight_of(uint32_t u) {
+  return u == 0xffffffffu ? __uint_as_float(0x7fc00000u) : __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
 // Which slots of a head stay: the (keep - recent) largest weights before the recent ones, and the recent ones.  A head is one
@@ -213,15 +218,19 @@ __device__ __forceinline__ uint32_t order_of(float f) {
 // order keys of up to KPT slots in registers (warp w of a CTA has 32 kpt consecutive slots, key i of lane l is slot 32 i + l).
 // The threshold is found two bits at a time from the top: three counts of keys above a candidate, added up over warps,
 // CTAs and the cluster; a candidate with exactly the wanted count ends the search (after about 11 of 16 rounds for
-// weights that differ).  Counting by comparison needs no atomics, whose same-address conflicts made histograms of
-// these skewed weights (most share an exponent) eight times slower: 397 us for 8 heads of 131k slots, 98 us for 256 heads
-// of 16k.  Then positions by ballots and prefix sums: kept slots are written in order, ties to the lowest slots.
-// Latency bound: rounds of compare, reduce and barrier.
+// weights that differ).  Once no more keys share the threshold's leading bits than a CTA has threads, those keys move to
+// one register each and a round is little more than its barrier.  Counting by comparison needs no atomics, whose same-address
+// conflicts made histograms of these skewed weights (most share an exponent) slow: 397 us for 8 heads of 131k slots,
+// 98 us for 256 heads of 16k.  Then positions by ballots and prefix sums: kept slots are written in order, ties to the
+// lowest slots.  Bound by instruction issue (six a key and round) and the rounds' barriers.
 template <int THREADS, int KPT, int CS>
 __global__ void __launch_bounds__(THREADS) kv8_select_kernel(EvictArgs a) {
   constexpr int W = THREADS / 32;
-  __shared__ unsigned int sh_warp[2][W];
+  __shared__ unsigned int sh_warp[2][2][W];
   __shared__ unsigned int sh_cta[2][CS][3];
+  __shared__ unsigned int sh_gt[W], sh_eq[W], sh_before[CS][2];
+  __shared__ uint32_t sh_key[THREADS];
+  __shared__ unsigned int sh_keys;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = CS > 1 ? (int)cluster_ctarank() : 0;
   const long long bh = blockIdx.x / CS;
@@ -247,47 +256,85 @@ __global__ void __launch_bounds__(THREADS) kv8_select_kernel(EvictArgs a) {
   const int j0 = (rank * W + warp) * 32 * kpt + lane;  // slot of key i: j0 + 32 i
   uint32_t key[KPT];  // 0: not a candidate (the key of -inf is 0x007fffff)
 #pragma unroll
-  for (int i = 0; i < KPT; i++) key[i] = i < kpt && j0 + 32 * i < N ? order_of(w[j0 + 32 * i]) : 0u;
-  // sums over the head of three counts (at most 1024 in a warp: two to a register)
+  for (int i = 0; i < KPT; i++) key[i] = i < kpt && j0 + 32 * i < N ? __float_as_uint(__ldg(w + j0 + 32 * i)) : 0u;  // all on their way
+#pragma unroll
+  for (int i = 0; i < KPT; i++) key[i] = i < kpt && j0 + 32 * i < N ? order_of(key[i]) : 0u;
+  // sums over the warps of a CTA of what lane i < W of each warp holds
+  auto over_warps = [&](unsigned int x) { return W > 1 ? __reduce_add_sync(0xffffffffu, lane < W ? x : 0u) : x; };
   int round = 0;
+  // sums over the head of three counts (at most 1024 in a warp: two to a register)
   auto total3 = [&](unsigned int c1, unsigned int c2, unsigned int c3, unsigned int (&sum)[3]) {
     const int f = round++ & 1;
     const unsigned int p12 = __reduce_add_sync(0xffffffffu, c1 | (c2 << 16));
     const unsigned int p3 = __reduce_add_sync(0xffffffffu, c3);
-    __shared__ unsigned int sh3[2][W];
-    if (lane == 0) sh_warp[f][warp] = p12, sh3[f][warp] = p3;
+    if (lane == 0) sh_warp[f][0][warp] = p12, sh_warp[f][1][warp] = p3;
     __syncthreads();
-    const unsigned int x = lane < W ? sh_warp[f][lane] : 0u, y = lane < W ? sh3[f][lane] : 0u;
-    sum[0] = __reduce_add_sync(0xffffffffu, x & 0xffffu);
-    sum[1] = __reduce_add_sync(0xffffffffu, x >> 16);
-    sum[2] = __reduce_add_sync(0xffffffffu, y);
+    if constexpr (W == 2) {
+      const unsigned int x = sh_warp[f][0][0], y = sh_warp[f][0][1];
+      sum[0] = (x & 0xffffu) + (y & 0xffffu), sum[1] = (x >> 16) + (y >> 16), sum[2] = sh_warp[f][1][0] + sh_warp[f][1][1];
+    } else {
+      const unsigned int x = lane < W ? sh_warp[f][0][lane] : 0u, y = lane < W ? sh_warp[f][1][lane] : 0u;
+      sum[0] = over_warps(x & 0xffffu), sum[1] = over_warps(x >> 16), sum[2] = over_warps(y);
+    }
     if constexpr (CS > 1) {
       if (tid < CS * 3) {  // this CTA's sums to every CTA of the cluster
         const uint32_t to = mapa_shared(smem_u32(&sh_cta[f][rank][tid % 3]), tid / 3);
-        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(sum[tid % 3]) : "memory");
+        const unsigned int v = tid % 3 == 0 ? sum[0] : tid % 3 == 1 ? sum[1] : sum[2];
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(v) : "memory");
       }
       cluster_sync();
 #pragma unroll
-      for (int k = 0; k < 3; k++) sum[k] = __reduce_add_sync(0xffffffffu, lane < CS ? sh_cta[f][lane][k] : 0u);
+      for (int k = 0; k < 3; k++) {
+        sum[k] = 0;
+#pragma unroll
+        for (int r = 0; r < CS; r++) sum[k] += sh_cta[f][r][k];
+      }
     }
   };
-  // T: the largest key with at least `want` keys >= T; above: how many are > T
-  unsigned int T = 0, above = 0;
-  if (want == 0) T = 0xffffffffu;
+  // T: the largest key with at least `want` keys >= T; above: how many are > T; upto: how many are >= T
+  unsigned int T = want ? 0u : 0xffffffffu, above = 0, upto = 0xffffffffu;
+  bool few = false;
+  uint32_t one = 0;  // this thread's key among the few that are left
 #pragma unroll 1
   for (int shift = 30; shift >= 0 && want > 0; shift -= 2) {
     unsigned int c1 = 0, c2 = 0, c3 = 0, sum[3];
     const uint32_t t1 = T + (1u << shift), t2 = T + (2u << shift), t3 = T + (3u << shift);
+    if (few) {
+      c1 = one >= t1, c2 = one >= t2, c3 = one >= t3;
+    } else {
 #pragma unroll
-    for (int i = 0; i < KPT; i++)
-      if (i < kpt) c1 += key[i] >= t1, c2 += key[i] >= t2, c3 += key[i] >= t3;
+      for (int i = 0; i < KPT; i += 4)
+        if (i < kpt) {
+#pragma unroll
+          for (int e = i; e < i + 4; e++) c1 += key[e] >= t1, c2 += key[e] >= t2, c3 += key[e] >= t3;
+        }
+    }
     total3(c1, c2, c3, sum);
+    if (few) sum[0] += above, sum[1] += above, sum[2] += above;  // the larger keys are not among the few
     const int d = sum[2] >= want ? 3 : sum[1] >= want ? 2 : sum[0] >= want ? 1 : 0;
-    if (d < 3) above = sum[d];
+    above = d == 3 ? above : d == 2 ? sum[2] : d == 1 ? sum[1] : sum[0];
+    if (d > 0) upto = d == 3 ? sum[2] : d == 2 ? sum[1] : sum[0];
     T += (unsigned int)d << shift;
-    if (d > 0 && sum[d - 1] == want) {  // exactly the keys >= T
+    if (d > 0 && upto == want) {  // exactly the keys >= T
       T--, above = want;
       break;
+    }
+    const uint32_t top = T + ((1u << shift) - 1u);  // keys T .. top share the leading bits
+    if (few) {
+      if (one < T || one > top) one = 0;
+    } else if (upto - above <= THREADS) {  // their number over the head (not known, and large, while T is 0)
+      if (tid == 0) sh_keys = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < KPT; i += 4)
+        if (i < kpt) {
+#pragma unroll
+          for (int e = i; e < i + 4; e++)
+            if (key[e] >= T && key[e] <= top && key[e] != 0u) sh_key[atomicAdd(&sh_keys, 1u)] = key[e];
+        }
+      __syncthreads();
+      one = tid < (int)sh_keys ? sh_key[tid] : 0u;
+      few = true;
     }
   }
   const unsigned int ties = want - above;  // of the keys equal to T
@@ -300,8 +347,6 @@ __global__ void __launch_bounds__(THREADS) kv8_select_kernel(EvictArgs a) {
       gt += __popc(__ballot_sync(0xffffffffu, key[i] > T || (j >= N && j < len)));
       eq += __popc(__ballot_sync(0xffffffffu, key[i] == T && key[i] != 0u));
     }
-  __shared__ unsigned int sh_gt[W], sh_eq[W];
-  __shared__ unsigned int sh_before[CS][2];
   if (lane == 0) sh_gt[warp] = gt, sh_eq[warp] = eq;
   __syncthreads();
   const unsigned int xg = lane < W ? sh_gt[lane] : 0u, xe = lane < W ? sh_eq[lane] : 0u;
@@ -326,7 +371,7 @@ __global__ void __launch_bounds__(THREADS) kv8_select_kernel(EvictArgs a) {
       if (sure || (even && e < ties)) {
         const unsigned int at = bg + __popc(mg & below) + min(e, ties);
         idx[at] = j;
-        dw[at] = w[j];
+        dw[at] = j < N ? weight_of(key[i]) : __ldg(w + j);  // from the register: a load behind each store costs its latency
       }
       bg += __popc(mg), be += __popc(me);
     }
@@ -334,90 +379,121 @@ __global__ void __launch_bounds__(THREADS) kv8_select_kernel(EvictArgs a) {
 
 // Largest |code| of 16, as a number.
 __device__ __forceinline__ int top_code(uint4 c) {
-
   uint32_t m = __vmaxu4(__vmaxu4(__vabsdiffs4(c.x, 0), __vabsdiffs4(c.y, 0)), __vmaxu4(__vabsdiffs4(c.z, 0), __vabsdiffs4(c.w, 0)));
   m = __vmaxu2(m & 0x00ff00ffu, (m >> 8) & 0x00ff00ffu);
   return (int)max(m & 0xffffu, m >> 16);
 }
-// Four codes times `s` (rounded), each divided by the new scale and rounded half to even: codes again.
-__device__ __forceinline__ uint32_t recode4(uint32_t c, float s, const Divisor& d) {
+// Four codes c times `s` (rounded), each divided by the new scale and rounded half to even: codes again.
+__noinline__ __device__ uint32_t recode4(uint32_t c, float s, float scale) {
+  const Divisor d(scale);
   c ^= 0x80808080u;
   // byte into the mantissa of 2^23: 2^23 + 128 + code
   auto value = [&](uint32_t sel) { return __fmul_rn(__uint_as_float(__byte_perm(c, 0x4b000000u, sel)) - 8388736.f, s); };
   return codes4(value(0x7440), value(0x7441), value(0x7442), value(0x7443), d);
 }
+// The same from the rounded ratio of the scales: code * ratio is within 127.1 * 4 * 2^-24 < 2^-15 of the quotient above, so it
+// rounds to the same integer unless it lies that near to a half; `worst` collects the distance from the integer.
+__device__ __forceinline__ uint32_t recode4_near(uint32_t c, unsigned long long ratio2, float& worst) {
+  const unsigned long long off = f2_pack(-8388736.f, -8388736.f), magic = f2_pack(12582912.f, 12582912.f),
+                           unmagic = f2_pack(-12582912.f, -12582912.f), minus = f2_pack(-1.f, -1.f);
+  c ^= 0x80808080u;
+  uint32_t o[2];
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const unsigned long long x = f2_add(f2_pack(__uint_as_float(__byte_perm(c, 0x4b000000u, 0x7440 + 2 * k)),
+                                                __uint_as_float(__byte_perm(c, 0x4b000000u, 0x7441 + 2 * k))), off);
+    const unsigned long long q = f2_mul(x, ratio2), r = f2_add(q, magic);
+    float r0, r1, t0, t1;
+    f2_unpack(r, r0, r1);
+    f2_unpack(f2_fma(f2_add(r, unmagic), minus, q), t0, t1);
+    worst = max3f(worst, fabsf(t0), fabsf(t1));
+    o[k] = __byte_perm(__float_as_uint(r0), __float_as_uint(r1), 0x0040);
+  }
+  return __byte_perm(o[0], o[1], 0x5410);
+}
 
 // CTA = one block of 64 kept tokens of one (sequence, head), K and V: values code * scale (rounded to fp32), the block's
-// scale max |value| / 127 and codes rint(value / scale).  All of a thread's rows are on their way at once.  The
-// quotient is code_of's.  Sequences that lost nothing are copied.
+// scale max |value| / 127 and codes rint(value / scale).  Rows come by 16-byte asynchronous copies, all on their way at once,
+// and the passes over them are short loops (unrolled over registers, they ran out of instruction cache).  Most pieces
+// of 16 codes need only a multiplication by the ratio of the scales; one in 500 has a value near a half and takes the
+// quotients.  Sequences that lost nothing are copied.  Bound: DRAM, rows of 64 or 128 bytes apart.
 template <int D>
 __global__ void __launch_bounds__(128) kv8_gather_kernel(EvictArgs a) {
-  constexpr int PC = D / 16, PER = BLK * PC / 128;  // 16-byte pieces of a row, pieces a thread takes of K and of V
-  __shared__ float red[2][4];
+  constexpr int PC = D / 16, PIECES = BLK * PC;  // 16-byte pieces of a row, of a block
+  __shared__ __align__(16) uint4 code[2][PIECES];
+  __shared__ float scale[2][BLK], ratio[2][BLK], red[2][4];
+  __shared__ int slot[BLK];
   const int tid = threadIdx.x;
   griddep_wait();
   griddep_launch();
   const int nb = a.keep / BLK, blk = (int)(blockIdx.x % nb);
   const size_t bh = blockIdx.x / nb;
   const int len = min(max(a.lens[bh / a.H], 0), a.C);
-  const int rows = min(len, a.keep) - blk * BLK;
+  const int rows = min(min(len, a.keep) - blk * BLK, BLK);
   if (rows <= 0) return;
-  const int* idx = a.index + bh * a.keep + blk * BLK;
   const bool copy = len <= a.keep;
-  uint4 c[2][PER];
-  float sc[2][PER];
-#pragma unroll
-  for (int k = 0; k < PER; k++) {
-    const int row = (tid + 128 * k) / PC, p = (tid + 128 * k) % PC;
-#pragma unroll
-    for (int v = 0; v < 2; v++) c[v][k] = make_uint4(0, 0, 0, 0), sc[v][k] = 0.f;
-    if (row >= rows) continue;
-    const int j = copy ? blk * BLK + row : idx[row];
-    const size_t at = (bh * a.C + j) * D + 16 * p, sat = bh * (a.C / BLK) + j / BLK;
-    c[0][k] = *reinterpret_cast<const uint4*>(a.kc + at);
-    c[1][k] = *reinterpret_cast<const uint4*>(a.vc + at);
-    sc[0][k] = a.ks[sat], sc[1][k] = a.vs[sat];
+  const int v = tid / BLK, r = tid % BLK;  // this thread's row of scales: K's or V's
+  if (r < rows) {
+    const int j = copy ? blk * BLK + r : a.index[bh * a.keep + blk * BLK + r];
+    if (v == 0) slot[r] = j;
+    scale[v][r] = (v ? a.vs : a.ks)[bh * (a.C / BLK) + j / BLK];
   }
-  float s[2];
+  __syncthreads();
+  for (int p = tid; p < rows * PC; p += 128) {
+    const size_t at = (bh * a.C + slot[p / PC]) * D + 16 * (p % PC);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&code[0][p])), "l"(a.kc + at) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&code[1][p])), "l"(a.vc + at) : "memory");
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  int8_t* dst[2] = {a.dkc + (bh * a.Cd + (size_t)blk * BLK) * D, a.dvc + (bh * a.Cd + (size_t)blk * BLK) * D};
+  float* ds[2] = {a.dks + bh * (a.Cd / BLK) + blk, a.dvs + bh * (a.Cd / BLK) + blk};
   if (copy) {
-    s[0] = sc[0][0], s[1] = sc[1][0];  // thread 0's first row is in this block
-  } else {
-#pragma unroll
-    for (int v = 0; v < 2; v++) {
-      float top = 0.f;  // rounding is monotonic: the largest rounded product is that of the largest code
-#pragma unroll
-      for (int k = 0; k < PER; k++) {
-        const float x = __fmul_rn((float)top_code(c[v][k]), fabsf(sc[v][k]));
-        top = isnan(sc[v][k]) ? INFINITY : fmaxf(top, x);
-      }
-      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-      if ((tid & 31) == 0) red[v][tid >> 5] = top;
+    for (int k = 0; k < 2; k++) {
+      for (int p = tid; p < rows * PC; p += 128) reinterpret_cast<uint4*>(dst[k])[p] = code[k][p];  // this thread's own copies
+      if (tid == 0) *ds[k] = scale[k][0];
     }
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < 2; v++) {
-      const float top = fmaxf(fmaxf(red[v][0], red[v][1]), fmaxf(red[v][2], red[v][3]));
-      s[v] = isinf(top) ? __uint_as_float(0x7fc00000u) : __fdiv_rn(top, 127.f);
-    }
+    return;
   }
 #pragma unroll
-  for (int v = 0; v < 2; v++) {
-    int8_t* dst = (v ? a.dvc : a.dkc) + (bh * a.Cd + (size_t)blk * BLK) * D;
-    const Divisor d(s[v]);
-#pragma unroll
-    for (int k = 0; k < PER; k++) {
-      const int row = (tid + 128 * k) / PC, p = (tid + 128 * k) % PC;
-      if (row >= rows) continue;
-      uint4 o = c[v][k];
-      if (!copy) {
-        if (s[v] > 0.f)
-          o = make_uint4(recode4(o.x, sc[v][k], d), recode4(o.y, sc[v][k], d), recode4(o.z, sc[v][k], d), recode4(o.w, sc[v][k], d));
-        else
-          o = make_uint4(0, 0, 0, 0);
-      }
-      *reinterpret_cast<uint4*>(dst + (size_t)row * D + 16 * p) = o;
+  for (int k = 0; k < 2; k++) {
+    float top = 0.f;  // rounding is monotonic: the largest rounded product is that of the largest code
+#pragma unroll 2
+    for (int p = tid; p < PIECES; p += 128) {  // a sequence that lost tokens fills its blocks
+      const float s = scale[k][p / PC];
+      top = isnan(s) ? INFINITY : fmaxf(top, __fmul_rn((float)top_code(code[k][p]), fabsf(s)));
     }
-    if (tid == 0) (v ? a.dvs : a.dks)[bh * (a.Cd / BLK) + blk] = s[v];
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    if ((tid & 31) == 0) red[k][tid >> 5] = top;
+  }
+  __syncthreads();
+  float s[2];
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const float top = fmaxf(fmaxf(red[k][0], red[k][1]), fmaxf(red[k][2], red[k][3]));
+    s[k] = isinf(top) ? __uint_as_float(0x7fc00000u) : __fdiv_rn(top, 127.f);
+  }
+  ratio[v][r] = __fdiv_rn(scale[v][r], v ? s[1] : s[0]);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    if (tid == 0) *ds[k] = s[k];
+    const bool fast = s[k] > 0x1p-80f && s[k] < 0x1p100f;
+#pragma unroll 1
+    for (int p = tid; p < PIECES; p += 128) {
+      const uint4 c = code[k][p];
+      uint4 o = make_uint4(0, 0, 0, 0);
+      if (s[k] > 0.f) {  // neither zero nor NaN
+        const float f = ratio[k][p / PC];
+        const unsigned long long f2 = f2_pack(f, f);
+        float worst = 0.f;
+        o = make_uint4(recode4_near(c.x, f2, worst), recode4_near(c.y, f2, worst), recode4_near(c.z, f2, worst), recode4_near(c.w, f2, worst));
+        if (!fast || !(worst < 0.5f - 0x1p-14f)) {
+          const float sp = scale[k][p / PC];
+          o = make_uint4(recode4(c.x, sp, s[k]), recode4(c.y, sp, s[k]), recode4(c.z, sp, s[k]), recode4(c.w, sp, s[k]));
+        }
+      }
+      reinterpret_cast<uint4*>(dst[k])[p] = o;
+    }
   }
 }
 
@@ -508,10 +584,10 @@ int vt_kv8_evict(cudaStream_t st, const int8_t* kc, const int8_t* vc, const floa
   if (units > 0x7fffffffLL || n > 0x0fffffffLL)
     return set_error(E_SHAPE, "vt_kv8_evict: grid too large (B=%d H=%d keep=%d)", B, H, keep);
   kv8::EvictArgs a{kc, vc, ks, vs, weights, lens, B, H, C, keep, recent, dst_C, dst_kc, dst_vc, dst_ks, dst_vs, dst_weights, dst_lens, index};
-  // 256 threads for up to 2048 slots, else 1024; as many CTAs a head as leave each thread at most 16 slots when there
+  // two warps for up to 2048 slots (a warp's share of a round is mostly not its keys), else 1024 threads; as many CTAs a head as leave each thread at most 16 slots when there
   // are fewer heads than SMs, 32 otherwise (one CTA then has a head of up to 32k slots; 256 heads fill the GPU)
   const int most = n < sm_count() ? 16 : 32;
-  if (C <= 2048) kv8::launch_select<256, 8, 1>(st, a);
+  if (C <= 2048) kv8::launch_select<64, 32, 1>(st, a);
   else if (C <= most * 1024) kv8::launch_select<1024, 32, 1>(st, a);
   else if (C <= most * 2048) kv8::launch_select<1024, 32, 2>(st, a);
   else if (C <= most * 4096) kv8::launch_select<1024, 32, 4>(st, a);
