@@ -5,7 +5,7 @@
 // one list that is cut into equal runs, one for each SM, whatever the sequences' lengths and the causal limits; an item
 // that spans CTAs leaves its parts (unnormalised O, row max, row sum) for attn_kv8_tc_join_kernel.
 //
-// CTA = 14 warps:
+// CTA = 16 warps (two of them idle):
 //   warps 0-3, 4-7   softmax of M tile 0 / 1, thread = row (TMEM lane): P = 2^(s - m) as bf16 over the scores;
 //   warps 8-11       codes -> bf16 operands in shared memory (ST stages), one tile's codes ahead in registers; q once an item;
 //   warps 12, 13     tcgen05.mma of M tile 0 / 1: S_(j+1), then O += P_j V_j (P from TMEM, V as an MN-major B operand).
@@ -24,10 +24,11 @@ namespace vt {
 namespace kv8 {
 namespace tc {
 
-constexpr int ROWS = 256, KEYS = 64, THREADS = 14 * 32, ST = 3, MAXB = 2048;
+constexpr int ROWS = 256, KEYS = 64, THREADS = 16 * 32, ST = 3, MAXB = 2048;
 constexpr uint32_t TMEM_COLS = 512;  // S of M tile t, buffer f: columns 128 t + 64 f; O of tile t: 256 + 128 t
 constexpr long long kDrainCycles = 200000000LL;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr int SOFTMAX_REGS = 168, CONVERT_REGS = 96, MMA_REGS = 80;
 constexpr float kTinyScale = 0x1p-100f;
 constexpr int WHOLE_TILES = 24;  // items of up to so many tiles stay whole when there are fewer of them than SMs
 
@@ -203,7 +204,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, ST_KV8_WAIT)) != 0;
   };
 
-  if (warp >= 12) {
+  // registers by role: 512 threads are launched with 128 each; the softmax holds 64 scores, and spills cost its tiles a fifth
+  static_assert(2 * SOFTMAX_REGS + CONVERT_REGS + MMA_REGS <= 4 * 128, "the split must come out of the launch's registers");
+  if (warp >= 14) {
+    set_regs_down<MMA_REGS>();  // idle; the issuers' warp group
+  } else if (warp >= 12) {
+    set_regs_down<MMA_REGS>();
     // ---------------- MMA issuer of M tile t (one warp each: issuing is what a tile's time is made of otherwise).  The
     // whole warp walks the loop, one lane issues.  j: key tiles of all segments; js: of those in which t had rows
     const int t = warp - 12;
@@ -222,7 +228,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       if (g.r0 + 128 * t >= g.s.cnt * a.G) {  // no rows in this M tile: only the barriers
         for (int i = 0; i < nt && ok; i++, next(st, ph)) {
           ok = wait(&kv_full[st], ph);
-          if (leader) mbar_arrive(&kv_empty[st]);
+          mbar_arrive_if(&kv_empty[st], leader != 0);
         }
         continue;
       }
@@ -264,6 +270,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       mbar_wait_drain(&drain[t], 0, kDrainCycles);
     }
   } else if (warp >= 8) {
+    set_regs_down<CONVERT_REGS>();
     // ---------------- converters: warp w rows 16 w .. of a block, 8 lanes = 8 rows of one 16-byte piece.  K's and V's codes of
     // the next tile are fetched as soon as this tile's are out of the registers
     constexpr int PER = D / 32;  // pieces of a K or V block that a lane takes
@@ -304,10 +311,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
         if (i + 1 < nt) fetch(vr, vp), vs = vsp[i + 1];
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&kv_full[st]);
+        mbar_arrive_if(&kv_full[st], lane == 0);
       }
     }
   } else {
+    set_regs_up<SOFTMAX_REGS>();
     // ---------------- softmax of M tile t: thread = row.  It brings in its row of q itself
     const int t = warp >> 2;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16, t_o = tmem + 256 + 128 * t + lane_off;
@@ -328,7 +336,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[t]);
+      mbar_arrive_if(&q_full[t], lane == 0);
     };
     Seg g;
     if (u_begin < u_end) load_q(g = segment(a, pre, u_begin, u_end));
@@ -347,16 +355,25 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       // the fewest keys that a row of this warp sees: tiles up to there need no mask
       const int lim_min = __reduce_min_sync(0xffffffffu, lim);
       float m = -INFINITY, l = 0.f;
-      float c, lvs, ivs;  // of the tile: K's scale times the softmax scale, log2 and inverse of V's scale
-      float ks_next = ksp[0], vs_next = vsp[0];
+      // of the tile: K's scale times the softmax scale, log2 and inverse of V's scale (the approximations err by 2^-22, both
+      // in the sum and in O); the next tile's are worked out while this one's scores arrive
+      float c, lvs, ivs, ks_next = ksp[0], vs_next = vsp[0], c_next, lvs_next, ivs_next;
+      auto next_scales = [&](int i) {
+        const float v = vs_next < kTinyScale ? 1.f : vs_next;  // the converters made V zero
+        c_next = ks_next * a.scale_log2, lvs_next = __log2f(v), ivs_next = __frcp_rn(v);
+        if (i + 1 < nt) ks_next = ksp[i + 1], vs_next = vsp[i + 1];
+      };
+      next_scales(0);
+      auto announce = [&](int f) {  // P in buffer f is complete
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_if(&p_full[2 * t + f], lane == 0);
+      };
       for (int i = 0; i < nt; i++) {
         const int f = (js + i) & 1, key0 = (g.ta + i) * KEYS;
         const uint32_t t_s = tmem + 128 * t + 64 * f + lane_off;
-        {
-          const float v = vs_next < kTinyScale ? 1.f : vs_next;  // the converters made V zero
-          c = ks_next * a.scale_log2, lvs = log2f(v), ivs = 1.f / v;
-          if (i + 1 < nt) ks_next = ksp[i + 1], vs_next = vsp[i + 1];
-        }
+        c = c_next, lvs = lvs_next, ivs = ivs_next;
         uint32_t r0[32], r1[32];
         float mx, sum;
         auto top32 = [&](const uint32_t (&r)[32]) {
@@ -390,6 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
         if (!ok) break;
         tc_fence_after();
         tmem_ld32(t_s, r0);
+        next_scales(i + 1);
         tmem_ld_wait();
         tmem_ld32(t_s + 32, r1);
         // a tile that every row sees whole, once a row has a maximum: P with the maximum so far, while the second half of
@@ -452,10 +470,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
           sum = exps(r0, 0, mu) + exps(r1, 16, mu);
         }
         l += sum * ivs;
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * t + f]);
+        announce(f);
       }
       if (!ok) break;
       const Seg done = g;
@@ -495,7 +510,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&o_empty[t]);
+      mbar_arrive_if(&o_empty[t], lane == 0);
       j += nt, js += nt, so++;
     }
   }
@@ -638,7 +653,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv8_weights_tc_kernel(Args a) {
       sh_lse[f][ct] = r0 + ct < rows ? a.lse[bh * a.rows + r0 + ct] : INFINITY;  // rows past the last add 2^-inf
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[f]);
+      mbar_arrive_if(&q_full[f], lane == 0);
     }
   } else {
     const int half = warp >> 2, key = key0 + (warp & 3) * 32 + lane;
@@ -659,7 +674,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv8_weights_tc_kernel(Args a) {
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s_empty[f]);
+      mbar_arrive_if(&s_empty[f], lane == 0);
       const bool edge = r0 < warp_max;
       const unsigned long long c2 = f2_pack(c, c), minus = f2_pack(-1.f, -1.f);
 #pragma unroll
@@ -684,7 +699,7 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv8_weights_tc_kernel(Args a) {
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_empty[f]);
+      mbar_arrive_if(&q_empty[f], lane == 0);
     }
     float lo, hi;
     f2_unpack(f2_add(acc2[0], acc2[1]), lo, hi);
