@@ -19,7 +19,7 @@ long long vt_attn_kv8_ws_bytes(int B, int n, int Hq, int H, int D, int C, int we
   // what n tokens need, and any fewer that may follow with the same workspace
   const int few = vt::kv8::FEW_ROWS / (Hq / H), nf = n < few ? n : few;
   const long long split = nf ? vt::kv8::split::make_plan(B, nf, Hq, H, D, C, weights != 0, vt::sm_count()).bytes : 0;
-  const long long many = n > few ? vt::kv8::tc::make_plan(B, n, Hq, H, D, weights != 0, vt::sm_count()).bytes : 0;
+  const long long many = n > few ? vt::kv8::tc::make_plan(B, n, Hq, H, D, C, weights != 0, vt::sm_count()).bytes : 0;
   return split > many ? split : many;
 }
 
@@ -46,15 +46,16 @@ int vt_attn_kv8(cudaStream_t st, const uint16_t* q, long long sq_b, long long sq
     kv8::split::Args a{q, sq_b, sq_t, sq_h, kc, vc, ks, vs, lens, counts, B, n, Hq / H, H, C, causal, p.rows, p.rg, p.ctas,
                        scale * kv8::LOG2E, out, so_b, so_t, so_h, (float*)(w8 + p.o_off), (float2*)(w8 + p.ml_off),
                        (float2*)(w8 + p.full_off), weights ? (float*)(w8 + p.s_off) : nullptr, weights, weights_in};
-    if (D == 64) return p.nt == 1 ? kv8::split::launch<64, 1>(st, a) : p.nt == 2 ? kv8::split::launch<64, 2>(st, a) : kv8::split::launch<64, 4>(st, a);
-    return p.nt == 1 ? kv8::split::launch<128, 1>(st, a) : kv8::split::launch<128, 2>(st, a);
+    if (D == 64) return p.nt == 1 ? kv8::split::launch<64, 1>(st, a, p.whole) : p.nt == 2 ? kv8::split::launch<64, 2>(st, a, p.whole) : kv8::split::launch<64, 4>(st, a, p.whole);
+    return p.nt == 1 ? kv8::split::launch<128, 1>(st, a, p.whole) : kv8::split::launch<128, 2>(st, a, p.whole);
   }
-  const kv8::tc::Plan p = kv8::tc::make_plan(B, n, Hq, H, D, weights != nullptr, sm_count());
+  const kv8::tc::Plan p = kv8::tc::make_plan(B, n, Hq, H, D, C, weights != nullptr, sm_count());
   const long long items = (p.rows + kv8::tc::ROWS - 1) / kv8::tc::ROWS;
   if (B > kv8::tc::MAXB || (long long)n * (Hq / H) > 0x3fffffffLL || B * items * H * (C / kv8::BLK) > 0x40000000LL)
     return set_error(E_SHAPE, "vt_attn_kv8: B=%d (at most %d) or B * H * n * C too large", B, kv8::tc::MAXB);
   char* w8 = static_cast<char*>(ws);
-  kv8::tc::Args a{q, sq_b, sq_t, sq_h, kc, vc, ks, vs, lens, counts, B, n, Hq / H, H, C, causal, p.rows, p.ctas, scale * kv8::LOG2E,
+  kv8::tc::Args a{q, sq_b, sq_t, sq_h, kc, vc, ks, vs, lens, counts, B, n, Hq / H, H, C, causal, p.rows, p.ctas,
+                  p.whole ? (int)items : 0, scale * kv8::LOG2E,
                   out, so_b, so_t, so_h, (float*)w8, (float2*)(w8 + p.ml_off), weights ? (float*)(w8 + p.lse_off) : nullptr,
                   weights, weights_in};
   return D == 64 ? kv8::tc::launch<64>(st, a) : kv8::tc::launch<128>(st, a);

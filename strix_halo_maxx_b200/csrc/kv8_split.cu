@@ -29,16 +29,22 @@ namespace vt {
 namespace kv8 {
 namespace split {
 
-constexpr int WARPS = 4, ST = 3;
+constexpr int ST = 3;
 constexpr int TILE = 4096;                         // bytes of K (or V) codes in a tile
 constexpr int RING = 2 * TILE * ST;                // a warp's ring
 constexpr int MAXB = 2048;                         // sequences a call takes (their tile counts sit in shared memory)
-constexpr int MIN_RUN = 4;                         // tiles of a CTA's run at least: one for each warp
+constexpr int WARPS = 4;                           // of a CTA with a run of tiles
+constexpr int MIN_RUN = WARPS;                     // tiles of a run at least
+// Where a head has at most so many tiles a CTA of eight warps takes a whole item: no parts, no second kernel, and the weights
+// come from the same CTA (32-token question over 730: 10.0 us, against 8.4 in runs and 5.1 to join; one token 6.4 against 5.1
+// and 4.7).
+constexpr int WHOLE_WARPS = 8, WHOLE_TILES = 16;
 constexpr long long kDrainCycles = 200000000LL;
 
 struct Plan {       // fixed on the host from sizes alone
   int rows, nt, rg;   // rows n G of a kv head, rows / 8 of a row group, row groups
   int ctas;
+  bool whole;         // a CTA for each item
   long long o_off, ml_off, full_off, s_off, bytes;  // workspace: partial O, their (m, l), (m, l) of every row, scores
 };
 
@@ -52,12 +58,13 @@ static Plan make_plan(int B, int n, int Hq, int H, int D, int C, bool weights, i
   p.nt = p.rows <= 8 ? 1 : (p.rows <= 16 || D == 128) ? 2 : 4;
   p.rg = (p.rows + 8 * p.nt - 1) / (8 * p.nt);
   p.ctas = 2 * sms;
+  p.whole = C / keys_per_tile(D) <= WHOLE_TILES && (p.rg == 1 || !weights);
   const long long slots = 2LL * p.ctas, gr = 8LL * p.nt;
   auto up = [](long long x) { return (x + 255) / 256 * 256; };
   p.o_off = 0;
-  p.ml_off = p.o_off + up(slots * gr * D * 4);
-  p.full_off = p.ml_off + up(slots * gr * 8);
-  p.s_off = p.full_off + up((long long)B * H * p.rg * gr * 8);
+  p.ml_off = p.o_off + (p.whole ? 0 : up(slots * gr * D * 4));
+  p.full_off = p.ml_off + (p.whole ? 0 : up(slots * gr * 8));
+  p.s_off = p.full_off + (p.whole ? 0 : up((long long)B * H * p.rg * gr * 8));
   p.bytes = p.s_off + (weights ? up((long long)B * H * p.rows * C * 4) : 0);
   return p;
 }
@@ -144,13 +151,14 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 }
 constexpr uint32_t H1152 = 0x64806480u;  // 1152 in both halves
 
-template <int D, int NT>
-__global__ void __launch_bounds__(WARPS * 32, 2) attn_kv8_split_kernel(Args a) {
+template <int D, int NT, bool WHOLE>
+__global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 : 2) attn_kv8_split_kernel(Args a) {
+  constexpr int WARPS = WHOLE ? WHOLE_WARPS : split::WARPS;
   constexpr int KT = TILE / D, GR = 8 * NT, WQ = D / 16, MT = KT / 16, OM = D / 16;
   extern __shared__ __align__(128) uint8_t sm[];
-  __shared__ int pre[MAXB + 1], warp_sum[WARPS];
+  __shared__ int pre[WHOLE ? 1 : MAXB + 1], warp_sum[WARPS];
   __shared__ __align__(8) uint64_t full[WARPS * ST];
-  __shared__ float sh_m[WARPS][GR], sh_l[WARPS][GR];
+  __shared__ float sh_m[WARPS][GR], sh_l[WARPS][GR], sh_lse[WHOLE ? GR : 1];
   __shared__ int sh_abort;
   volatile int* abort_flag = &sh_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -163,18 +171,26 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn_kv8_split_kernel(Args a) {
   }
   griddep_wait();  // programmatic dependent launch: the previous kernel has completed
   griddep_launch();
-  tile_list(a, KT, pre, warp_sum);  // its barriers also publish the mbarriers
-  const int total = pre[a.B], run = run_of(total, a.ctas);
-  const long long u_begin = (long long)blockIdx.x * run;
-  const int u_end = (int)min(u_begin + run, (long long)total);
+  long long u_begin = 0;
+  int total = 1, u_end = 1;  // this CTA's run of tiles (a whole item: one round)
+  if (WHOLE) {
+    __syncthreads();
+  } else {
+    tile_list(a, KT, pre, warp_sum);  // its barriers also publish the mbarriers
+    total = pre[a.B];
+    const int run = run_of(total, a.ctas);
+    u_begin = (long long)blockIdx.x * run;
+    u_end = (int)min(u_begin + run, (long long)total);
+  }
   int consumed = 0;  // tiles this warp has taken from its ring
   bool ok = true;
   for (int u = (int)min(u_begin, (long long)total); u < u_end;) {
-    const int b = find_seq(pre, a.B, u);
+    const int b = WHOLE ? blockIdx.x / (a.H * a.rg) : find_seq(pre, a.B, u);
     const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C);
     const int T = s.len + s.cnt, tiles = (T + KT - 1) / KT;
-    const int item = (u - pre[b]) / tiles, ta = (u - pre[b]) % tiles;
-    const int tb = min(tiles, ta + (u_end - u));  // this CTA's tiles of the item: [ta, tb)
+    const int item = WHOLE ? blockIdx.x % (a.H * a.rg) : (u - pre[b]) / tiles, ta = WHOLE ? 0 : (u - pre[b]) % tiles;
+    // this CTA's tiles of the item: [ta, tb)
+    const int tb = WHOLE ? (item % a.rg * GR < s.cnt * a.G ? tiles : 0) : min(tiles, ta + (u_end - u));
     const int h = item / a.rg, r0 = (item % a.rg) * GR;
     const size_t bh = (size_t)b * a.H + h;
     const int8_t *kp = a.kc + bh * a.C * D, *vp = a.vc + bh * a.C * D;
@@ -408,7 +424,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn_kv8_split_kernel(Args a) {
               make_float4(o[2 * w][nt][k], o[2 * w][nt][2 + k], o[2 * w + 1][nt][k], o[2 * w + 1][nt][2 + k]);
       }
     __syncthreads();
-    const bool whole = ta == 0 && tb == tiles;
+    const bool whole = WHOLE || (ta == 0 && tb == tiles);
     const int slot = 2 * blockIdx.x + (u == u_begin ? 0 : 1);  // of a part; a run has two at most: its first and its last
     for (int e = tid; e < GR * D / 4; e += WARPS * 32) {
       const int r = e / (D / 4), d = e % (D / 4) * 4, row = r0 + r;
@@ -429,11 +445,26 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn_kv8_split_kernel(Args a) {
         const float inv = 1.f / sum;
         uint16_t* op = a.out + b * a.so_b + row / a.G * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
         *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
-        if (d == 0 && a.w) a.full_ml[(bh * a.rg + item % a.rg) * GR + r] = make_float2(mx, sum);
+        if (d == 0 && a.w) {
+          if (WHOLE) sh_lse[r] = mx + log2f(sum);
+          else a.full_ml[(bh * a.rg + item % a.rg) * GR + r] = make_float2(mx, sum);
+        }
       } else {
         *reinterpret_cast<float4*>(a.part_o + ((size_t)slot * GR + r) * D + d) = v;
         if (d == 0) a.part_ml[(size_t)slot * GR + r] = make_float2(mx, sum);
       }
+    }
+    if (WHOLE) {
+      if (a.w) {  // one row group: the item's rows are all the rows of (b, h)
+        __syncthreads();
+        for (int j = tid; j < T; j += WARPS * 32) {
+          const size_t at = bh * a.C + j;
+          float acc = a.w_in && j < s.len ? a.w_in[at] : 0.f;
+          for (int r = 0; r < s.cnt * a.G; r++) acc += ex2_approx(a.scores[(bh * a.rows + r) * a.C + j] - sh_lse[r]);
+          a.w[at] = acc;
+        }
+      }
+      return;
     }
     fence_proxy_async_smem();  // these reads and writes come before the next item's copies into the rings
     __syncthreads();
@@ -528,11 +559,19 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
 }
 
 template <int D, int NT>
-static int launch(cudaStream_t st, const Args& a) {
-  constexpr int SMEM = WARPS * RING, ROWS = 128 * 4 / D;
-  const int rc = smem_attr_once((const void*)attn_kv8_split_kernel<D, NT>, SMEM, "vt_attn_kv8");
+static int launch(cudaStream_t st, const Args& a, bool whole) {
+  constexpr int ROWS = 128 * 4 / D;
+  if (whole) {
+    constexpr int SMEM = WHOLE_WARPS * RING;
+    const int rc = smem_attr_once((const void*)attn_kv8_split_kernel<D, NT, true>, SMEM, "vt_attn_kv8");
+    if (rc) return rc;
+    launch_k(attn_kv8_split_kernel<D, NT, true>, (unsigned)(a.B * a.H * a.rg), WHOLE_WARPS * 32, SMEM, st, a);
+    return check_launch("vt_attn_kv8");
+  }
+  constexpr int SMEM = WARPS * RING;
+  const int rc = smem_attr_once((const void*)attn_kv8_split_kernel<D, NT, false>, SMEM, "vt_attn_kv8");
   if (rc) return rc;
-  launch_k(attn_kv8_split_kernel<D, NT>, a.ctas, WARPS * 32, SMEM, st, a);
+  launch_k(attn_kv8_split_kernel<D, NT, false>, a.ctas, WARPS * 32, SMEM, st, a);
   const int rows = 8 * NT < a.rows ? 8 * NT : a.rows;
   const int merge = a.B * a.H * a.rg * ((rows + ROWS - 1) / ROWS);
   const int chunks = a.w ? a.B * a.H * ((a.C + 511) / 512) : 0;

@@ -30,7 +30,9 @@ constexpr long long kDrainCycles = 200000000LL;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr int SOFTMAX_REGS = 168, CONVERT_REGS = 96, MMA_REGS = 80;
 constexpr float kTinyScale = 0x1p-100f;
-constexpr int WHOLE_TILES = 24;  // items of up to so many tiles stay whole when there are fewer of them than SMs
+// With caches of up to so many blocks a CTA takes a whole item: equal runs for all SMs would cost more in parts to write and
+// join than they gain (the 730-token prefix, 96 items of 12 tiles: 20.5 us whole, 24.8 in runs and 12.4 to join them).
+constexpr int WHOLE_TILES = 24;
 
 template <int D>
 struct Smem {
@@ -46,6 +48,7 @@ struct Args {
   const float *ks, *vs;
   const int *lens, *counts;
   int B, n, G, H, C, causal, rows, ctas;
+  int items;  // > 0: items of a head, and a CTA for each item (no runs, nothing to join)
   float scale_log2;
   uint16_t* out;
   long long so_b, so_t, so_h;
@@ -58,15 +61,17 @@ struct Args {
 
 struct Plan {
   int rows, ctas;
+  bool whole;  // a CTA for each item
   long long ml_off, lse_off, bytes;
 };
-static Plan make_plan(int B, int n, int Hq, int H, int D, bool weights, int sms) {
+static Plan make_plan(int B, int n, int Hq, int H, int D, int C, bool weights, int sms) {
   Plan p;
+  p.whole = C / BLK <= WHOLE_TILES;
   p.rows = n * (Hq / H);
   p.ctas = sms;
   auto up = [](long long x) { return (x + 255) / 256 * 256; };
-  p.ml_off = up(2LL * sms * ROWS * D * 4);
-  p.lse_off = p.ml_off + up(2LL * sms * ROWS * 8);
+  p.ml_off = p.whole ? 0 : up(2LL * sms * ROWS * D * 4);
+  p.lse_off = p.ml_off + (p.whole ? 0 : up(2LL * sms * ROWS * 8));
   p.bytes = p.lse_off + (weights ? up((long long)B * H * p.rows * 4) : 0);
   return p;
 }
@@ -80,11 +85,9 @@ __device__ __forceinline__ int seq_items(const Args& a, const Seq& s) { return (
 
 // The list of all tiles, sequence by sequence, head by head, item by item: pre[b] first tile of sequence b; and the run.
 __device__ __forceinline__ int tile_list(const Args& a, int* pre, int* scratch) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x / 32;
-  if (tid == 0) scratch[nw] = 0;
-  __syncthreads();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.B + (int)blockDim.x - 1) / (int)blockDim.x, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
-  int sum = 0, most = 0;
+  int sum = 0;
   for (int b = b0; b < b1; b++) {
     Seq s;
     s.len = min(max(a.lens[b], 0), a.C);
@@ -95,7 +98,6 @@ __device__ __forceinline__ int tile_list(const Args& a, int* pre, int* scratch) 
       for (int q = 0; q < items; q++) t += item_tiles(a, s, q);
     else if (items)
       t = items * item_tiles(a, s, 0);
-    if (items) most = max(most, item_tiles(a, s, items - 1));
     pre[b] = t * a.H;
     sum += t * a.H;
   }
@@ -105,9 +107,7 @@ __device__ __forceinline__ int tile_list(const Args& a, int* pre, int* scratch) 
     const int y = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += y;
   }
-  most = __reduce_max_sync(0xffffffffu, most);
   if (lane == 31) scratch[warp] = inc;
-  if (lane == 0) atomicMax(&scratch[nw], most);
   __syncthreads();
   int at = inc - sum;
   for (int i = 0; i < warp; i++) at += scratch[i];
@@ -119,8 +119,7 @@ __device__ __forceinline__ int tile_list(const Args& a, int* pre, int* scratch) 
   if (tid == (int)blockDim.x - 1) pre[a.B] = at;
   __syncthreads();
   const int run = max((pre[a.B] + a.ctas - 1) / a.ctas, 1);
-  // fewer tiles for each CTA than the largest item has, and not many: whole items, no parts to join
-  return run < scratch[nw] && scratch[nw] <= WHOLE_TILES ? scratch[nw] : run;
+  return run;
 }
 
 // A CTA's share of one item: rows r0 .. of (b, h), key tiles [ta, tb) of `tiles`.
@@ -130,6 +129,13 @@ struct Seg {
 };
 __device__ __forceinline__ Seg segment(const Args& a, const int* pre, int u, int u_end) {
   Seg g;
+  if (a.items > 0) {  // CTA = item
+    const int bh = blockIdx.x / a.items, qt = blockIdx.x % a.items;
+    g.b = bh / a.H, g.h = bh % a.H, g.r0 = qt * ROWS, g.ta = 0;
+    g.s = seq_of(a.lens, a.counts, g.b, a.n, a.C);
+    g.tb = g.tiles = g.r0 < g.s.cnt * a.G ? item_tiles(a, g.s, qt) : 0;
+    return g;
+  }
   g.b = split::find_seq(pre, a.B, u);
   g.s = seq_of(a.lens, a.counts, g.b, a.n, a.C);
   const int head = (pre[g.b + 1] - pre[g.b]) / a.H;  // tiles of one head
@@ -167,7 +173,7 @@ template <int D>
 __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
   using L = Smem<D>;
   extern __shared__ __align__(1024) uint8_t sm[];
-  __shared__ int pre[MAXB + 1], scratch[THREADS / 32 + 1];
+  __shared__ int pre[MAXB + 1], scratch[THREADS / 32];
   __shared__ __align__(8) uint64_t bars[2 + 2 * ST + 4 + 4 + 4 + 2];
   __shared__ uint32_t tmem_slot;
   __shared__ int sh_abort;
@@ -196,9 +202,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
   const uint32_t tmem = tmem_slot;
   griddep_wait();  // programmatic dependent launch: the previous kernel has completed
   griddep_launch();
-  const int run = tile_list(a, pre, scratch), total = pre[a.B];
-  const int u_begin = (int)min((long long)blockIdx.x * run, (long long)total);
-  const int u_end = (int)min((long long)u_begin + run, (long long)total);
+  int u_begin = 0, u_end;  // this CTA's run of tiles
+  if (a.items > 0) {
+    u_end = segment(a, pre, 0, 0).tiles;
+  } else {
+    const int run = tile_list(a, pre, scratch), total = pre[a.B];
+    u_begin = (int)min((long long)blockIdx.x * run, (long long)total);
+    u_end = (int)min((long long)u_begin + run, (long long)total);
+  }
   // a wait of the whole warp: every lane gives up when one does
   auto wait = [&](uint64_t* bar, int parity) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, ST_KV8_WAIT)) != 0;
@@ -527,7 +538,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
 // in c's run; blockIdx.y: 16 of its rows; thread = 4 dims of a row.
 template <int D>
 __global__ void __launch_bounds__(128) attn_kv8_tc_join_kernel(Args a) {
-  __shared__ int pre[MAXB + 1], scratch[5];
+  __shared__ int pre[MAXB + 1], scratch[4];
   constexpr int PER = 128 * 4 / D;
   griddep_wait();
   griddep_launch();
@@ -576,7 +587,7 @@ struct WSmem {
   static constexpr int K = 0, Q = WK * D * 2, QT = WR * D * 2, BYTES = Q + 2 * QT;
 };
 template <int D>
-__global__ void __launch_bounds__(WTHREADS, 1) kv8_weights_tc_kernel(Args a) {
+__global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
   using L = WSmem<D>;
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ __align__(16) float sh_lse[2][WR], half_sum[WK];
@@ -612,27 +623,46 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv8_weights_tc_kernel(Args a) {
   const uint32_t tmem = tmem_slot;
   float acc = 0.f;
   bool ok = true;
+  // a wait of the whole warp: every lane gives up when one does
+  auto wait = [&](uint64_t* bar, int parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, ST_KV8_WAIT)) != 0;
+  };
   if (warp == 12) {
-    if (lane == 0) {
-      const uint32_t sk = smem_u32(sm + L::K), sq = smem_u32(sm + L::Q);
-      for (int i = 0; i < nt && ok; i++) {
-        const int f = i & 1;
-        ok = mbar_wait(&q_full[f], (i >> 1) & 1, abort_flag, ST_KV8_WAIT) &&
-             (i < 2 || mbar_wait(&s_empty[f], ((i >> 1) - 1) & 1, abort_flag, ST_KV8_WAIT));
-        if (!ok) break;
-        tc_fence_after();
+    const uint32_t leader = elect_one();
+    const uint64_t dk = sdesc_noswz(smem_u32(sm + L::K), 2048, 128), dq = sdesc_noswz(smem_u32(sm + L::Q), 2048, 128);
+    for (int i = 0; i < nt; i++) {
+      const int f = i & 1;
+      ok = wait(&q_full[f], (i >> 1) & 1) && (i < 2 || wait(&s_empty[f], ((i >> 1) - 1) & 1));
+      if (!ok) break;
+      tc_fence_after();
+      if (leader) {
 #pragma unroll
         for (int k = 0; k < D / 16; k++)
-          umma_f16(tmem + 128 * f, sdesc_noswz(sk + k * 4096, 2048, 128), sdesc_noswz(sq + f * L::QT + k * 4096, 2048, 128),
-                   idesc_bf16(WK, WR), k > 0 ? 1u : 0u);
+          umma_f16(tmem + 128 * f, dk + k * (4096 >> 4), dq + f * (L::QT >> 4) + k * (4096 >> 4), idesc_bf16(WK, WR), k > 0 ? 1u : 0u);
         umma_commit(&s_full[f]);
       }
+      __syncwarp();
+    }
+    if (leader) {
       umma_commit(drain);
       mbar_wait_drain(drain, 0, kDrainCycles);
     }
   } else if (warp >= 8) {
     const int w = warp - 8, ct = tid - 256;
     const int8_t* kp = a.kc + bh * a.C * D;
+    // thread = row of the row tile: its q on its way a tile ahead
+    float lse;
+    auto fetch = [&](int i) {
+      const int f = i & 1, r = (first + i) * WR + ct;
+      const uint16_t* src = q_row(a, b, h, min(r, rows - 1));
+      const uint32_t dst = smem_u32(sm + L::Q + f * L::QT + ct * 16);
+#pragma unroll
+      for (int c = 0; c < D / 8; c++)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c * WR * 16), "l"(src + 8 * c) : "memory");
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      lse = r < rows ? a.lse[bh * a.rows + r] : INFINITY;  // rows past the last add 2^-inf
+    };
+    if (nt > 0) fetch(0);
     for (int x = 0; x < 4 * (D / 64); x++) {  // warp w rows 32 w ..; slots behind the cache's last one are zero
       const int row = 32 * w + 8 * (x & 3) + (lane & 7), p = (lane >> 3) + 4 * (x >> 2);
       uint4 c = make_uint4(0, 0, 0, 0);
@@ -640,21 +670,22 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv8_weights_tc_kernel(Args a) {
       store_codes<WK>(sm + L::K, row, p, c);
     }
     for (int i = 0; i < nt; i++) {
-      const int f = i & 1, r0 = (first + i) * WR;
-      // the stage is free when both halves have read its lse, which comes after its products
-      if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[f], ((i >> 1) - 1) & 1, abort_flag, ST_KV8_WAIT));
-      if (!ok) break;
-      for (int e = ct; e < WR * D / 8; e += 128) {
-        const int r = e % WR, c = e / WR;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r0 + r < rows) v = *reinterpret_cast<const uint4*>(q_row(a, b, h, r0 + r) + 8 * c);
-        *reinterpret_cast<uint4*>(sm + L::Q + f * L::QT + (c * WR + r) * 16) = v;
+      const int f = i & 1;
+      sh_lse[f][ct] = lse;
+      if (i + 1 < nt) {
+        // the stage is free when both halves have read its lse, which comes after its products
+        if (i >= 1) ok = wait(&q_empty[f ^ 1], ((i - 1) >> 1) & 1);
+        if (!ok) break;
+        fetch(i + 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      } else {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
       }
-      sh_lse[f][ct] = r0 + ct < rows ? a.lse[bh * a.rows + r0 + ct] : INFINITY;  // rows past the last add 2^-inf
       fence_proxy_async_smem();
       __syncwarp();
       mbar_arrive_if(&q_full[f], lane == 0);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     const int half = warp >> 2, key = key0 + (warp & 3) * 32 + lane;
     const uint32_t t_s = tmem + 64 * half + ((uint32_t)((warp & 3) * 32) << 16);
@@ -662,24 +693,24 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv8_weights_tc_kernel(Args a) {
     const int r_min = a.causal ? (key - s.len) * a.G : 0;  // rows before it do not see this key
     const int warp_max = __reduce_max_sync(0xffffffffu, r_min);
     unsigned long long acc2[2] = {0ull, 0ull};
+    const unsigned long long c2 = f2_pack(c, c), minus = f2_pack(-1.f, -1.f);
     for (int i = 0; i < nt; i++) {
-      const int f = i & 1, r0 = (first + i) * WR + 64 * half;
-      ok = __all_sync(0xffffffffu, mbar_wait(&q_full[f], (i >> 1) & 1, abort_flag, ST_KV8_WAIT) &&  // lse
-                                       mbar_wait(&s_full[f], (i >> 1) & 1, abort_flag, ST_KV8_WAIT));
+      const int f = i & 1;
+      ok = wait(&q_full[f], (i >> 1) & 1) && wait(&s_full[f], (i >> 1) & 1);  // lse, scores
       if (!ok) break;
       tc_fence_after();
-      uint32_t x0[32], x1[32];
-      tmem_ld32(t_s + 128 * f, x0);
-      tmem_ld32(t_s + 128 * f + 32, x1);
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      mbar_arrive_if(&s_empty[f], lane == 0);
-      const bool edge = r0 < warp_max;
-      const unsigned long long c2 = f2_pack(c, c), minus = f2_pack(-1.f, -1.f);
 #pragma unroll
       for (int hf = 0; hf < 2; hf++) {
-        const uint32_t* x = hf ? x1 : x0;
+        uint32_t x[32];
+        tmem_ld32(t_s + 128 * f + 32 * hf, x);
+        tmem_ld_wait();
+        if (hf == 1) {
+          tc_fence_before();
+          __syncwarp();
+          mbar_arrive_if(&s_empty[f], lane == 0);
+        }
+        const int r0 = (first + i) * WR + 64 * half + 32 * hf;
+        const bool edge = r0 < warp_max;
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           const float4 z = *reinterpret_cast<const float4*>(&sh_lse[f][64 * half + 32 * hf + e]);
@@ -691,8 +722,8 @@ __global__ void __launch_bounds__(WTHREADS, 1) kv8_weights_tc_kernel(Args a) {
             f2_unpack(y, y0, y1);
             y0 = ex2_approx(y0), y1 = ex2_approx(y1);
             if (edge) {
-              if (r0 + 32 * hf + e + 2 * k < r_min) y0 = 0.f;
-              if (r0 + 32 * hf + e + 2 * k + 1 < r_min) y1 = 0.f;
+              if (r0 + e + 2 * k < r_min) y0 = 0.f;
+              if (r0 + e + 2 * k + 1 < r_min) y1 = 0.f;
             }
             acc2[k] = f2_add(acc2[k], f2_pack(y0, y1));
           }
@@ -727,8 +758,12 @@ static int launch(cudaStream_t st, const Args& a) {
   int rc = smem_attr_once((const void*)attn_kv8_tc_kernel<D>, Smem<D>::BYTES, "vt_attn_kv8");
   if (!rc) rc = smem_attr_once((const void*)kv8_weights_tc_kernel<D>, WSmem<D>::BYTES, "vt_attn_kv8");
   if (rc) return rc;
-  launch_k(attn_kv8_tc_kernel<D>, a.ctas, THREADS, Smem<D>::BYTES, st, a);
-  launch_k(attn_kv8_tc_join_kernel<D>, dim3(a.ctas, ROWS / 16), 128, 0, st, a);
+  if (a.items > 0) {
+    launch_k(attn_kv8_tc_kernel<D>, (unsigned)(a.B * a.H * a.items), THREADS, Smem<D>::BYTES, st, a);
+  } else {
+    launch_k(attn_kv8_tc_kernel<D>, a.ctas, THREADS, Smem<D>::BYTES, st, a);
+    launch_k(attn_kv8_tc_join_kernel<D>, dim3(a.ctas, ROWS / 16), 128, 0, st, a);
+  }
   if (a.w) launch_k(kv8_weights_tc_kernel<D>, (unsigned)(a.B * a.H * ((a.C + WK - 1) / WK)), WTHREADS, WSmem<D>::BYTES, st, a);
   return check_launch("vt_attn_kv8");
 }

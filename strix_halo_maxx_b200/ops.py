@@ -521,7 +521,7 @@ def rope_kv8(qkv, cache, lens, cos_t, sin_t, q, pos=None, counts=None):
 
 def attn_kv8_workspace(B, n, Hq, H, D, C, device, weights=False):
     """A workspace for attn_kv8 calls of these sizes, one call at a time (vt_attn_kv8_ws_bytes)."""
-    return torch.empty(max(lib().vt_attn_kv8_ws_bytes(B, n, Hq, H, D, C, int(weights)), 16), dtype=torch.uint8, device=device)
+    return torch.empty(lib().vt_attn_kv8_ws_bytes(B, n, Hq, H, D, C, int(weights)), dtype=torch.uint8, device=device)
 
 
 def attn_kv8(q, cache, lens, out=None, counts=None, causal=True, scale=None, weights=None, weights_in=None, ws=None):
@@ -539,7 +539,9 @@ def attn_kv8(q, cache, lens, out=None, counts=None, causal=True, scale=None, wei
             out.get_device() != dev or sq[3] != 1 or so[2] != 1:
         _kv8_fail(what, f"q {tuple(q.shape)}, out {tuple(out.shape)} for a cache of B={B} H={H} D={D} (bf16, contiguous rows)")
     if ws is None:
-        ws = attn_kv8_workspace(B, n, Hq, H, D, C, q.device, weights is not None)
+        nb = lib().vt_attn_kv8_ws_bytes(B, n, Hq, H, D, C, 0 if weights is None else 1)
+        if nb:  # held until the call is on the stream; its memory is reused on this stream only
+            ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
     elif ws.get_device() != dev or not ws.is_contiguous():
         _kv8_fail(what, "the workspace must be contiguous on the tensors' device")
     _kv8_call(lib().vt_attn_kv8, "vt_attn_kv8", dev, q.data_ptr(), sq[0], sq[1], sq[2],
@@ -549,7 +551,7 @@ def attn_kv8(q, cache, lens, out=None, counts=None, causal=True, scale=None, wei
               int(bool(causal)), D ** -0.5 if scale is None else float(scale), out.data_ptr(), so[0], so[1], D,
               None if weights is None else _kv8_vec(what, "weights", weights, (B, H, C), torch.float32, dev),
               None if weights_in is None else _kv8_vec(what, "weights_in", weights_in, (B, H, C), torch.float32, dev),
-              ws.data_ptr(), ws.nbytes)
+              None if ws is None else ws.data_ptr(), 0 if ws is None else ws.nbytes)
     return out
 
 
