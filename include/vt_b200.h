@@ -296,7 +296,8 @@ int vt_attn_causal(cudaStream_t stream, const uint16_t* q, const uint16_t* kc, c
  * takes the scale max|x| / 127 of its new ones; a block that holds tokens keeps its scale, doubled as often as the
  * new ones need, its codes halved as often (rint): a value is then at most one step off however it arrived, half a
  * step when its block was written in one call.  A NaN or an infinity makes its block's scale NaN.  A call may be
- * repeated from the same lens (a question asked again over the same prefix). */
+ * repeated from the same lens (a question asked again over the same prefix); with other tokens, the block that holds
+ * tokens before lens keeps the larger of the scales it had. */
 int vt_rope_kv8(cudaStream_t stream, const uint16_t* qkv, long long sx_b, long long sx_t, int B, int n, int Hq, int H,
                 int D, const float* cos_t, const float* sin_t, int tab, const int* lens, const int* pos,
                 const int* counts, uint16_t* q, long long sq_b, long long sq_t, long long sq_h, int8_t* kc, int8_t* vc,
@@ -308,7 +309,7 @@ long long vt_attn_kv8_ws_bytes(int B, int n, int Hq, int H, int D, int C, int we
 
 /* Attention of the n new rows of each sequence over its cache, their own tokens already in it: row i of sequence b
  * sees slots 0 .. lens[b] + i (causal != 0) or 0 .. lens[b] + counts[b] - 1; softmax(scale q k^T) v, sums in fp32, out
- * bf16 at out + b*so_b + i*so_t + hq*so_h.  weights fp32 [B][H][C] (NULL: none) receives the attention weight of each
+ * bf16 at out + b*so_b + i*so_t + hq*so_h (not over q).  V scales of 2^-100 .. 2^100.  weights fp32 [B][H][C] (NULL: none) receives the attention weight of each
  * slot j < lens[b] + counts[b]: its probabilities summed over the sequence's rows and the group's query heads, plus
  * weights_in[b][h][j] (NULL: none; may be weights) for j < lens[b].  ws: vt_attn_kv8_ws_bytes bytes, 16-byte
  * aligned, one call at a time.  Results do not depend on the other sequences of the batch beyond the rounding of

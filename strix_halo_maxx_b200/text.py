@@ -17,6 +17,11 @@ LayerNorm kernel (vt_layernorm_quant), and shared by qkv and fc1 (md2fast.py:174
 fc1 output (GELU fused into its epilogue) are quantised before proj and fc2 (vt_quant_rows + vt_gemm_i8,
 ops.I8Lin).  The KV caches ([layers][H][762][64]
 bf16) live on the device, owned by this object: encode() fills positions 0 .. 729, query() 730 .. 761.
+
+kv8=True holds the caches in 8 bits with a scale per 64 tokens and head (ops.Kv8: half the bytes): vt_rope_kv8 writes
+them and vt_attn_kv8 reads them, for the prefix (no mask) and for the question (causal).  keep=N then evicts: each
+head of each layer keeps the N image-prefix tokens that the prefix's own attention weighed most (the last keep_recent
+among them in any case), and questions attend to those; their positions go on at 730.
 """
 import torch
 
@@ -36,10 +41,16 @@ def rope_tables(cfg: TextConfig, device):
 
 
 class TextDecoder:
-    def __init__(self, weights, cfg: TextConfig = TEXT, device="cuda", graphs=True, int8=False):
+    def __init__(self, weights, cfg: TextConfig = TEXT, device="cuda", graphs=True, int8=False, kv8=False, keep=None,
+                 keep_recent=32):
+        if keep is not None and (not kv8 or keep <= 0 or keep % ops.KV8_BLOCK or keep >= cfg.prefix or
+                                 not 0 <= keep_recent <= keep):
+            raise ValueError(f"keep={keep}: needs kv8, a multiple of {ops.KV8_BLOCK} below the prefix of {cfg.prefix} tokens, "
+                             f"and 0 <= keep_recent={keep_recent} <= keep")
         self.cfg = cfg
         self.use_graphs = graphs
         self.int8 = int8
+        self.kv8, self.keep, self.keep_recent = kv8, keep, keep_recent
         self._qgraph = self._egraph = None
         dev = self.dev = torch.device(device)
         if dev.type == "cuda" and dev.index is None:
@@ -69,8 +80,11 @@ class TextDecoder:
         self.qflat = torch.empty(H * P * hd, dtype=BF16, device=dev)
         self.a = torch.empty(P, D, dtype=BF16, device=dev)
         self.f = torch.empty(P, cfg.ff, dtype=BF16, device=dev)
-        self.kc = torch.zeros(self.n_layers, H, cfg.ctx, hd, dtype=BF16, device=dev)
-        self.vc = torch.zeros(self.n_layers, H, cfg.ctx, hd, dtype=BF16, device=dev)
+        if kv8:
+            self._init_kv8(dev)
+        else:
+            self.kc = torch.zeros(self.n_layers, H, cfg.ctx, hd, dtype=BF16, device=dev)
+            self.vc = torch.zeros(self.n_layers, H, cfg.ctx, hd, dtype=BF16, device=dev)
         self.hl = torch.empty(1, D, dtype=BF16, device=dev)
         self.xl = torch.empty(1, D, dtype=F32, device=dev)
         self._ids = torch.zeros(cfg.q_len, dtype=torch.int64, device=dev)
@@ -88,6 +102,38 @@ class TextDecoder:
         # split-K workspace of the question's GEMMs (32 rows; the widest output is fc1's)
         self.ws = ops.gemm_workspace(cfg.q_len, max(3 * D, cfg.ff), dev)
 
+    def _init_kv8(self, dev):
+        """The layers' 8-bit caches: the layers are the batch of one eviction call, each alone a batch of one sequence."""
+        cfg, L = self.cfg, self.n_layers
+        H, hd, P = cfg.heads, cfg.head_dim, cfg.prefix
+        i32 = lambda x, n: torch.full((n,), x, dtype=torch.int32, device=dev)
+        self.kv = self.kv_q = ops.kv8_cache(L, H, cfg.ctx, hd, dev)  # the prefix's, the question's
+        self.len_0, self.len_p = i32(0, 1), i32(P, L)
+        self.len_q = self.len_p                                      # tokens before the question
+        if self.keep is not None:
+            self.kv_q = ops.kv8_cache(L, H, self.keep + cfg.q_len, hd, dev)
+            self.len_q = i32(0, L)
+            self.attn_w = torch.zeros(L, H, self.kv.k.shape[2], device=dev)
+            self.attn_w_q = torch.zeros(L, H, self.kv_q.k.shape[2], device=dev)
+            self.kept = torch.zeros(L, H, self.keep, dtype=torch.int32, device=dev)
+        # The prefix ends inside a block, whose scale a question's tokens may double for good: its codes and scales are put back
+        # before each question, so that no answer depends on the questions before it
+        b = P // ops.KV8_BLOCK
+        self.tail = [t[:, :, b * ops.KV8_BLOCK:P] for t in (self.kv.k, self.kv.v)] + [t[:, :, b] for t in (self.kv.ks, self.kv.vs)] \
+            if self.keep is None and P % ops.KV8_BLOCK else []
+        self.tail_saved = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in self.tail]
+        self.ws8 = ops.attn_kv8_workspace(1, P, H, H, hd, self.kv.k.shape[2], dev, self.keep is not None)
+
+    def _attend_kv8(self, i, qkv, n, full, a):
+        """Rotary, cache write and attention of layer i's n new tokens on the 8-bit cache, into a [n, D]."""
+        cfg = self.cfg
+        cache = ops.Kv8(*(t[i:i + 1] for t in (self.kv if full else self.kv_q)))
+        lens = self.len_0 if full else self.len_q[i:i + 1]
+        q = self.qflat[:n * cfg.dim].view(1, n, cfg.heads, cfg.head_dim)
+        ops.rope_kv8(qkv[None], cache, lens, self.cos, self.sin, q, pos=self.len_0 if full else self.len_p[i:i + 1])
+        w = self.attn_w[i:i + 1] if full and self.keep is not None else None
+        ops.attn_kv8(q, cache, lens, a[None], causal=not full, weights=w, ws=self.ws8)
+
     def _layers(self, n, pos0, full):
         cfg = self.cfg
         D, H, hd, Fh = cfg.dim, cfg.heads, cfg.head_dim, cfg.ff
@@ -99,14 +145,20 @@ class TextDecoder:
         for i, b in enumerate(self.layers):
             ops.layer_norm(x, b["ln_w"], b["ln_b"], cfg.eps, out=h)
             ops.gemm(h, b["qkv_w"], b["qkv_ld"], D, 3 * D, b["qkv_b"], out=qkv, ws=ws)
-            ops.rope_qkv(qkv, pos0, self.cos, self.sin, q, self.kc[i], self.vc[i])
-            if full:  # the prefix: no mask, its own n keys (md2fast.py:182-183)
-                self.attn(q[None], self.kc[i][None, :, pos0:pos0 + n], self.vc[i][None, :, pos0:pos0 + n], out=a[None])
-            else:     # the question: causal over the cache (md2fast.py:184-185 with the query mask)
-                ops.attn_causal(q, self.kc[i], self.vc[i], pos0, a)
+            self._attend(i, qkv, q, n, pos0, full, a)
             ops.gemm(a, b["proj_w"], b["proj_ld"], D, D, b["proj_b"], res=x, out=x, ws=ws)
             ops.gemm(h, b["fc1_w"], b["fc1_ld"], D, Fh, b["fc1_b"], gelu=True, out=f, ws=ws)
             ops.gemm(f, b["fc2_w"], b["fc2_ld"], Fh, D, b["fc2_b"], res=x, out=x, ws=ws)
+
+    def _attend(self, i, qkv, q, n, pos0, full, a):
+        """Rotary, cache write and attention of layer i's n new tokens at pos0 .., into a [n, D]."""
+        if self.kv8:
+            return self._attend_kv8(i, qkv, n, full, a)
+        ops.rope_qkv(qkv, pos0, self.cos, self.sin, q, self.kc[i], self.vc[i])
+        if full:  # the prefix: no mask, its own n keys (md2fast.py:182-183)
+            self.attn(q[None], self.kc[i][None, :, pos0:pos0 + n], self.vc[i][None, :, pos0:pos0 + n], out=a[None])
+        else:     # the question: causal over the cache (md2fast.py:184-185 with the query mask)
+            ops.attn_causal(q, self.kc[i], self.vc[i], pos0, a)
 
     def _layers_i8(self, n, pos0, full, q, ws):
         """The same layers with the W8A8 linears (HI8Lin, md2fast.py:169-199 with SHARE_QUANT)."""
@@ -118,11 +170,7 @@ class TextDecoder:
             # LN + per-token quantisation in one kernel; the int8 rows are shared by qkv and fc1 (md2fast.py:174)
             pre = ops.layer_norm_quant(x, b["ln_w"], b["ln_b"], cfg.eps, hq, hs)
             b["qkv"](h, pre=pre, out=qkv, ws=ws)
-            ops.rope_qkv(qkv, pos0, self.cos, self.sin, q, self.kc[i], self.vc[i])
-            if full:
-                self.attn(q[None], self.kc[i][None, :, pos0:pos0 + n], self.vc[i][None, :, pos0:pos0 + n], out=a[None])
-            else:
-                ops.attn_causal(q, self.kc[i], self.vc[i], pos0, a)
+            self._attend(i, qkv, q, n, pos0, full, a)
             b["proj"](a, pre=b["proj"].quant(a, aq, as_), res=x, out=x, ws=ws)
             b["fc1"](h, gelu=True, pre=pre, out=f, ws=ws)
             b["fc2"](f, pre=b["fc2"].quant(f, fq, fs), res=x, out=x, ws=ws)
@@ -148,6 +196,12 @@ class TextDecoder:
         torch.index_select(self.wte, 0, self._bos, out=self.x[:1])
         self.x[1:self.cfg.prefix].copy_(self._emb)
         self._layers(self.cfg.prefix, 0, True)
+        if self.keep is not None:
+            ops.kv8_evict(self.kv, self.attn_w, self.len_p, self.keep, self.keep_recent, self.kv_q, self.attn_w_q,
+                          self.len_q, index=self.kept)
+        if self.kv8:
+            for t, saved in zip(self.tail, self.tail_saved):
+                saved.copy_(t)
 
     def query(self, ids, last):
         """Question prefill (md2fast.py:208-212): ids [q_len] int64 on the device, `last` the index of the
@@ -171,6 +225,9 @@ class TextDecoder:
     def _query(self):
         cfg = self.cfg
         torch.index_select(self.wte, 0, self._ids, out=self.x[:cfg.q_len])
+        if self.kv8:
+            for t, saved in zip(self.tail, self.tail_saved):
+                t.copy_(saved)
         self._layers(cfg.q_len, cfg.prefix, False)
         torch.index_select(self.x, 0, self._last, out=self.xl)
         ops.layer_norm(self.xl, self.post_w, self.post_b, cfg.eps, out=self.hl)
@@ -235,7 +292,7 @@ def op_times(dev, n=20, reps=5):
 
 
 def main(argv=None):
-    """python -m strix_halo_maxx_b200.text [--int8] [--bf16] [--reps N] [--eager] [--layers L] [--ops]: the decoder on
+    """python -m strix_halo_maxx_b200.text [--int8] [--bf16] [--kv8 [--keep N]] [--reps N] [--eager] [--layers L] [--ops]: the decoder on
     device-random weights (weights.text_weights_device); prints the mean prefill / question ms of each
     selected variant (both by default).  With --reps 0 it runs one eager prefill and one question per variant
     and prints nothing else: the command to put under a profiler's launch list."""
@@ -244,6 +301,8 @@ def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("--int8", action="store_true")
     ap.add_argument("--bf16", action="store_true")
+    ap.add_argument("--kv8", action="store_true", help="the KV cache in 8 bits")
+    ap.add_argument("--keep", type=int, default=None, help="with --kv8: image-prefix tokens a head keeps for the questions")
     ap.add_argument("--reps", type=int, default=20)
     ap.add_argument("--eager", action="store_true", help="no CUDA-graph replay")
     ap.add_argument("--layers", type=int, default=None, help="fewer layers than the model's 24 (small profiles)")
@@ -260,7 +319,8 @@ def main(argv=None):
     emb = torch.randn(TEXT.prefix - 1, TEXT.dim, device=dev, generator=g)
     ids = torch.randint(1, TEXT.vocab, (TEXT.q_len,), device=dev, generator=g)
     for v in variants:
-        dec = TextDecoder(W, TEXT, device=dev, graphs=not a.eager and a.reps > 0, int8=(v == "int8"))
+        dec = TextDecoder(W, TEXT, device=dev, graphs=not a.eager and a.reps > 0, int8=(v == "int8"), kv8=a.kv8,
+                          keep=a.keep)
         res = {}
         for name, fn in (("prefill_ms", lambda: dec.encode(emb, 0)), ("question_ms", lambda: dec.query(ids, TEXT.q_len - 1))):
             if a.reps <= 0:
@@ -278,7 +338,7 @@ def main(argv=None):
             res[name] = round(e0.elapsed_time(e1) / a.reps, 4)
         torch.cuda.synchronize()
         if res:
-            print(v, res, flush=True)
+            print(v + ("_kv8" if a.kv8 else ""), res, flush=True)
         del dec
 
 
