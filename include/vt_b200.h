@@ -287,7 +287,8 @@ int vt_attn_causal(cudaStream_t stream, const uint16_t* q, const uint16_t* kc, c
  * read into a result, and left as they were in every output.  Lengths on the device cannot be refused by the host: a
  * negative one, a count outside 0 .. n, tokens past C and positions past the rotary table are clamped and set bit 9
  * of the status word (vt_device_status).  Query head hq reads head hq / (Hq / H).  The reference has a bf16 cache only
- * (moondream/gpu/md2fast.py:186-191); these stand beside vt_rope_qkv and vt_attn_causal. */
+ * (moondream/gpu/md2fast.py:186-191); these stand beside vt_rope_qkv and vt_attn_causal.
+ * Limits: vt_attn_kv8 B <= 2048, 0 <= scale < 2^100; vt_kv8_evict C <= 262144. */
 
 /* Rotary embedding (vt_rope_qkv's: the first 32 dims of each q / k head) and quantised cache write of n new tokens for
  * each of B sequences: qkv bf16, row (b, i) at qkv + b*sx_b + i*sx_t = q [Hq][D] | k [H][D] | v [H][D]; cos_t / sin_t

@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(128) rope_kv8_kernel(AppendArgs a) {
       const int i = (int)(row % a.n), b = (int)(row / a.n);
       const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C);
       if (i >= s.cnt) continue;
-      const int p = min(max((a.pos ? a.pos[b] : s.len) + i, 0), a.tab - 1);
+      const int p = min(min(max(a.pos ? a.pos[b] : s.len, 0), a.tab) + i, a.tab - 1);
       const uint16_t* x = a.qkv + b * a.sx_b + i * a.sx_t + (size_t)hq * D;
       *reinterpret_cast<uint4*>(a.q + b * a.sq_b + i * a.sq_t + hq * a.sq_h + 8 * c) =
           head_chunk(x, c, true, a.cos_t + (size_t)p * (ROT / 2), a.sin_t + (size_t)p * (ROT / 2));
@@ -121,8 +121,8 @@ __global__ void __launch_bounds__(128) rope_kv8_kernel(AppendArgs a) {
   const int lo = max(blk * BLK, s.len), hi = min((blk + 1) * BLK, s.len + s.cnt);
   if (lo >= hi) return;
   const int i0 = lo - s.len, m = hi - lo, held = lo - blk * BLK;
-  const int p0 = a.pos ? a.pos[b] : s.len;
-  if (tid == 0 && w == 0 && (p0 < 0 || p0 + i0 + m > a.tab)) atomicOr(&g_status, (unsigned int)ST_KV8_RANGE);
+  const int p_in = a.pos ? a.pos[b] : s.len, p0 = min(max(p_in, 0), a.tab);
+  if (tid == 0 && w == 0 && (p_in != p0 || p0 + i0 + m > a.tab)) atomicOr(&g_status, (unsigned int)ST_KV8_RANGE);
   const size_t bh = (size_t)b * a.H + h;
   int8_t* codes = (w ? a.vc : a.kc) + (bh * a.C + (size_t)blk * BLK) * D;
   float* scale = (w ? a.vs : a.ks) + bh * (a.C / BLK) + blk;
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(128) rope_kv8_kernel(AppendArgs a) {
     const int t = tid + 128 * k, row = t / CH, c = t % CH;
     v[k] = make_uint4(0, 0, 0, 0);
     if (row < m) {
-      const int p = min(max(p0 + i0 + row, 0), a.tab - 1);
+      const int p = min(p0 + i0 + row, a.tab - 1);
       v[k] = head_chunk(src + (i0 + row) * a.sx_t, c, w == 0, a.cos_t + (size_t)p * (ROT / 2),
                         a.sin_t + (size_t)p * (ROT / 2));
     }
@@ -581,7 +581,7 @@ int vt_kv8_evict(cudaStream_t st, const int8_t* kc, const int8_t* vc, const floa
     for (const auto& d : dst)
       if (kv8::overlap(s.p, s.n, d.p, d.n)) return set_error(E_SHAPE, "vt_kv8_evict: the destination overlaps the source");
   const long long units = n * (keep / kv8::BLK);
-  if (units > 0x7fffffffLL || n > 0x0fffffffLL)
+  if (units > 0x7fffffffLL || n > 0x07ffffffLL)
     return set_error(E_SHAPE, "vt_kv8_evict: grid too large (B=%d H=%d keep=%d)", B, H, keep);
   kv8::EvictArgs a{kc, vc, ks, vs, weights, lens, B, H, C, keep, recent, dst_C, dst_kc, dst_vc, dst_ks, dst_vs, dst_weights, dst_lens, index};
   // two warps for up to 2048 slots (a warp's share of a round is mostly not its keys), else 1024 threads; as many CTAs a head as leave each thread at most 16 slots when there

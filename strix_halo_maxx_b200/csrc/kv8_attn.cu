@@ -34,6 +34,7 @@ int vt_attn_kv8(cudaStream_t st, const uint16_t* q, long long sq_b, long long sq
   if (B == 0 || n == 0) return OK;
   if (!q || !lens || !out || !aligned16(q) || !aligned16(out) || (sq_b | sq_t | sq_h | so_b | so_t | so_h) % 8)
     return set_error(E_SHAPE, "vt_attn_kv8: null pointer, or pointers / strides not 16-byte aligned");
+  if (!(scale >= 0.f && scale < 0x1p100f)) return set_error(E_SHAPE, "vt_attn_kv8: scale %g is not 0 .. 2^100", scale);
   if (weights_in && !weights) return set_error(E_SHAPE, "vt_attn_kv8: weights_in without weights");
   const long long need = vt_attn_kv8_ws_bytes(B, n, Hq, H, D, C, weights != nullptr);
   if (need && (!ws || !aligned16(ws) || ws_bytes < need))

@@ -146,8 +146,9 @@ def test_lengths_beyond_the_cache_are_cut_off_and_recorded():
     R.append(np_(qkv.float()), ref, [127, 10, 0, 0], np_(cos), np_(sin), 1, counts=[1, 3, 0, 0])
     for got, want in zip(as_np(cache), ref):
         assert np.array_equal(got, want)
-    ops.rope_kv8(qkv[:1, :1], ops.Kv8(*(t[:1] for t in cache)), i32([3]), cos, sin, q[:1, :1], pos=i32([cos.shape[0]]))
-    assert device_status(clear=True) == RANGE_BIT
+    for pos in (cos.shape[0], -1, 2 ** 31 - 1, -2 ** 31):
+        ops.rope_kv8(qkv[:1, :1], ops.Kv8(*(t[:1] for t in cache)), i32([3]), cos, sin, q[:1, :1], pos=i32([pos]))
+        assert device_status(clear=True) == RANGE_BIT, pos
     out = torch.full((B, 3, D), 5.0, dtype=BF, device=DEV)
     ops.attn_kv8(q, cache, i32([127, 10, -5, 500]), out, counts=i32([3, 9, 0, 3]))
     assert device_status(clear=True) == RANGE_BIT
@@ -263,6 +264,53 @@ def test_attn_kv8_large_scores_and_peaked_rows():
         ro, _, mag, _ = R.attention(np_(q.float()), as_np(cache), [T - n])
         # integer scores times a power of two: exact in fp32, so only the roundings of P and the output remain
         assert (np.abs(np_(out.float()) - ro) <= (np.abs(ro) + mag) * 2.0 ** -8 * 1.02 + 1e-6).all()
+
+
+@pytest.mark.parametrize("n", [1, 40, 150])
+def test_attn_kv8_odd_queries_and_a_zero_scale(n):
+    """Rows of q that are zero, subnormal, huge, infinite or NaN change no other row; scale 0 weighs every key the same."""
+    H, D, L = 2, 64, 190
+    cache = filled(1, H, 384, D, 21)
+    g = torch.Generator(DEV).manual_seed(n)
+    q = torch.randn(1, n, 2 * H, D, device=DEV, generator=g).to(BF)
+    q[0, 0, 0], q[0, 0, 1], q[0, n // 2, 2] = 0, q[0, 0, 1] * 1e-39, q[0, n // 2, 2] * 1e-30
+    out = ops.attn_kv8(q, cache, i32([L]))
+    check_attn(q, cache, [L], None, True, out)
+    bad = q.clone()
+    bad[0, 0, 3, 5], bad[0, n - 1, 1, 0], bad[0, n // 3, 2] = float("inf"), float("nan"), 3e38
+    o2 = ops.attn_kv8(bad, cache, i32([L]))
+    same = torch.ones(n, 2 * H, dtype=torch.bool)
+    same[0, 3], same[n - 1, 1], same[n // 3, 2] = False, False, False
+    a, b = out.view(n, 2 * H, D)[same.to(DEV)], o2.view(n, 2 * H, D)[same.to(DEV)]
+    assert torch.equal(a, b) and torch.isnan(o2.view(n, 2 * H, D)[n - 1, 1]).all()
+    flat = ops.attn_kv8(q, cache, i32([L]), scale=0.0)
+    check_attn(q, cache, [L], None, True, flat, scale=0.0)
+
+
+def test_attn_kv8_one_workspace_for_calls_of_every_size_and_two_streams():
+    """A workspace for the largest call serves the smaller ones after it; calls on two streams with workspaces of their own
+    give what they give alone."""
+    H, D = 2, 64
+    cache = filled(1, H, 2048, D, 2)
+    ws = ops.attn_kv8_workspace(1, 300, 4, H, D, 2048, DEV, True)
+    want = {}
+    for n in (300, 16, 1, 90):
+        g = torch.Generator(DEV).manual_seed(n)
+        q, w = torch.randn(1, n, 4, D, device=DEV, generator=g).to(BF), torch.zeros(1, H, 2048, device=DEV)
+        o = ops.attn_kv8(q, cache, i32([1500]), weights=w, ws=ws)
+        want[n] = (q, o, w)
+        check_attn(q, cache, [1500], None, True, o, w)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for r in range(10):
+        for s, n in ((s1, 300), (s2, 90), (s1, 16), (s2, 1)):
+            with torch.cuda.stream(s):
+                w = torch.zeros(1, H, 2048, device=DEV)
+                got.append((n, ops.attn_kv8(want[n][0], cache, i32([1500]), weights=w), w))
+    torch.cuda.synchronize()
+    for n, o, w in got:
+        assert torch.equal(o, want[n][1]) and torch.equal(w, want[n][2]), n
 
 
 def test_attn_kv8_of_one_row_does_not_depend_on_its_batch():

@@ -35,15 +35,17 @@ def test_rope_kv8_refuses_on_the_host(L, kw, rc, word):
     assert word is None or word in _msg(L), _msg(L)
 
 
-def _attn(L, B=1, n=1, Hq=4, H=2, D=64, C=64, q=4096, sq=64, out=4096, so=64, w=None, w_in=None, ws=4096, ws_bytes=1 << 40, lens=4096):
-    return L.vt_attn_kv8(None, q, 256, 256, sq, 4096, 4096, 4096, 4096, C, lens, None, B, n, Hq, H, D, 1, 0.125, out, 256, 256, so,
+def _attn(L, B=1, n=1, Hq=4, H=2, D=64, C=64, q=4096, sq=64, out=4096, so=64, w=None, w_in=None, ws=4096, ws_bytes=1 << 40, lens=4096,
+          scale=0.125):
+    return L.vt_attn_kv8(None, q, 256, 256, sq, 4096, 4096, 4096, 4096, C, lens, None, B, n, Hq, H, D, 1, scale, out, 256, 256, so,
                          w, w_in, ws, ws_bytes)
 
 
 @pytest.mark.parametrize("kw,rc,word", [
     (dict(D=80), -1, b"head_dim"), (dict(C=65), -2, b"multiple of 64"), (dict(Hq=5), -2, b"multiple of H"), (dict(q=None), -2, b"null"),
     (dict(out=4104), -2, b"16-byte"), (dict(sq=12), -2, b"16-byte"), (dict(so=100), -2, b"16-byte"), (dict(lens=None), -2, b"null"),
-    (dict(w_in=4096), -2, b"weights_in without weights"), (dict(w=4096, ws=None), -2, b"workspace"),
+    (dict(w_in=4096), -2, b"weights_in without weights"), (dict(scale=-0.1), -2, b"scale"), (dict(scale=float("nan")), -2, b"scale"),
+    (dict(scale=float("inf")), -2, b"scale"), (dict(B=2049, C=4096), -2, b"at most 2048"), (dict(w=4096, ws=None), -2, b"workspace"),
     (dict(w=4096, ws_bytes=4), -2, b"workspace"), (dict(w=4096, ws=4100), -2, b"workspace"), (dict(n=0), 0, None), (dict(B=0), 0, None)])
 def test_attn_kv8_refuses_on_the_host(L, kw, rc, word):
     assert _attn(L, **kw) == rc
@@ -58,7 +60,7 @@ def _evict(L, B=1, H=2, D=64, C=128, keep=64, recent=8, base=1 << 20, dst=1 << 2
 @pytest.mark.parametrize("kw,rc,word", [
     (dict(D=96), -1, b"head_dim"), (dict(keep=0), -2, b"keep=0"), (dict(keep=63), -2, b"keep=63"), (dict(keep=128), -2, b"keep=128"),
     (dict(recent=65), -2, b"recent=65"), (dict(recent=-1), -2, b"recent=-1"), (dict(Cd=96), -2, b"multiple of 64"),
-    (dict(w=None), -2, b"null"), (dict(dst=1 << 20), -2, b"overlaps"), (dict(dst=(1 << 20) + 64 * 64), -2, b"overlaps"),
+    (dict(w=None), -2, b"null"), (dict(C=262144 + 64), -2, b"at most 262144"), (dict(dst=1 << 20), -2, b"overlaps"), (dict(dst=(1 << 20) + 64 * 64), -2, b"overlaps"),
     (dict(dlens=1 << 23), -2, b"overlaps"), (dict(B=0), 0, None)])
 def test_kv8_evict_refuses_on_the_host(L, kw, rc, word):
     assert _evict(L, **kw) == rc
