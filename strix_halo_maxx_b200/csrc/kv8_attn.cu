@@ -5,9 +5,7 @@
 namespace vt {
 namespace kv8 {
 
-// Rows of a kv head that the split kernel takes.
-constexpr int FEW_ROWS = 32;
-static bool few_rows(int n, int Hq, int H) { return (long long)n * (Hq / H) <= FEW_ROWS; }
+static bool few_rows(int n, int Hq, int H) { return (long long)n * (Hq / H) <= split::FEW_ROWS; }
 
 }  // namespace kv8
 }  // namespace vt
@@ -17,7 +15,7 @@ extern "C" {
 long long vt_attn_kv8_ws_bytes(int B, int n, int Hq, int H, int D, int C, int weights) {
   if (B <= 0 || n <= 0 || Hq <= 0 || H <= 0 || Hq % H || C <= 0 || (D != 64 && D != 128)) return 0;
   // what n tokens need, and any fewer that may follow with the same workspace
-  const int few = vt::kv8::FEW_ROWS / (Hq / H), nf = n < few ? n : few;
+  const int few = vt::kv8::split::FEW_ROWS / (Hq / H), nf = n < few ? n : few;
   const long long split = nf ? vt::kv8::split::make_plan(B, nf, Hq, H, D, C, weights != 0, vt::sm_count()).bytes : 0;
   const long long many = n > few ? vt::kv8::tc::make_plan(B, n, Hq, H, D, C, weights != 0, vt::sm_count()).bytes : 0;
   return split > many ? split : many;

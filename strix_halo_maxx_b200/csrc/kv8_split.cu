@@ -29,7 +29,7 @@ namespace vt {
 namespace kv8 {
 namespace split {
 
-constexpr int ST = 3;
+constexpr int ST = 3, FEW_ROWS = 32;                // stages; rows of a kv head that this kernel takes
 constexpr int TILE = 4096;                         // bytes of K (or V) codes in a tile
 constexpr int RING = 2 * TILE * ST;                // a warp's ring
 constexpr int MAXB = 2048;                         // sequences a call takes (their tile counts sit in shared memory)
@@ -472,50 +472,73 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
   }
 }
 
-// Merges the parts of items that span CTAs, in the CTAs' order, and turns scores into weights.
-// CTAs [0, merge_ctas): ROWS rows of one item, thread = 4 dims of a row.  The others: 512 keys of one (sequence, head):
-// weight = (key before len ? weights_in : 0) + sum over rows of 2^(score - m - log2 l).
+// Merges the parts of items that span CTAs and turns scores into weights.
+// CTAs [0, merge_ctas): one row of an item; each of 128 * 4 / D groups of threads (thread = 4 dims) takes every so many'th
+// part, the groups' sums are added in order.  The others: 512 keys of one (sequence, head):
+// weight = (key before len ? weights_in : 0) + sum over rows of 2^(score - m - log2 l), a row's (m, l) by a warp.
 template <int D, int NT>
 __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ctas) {
-  constexpr int KT = TILE / D, GR = 8 * NT, ROWS = 128 * 4 / D;
+  constexpr int KT = TILE / D, GR = 8 * NT, GROUPS = 128 * 4 / D;
   __shared__ int pre[MAXB + 1], warp_sum[4];
-  __shared__ float lse[64];
-  const int tid = threadIdx.x;
+  __shared__ float lse[FEW_ROWS];
+  __shared__ __align__(16) float4 sh_o[128];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   griddep_wait();
   griddep_launch();
   tile_list(a, KT, pre, warp_sum);
   const int run = run_of(pre[a.B], a.ctas);
-  // (m, l) of row `row` of (b, h), and the first and last CTA that hold a part of it
+  // the first and last CTA that hold a part of an item, and the first part's slot (the others begin their CTA's run: 2 c)
   auto parts = [&](int b, int h, int rg, int tiles, int& c0, int& c1, int& first) {
     const int u0 = pre[b] + (h * a.rg + rg) * tiles;
     c0 = u0 / run, c1 = (u0 + tiles - 1) / run;
-    first = 2 * c0 + (u0 == c0 * run ? 0 : 1);  // slot of the first part; the others begin their CTA's run: 2 c
+    first = 2 * c0 + (u0 == c0 * run ? 0 : 1);
+  };
+  auto slot = [&](int c, int c0, int first) { return (size_t)(c == c0 ? first : 2 * c) * GR; };
+  // a row's maximum and sum over its parts, lane c taking part c0 + c and so on: the same in every warp that asks
+  auto row_ml = [&](int c0, int c1, int first, int r, float& mx, float& sum) {
+    mx = -INFINITY, sum = 0.f;
+    for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, a.part_ml[slot(c, c0, first) + r].x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    for (int c = c0 + lane; c <= c1; c += 32) {
+      const float2 ml = a.part_ml[slot(c, c0, first) + r];
+      sum += ml.x == -INFINITY ? 0.f * ml.y : ml.y * ex2_approx(ml.x - mx);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   };
   if ((int)blockIdx.x < merge_ctas) {
-    const int groups = (min(GR, a.rows) + ROWS - 1) / ROWS;
-    const int item = blockIdx.x / groups, r = blockIdx.x % groups * ROWS + tid / (D / 4), d = tid % (D / 4) * 4;
+    const int rows = min(GR, a.rows), item = blockIdx.x / rows, r = blockIdx.x % rows;
     const int rg = item % a.rg, h = item / a.rg % a.H, b = item / a.rg / a.H;
     const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C);
     const int row = rg * GR + r, tiles = (s.len + s.cnt + KT - 1) / KT;
-    if (r >= GR || row >= s.cnt * a.G) return;
+    if (row >= s.cnt * a.G) return;
     int c0, c1, first;
     parts(b, h, rg, tiles, c0, c1, first);
     if (c0 == c1) return;
-    float mx = -INFINITY;
-    for (int c = c0; c <= c1; c++) mx = fmaxf(mx, a.part_ml[(size_t)(c == c0 ? first : 2 * c) * GR + r].x);
-    float sum = 0.f;
+    float mx, sum;
+    row_ml(c0, c1, first, r, mx, sum);
+    const int grp = tid / (D / 4), d = tid % (D / 4) * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int c = c0; c <= c1; c++) {
-      const size_t at = (size_t)(c == c0 ? first : 2 * c) * GR + r;
-      const float2 ml = a.part_ml[at];
+    for (int c = c0 + grp; c <= c1; c += GROUPS) {
+      const size_t at = slot(c, c0, first) + r;
+      const float m = a.part_ml[at].x;
       const float4 x = *reinterpret_cast<const float4*>(a.part_o + at * D + d);
-      const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - mx);
-      sum += ml.y * f, v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+      const float f = m == -INFINITY ? 0.f : ex2_approx(m - mx);
+      v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
     }
-    const float inv = 1.f / sum;
-    uint16_t* op = a.out + b * a.so_b + row / a.G * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
-    *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
+    sh_o[tid] = v;
+    __syncthreads();
+    if (grp == 0) {
+      for (int k = 1; k < GROUPS; k++) {
+        const float4 x = sh_o[tid + k * (D / 4)];
+        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+      }
+      const float inv = 1.f / sum;
+      uint16_t* op = a.out + b * a.so_b + row / a.G * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
+      *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
+    }
     return;
   }
   const int chunks = (a.C + 511) / 512, x = blockIdx.x - merge_ctas;
@@ -523,7 +546,7 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
   const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C);
   const int T = s.len + s.cnt, rows = s.cnt * a.G, tiles = (T + KT - 1) / KT;
   if (x % chunks * 512 >= T) return;
-  for (int r = tid; r < rows; r += 128) {
+  for (int r = warp; r < rows; r += 4) {
     int c0, c1, first;
     parts(b, h, r / GR, tiles, c0, c1, first);
     float mx, sum;
@@ -531,14 +554,9 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
       const float2 ml = a.full_ml[((size_t)bh * a.rg + r / GR) * GR + r % GR];
       mx = ml.x, sum = ml.y;
     } else {
-      mx = -INFINITY, sum = 0.f;
-      for (int c = c0; c <= c1; c++) mx = fmaxf(mx, a.part_ml[(size_t)(c == c0 ? first : 2 * c) * GR + r % GR].x);
-      for (int c = c0; c <= c1; c++) {
-        const float2 ml = a.part_ml[(size_t)(c == c0 ? first : 2 * c) * GR + r % GR];
-        sum += ml.x == -INFINITY ? 0.f * ml.y : ml.y * ex2_approx(ml.x - mx);
-      }
+      row_ml(c0, c1, first, r % GR, mx, sum);
     }
-    lse[r] = mx + log2f(sum);
+    if (lane == 0) lse[r] = mx + log2f(sum);
   }
   __syncthreads();
   if (j >= T) return;
@@ -560,7 +578,6 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
 
 template <int D, int NT>
 static int launch(cudaStream_t st, const Args& a, bool whole) {
-  constexpr int ROWS = 128 * 4 / D;
   if (whole) {
     constexpr int SMEM = WHOLE_WARPS * RING;
     const int rc = smem_attr_once((const void*)attn_kv8_split_kernel<D, NT, true>, SMEM, "vt_attn_kv8");
@@ -573,7 +590,7 @@ static int launch(cudaStream_t st, const Args& a, bool whole) {
   if (rc) return rc;
   launch_k(attn_kv8_split_kernel<D, NT, false>, a.ctas, WARPS * 32, SMEM, st, a);
   const int rows = 8 * NT < a.rows ? 8 * NT : a.rows;
-  const int merge = a.B * a.H * a.rg * ((rows + ROWS - 1) / ROWS);
+  const int merge = a.B * a.H * a.rg * rows;
   const int chunks = a.w ? a.B * a.H * ((a.C + 511) / 512) : 0;
   launch_k(attn_kv8_join_kernel<D, NT>, merge + chunks, 128, 0, st, a, merge);
   return check_launch("vt_attn_kv8");

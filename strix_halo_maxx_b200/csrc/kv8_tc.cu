@@ -590,7 +590,7 @@ template <int D>
 __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
   using L = WSmem<D>;
   extern __shared__ __align__(1024) uint8_t sm[];
-  __shared__ __align__(16) float sh_lse[2][WR], half_sum[WK];
+  __shared__ __align__(16) float sh_lse[2][WR], half_sum[WK];  // sh_lse: minus the row's
   __shared__ __align__(8) uint64_t bars[2 + 2 + 2 + 2 + 1];
   __shared__ uint32_t tmem_slot;
   __shared__ int sh_abort;
@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
       for (int c = 0; c < D / 8; c++)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c * WR * 16), "l"(src + 8 * c) : "memory");
       asm volatile("cp.async.commit_group;" ::: "memory");
-      lse = r < rows ? a.lse[bh * a.rows + r] : INFINITY;  // rows past the last add 2^-inf
+      lse = r < rows ? -a.lse[bh * a.rows + r] : -INFINITY;  // rows past the last add 2^-inf
     };
     if (nt > 0) fetch(0);
     for (int x = 0; x < 4 * (D / 64); x++) {  // warp w rows 32 w ..; slots behind the cache's last one are zero
@@ -693,7 +693,7 @@ __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
     const int r_min = a.causal ? (key - s.len) * a.G : 0;  // rows before it do not see this key
     const int warp_max = __reduce_max_sync(0xffffffffu, r_min);
     unsigned long long acc2[2] = {0ull, 0ull};
-    const unsigned long long c2 = f2_pack(c, c), minus = f2_pack(-1.f, -1.f);
+    const unsigned long long c2 = f2_pack(c, c);
     for (int i = 0; i < nt; i++) {
       const int f = i & 1;
       ok = wait(&q_full[f], (i >> 1) & 1) && wait(&s_full[f], (i >> 1) & 1);  // lse, scores
@@ -717,7 +717,7 @@ __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
 #pragma unroll
           for (int k = 0; k < 2; k++) {
             const unsigned long long lz = k ? f2_pack(z.z, z.w) : f2_pack(z.x, z.y);
-            const unsigned long long y = f2_fma(f2_pack(__uint_as_float(x[e + 2 * k]), __uint_as_float(x[e + 2 * k + 1])), c2, f2_mul(lz, minus));
+            const unsigned long long y = f2_fma(f2_pack(__uint_as_float(x[e + 2 * k]), __uint_as_float(x[e + 2 * k + 1])), c2, lz);
             float y0, y1;
             f2_unpack(y, y0, y1);
             y0 = ex2_approx(y0), y1 = ex2_approx(y1);
