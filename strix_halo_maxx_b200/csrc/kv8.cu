@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(128) kv8_gather_kernel(EvictArgs a) {
 }
 
 template <int THREADS, int KPT, int CS>
-static void launch_select(cudaStream_t st, const EvictArgs& a) {
+static int launch_select(cudaStream_t st, const EvictArgs& a) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.B * a.H * CS));
   cfg.blockDim = dim3(THREADS);
@@ -511,6 +511,7 @@ static void launch_select(cudaStream_t st, const EvictArgs& a) {
   cfg.attrs = at;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   cudaLaunchKernelEx(&cfg, kv8_select_kernel<THREADS, KPT, CS>, a);
+  return check_launch("vt_kv8_evict");
 }
 
 static bool overlap(const void* p, long long n, const void* q, long long m) {
@@ -584,14 +585,16 @@ int vt_kv8_evict(cudaStream_t st, const int8_t* kc, const int8_t* vc, const floa
   if (units > 0x7fffffffLL || n > 0x07ffffffLL)
     return set_error(E_SHAPE, "vt_kv8_evict: grid too large (B=%d H=%d keep=%d)", B, H, keep);
   kv8::EvictArgs a{kc, vc, ks, vs, weights, lens, B, H, C, keep, recent, dst_C, dst_kc, dst_vc, dst_ks, dst_vs, dst_weights, dst_lens, index};
-  // two warps for up to 2048 slots (a warp's share of a round is mostly not its keys), else 1024 threads; as many CTAs a head as leave each thread at most 16 slots when there
-  // are fewer heads than SMs, 32 otherwise (one CTA then has a head of up to 32k slots; 256 heads fill the GPU)
+  // Two warps for up to 2048 slots: a warp's share of a round is mostly not its keys.  Beyond, 1024 threads, and as many CTAs a
+  // head as leave each thread at most 16 slots when there are fewer heads than SMs (8 heads of 131k slots, clusters of 8:
+  // 39 us; clusters of 16 with half the threads 52 us, their barriers cost more than the keys), 32 otherwise
   const int most = n < sm_count() ? 16 : 32;
-  if (C <= 2048) kv8::launch_select<64, 32, 1>(st, a);
-  else if (C <= most * 1024) kv8::launch_select<1024, 32, 1>(st, a);
-  else if (C <= most * 2048) kv8::launch_select<1024, 32, 2>(st, a);
-  else if (C <= most * 4096) kv8::launch_select<1024, 32, 4>(st, a);
-  else kv8::launch_select<1024, 32, 8>(st, a);
+  if (C <= 2048) rc = kv8::launch_select<64, 32, 1>(st, a);
+  else if (C <= most * 1024) rc = kv8::launch_select<1024, 32, 1>(st, a);
+  else if (C <= most * 2048) rc = kv8::launch_select<1024, 32, 2>(st, a);
+  else if (C <= most * 4096) rc = kv8::launch_select<1024, 32, 4>(st, a);
+  else rc = kv8::launch_select<1024, 32, 8>(st, a);
+  if (rc) return rc;
   if (D == 64) launch_k(kv8::kv8_gather_kernel<64>, (unsigned)units, 128, 0, st, a);
   else launch_k(kv8::kv8_gather_kernel<128>, (unsigned)units, 128, 0, st, a);
   return check_launch("vt_kv8_evict");

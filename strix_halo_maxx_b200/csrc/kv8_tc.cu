@@ -54,7 +54,7 @@ struct Args {
   long long so_b, so_t, so_h;
   float* part_o;     // [2 ctas][ROWS][D]
   float2* part_ml;   // [2 ctas][ROWS]
-  float* lse;        // [B][H][rows], or null
+  float* lse;        // [B][H][rows] minus log2 of the row's sum, or null
   float* w;
   const float* w_in;
 };
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       }
       if (row < valid) {
         if (!whole) a.part_ml[slot] = make_float2(m, l);
-        else if (a.lse) a.lse[bh * a.rows + row] = m + log2f(l);
+        else if (a.lse) a.lse[bh * a.rows + row] = -(m + log2f(l));
       }
       tc_fence_before();
       __syncwarp();
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(128) attn_kv8_tc_join_kernel(Args a) {
     const float inv = 1.f / sum;
     uint16_t* op = a.out + g.b * a.so_b + row / a.G * a.so_t + (size_t)(g.h * a.G + row % a.G) * a.so_h + d;
     *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
-    if (d == 0 && a.lse) a.lse[bh * a.rows + row] = mx + log2f(sum);
+    if (d == 0 && a.lse) a.lse[bh * a.rows + row] = -(mx + log2f(sum));
   }
 }
 
@@ -578,24 +578,26 @@ __global__ void __launch_bounds__(128) attn_kv8_tc_join_kernel(Args a) {
 // a thread owns a key and adds up along its TMEM lane: no atomics, one order.  CTA = 128 keys of one (sequence, head);
 // rows 128 at a time:
 //   warps 0-3, 4-7   rows 0-63 / 64-127 of the row tile, thread = key;
-//   warps 8-11       K's codes -> the A operand once; q rows and lse of each row tile (2 stages);
+//   warps 8-11       K's codes -> the A operand once; q rows and lse of each row tile, ST tiles in flight;
 //   warp 12          tcgen05.mma into two S buffers.
 // Bound: MUFU, one ex2 a score.
 constexpr int WK = 128, WR = 128, WTHREADS = 13 * 32;
 template <int D>
 struct WSmem {
-  static constexpr int K = 0, Q = WK * D * 2, QT = WR * D * 2, BYTES = Q + 2 * QT;
+  static constexpr int ST = D == 64 ? 4 : 2;  // row tiles in flight; two CTAs share an SM
+  static constexpr int K = 0, Q = WK * D * 2, QT = WR * D * 2, BYTES = Q + ST * QT;
 };
 template <int D>
 __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
   using L = WSmem<D>;
   extern __shared__ __align__(1024) uint8_t sm[];
-  __shared__ __align__(16) float sh_lse[2][WR], half_sum[WK];  // sh_lse: minus the row's
-  __shared__ __align__(8) uint64_t bars[2 + 2 + 2 + 2 + 1];
+  constexpr int ST = L::ST;
+  __shared__ __align__(16) float sh_lse[ST][WR], half_sum[WK];
+  __shared__ __align__(8) uint64_t bars[2 * ST + 2 + 2 + 1];
   __shared__ uint32_t tmem_slot;
   __shared__ int sh_abort;
   volatile int* abort_flag = &sh_abort;
-  uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *s_empty = bars + 6, *drain = bars + 8;
+  uint64_t *q_full = bars, *q_empty = bars + ST, *s_full = q_empty + ST, *s_empty = s_full + 2, *drain = s_empty + 2;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kt = (a.C + WK - 1) / WK, key0 = blockIdx.x % kt * WK;
   const size_t bh = blockIdx.x / kt;
@@ -607,7 +609,8 @@ __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
   // the first row that sees a key of this CTA, down to a whole tile
   const int first = a.causal ? max(key0 - s.len, 0) * a.G / WR : 0, nt = (rows + WR - 1) / WR - first;
   if (tid == 0) {
-    for (int i = 0; i < 2; i++) mbar_init(&q_full[i], 4), mbar_init(&q_empty[i], 8), mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], 8);
+    for (int i = 0; i < ST; i++) mbar_init(&q_full[i], 4), mbar_init(&q_empty[i], 8);
+    for (int i = 0; i < 2; i++) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], 8);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -631,14 +634,14 @@ __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
     const uint32_t leader = elect_one();
     const uint64_t dk = sdesc_noswz(smem_u32(sm + L::K), 2048, 128), dq = sdesc_noswz(smem_u32(sm + L::Q), 2048, 128);
     for (int i = 0; i < nt; i++) {
-      const int f = i & 1;
-      ok = wait(&q_full[f], (i >> 1) & 1) && (i < 2 || wait(&s_empty[f], ((i >> 1) - 1) & 1));
+      const int f = i & 1, st = i % ST;
+      ok = wait(&q_full[st], (i / ST) & 1) && (i < 2 || wait(&s_empty[f], ((i >> 1) - 1) & 1));
       if (!ok) break;
       tc_fence_after();
       if (leader) {
 #pragma unroll
         for (int k = 0; k < D / 16; k++)
-          umma_f16(tmem + 128 * f, dk + k * (4096 >> 4), dq + f * (L::QT >> 4) + k * (4096 >> 4), idesc_bf16(WK, WR), k > 0 ? 1u : 0u);
+          umma_f16(tmem + 128 * f, dk + k * (4096 >> 4), dq + st * (L::QT >> 4) + k * (4096 >> 4), idesc_bf16(WK, WR), k > 0 ? 1u : 0u);
         umma_commit(&s_full[f]);
       }
       __syncwarp();
@@ -650,19 +653,26 @@ __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
   } else if (warp >= 8) {
     const int w = warp - 8, ct = tid - 256;
     const int8_t* kp = a.kc + bh * a.C * D;
-    // thread = row of the row tile: its q on its way a tile ahead
-    float lse;
+    // a warp's copies take 32 bytes of 16 rows at a time: whole sectors, and two lanes to a bank at most
     auto fetch = [&](int i) {
-      const int f = i & 1, r = (first + i) * WR + ct;
-      const uint16_t* src = q_row(a, b, h, min(r, rows - 1));
-      const uint32_t dst = smem_u32(sm + L::Q + f * L::QT + ct * 16);
+      const int st = i % ST, r0 = (first + i) * WR;
 #pragma unroll
-      for (int c = 0; c < D / 8; c++)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c * WR * 16), "l"(src + 8 * c) : "memory");
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      lse = r < rows ? -a.lse[bh * a.rows + r] : -INFINITY;  // rows past the last add 2^-inf
+      for (int x = 0; x < 2; x++) {
+        const int r = 32 * w + 16 * x + (lane >> 1);
+        const uint16_t* src = q_row(a, b, h, min(r0 + r, rows - 1)) + 8 * (lane & 1);
+        const uint32_t dst = smem_u32(sm + L::Q + st * L::QT + ((lane & 1) * WR + r) * 16);
+#pragma unroll
+        for (int c = 0; c < D / 16; c++)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 2 * c * WR * 16), "l"(src + 16 * c) : "memory");
+      }
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&sh_lse[st][ct])), "l"(a.lse + bh * a.rows + min(r0 + ct, rows - 1))
+                   : "memory");
     };
-    if (nt > 0) fetch(0);
+    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+    for (int i = 0; i < ST - 1; i++) {
+      if (i < nt) fetch(i);
+      commit();
+    }
     for (int x = 0; x < 4 * (D / 64); x++) {  // warp w rows 32 w ..; slots behind the cache's last one are zero
       const int row = 32 * w + 8 * (x & 3) + (lane & 7), p = (lane >> 3) + 4 * (x >> 2);
       uint4 c = make_uint4(0, 0, 0, 0);
@@ -670,20 +680,17 @@ __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
       store_codes<WK>(sm + L::K, row, p, c);
     }
     for (int i = 0; i < nt; i++) {
-      const int f = i & 1;
-      sh_lse[f][ct] = lse;
-      if (i + 1 < nt) {
-        // the stage is free when both halves have read its lse, which comes after its products
-        if (i >= 1) ok = wait(&q_empty[f ^ 1], ((i - 1) >> 1) & 1);
-        if (!ok) break;
-        fetch(i + 1);
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-      } else {
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
       fence_proxy_async_smem();
       __syncwarp();
-      mbar_arrive_if(&q_full[f], lane == 0);
+      mbar_arrive_if(&q_full[i % ST], lane == 0);
+      const int n = i + ST - 1;  // the next tile to bring in; its stage was tile i - 1's, free when both halves have read its lse
+      if (n < nt) {
+        if (i > 0) ok = wait(&q_empty[n % ST], ((i - 1) / ST) & 1);
+        if (!ok) break;
+        fetch(n);
+      }
+      commit();
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
@@ -695,8 +702,8 @@ __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
     unsigned long long acc2[2] = {0ull, 0ull};
     const unsigned long long c2 = f2_pack(c, c);
     for (int i = 0; i < nt; i++) {
-      const int f = i & 1;
-      ok = wait(&q_full[f], (i >> 1) & 1) && wait(&s_full[f], (i >> 1) & 1);  // lse, scores
+      const int f = i & 1, st = i % ST;
+      ok = wait(&q_full[st], (i / ST) & 1) && wait(&s_full[f], (i >> 1) & 1);  // lse, scores
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
@@ -710,10 +717,10 @@ __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
           mbar_arrive_if(&s_empty[f], lane == 0);
         }
         const int r0 = (first + i) * WR + 64 * half + 32 * hf;
-        const bool edge = r0 < warp_max;
+        const bool edge = r0 < warp_max || r0 + 32 > rows;
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-          const float4 z = *reinterpret_cast<const float4*>(&sh_lse[f][64 * half + 32 * hf + e]);
+          const float4 z = *reinterpret_cast<const float4*>(&sh_lse[st][64 * half + 32 * hf + e]);
 #pragma unroll
           for (int k = 0; k < 2; k++) {
             const unsigned long long lz = k ? f2_pack(z.z, z.w) : f2_pack(z.x, z.y);
@@ -722,15 +729,16 @@ __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
             f2_unpack(y, y0, y1);
             y0 = ex2_approx(y0), y1 = ex2_approx(y1);
             if (edge) {
-              if (r0 + e + 2 * k < r_min) y0 = 0.f;
-              if (r0 + e + 2 * k + 1 < r_min) y1 = 0.f;
+              const int ra = r0 + e + 2 * k;
+              if (ra < r_min || ra >= rows) y0 = 0.f;
+              if (ra + 1 < r_min || ra + 1 >= rows) y1 = 0.f;
             }
             acc2[k] = f2_add(acc2[k], f2_pack(y0, y1));
           }
         }
       }
       __syncwarp();
-      mbar_arrive_if(&q_empty[f], lane == 0);
+      mbar_arrive_if(&q_empty[st], lane == 0);
     }
     float lo, hi;
     f2_unpack(f2_add(acc2[0], acc2[1]), lo, hi);

@@ -329,7 +329,9 @@ def test_attn_kv8_of_one_row_does_not_depend_on_its_batch():
 EVICT = [  # B, H, D, C, lens, keep, recent, dst C
     (1, 1, 64, 128, [128], 64, 0, 64), (1, 2, 64, 832, [730], 256, 32, 320), (2, 3, 128, 512, [500, 300], 448, 448, 448),
     (4, 2, 64, 1024, [1000, 64, 0, 65], 64, 7, 128), (1, 2, 128, 5056, [5001], 1024, 100, 2048), (3, 1, 64, 256, [200, 256, 193], 192, 1, 256),
-    (1, 1, 128, 20480, [20001], 128, 0, 128)]
+    (1, 1, 128, 20480, [20001], 128, 0, 128), (1, 2, 64, 9024, [9000], 64, 0, 64), (2, 1, 64, 40000, [39999, 33000], 4096, 5, 4096),
+    (1, 1, 64, 70016, [70016], 640, 1, 640), (150, 1, 64, 2112, [2100 - i for i in range(150)], 1024, 100, 1024),
+    (150, 1, 64, 33024, [33000] * 2 + [500] * 148, 512, 1, 512), (1, 1, 64, 262144, [262100], 128, 64, 128)]
 
 
 @pytest.mark.parametrize("ties", [False, True])
