@@ -286,7 +286,7 @@ int vt_attn_causal(cudaStream_t stream, const uint16_t* q, const uint16_t* kc, c
  * (int, device memory, NULL: n for all) the number of its new tokens, 0 .. n; rows past counts[b] are padding: never
  * read into a result, and left as they were in every output.  Lengths on the device cannot be refused by the host: a
  * negative one, a count outside 0 .. n, tokens past C and positions past the rotary table are clamped and set bit 9
- * of the status word (vt_device_status).  Query head hq reads head hq / (Hq / H).  The reference has a bf16 cache only
+ * of the status word (vt_device_status; bit 10: a bounded wait of vt_attn_kv8 gave up).  Query head hq reads head hq / (Hq / H).  The reference has a bf16 cache only
  * (moondream/gpu/md2fast.py:186-191); these stand beside vt_rope_qkv and vt_attn_causal.
  * Limits: vt_attn_kv8 B <= 2048, 0 <= scale < 2^100; vt_kv8_evict C <= 262144. */
 

@@ -14,9 +14,10 @@
 // Scales cost nothing per score: K's joins the softmax scale of the tile; V's shifts the exponent, P' = vs P = 2^(s - (m - log2
 // vs)), and the row sum takes sum(P') / vs.  So P' is rounded to bf16 with its scale in the exponent, whatever its size
 // (scales of 2^-100 .. 2^100; V blocks with a smaller one are zeros).
-// Bound: MUFU (one ex2 a score, 16 a clock and SM) for D = 64, the tensor pipe nearly as much for D = 128.
-#include <type_traits>
-
+// A 2048-token chunk over 6001 slots (32 / 8 heads x 128, 236 GFLOP): 277 us, 850 TFLOP/s.  A tile takes about 2,040 cycles: the
+// exponentials occupy the MUFU for 1,024 (16 a clock and SM), the MMAs are issued over about 1,500, and P -> PV -> S of a
+// score buffer is a chain of which two are in flight.  128-key tiles with one score buffer were slower (346 us), so were
+// four stages (299) and P announced one tile late (294).
 #include "vt_common.cuh"
 #include "vt_host.h"
 
@@ -215,14 +216,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, ST_KV8_WAIT)) != 0;
   };
 
-  // registers by role: 512 threads are launched with 128 each; the softmax holds 64 scores, and spills cost its tiles a fifth
+  // registers by role: 512 threads are launched with 128 each; the softmax holds 64 scores, and its spills cost 307 against
+  // 284 us for the 2048-token chunk
   static_assert(2 * SOFTMAX_REGS + CONVERT_REGS + MMA_REGS <= 4 * 128, "the split must come out of the launch's registers");
   if (warp >= 14) {
     set_regs_down<MMA_REGS>();  // idle; the issuers' warp group
   } else if (warp >= 12) {
     set_regs_down<MMA_REGS>();
-    // ---------------- MMA issuer of M tile t (one warp each: issuing is what a tile's time is made of otherwise).  The
-    // whole warp walks the loop, one lane issues.  j: key tiles of all segments; js: of those in which t had rows
+    // ---------------- MMA issuer of M tile t, one warp each (one thread for both tiles: 435 against 335 us for the 2048-token
+    // chunk).  The whole warp walks the loop, one lane issues.  j: key tiles of all segments; js: of those in which t had rows
     const int t = warp - 12;
     const uint32_t leader = elect_one();
     constexpr uint32_t IDESC_S = idesc_bf16(128, KEYS), IDESC_O = idesc_bf16(128, D) | (1u << 16);  // V MN-major
@@ -580,7 +582,7 @@ __global__ void __launch_bounds__(128) attn_kv8_tc_join_kernel(Args a) {
 //   warps 0-3, 4-7   rows 0-63 / 64-127 of the row tile, thread = key;
 //   warps 8-11       K's codes -> the A operand once; q rows and lse of each row tile, ST tiles in flight;
 //   warp 12          tcgen05.mma into two S buffers.
-// Bound: MUFU, one ex2 a score.
+// Bound: MUFU, one ex2 a score (730 x 730 x 32 heads: 22 us, most of it on the SMs that have two of the 192 CTAs).
 constexpr int WK = 128, WR = 128, WTHREADS = 13 * 32;
 template <int D>
 struct WSmem {
