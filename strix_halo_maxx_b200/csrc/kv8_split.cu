@@ -36,9 +36,10 @@ constexpr int RING = 2 * TILE * ST;                // a warp's ring
 constexpr int MAXB = 2048;                         // sequences a call takes (their tile counts sit in shared memory)
 constexpr int WARPS = 4;                           // of a CTA with a run of tiles
 constexpr int MIN_RUN = WARPS;                     // tiles of a run at least
-// Where a head has at most so many tiles a CTA of eight warps takes a whole item: no parts, no second kernel, and the weights
-// come from the same CTA (32-token question over 730: 10.0 us, against 8.4 in runs and 5.1 to join; one token 6.4 against 5.1
-// and 4.7).
+// Where a head has at most so many tiles, and there are at most four items for each SM, a CTA of eight warps takes a whole item:
+// no parts, no second kernel, and the weights come from the same CTA (32-token question over 730: 10.0 us, against 8.4 in runs
+// and 5.1 to join; one token 6.4 against 5.1 and 4.7; 12 x 32 heads of 800: 13.8 against 17.5 together; but 34 x 32 heads of
+// 531 with weights 40.3 against 36.1).
 constexpr int WHOLE_WARPS = 8, WHOLE_TILES = 16;
 constexpr long long kDrainCycles = 200000000LL;
 
@@ -59,7 +60,7 @@ static Plan make_plan(int B, int n, int Hq, int H, int D, int C, bool weights, i
   p.nt = p.rows <= 8 ? 1 : (p.rows <= 16 || D == 128) ? 2 : 4;
   p.rg = (p.rows + 8 * p.nt - 1) / (8 * p.nt);
   p.ctas = 2 * sms;
-  p.whole = C / keys_per_tile(D) <= WHOLE_TILES && (p.rg == 1 || !weights);
+  p.whole = C / keys_per_tile(D) <= WHOLE_TILES && (p.rg == 1 || !weights) && (long long)B * H * p.rg <= 4LL * sms;
   const long long slots = 2LL * p.ctas, gr = 8LL * p.nt;
   auto up = [](long long x) { return (x + 255) / 256 * 256; };
   p.o_off = 0;
