@@ -236,6 +236,7 @@ __global__ void __launch_bounds__(THREADS) kv8_select_kernel(EvictArgs a) {
   const int rank = CS > 1 ? (int)cluster_ctarank() : 0;
   const long long bh = blockIdx.x / CS;
   const int h = (int)(bh % a.H), b = (int)(bh / a.H);
+  if constexpr (CS > 1) cluster_sync();  // every CTA of the cluster has started before another one writes its shared memory
   griddep_wait();
   griddep_launch();
   int len = a.lens[b];
@@ -283,6 +284,7 @@ __global__ void __launch_bounds__(THREADS) kv8_select_kernel(EvictArgs a) {
         const unsigned int v = tid % 3 == 0 ? sum[0] : tid % 3 == 1 ? sum[1] : sum[2];
         asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(v) : "memory");
       }
+      __syncwarp();  // the barrier below is one for whole warps
       cluster_sync();
 #pragma unroll
       for (int k = 0; k < 3; k++) {
@@ -358,6 +360,7 @@ __global__ void __launch_bounds__(THREADS) kv8_select_kernel(EvictArgs a) {
       const uint32_t to = mapa_shared(smem_u32(&sh_before[rank][tid & 1]), tid / 2);
       asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(tid & 1 ? te : tg) : "memory");
     }
+    __syncwarp();
     cluster_sync();  // the last access to another CTA's shared memory is before it
     for (int r = 0; r < rank; r++) bg += sh_before[r][0], be += sh_before[r][1];
   }
