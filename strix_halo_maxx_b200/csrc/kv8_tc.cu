@@ -219,13 +219,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
   // registers by role: 512 threads are launched with 128 each; the softmax holds 64 scores, and its spills cost 307 against
   // 284 us for the 2048-token chunk
   static_assert(2 * SOFTMAX_REGS + CONVERT_REGS + MMA_REGS <= 4 * 128, "the split must come out of the launch's registers");
-  if (warp >= 14) {
-    set_regs_down<MMA_REGS>();  // idle; the issuers' warp group
-  } else if (warp >= 12) {
-    set_regs_down<MMA_REGS>();
+  if (warp >= 12) {
+    set_regs_down<MMA_REGS>();  // one instruction for the whole warp group
     // ---------------- MMA issuer of M tile t, one warp each (one thread for both tiles: 435 against 335 us for the 2048-token
     // chunk).  The whole warp walks the loop, one lane issues.  j: key tiles of all segments; js: of those in which t had rows
-    const int t = warp - 12;
+    const int t = warp - 12, end = t < 2 ? u_end : u_begin;  // warps 14 and 15 are idle
     const uint32_t leader = elect_one();
     constexpr uint32_t IDESC_S = idesc_bf16(128, KEYS), IDESC_O = idesc_bf16(128, D) | (1u << 16);  // V MN-major
     const uint64_t dq = sdesc_noswz(smem_u32(sm) + t * L::QT, 2048, 128), dk = sdesc_noswz(smem_u32(sm + L::K), 1024, 128);
@@ -234,7 +232,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
     bool ok = true;
     int st = 0, ph = 0, js = 0, so = 0;  // stage and phase of the next tile's operands; tiles, segments in which t had rows
     auto next = [](int& x, int& y) { if (++x == ST) x = 0, y ^= 1; };
-    for (int u = u_begin; u < u_end && ok;) {
+    for (int u = u_begin; u < end && ok;) {
       const Seg g = segment(a, pre, u, u_end);
       const int nt = g.tb - g.ta;
       u += nt;
@@ -278,7 +276,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       }
       js += nt, so++;
     }
-    if (leader) {
+    if (leader && t < 2) {
       umma_commit(&drain[t]);
       mbar_wait_drain(&drain[t], 0, kDrainCycles);
     }

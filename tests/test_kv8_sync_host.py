@@ -21,3 +21,12 @@ def test_no_store_into_another_cta_before_its_cluster_has_started():
     for m in re.finditer(r"st\.shared::cluster", k):
         rest = k[m.end():]
         assert "__syncwarp();" in rest[:rest.index("cluster_sync();")]
+
+
+def test_a_warp_group_changes_its_registers_at_one_instruction():
+    """setmaxnreg is one instruction for all four warps of a group, so no branch that leads to one may part a group."""
+    k = _kernel("attn_kv8_tc_kernel", "kv8_tc.cu")
+    uses = [m.start() for m in re.finditer(r"set_regs_(up|down)<", k)]
+    assert len(uses) == 3
+    for at in uses:
+        assert int(re.findall(r"if \(warp >= (\d+)\)", k[:at])[-1]) % 4 == 0
