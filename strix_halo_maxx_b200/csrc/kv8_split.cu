@@ -16,7 +16,10 @@
 //           largest value, below that off by 2^-25 of it;
 //   scores  fp32 accumulators times (row's power of two * scale * log2 e * the block's K scale): the scale is
 //           applied to the exact sum of products of codes, so it costs one multiplication a score;
-//   P       2^(s - m) in f16 (11 bits); S^T's accumulator layout becomes the B operand of O^T = V^T P^T by movmatrix;
+//   P       2^(s - m) in f16, with m 15 below the largest score so far, so that P uses f16's range up to 2^15: 11 bits down to 2^-29
+//           of a row's largest weight, below that off by 2^-40 of it at most (the sum takes P before it is rounded; with
+//           m at the largest score itself, keys 15 nats below a sink lost 0.5 % and 17.6 nats below it 17 %); S^T's
+//           accumulator layout becomes the B operand of O^T = V^T P^T by movmatrix;
 //   V^T     needs two keys of one dim in a register: four words of four keys are transposed by byte permutes.  Which
 //           of a tile's keys is which row of the MMA is free, so lane t takes keys t, 4 + t, 8 + t, 12 + t: its reads are
 //           free of bank conflicts (rows 64 B apart), and K's rows follow the same order;
@@ -42,6 +45,7 @@ constexpr int MIN_RUN = WARPS;                     // tiles of a run at least
 // 531 with weights 40.3 against 36.1).
 constexpr int WHOLE_WARPS = 8, WHOLE_TILES = 16;
 constexpr long long kDrainCycles = 200000000LL;
+constexpr float P_UP = 15.f, P_SCALE = 0x1p15f;  // how far m is below the largest score (log2 units); O is kept divided by 2^15, see vc
 
 struct Plan {       // fixed on the host from sizes alone
   int rows, nt, rg;   // rows n G of a kv head, rows / 8 of a row group, row groups
@@ -338,12 +342,12 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
         float mu[2];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-          float mx = m[nt][k];
+          float mx = -INFINITY;
 #pragma unroll
           for (int x = 0; x < MT; x++) mx = max3f(mx, sc[x][nt][k], sc[x][nt][2 + k]);
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          mx = fmaxf(m[nt][k], fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)) - P_UP);
           mu[k] = mx == -INFINITY ? 0.f : mx;  // no key in sight yet: every exponential below is 0
           al[nt][k] = ex2_approx(m[nt][k] - mu[k]);
           m[nt][k] = mx;
@@ -364,12 +368,12 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
         for (int k = 0; k < 2; k++) l[nt][k] = l[nt][k] * al[nt][k] + sum[k];
       }
       // ---- O^T = alpha O^T + vs V^T P^T: word w of lane g is dims g D/8 + 4w .. + 3, two m-tiles.  A row that sees
-      // nothing of the tile gets no product with its scale, which may be NaN
+      // nothing of the tile gets no product with its scale, which may be NaN; P's 2^15 is taken out, so that no scale overflows
       float vc[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int k = 0; k < 2; k++) vc[nt][k] = edge && key0 >= lim[nt][k] ? 0.f : vs;
+        for (int k = 0; k < 2; k++) vc[nt][k] = edge && key0 >= lim[nt][k] ? 0.f : vs * (1.f / P_SCALE);
 #pragma unroll
       for (int w = 0; w < D / 32; w++) {
         float acc[2][NT][4];
@@ -444,7 +448,7 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
         sum += sh_l[w][r] * f, v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
       }
       if (whole) {
-        const float inv = 1.f / sum;
+        const float inv = P_SCALE / sum;
         uint16_t* op = a.out + b * a.so_b + row / a.G * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
         *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
         if (d == 0 && a.w) {
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
         const float4 x = sh_o[tid + k * (D / 4)];
         v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
       }
-      const float inv = 1.f / sum;
+      const float inv = P_SCALE / sum;
       uint16_t* op = a.out + b * a.so_b + row / a.G * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
       *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
     }

@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 from strix_halo_maxx_b200 import ops
 from strix_halo_maxx_b200._lib import device_status
 from oracle import kv8_ref as R
-from test_kv8_gpu import DEV, as_np, filled, i32, np_
+from test_kv8_gpu import BF, DEV, as_np, filled, i32, np_
 
 
 @pytest.fixture(autouse=True)
@@ -39,3 +39,76 @@ def test_kv8_evict_over_clusters_with_few_or_no_places_left_for_weights(B, H, D,
             assert np.array_equal(np_(dw)[b], np.take_along_axis(np_(w)[b], ref[b][0], -1))
             for got, want in zip(as_np(dst), ref[b][1:]):
                 assert np.array_equal(got[b], want)
+
+
+# ------------------------------------------------------------------------------------------------ attention
+def attention64(q, cache, lens, counts=None, causal=True, scale=None, w_in=None):
+    """out, weights, the sums of p |v| behind each output and a bound on the error of each weight (scores in fp32, as in
+    oracle.kv8_ref.attention), in 64 bits on the GPU; rows past the count and slots past the end NaN."""
+    B, H, C, D = cache.k.shape
+    n, Hq = q.shape[1:3]
+    G, scale = Hq // H, D ** -0.5 if scale is None else scale
+    nan = lambda *s: torch.full(s, float("nan"), dtype=torch.float64, device=DEV)
+    out, mag, w, werr = nan(B, n, Hq, D), nan(B, n, Hq, D), nan(B, H, C), nan(B, H, C)
+    for b in range(B):
+        L, m = lens[b], n if counts is None else counts[b]
+        T = L + m
+        blk = torch.arange(T, device=DEV) // 64
+        w[b, :, :T], werr[b, :, :T] = 0, 0
+        if w_in is not None:
+            w[b, :, :L] = w_in[b, :, :L].double()
+        for h in range(H if m else 0):
+            k, v = (c[b, h, :T].double() * s[b, h, blk].double()[:, None] for c, s in ((cache.k, cache.ks), (cache.v, cache.vs)))
+            x = q[b, :m, h * G:h * G + G].double().reshape(m * G, D)
+            z = x @ k.T * scale
+            d = ((x.abs() @ k.abs().T) * (abs(scale) * D * 2.0 ** -24) + z.abs() * 2.0 ** -22)
+            if causal:
+                i = torch.arange(m, device=DEV).repeat_interleave(G)[:, None]
+                hide = torch.arange(T, device=DEV)[None] > L + i
+                z.masked_fill_(hide, -float("inf"))
+                d.masked_fill_(hide, 0)
+            p = torch.softmax(z, -1)
+            out[b, :m, h * G:h * G + G] = (p @ v).view(m, G, D)
+            mag[b, :m, h * G:h * G + G] = (p @ v.abs()).view(m, G, D)
+            w[b, h, :T] += p.sum(0)
+            werr[b, h, :T] += (p * 2 * d.amax(-1, keepdim=True)).sum(0)
+    return out.flatten(2), w, mag.flatten(2), werr
+
+
+def check64(q, cache, lens, counts, causal, out, w=None, w_in=None, scale=None, random_v=True):
+    """Outputs: the rounding to bf16, half a step or 2^-8 of the value; P in 11 bits, 2^-11 of each term p |v|; scores and sums
+    in fp32, below 2^-12 of the terms (|score| < 100).  Where V has both signs the roundings of P are independent and
+    add in squares to an eighth of the output's own: 1.01 of it in the 2-norm, 1.1 allowed."""
+    ro, rw, mag, werr = attention64(q, cache, lens, counts, causal, scale, w_in)
+    at = ~torch.isnan(ro)
+    err, bound = (out.double() - ro).abs()[at], (ro.abs() * 2.0 ** -8 + mag * (2.0 ** -11 + 2.0 ** -12))[at]
+    assert (err <= bound * (1 + 2.0 ** -7)).all(), float((err / bound).max())
+    if random_v:
+        own = (ro.to(torch.bfloat16).double() - ro)[at].norm()
+        assert err.norm() <= 1.1 * own, float(err.norm() / own)
+    if w is not None:
+        n, G, at = q.shape[1], q.shape[2] // cache.k.shape[1], ~torch.isnan(rw)
+        tol = werr + rw.abs() * (2.0 ** -18 + (n * G + 1) * 2.0 ** -24) + 1e-30
+        err, tol = (w.double() - rw).abs()[at], tol[at]
+        assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("gap", [9.0, 15.0, 17.0, 17.6])
+@pytest.mark.parametrize("n,D,T,Hq", [(1, 64, 730, 2), (1, 128, 500, 8), (32, 64, 762, 2), (32, 128, 400, 2), (5, 64, 2500, 6), (1, 128, 2500, 4)])
+def test_attn_kv8_few_rows_keep_what_stands_beside_a_sink(n, D, T, Hq, gap):
+    """One key takes nearly all the weight and its value is zero, so the output is made of weights e^-gap: as exact as others."""
+    _sink(n, D, T, Hq, gap)
+
+
+def _sink(n, D, T, Hq, gap):
+    H, C = 2, (T + 63) // 64 * 64
+    cache = filled(1, H, C, D, n)
+    cache.k.zero_()
+    cache.ks.fill_(1 / 128)
+    cache.v.copy_(cache.v.abs() // 4 + 90)   # one sign: the losses would add up
+    cache.k[:, :, 3, 0] = 127
+    cache.v[:, :, 3] = 0
+    q = torch.randn(1, n, Hq, D, device=DEV, generator=torch.Generator(DEV).manual_seed(2)).to(BF)
+    q[..., 0] = 1
+    out = ops.attn_kv8(q, cache, i32([T - n]), scale=gap * 128 / 127)
+    check64(q, cache, [T - n], None, True, out, scale=gap * 128 / 127, random_v=False)
