@@ -12,8 +12,8 @@
 // operands; here a code goes from shared memory through two byte permutes and a subtraction into a register of
 // the operand.  S^T = K Q^T: keys are the M dimension (16 a step), rows the N dimension (8).
 //   codes   byte b -> 0x6400 | (b ^ 0x80) = 1152 + code in f16, minus 1152: exact;
-//   q       bf16 -> f16 after scaling each row by a power of two to max 1 .. 2: exact down to 2^-14 of the row's
-//           largest value, below that off by 2^-25 of it;
+//   q       bf16 -> f16 after scaling each row by a power of two to max 2^15 .. 2^16 (f16 ends there): exact down to 2^-32
+//           of the row's largest value, below that off by 2^-40 of it;
 //   scores  fp32 accumulators times (row's power of two * scale * log2 e * the block's K scale): the scale is
 //           applied to the exact sum of products of codes, so it costs one multiplication a score;
 //   P       2^(s - m) in f16, with m 15 below the largest score so far, so that P uses f16's range up to 2^15: 11 bits down to 2^-29
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
       for (int j = 0; j < min(mine, ST); j++) load(j);
     float ks_next = 0.f, vs_next = 0.f;  // scales of the next tile
     if (mine > 0) ks_next = ksp[(ta + warp) * KT / BLK], vs_next = vsp[(ta + warp) * KT / BLK];
-    // q of rows r0 + 8 nt + g, this lane's dims t D/4 .. as f16 pairs, scaled to a largest value of 1 .. 2
+    // q of rows r0 + 8 nt + g, this lane's dims t D/4 .. as f16 pairs, scaled to a largest value of 2^15 .. 2^16
     uint32_t qf[NT][WQ][2];
     float cq[NT][2];  // scale of columns 2t, 2t + 1: scale * log2 e * the row's power of two
     int lim[NT][2];   // keys that they see
@@ -238,8 +238,8 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
       top = max(top & 0xffffu, top >> 16);
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // exponent e of the row's largest value: 2^-e as a float; zero rows and non-finite ones stay as they are
-      const int e = (int)(top >> 7), sh = top == 0 || e == 255 ? 0 : e == 0 ? -126 : max(min(e - 127, 126), -126);
+      // exponent e of the row's largest value: 2^(15 - e) as a float (2^126 at most); zero rows and non-finite ones stay as they are
+      const int e = (int)(top >> 7), sh = top == 0 || e == 255 ? 0 : max(e - 127 - 15, -126);
       const float f = __uint_as_float((uint32_t)(127 - sh) << 23);
 #pragma unroll
       for (int w = 0; w < WQ; w++)

@@ -112,3 +112,17 @@ def _sink(n, D, T, Hq, gap):
     q[..., 0] = 1
     out = ops.attn_kv8(q, cache, i32([T - n]), scale=gap * 128 / 127)
     check64(q, cache, [T - n], None, True, out, scale=gap * 128 / 127, random_v=False)
+
+
+@pytest.mark.parametrize("n,D,T,Hq", [(1, 64, 730, 2), (2, 128, 2500, 8), (32, 64, 762, 2)])
+def test_attn_kv8_queries_with_one_value_far_above_the_others(n, D, T, Hq):
+    """The scores come from values 2^-22 of the row's largest, which meets keys that are zero there."""
+    H, C = 2, (T + 63) // 64 * 64
+    cache = filled(1, H, C, D, n)
+    cache.k[..., 7] = 0
+    cache.ks.fill_(1.0)
+    q = (torch.randn(1, n, Hq, D, device=DEV, generator=torch.Generator(DEV).manual_seed(2)) * 2.0 ** -12).to(BF)
+    q[..., 7] = 1024
+    w = torch.zeros(1, H, C, device=DEV)
+    out = ops.attn_kv8(q, cache, i32([T - n]), scale=16.0, weights=w)
+    check64(q, cache, [T - n], None, True, out, w, scale=16.0)
