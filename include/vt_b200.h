@@ -309,8 +309,11 @@ int vt_rope_kv8(cudaStream_t stream, const uint16_t* qkv, long long sx_b, long l
 long long vt_attn_kv8_ws_bytes(int B, int n, int Hq, int H, int D, int C, int weights);
 
 /* Attention of the n new rows of each sequence over its cache, their own tokens already in it: row i of sequence b
- * sees slots 0 .. lens[b] + i (causal != 0) or 0 .. lens[b] + counts[b] - 1; softmax(scale q k^T) v, sums in fp32, out
- * bf16 at out + b*so_b + i*so_t + hq*so_h (not over q).  V scales of 2^-100 .. 2^100.  weights fp32 [B][H][C] (NULL: none) receives the attention weight of each
+ * sees slots 0 .. lens[b] + i (causal != 0) or 0 .. lens[b] + counts[b] - 1; softmax(scale q k^T) v, out
+ * bf16 at out + b*so_b + i*so_t + hq*so_h (not over q).  Scores, maxima, sums, O and weights are fp32; before they meet V the
+ * probabilities are rounded to f16's 11 bits, terms p * V scale below 2^-21 of the row's largest to 2^-32 of that.  With n Hq / H <= 32
+ * q values below 2^-32 of their row's largest are rounded to 2^-40 of it; all else of q, k and v is exact.  V scales of 2^-100 .. 2^100,
+ * those of a head within 2^64 of one another; smaller ones count as zero.  weights fp32 [B][H][C] (NULL: none) receives the attention weight of each
  * slot j < lens[b] + counts[b]: its probabilities summed over the sequence's rows and the group's query heads, plus
  * weights_in[b][h][j] (NULL: none; may be weights) for j < lens[b].  ws: vt_attn_kv8_ws_bytes bytes, 16-byte
  * aligned, one call at a time.  Results do not depend on the other sequences of the batch beyond the rounding of

@@ -6,14 +6,18 @@
 // that spans CTAs leaves its parts (unnormalised O, row max, row sum) for attn_kv8_tc_join_kernel.
 //
 // CTA = 16 warps (two of them idle):
-//   warps 0-3, 4-7   softmax of M tile 0 / 1, thread = row (TMEM lane): P = 2^(s - m) as bf16 over the scores;
-//   warps 8-11       codes -> bf16 operands in shared memory (ST stages), one tile's codes ahead in registers; q once an item;
+//   warps 0-3, 4-7   softmax of M tile 0 / 1, thread = row (TMEM lane): q once an item, then P as f16 over the scores;
+//   warps 8-11       codes -> operands in shared memory (ST stages), K's as bf16 and V's as f16, one tile's codes ahead in registers;
 //   warps 12, 13     tcgen05.mma of M tile 0 / 1: S_(j+1), then O += P_j V_j (P from TMEM, V as an MN-major B operand).
-// Codes are exact in bf16: byte b -> 0x4300 | b, and (that & ~0x80) - (that & 0x80 | 0x4300) = 128 + low bits - (128 or 256).
-// K and V tiles have the same layout (no-swizzle core matrices, [D/8][64][8]), so both take the same conversion.
-// Scales cost nothing per score: K's joins the softmax scale of the tile; V's shifts the exponent, P' = vs P = 2^(s - (m - log2
-// vs)), and the row sum takes sum(P') / vs.  So P' is rounded to bf16 with its scale in the exponent, whatever its size
-// (scales of 2^-100 .. 2^100; V blocks with a smaller one are zeros).
+// Codes are exact in both types: in bf16 byte b -> 0x4300 | b, and (that & ~0x80) - (that & 0x80 | 0x4300) = 128 + low bits -
+// (128 or 256); in f16 (0x6400 | b ^ 0x80) - 1152.  K and V tiles have the same layout (no-swizzle core matrices, [D/8][64][8]).
+// Scales cost nothing per score: K's joins the softmax scale of the tile; V's shifts the exponent, P' = vs P = 2^(s + log2 vs - m),
+// and the row sum takes sum(P') / vs before P' is rounded.  P' is at most 2^15.9: m begins P_UP below the row's largest s + log2 vs and
+// moves, O through registers, when that has grown by P_MOVE (by 4 instead of 8: 319 against 275 us below).  So P' has f16's 11 bits
+// down to 2^-21 of the row's largest term and is off by 2^-32 of it below that; where one key is far above all before it and
+// beside it, such as a sink, m goes P_UP_SINK below it and these are 2^-27 and 2^-38.  (In bf16, with its 8 bits, an output's error
+// against 64 bits was 1.4 times its own rounding.)  V blocks with a scale below 2^-100 are zeros and take another block's scale
+// for P'.  The scales of a head's other blocks may differ by 2^64.
 // A 2048-token chunk over 6001 slots (32 / 8 heads x 128, 236 GFLOP): 277 us, 850 TFLOP/s.  A tile takes about 2,040 cycles: the
 // exponentials occupy the MUFU for 1,024 (16 a clock and SM), the MMAs are issued over about 1,500, and P -> PV -> S of a
 // score buffer is a chain of which two are in flight.  128-key tiles with one score buffer were slower (346 us), so were
@@ -28,7 +32,8 @@ namespace tc {
 constexpr int ROWS = 256, KEYS = 64, THREADS = 16 * 32, ST = 3, MAXB = 2048;
 constexpr uint32_t TMEM_COLS = 512;  // S of M tile t, buffer f: columns 128 t + 64 f; O of tile t: 256 + 128 t
 constexpr long long kDrainCycles = 200000000LL;
-constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr float P_TOP = 15.9f, P_MOVE = 8.f, P_UP = P_TOP - P_MOVE, P_UP_SINK = P_TOP - 2.f;  // log2 units
+constexpr float L_SCALE = 0x1p-20f, L_LOG2 = -20.f;  // row sums are kept times 2^-20, so that 2^15 / vs does not overflow
 constexpr int SOFTMAX_REGS = 168, CONVERT_REGS = 96, MMA_REGS = 80;
 constexpr float kTinyScale = 0x1p-100f;
 // With caches of up to so many blocks a CTA takes a whole item: equal runs for all SMs would cost more in parts to write and
@@ -152,18 +157,22 @@ __device__ __forceinline__ uint32_t sub_bf2(uint32_t a, uint32_t b) {
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// Two codes (bytes lo, lo + 1 of x) as bf16.
-template <int SEL>
-__device__ __forceinline__ uint32_t bf_of_codes(uint32_t x) {
+// Two codes (bytes lo, lo + 1 of x) as bf16 or f16; x of the latter with its bytes' top bits flipped.
+template <int SEL, bool F16>
+__device__ __forceinline__ uint32_t two_codes(uint32_t x) {
+  if (F16) return split::hsub2(__byte_perm(x, 0x64646464u, SEL), split::H1152);
   const uint32_t w = __byte_perm(x, 0x43434343u, SEL);
   return sub_bf2(w & 0xff7fff7fu, w & 0xff80ff80u);
 }
 // 16 codes of a row: dims 16 p .. of row `row` into operand chunks 2p, 2p + 1 (CR rows each).
-template <int CR>
+template <int CR, bool F16>
 __device__ __forceinline__ void store_codes(uint8_t* tile, int row, int p, uint4 c) {
   uint8_t* at = tile + (2 * p * CR + row) * 16;
-  *reinterpret_cast<uint4*>(at) = make_uint4(bf_of_codes<0x4140>(c.x), bf_of_codes<0x4342>(c.x), bf_of_codes<0x4140>(c.y), bf_of_codes<0x4342>(c.y));
-  *reinterpret_cast<uint4*>(at + CR * 16) = make_uint4(bf_of_codes<0x4140>(c.z), bf_of_codes<0x4342>(c.z), bf_of_codes<0x4140>(c.w), bf_of_codes<0x4342>(c.w));
+  if (F16) c.x ^= 0x80808080u, c.y ^= 0x80808080u, c.z ^= 0x80808080u, c.w ^= 0x80808080u;
+  auto lo = [](uint32_t x) { return two_codes<0x4140, F16>(x); };
+  auto hi = [](uint32_t x) { return two_codes<0x4342, F16>(x); };
+  *reinterpret_cast<uint4*>(at) = make_uint4(lo(c.x), hi(c.x), lo(c.y), hi(c.y));
+  *reinterpret_cast<uint4*>(at + CR * 16) = make_uint4(lo(c.z), hi(c.z), lo(c.w), hi(c.w));
 }
 // The address of q row r of (b, h).
 __device__ __forceinline__ const uint16_t* q_row(const Args& a, int b, int h, int r) {
@@ -225,7 +234,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
     // chunk).  The whole warp walks the loop, one lane issues.  j: key tiles of all segments; js: of those in which t had rows
     const int t = warp - 12, end = t < 2 ? u_end : u_begin;  // warps 14 and 15 are idle
     const uint32_t leader = elect_one();
-    constexpr uint32_t IDESC_S = idesc_bf16(128, KEYS), IDESC_O = idesc_bf16(128, D) | (1u << 16);  // V MN-major
+    constexpr uint32_t IDESC_S = idesc_bf16(128, KEYS), IDESC_O = idesc_f16(128, D) | (1u << 16);  // V MN-major
     const uint64_t dq = sdesc_noswz(smem_u32(sm) + t * L::QT, 2048, 128), dk = sdesc_noswz(smem_u32(sm + L::K), 1024, 128);
     const uint64_t dv = sdesc_noswz(smem_u32(sm + L::V), 128, 1024);
     const uint32_t t_s = tmem + 128 * t, t_o = tmem + 256 + 128 * t;
@@ -303,11 +312,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
         for (int x = 0; x < PER; x++)
           to[x] = *reinterpret_cast<const uint4*>(from + (row + 8 * (x & 1)) * D + 16 * (piece + 4 * (x >> 1)));
       };
-      auto convert = [&](uint8_t* tile, const uint4 (&from)[PER], bool zero) {
-#pragma unroll
-        for (int x = 0; x < PER; x++)
-          store_codes<KEYS>(tile, row + 8 * (x & 1), piece + 4 * (x >> 1), zero ? make_uint4(0, 0, 0, 0) : from[x]);
-      };
       fetch(kr, kp);
       fetch(vr, vp);
       vs = vsp[0];
@@ -316,9 +320,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
         if (j >= ST) ok = wait(&kv_empty[st], (j / ST - 1) & 1);
         if (!ok) break;
         kp += KEYS * D, vp += KEYS * D;
-        convert(sm + L::K + st * L::KT, kr, false);
+#pragma unroll
+        for (int x = 0; x < PER; x++) store_codes<KEYS, false>(sm + L::K + st * L::KT, row + 8 * (x & 1), piece + 4 * (x >> 1), kr[x]);
         if (i + 1 < nt) fetch(kr, kp);
-        convert(sm + L::V + st * L::KT, vr, vs < kTinyScale);
+#pragma unroll
+        for (int x = 0; x < PER; x++)
+          store_codes<KEYS, true>(sm + L::V + st * L::KT, row + 8 * (x & 1), piece + 4 * (x >> 1), vs < kTinyScale ? make_uint4(0, 0, 0, 0) : vr[x]);
         if (i + 1 < nt) fetch(vr, vp), vs = vsp[i + 1];
         fence_proxy_async_smem();
         __syncwarp();
@@ -366,12 +373,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       // the fewest keys that a row of this warp sees: tiles up to there need no mask
       const int lim_min = __reduce_min_sync(0xffffffffu, lim);
       float m = -INFINITY, l = 0.f;
-      // of the tile: K's scale times the softmax scale, log2 and inverse of V's scale (the approximations err by 2^-22, both
-      // in the sum and in O); the next tile's are worked out while this one's scores arrive
-      float c, lvs, ivs, ks_next = ksp[0], vs_next = vsp[0], c_next, lvs_next, ivs_next;
+      // of the tile: K's scale times the softmax scale, log2 and inverse (times L_SCALE) of V's scale (the approximations err by
+      // 2^-22, both in the sum and in O); the next tile's are worked out while this one's scores arrive
+      float c, lvs, ivs, ks_next = ksp[0], vs_next = vsp[0], c_next, lvs_next, ivs_next, v = vs_next;
+      if (!(v >= kTinyScale)) {  // the first scale of the run that is one
+        v = 1.f;
+        for (int i = nt - 1; i >= 0; i--) v = vsp[i] >= kTinyScale ? vsp[i] : v;
+      }
       auto next_scales = [&](int i) {
-        const float v = vs_next < kTinyScale ? 1.f : vs_next;  // the converters made V zero
-        c_next = ks_next * a.scale_log2, lvs_next = __log2f(v), ivs_next = __frcp_rn(v);
+        v = vs_next < kTinyScale ? v : vs_next;  // the converters made V zero
+        c_next = ks_next * a.scale_log2, lvs_next = __log2f(v), ivs_next = __frcp_rn(v) * L_SCALE;
         if (i + 1 < nt) ks_next = ksp[i + 1], vs_next = vsp[i + 1];
       };
       next_scales(0);
@@ -396,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
           for (int e = 0; e < 3; e++) x[e] = max3f(x[3 * e], x[3 * e + 1], x[3 * e + 2]);
           return max3f(max3f(x[0], x[1], x[2]), x[9], x[10]);
         };
-        // P' = 2^(s c - (m - log2 vs)) of 32 scores into columns `at` of P; returns their sum
+        // P' = 2^(s c + log2 vs - m) of 32 scores into columns `at` of P; returns their sum
         auto exps = [&](const uint32_t (&r)[32], uint32_t at, float mu) {
           const unsigned long long c2 = f2_pack(c, c), sh2 = f2_pack(lvs - mu, lvs - mu);
           unsigned long long sum2[2] = {0ull, 0ull};
@@ -407,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
             f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), c2, sh2), x0, x1);
             const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
             sum2[e & 1] = f2_add(sum2[e & 1], f2_pack(p0, p1));
-            pk[e] = pack_bf2(p0, p1);
+            pk[e] = split::pack_h2(p0, p1);
           }
           tmem_st16(t_s + at, pk);
           float lo, hi;
@@ -422,7 +433,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
         tmem_ld_wait();
         tmem_ld32(t_s + 32, r1);
         // a tile that every row sees whole, once a row has a maximum: P with the maximum so far, while the second half of
-        // the scores arrives and the new maximum is found beside the exponentials; they stand unless it grew by 2^8
+        // the scores arrives and the new maximum is found beside the exponentials; they stand unless it grew too far
         const bool edge = key0 + KEYS > lim_min;
         bool again = i == 0 || edge;
         if (!again) {
@@ -430,8 +441,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
           const float ma = top32(r0);
           tmem_ld_wait();
           sum += exps(r1, 16, m);
-          mx = fmaxf(ma, top32(r1)) * c;
-          again = __any_sync(0xffffffffu, mx > m + kRescaleThreshold);
+          mx = fmaf(fmaxf(ma, top32(r1)), c, lvs);
+          again = __any_sync(0xffffffffu, mx > m + P_TOP);
         }
         if (again) {
           tmem_ld_wait();
@@ -443,9 +454,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
               if (32 + e >= left) r1[e] = 0xff800000u;
             }
           }
-          mx = left > 0 ? fmaxf(top32(r0), top32(r1)) * c : -INFINITY;
-          const bool need = mx > m + kRescaleThreshold;
-          const float mn = i == 0 || need ? mx : m;
+          mx = left > 0 ? fmaf(fmaxf(top32(r0), top32(r1)), c, lvs) : -INFINITY;
+          const bool need = mx > m + P_TOP;
+          const float mn = i == 0 ? mx - P_UP : need ? mx - (mx > m + (P_TOP + 12.f) ? P_UP_SINK : P_UP) : m;
           if (i > 0 && __any_sync(0xffffffffu, need)) {  // O through registers (warp-collective)
             // O must hold every product up to tile i - 1; the barrier's next arrival, ST tiles on, needs P of this row
             ok = wait(&kv_empty[(j + i - 1) % ST], ((j + i - 1) / ST) & 1);
@@ -479,6 +490,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
             }
           }
           sum = exps(r0, 0, mu) + exps(r1, 16, mu);
+          if (i == 0) {  // a tile whose other keys add up to a twentieth of its largest one
+            const bool sink = sum < 1.05f * exp2f(P_UP);
+            if (__any_sync(0xffffffffu, sink)) {
+              m -= sink ? P_UP_SINK - P_UP : 0.f;
+              const float ms = m == -INFINITY ? 0.f : m;
+              sum = exps(r0, 0, ms) + exps(r1, 16, ms);
+            }
+          }
         }
         l += sum * ivs;
         announce(f);
@@ -490,7 +509,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       if (!ok) break;
       tc_fence_after();
       const bool whole = done.ta == 0 && done.tb == done.tiles;
-      const float inv = 1.f / l;
+      const float inv = L_SCALE / l;
       const int at = row - done.r0;
       const size_t slot = (2 * (size_t)blockIdx.x + (first ? 0 : 1)) * ROWS + at;
       uint16_t* op = a.out + done.b * a.so_b + row / a.G * a.so_t + (size_t)(done.h * a.G + row % a.G) * a.so_h;
@@ -517,7 +536,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       }
       if (row < valid) {
         if (!whole) a.part_ml[slot] = make_float2(m, l);
-        else if (a.lse) a.lse[bh * a.rows + row] = -(m + log2f(l));
+        else if (a.lse) a.lse[bh * a.rows + row] = -(m - L_LOG2 + log2f(l));
       }
       tc_fence_before();
       __syncwarp();
@@ -566,10 +585,10 @@ __global__ void __launch_bounds__(128) attn_kv8_tc_join_kernel(Args a) {
       const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - mx);
       sum += ml.y * f, v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
     }
-    const float inv = 1.f / sum;
+    const float inv = L_SCALE / sum;
     uint16_t* op = a.out + g.b * a.so_b + row / a.G * a.so_t + (size_t)(g.h * a.G + row % a.G) * a.so_h + d;
     *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
-    if (d == 0 && a.lse) a.lse[bh * a.rows + row] = -(mx + log2f(sum));
+    if (d == 0 && a.lse) a.lse[bh * a.rows + row] = -(mx - L_LOG2 + log2f(sum));
   }
 }
 
@@ -677,7 +696,7 @@ __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
       const int row = 32 * w + 8 * (x & 3) + (lane & 7), p = (lane >> 3) + 4 * (x >> 2);
       uint4 c = make_uint4(0, 0, 0, 0);
       if (key0 + row < a.C) c = *reinterpret_cast<const uint4*>(kp + (size_t)(key0 + row) * D + 16 * p);
-      store_codes<WK>(sm + L::K, row, p, c);
+      store_codes<WK, false>(sm + L::K, row, p, c);
     }
     for (int i = 0; i < nt; i++) {
       asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");

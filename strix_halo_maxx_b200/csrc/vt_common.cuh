@@ -307,7 +307,7 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
                : "memory");
 }
 // 32 lanes x 32 consecutive 32-bit columns: thread i of the warp gets lane (base lane + i).
-// The same with A in tensor memory (rows = lanes, two bf16 per 32-bit column, K-major).
+// The same with A in tensor memory (rows = lanes, two bf16 or f16 per 32-bit column, K-major); A's and B's type as idesc says.
 __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
                                             uint32_t accumulate) {
   asm volatile(
@@ -475,6 +475,10 @@ __device__ __forceinline__ uint64_t sdesc_k_sw128(uint32_t saddr) {
 // Instruction descriptor, kind::f16: D fp32, A and B bf16, both K-major, shape M x N.
 __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// The same with A and B f16 (format 0).
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 // kind::i8: s32 accumulator (bits 4-5 = 2), signed 8-bit A and B (bits 7-9, 10-12 = 1), both K-major.
 __host__ __device__ constexpr uint32_t idesc_i8(int M, int N) {

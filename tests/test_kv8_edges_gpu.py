@@ -114,7 +114,7 @@ def _sink(n, D, T, Hq, gap):
     check64(q, cache, [T - n], None, True, out, scale=gap * 128 / 127, random_v=False)
 
 
-@pytest.mark.parametrize("n,D,T,Hq", [(1, 64, 730, 2), (2, 128, 2500, 8), (32, 64, 762, 2)])
+@pytest.mark.parametrize("n,D,T,Hq", [(1, 64, 730, 2), (2, 128, 2500, 8), (32, 64, 762, 2), (60, 64, 762, 2)])
 def test_attn_kv8_queries_with_one_value_far_above_the_others(n, D, T, Hq):
     """The scores come from values 2^-22 of the row's largest, which meets keys that are zero there."""
     H, C = 2, (T + 63) // 64 * 64
@@ -126,3 +126,40 @@ def test_attn_kv8_queries_with_one_value_far_above_the_others(n, D, T, Hq):
     w = torch.zeros(1, H, C, device=DEV)
     out = ops.attn_kv8(q, cache, i32([T - n]), scale=16.0, weights=w)
     check64(q, cache, [T - n], None, True, out, w, scale=16.0)
+
+
+@pytest.mark.parametrize("gap", [9.0, 15.0, 17.0, 17.6])
+@pytest.mark.parametrize("n,D,T,Hq", [(64, 64, 730, 2), (200, 128, 1000, 4), (70, 64, 2500, 2), (300, 128, 2500, 2)])
+def test_attn_kv8_many_rows_keep_what_stands_beside_a_sink(n, D, T, Hq, gap):
+    _sink(n, D, T, Hq, gap)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n,Hq,H,D,L", [(730, 4, 4, 64, 0), (40, 8, 2, 128, 700), (513, 4, 2, 128, 2000), (129, 2, 2, 64, 3000), (16, 4, 2, 64, 500)])
+def test_attn_kv8_rounds_its_probabilities_to_11_bits(n, Hq, H, D, L, causal):
+    """The output's own rounding to bf16 is what is left of the error; V's scales differ from block to block by up to 2^12, some
+    blocks are all zeros, and rows rescale (the largest scores come late)."""
+    C = (L + n + 63) // 64 * 64
+    cache = filled(1, H, C, D, n)
+    g = torch.Generator(DEV).manual_seed(L + n)
+    cache.vs.copy_(2.0 ** (torch.rand(cache.vs.shape, device=DEV, generator=g) * 12 - 6))
+    cache.vs[:, :, 1::7] = 0
+    cache.ks.mul_(torch.linspace(0.5, 3, C // 64, device=DEV))
+    q = (torch.randn(1, n, Hq, D, device=DEV, generator=g) * 1.5).to(BF)
+    w = torch.zeros(1, H, C, device=DEV)
+    out = ops.attn_kv8(q, cache, i32([L]), causal=causal, weights=w)
+    check64(q, cache, [L], None, causal, out, w)
+
+
+def test_attn_kv8_many_rows_take_scales_over_their_whole_range():
+    """V scales of 2^-100 and of 2^100, beside zeros; weights count every key."""
+    H, D, n, C = 2, 64, 80, 512
+    for e in (-100, -60, 60, 99):
+        cache = filled(1, H, C, D, 3)
+        cache.vs.mul_(2.0 ** e / 0.03)
+        cache.vs.clamp_(min=2.0 ** -100)
+        cache.vs[:, :, 2] = 0
+        q = torch.randn(1, n, H, D, device=DEV, generator=torch.Generator(DEV).manual_seed(2)).to(BF)
+        w = torch.zeros(1, H, C, device=DEV)
+        out = ops.attn_kv8(q, cache, i32([C - n]), weights=w)
+        check64(q, cache, [C - n], None, True, out, w)
