@@ -18,13 +18,16 @@ constexpr float LOG2E = 1.4426950408889634f;
 struct Seq {
   int len, cnt;
 };
-__device__ __forceinline__ Seq seq_of(const int* lens, const int* counts, int b, int n, int C) {
+__device__ __forceinline__ Seq seq_of(const int* lens, const int* counts, int b, int n, int C, bool record) {
   int len = lens[b], cnt = counts ? counts[b] : n;
   const bool bad = len < 0 || len > C || cnt < 0 || cnt > n || cnt > C - len;
   len = min(max(len, 0), C);
   cnt = min(min(max(cnt, 0), n), C - len);
-  if (bad && threadIdx.x == 0) atomicOr(&g_status, (unsigned int)ST_KV8_RANGE);
+  if (bad && record) atomicOr(&g_status, (unsigned int)ST_KV8_RANGE);
   return {len, cnt};
+}
+__device__ __forceinline__ Seq seq_of(const int* lens, const int* counts, int b, int n, int C) {
+  return seq_of(lens, counts, b, n, C, threadIdx.x == 0);
 }
 
 // ---------------------------------------------------------------- append

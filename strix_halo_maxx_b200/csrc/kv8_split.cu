@@ -99,9 +99,8 @@ __device__ __forceinline__ void tile_list(const Args& a, int kt, int* pre, int* 
   const int per = (a.B + nth - 1) / nth, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
   int sum = 0;
   for (int b = b0; b < b1; b++) {
-    int len = min(max(a.lens[b], 0), a.C);
-    const int cnt = min(min(max(a.counts ? a.counts[b] : a.n, 0), a.n), a.C - len);
-    const int t = cnt ? (len + cnt + kt - 1) / kt * a.H * a.rg : 0;
+    const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C, blockIdx.x == 0);  // those without work are looked at here only
+    const int t = s.cnt ? (s.len + s.cnt + kt - 1) / kt * a.H * a.rg : 0;
     pre[b] = t;
     sum += t;
   }

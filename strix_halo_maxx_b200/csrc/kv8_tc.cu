@@ -95,9 +95,7 @@ __device__ __forceinline__ int tile_list(const Args& a, int* pre, int* scratch) 
   const int per = (a.B + (int)blockDim.x - 1) / (int)blockDim.x, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
   int sum = 0;
   for (int b = b0; b < b1; b++) {
-    Seq s;
-    s.len = min(max(a.lens[b], 0), a.C);
-    s.cnt = min(min(max(a.counts ? a.counts[b] : a.n, 0), a.n), a.C - s.len);
+    const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C, blockIdx.x == 0 && blockIdx.y == 0);  // those without work are looked at here only
     int t = 0;
     const int items = seq_items(a, s);
     if (a.causal)

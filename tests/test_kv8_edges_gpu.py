@@ -163,3 +163,18 @@ def test_attn_kv8_many_rows_take_scales_over_their_whole_range():
         w = torch.zeros(1, H, C, device=DEV)
         out = ops.attn_kv8(q, cache, i32([C - n]), weights=w)
         check64(q, cache, [C - n], None, True, out, w)
+
+
+@pytest.mark.parametrize("n,C", [(40, 2048), (40, 512), (1, 2048), (1, 512)])
+@pytest.mark.parametrize("lens,counts", [([5000, 100], None), ([100, 2 ** 31 - 1], [1, 0]), ([-7, 100], [0, 1]), ([100, 64], [1, -1]), ([100, 64], [1, 2 ** 31 - 1])])
+def test_attn_kv8_records_every_length_beyond_the_cache(n, C, lens, counts):
+    """In every plan, and for sequences that are left without work by it; their rows stay as they were."""
+    cache = filled(2, 2, C, 64, 5)
+    q = torch.randn(2, n, 2, 64, device=DEV, generator=torch.Generator(DEV).manual_seed(2)).to(BF)
+    out = torch.full((2, n, 128), 3.0, dtype=BF, device=DEV)
+    ops.attn_kv8(q, cache, i32(lens), out, counts=None if counts is None else i32(counts))
+    assert device_status(clear=True) == 1 << 9
+    for b in range(2):
+        L, m = min(max(lens[b], 0), C), n if counts is None else min(max(counts[b], 0), n)
+        m = min(m, C - L)
+        assert (out[b, m:] == 3).all() and (out[b, :m] != 3).any(-1).all()
