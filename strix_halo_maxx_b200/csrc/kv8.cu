@@ -533,6 +533,7 @@ static int check_cache(const char* what, const void* kc, const void* vc, const v
   if (B < 0 || H <= 0 || C <= 0 || C % BLK)
     return set_error(E_SHAPE, "%s: B=%d H=%d C=%d (C a multiple of %d)", what, B, H, C, BLK);
   if ((long long)B * H > (1LL << 31) / 2) return set_error(E_SHAPE, "%s: B * H = %lld too large", what, (long long)B * H);
+  if (B == 0) return OK;  // nothing is read: the pointers of an empty batch may be null
   if (!kc || !vc || !ks || !vs || !aligned16(kc) || !aligned16(vc) || (reinterpret_cast<uintptr_t>(ks) & 3) ||
       (reinterpret_cast<uintptr_t>(vs) & 3))
     return set_error(E_SHAPE, "%s: null or unaligned cache pointer (codes 16 bytes, scales 4)", what);

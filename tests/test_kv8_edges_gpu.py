@@ -178,3 +178,15 @@ def test_attn_kv8_records_every_length_beyond_the_cache(n, C, lens, counts):
         L, m = min(max(lens[b], 0), C), n if counts is None else min(max(counts[b], 0), n)
         m = min(m, C - L)
         assert (out[b, m:] == 3).all() and (out[b, :m] != 3).any(-1).all()
+
+
+def test_an_empty_batch_and_no_new_tokens_are_calls_that_do_nothing():
+    for B, n in ((0, 3), (0, 0), (2, 0)):
+        cache, q = ops.kv8_cache(B, 2, 128, 64, DEV), torch.zeros(B, n, 4, 64, dtype=BF, device=DEV)
+        cos = torch.zeros(8, 16, device=DEV)
+        assert ops.rope_kv8(torch.zeros(B, n, 512, dtype=BF, device=DEV), cache, i32([0] * B), cos, cos, q) is q
+        assert ops.attn_kv8(q, cache, i32([0] * B)).shape == (B, n, 256)
+        assert ops.attn_kv8(q, cache, i32([0] * B), weights=torch.zeros(B, 2, 128, device=DEV)).shape == (B, n, 256)
+    cache = ops.kv8_cache(0, 2, 128, 64, DEV)
+    w = torch.zeros(0, 2, 128, device=DEV)
+    assert ops.kv8_evict(cache, w, i32([]), 64, 8, ops.kv8_cache(0, 2, 64, 64, DEV), w[:, :, :64].contiguous(), i32([])).shape == (0, 2, 64)
