@@ -479,7 +479,8 @@ __global__ void __launch_bounds__(128) kv8_gather_kernel(EvictArgs a) {
     const float top = fmaxf(fmaxf(red[k][0], red[k][1]), fmaxf(red[k][2], red[k][3]));
     s[k] = isinf(top) ? __uint_as_float(0x7fc00000u) : __fdiv_rn(top, 127.f);
   }
-  ratio[v][r] = __fdiv_rn(scale[v][r], v ? s[1] : s[0]);
+  // above 2^100 every code of the row is 0 (its value would be the block's largest); an infinite ratio would make them NaN
+  ratio[v][r] = fminf(__fdiv_rn(scale[v][r], v ? s[1] : s[0]), 0x1p100f);
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < 2; k++) {

@@ -190,3 +190,20 @@ def test_an_empty_batch_and_no_new_tokens_are_calls_that_do_nothing():
     cache = ops.kv8_cache(0, 2, 128, 64, DEV)
     w = torch.zeros(0, 2, 128, device=DEV)
     assert ops.kv8_evict(cache, w, i32([]), 64, 8, ops.kv8_cache(0, 2, 64, 64, DEV), w[:, :, :64].contiguous(), i32([])).shape == (0, 2, 64)
+
+
+def test_kv8_evict_zero_codes_under_scales_far_apart():
+    """Zeros stay zeros whatever their block's scale was: 1e30 beside 1e-20, whose ratio is no finite number."""
+    cache = filled(1, 2, 256, 64, 2)
+    cache.k[:, :, :64] = 0
+    cache.v[:, :, 64:128] = 0
+    cache.ks[:, :, 0], cache.vs[:, :, 1] = 1e30, 1e30
+    cache.ks[:, :, 1:] = 1e-20
+    cache.vs[:, :, 0], cache.vs[:, :, 2:] = 1e-20, 1e-20
+    w = torch.rand(1, 2, 256, device=DEV, generator=torch.Generator(DEV).manual_seed(4))
+    dst, dw, dl = ops.kv8_cache(1, 2, 128, 64, DEV), torch.zeros(1, 2, 128, device=DEV), i32([0])
+    idx = ops.kv8_evict(cache, w, i32([256]), 128, 0, dst, dw, dl)
+    (ri, *want), = R.evict(as_np(cache), np_(w), [256], 128, 0)
+    assert np.array_equal(np_(idx)[0], ri)
+    for got, x in zip(as_np(dst), want):
+        assert np.array_equal(got[0], x)
