@@ -714,7 +714,7 @@ __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
     const int half = warp >> 2, key = key0 + (warp & 3) * 32 + lane;
     const uint32_t t_s = tmem + 64 * half + ((uint32_t)((warp & 3) * 32) << 16);
     const float c = key < T ? a.ks[bh * (a.C / BLK) + key / BLK] * a.scale_log2 : 0.f;
-    const int r_min = a.causal ? (key - s.len) * a.G : 0;  // rows before it do not see this key
+    const int r_min = a.causal ? max(key - s.len, 0) * a.G : 0;  // rows before it do not see this key
     const int warp_max = __reduce_max_sync(0xffffffffu, r_min);
     unsigned long long acc2[2] = {0ull, 0ull};
     const unsigned long long c2 = f2_pack(c, c);

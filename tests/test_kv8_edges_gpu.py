@@ -207,3 +207,26 @@ def test_kv8_evict_zero_codes_under_scales_far_apart():
     assert np.array_equal(np_(idx)[0], ri)
     for got, x in zip(as_np(dst), want):
         assert np.array_equal(got[0], x)
+
+
+def test_attn_kv8_weights_of_many_heads_over_a_very_long_cache():
+    """128 query heads on one kv head over 17 million slots: (slots - length) * heads passes 31 bits."""
+    C, D, G = 17_000_000, 64, 128
+    g = torch.Generator(DEV).manual_seed(1)
+    k, v = (torch.randint(-127, 128, (1, 1, C, D), dtype=torch.int8, device=DEV, generator=g) for _ in range(2))
+    ks, vs = (torch.rand(1, 1, C // 64, device=DEV, generator=g) * 0.01 + 0.01 for _ in range(2))
+    cache = ops.Kv8(k, v, ks, vs)
+    q = torch.randn(1, 1, G, D, device=DEV, generator=g).to(BF)
+    w = torch.zeros(1, 1, C, device=DEV)
+    out = ops.attn_kv8(q, cache, i32([C - 1]), weights=w)
+    x, step = q[0, 0].double() * D ** -0.5, 64 * 15625
+    vals = lambda c, s, at: c[0, 0, at:at + step].double() * s[0, 0, at // 64:(at + step) // 64].double().repeat_interleave(64)[:, None]
+    lse = torch.stack([torch.logsumexp(x @ vals(k, ks, at).T, -1) for at in range(0, C, step)]).logsumexp(0)
+    o = torch.zeros(G, D, dtype=torch.float64, device=DEV)
+    for at in range(0, C, step):
+        p = torch.exp(x @ vals(k, ks, at).T - lse[:, None])
+        o += p @ vals(v, vs, at)
+        # scores of up to 30 in fp32, 128 rows: far below 2^-12 of a weight
+        assert torch.allclose(w[0, 0, at:at + step].double(), p.sum(0), rtol=2.0 ** -12, atol=0), at
+    # means of 17 million values of both signs: small beside the values, whose rounded weights and fp32 sums leave 2^-12 of their size
+    assert (out[0, 0].view(G, D).double() - o).abs().max() <= o.abs().max() * 2.0 ** -8 + 2.0 ** -12
