@@ -121,7 +121,7 @@ class TextDecoder:
         b = P // ops.KV8_BLOCK
         self.tail = [t[:, :, b * ops.KV8_BLOCK:P] for t in (self.kv.k, self.kv.v)] + [t[:, :, b] for t in (self.kv.ks, self.kv.vs)] \
             if self.keep is None and P % ops.KV8_BLOCK else []
-        self.tail_saved = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in self.tail]
+        self.tail_saved = [t.clone(memory_format=torch.contiguous_format) for t in self.tail]
         self.ws8 = ops.attn_kv8_workspace(1, P, H, H, hd, self.kv.k.shape[2], dev, self.keep is not None)
 
     def _attend_kv8(self, i, qkv, n, full, a):
