@@ -230,3 +230,46 @@ def test_attn_kv8_weights_of_many_heads_over_a_very_long_cache():
         assert torch.allclose(w[0, 0, at:at + step].double(), p.sum(0), rtol=2.0 ** -12, atol=0), at
     # means of 17 million values of both signs: small beside the values, whose rounded weights and fp32 sums leave 2^-12 of their size
     assert (out[0, 0].view(G, D).double() - o).abs().max() <= o.abs().max() * 2.0 ** -8 + 2.0 ** -12
+
+
+FEW = [  # B, n, Hq, H, D, C, lens, counts: D = 128 with two row groups (17 to 32 rows), whole items and runs; two of eight rows in runs
+    (3, 8, 8, 2, 128, 512, [400, 0, 33], [8, 3, 5]), (2, 5, 4, 1, 128, 512, [500, 31], [5, 1]), (4, 8, 8, 2, 128, 2048, [2000, 1, 64, 1500], [8, 4, 0, 2]),
+    (2, 6, 20, 4, 128, 4096, [4000, 900], None), (3, 7, 8, 2, 128, 1024, [512, 1000, 0], [7, 0, 4]), (2, 4, 8, 2, 128, 2048, [1111, 2000], None),
+    (3, 4, 12, 3, 64, 2048, [1999, 5, 1025], [4, 1, 3]), (5, 8, 12, 3, 64, 4096, [3000, 0, 4088, 64, 2000], [8, 5, 2, 0, 8]), (40, 1, 32, 8, 128, 2048, [50 * i for i in range(40)], None)]
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("B,n,Hq,H,D,C,lens,counts", FEW)
+def test_attn_kv8_few_rows_in_every_plan(B, n, Hq, H, D, C, lens, counts, causal, weights):
+    _attend(B, n, Hq, H, D, C, lens, counts, causal, weights)
+
+
+MANY = [  # runs of tiles that end inside an item, hold whole ones and begin another; sequences of every length, idle ones among them
+    (6, 300, 32, 16, 64, 1856, [1500, 300, 0, 700, 64, 1000], [300, 211, 300, 0, 1, 130]), (5, 90, 16, 8, 128, 2176, [2000, 1500, 0, 1900, 37], [90, 0, 60, 17, 90]),
+    (4, 140, 8, 8, 128, 1664, [1500, 640, 1, 1024], None), (1, 600, 12, 4, 64, 2560, [1900], None), (7, 64, 32, 8, 128, 1600, [1536, 1000, 500, 250, 100, 50, 0], [64, 0, 64, 33, 64, 0, 64]),
+    (3, 65, 5, 1, 64, 4160, [4000, 0, 2048], [65, 65, 30]), (12, 40, 20, 10, 64, 1600, [130 * i for i in range(12)], [40 - 3 * i for i in range(12)]),
+    (3, 200, 4, 2, 64, 1536, [1300, 0, 512], [200, 200, 0])]
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("B,n,Hq,H,D,C,lens,counts", MANY)
+def test_attn_kv8_many_rows_in_every_plan(B, n, Hq, H, D, C, lens, counts, causal, weights):
+    _attend(B, n, Hq, H, D, C, lens, counts, causal, weights)
+
+
+def _attend(B, n, Hq, H, D, C, lens, counts, causal, weights):
+    cache = filled(B, H, C, D, n + Hq)
+    g = torch.Generator(DEV).manual_seed(n)
+    # keys that grow along the cache, so that rows rescale late in a run
+    cache.ks.mul_(torch.linspace(0.4, 2.5, C // 64, device=DEV))
+    q = (torch.randn(B, n, Hq, D, device=DEV, generator=g) * 1.5).to(BF)
+    out = torch.full((B, n, Hq * D), 3.0, dtype=BF, device=DEV)
+    w = torch.full((B, H, C), -1.0, device=DEV) if weights else None
+    w_in = torch.rand(B, H, C, device=DEV, generator=g) if weights else None
+    ops.attn_kv8(q, cache, i32(lens), out, counts=None if counts is None else i32(counts), causal=causal, weights=w, weights_in=w_in)
+    check64(q, cache, lens, counts, causal, out, w, w_in)
+    for b in range(B):
+        m = n if counts is None else counts[b]
+        assert (out[b, m:] == 3).all() and (w is None or (w[b, :, lens[b] + m:] == -1).all())
