@@ -92,15 +92,17 @@ struct Args {
   const float* w_in;
 };
 
-// First tile of each sequence in the list of all tiles, pre[0 .. B]; a sequence's tiles are those of its H * rg (head,
-// row group) items one after another.  Every CTA computes it for itself.
-__device__ __forceinline__ void tile_list(const Args& a, int kt, int* pre, int* warp_sum) {
+// Row groups of gr rows that a sequence's new tokens fill (rg of the plan at most).
+__device__ __forceinline__ int row_groups(const Args& a, const Seq& s, int gr) { return (s.cnt * a.G + gr - 1) / gr; }
+// First tile of each sequence in the list of all tiles, pre[0 .. B]; a sequence's tiles are those of its (head, row group)
+// items one after another.  Every CTA computes it for itself.
+__device__ __forceinline__ void tile_list(const Args& a, int kt, int gr, int* pre, int* warp_sum) {
   const int tid = threadIdx.x, nth = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.B + nth - 1) / nth, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
   int sum = 0;
   for (int b = b0; b < b1; b++) {
     const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C, blockIdx.x == 0);  // those without work are looked at here only
-    const int t = s.cnt ? (s.len + s.cnt + kt - 1) / kt * a.H * a.rg : 0;
+    const int t = (s.len + s.cnt + kt - 1) / kt * a.H * row_groups(a, s, gr);
     pre[b] = t;
     sum += t;
   }
@@ -181,7 +183,7 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
   if (WHOLE) {
     __syncthreads();
   } else {
-    tile_list(a, KT, pre, warp_sum);  // its barriers also publish the mbarriers
+    tile_list(a, KT, GR, pre, warp_sum);  // its barriers also publish the mbarriers
     total = pre[a.B];
     const int run = run_of(total, a.ctas);
     u_begin = (long long)blockIdx.x * run;
@@ -193,10 +195,11 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
     const int b = WHOLE ? blockIdx.x / (a.H * a.rg) : find_seq(pre, a.B, u);
     const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C);
     const int T = s.len + s.cnt, tiles = (T + KT - 1) / KT;
-    const int item = WHOLE ? blockIdx.x % (a.H * a.rg) : (u - pre[b]) / tiles, ta = WHOLE ? 0 : (u - pre[b]) % tiles;
+    const int rgs = WHOLE ? a.rg : row_groups(a, s, GR);
+    const int item = WHOLE ? blockIdx.x % (a.H * rgs) : (u - pre[b]) / tiles, ta = WHOLE ? 0 : (u - pre[b]) % tiles;
+    const int h = item / rgs, rg = item % rgs, r0 = rg * GR;
     // this CTA's tiles of the item: [ta, tb)
-    const int tb = WHOLE ? (item % a.rg * GR < s.cnt * a.G ? tiles : 0) : min(tiles, ta + (u_end - u));
-    const int h = item / a.rg, r0 = (item % a.rg) * GR;
+    const int tb = WHOLE ? (r0 < s.cnt * a.G ? tiles : 0) : min(tiles, ta + (u_end - u));
     const size_t bh = (size_t)b * a.H + h;
     const int8_t *kp = a.kc + bh * a.C * D, *vp = a.vc + bh * a.C * D;
     const float *ksp = a.ks + bh * (a.C / BLK), *vsp = a.vs + bh * (a.C / BLK);
@@ -452,7 +455,7 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
         *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
         if (d == 0 && a.w) {
           if (WHOLE) sh_lse[r] = mx + log2f(sum);
-          else a.full_ml[(bh * a.rg + item % a.rg) * GR + r] = make_float2(mx, sum);
+          else a.full_ml[(bh * a.rg + rg) * GR + r] = make_float2(mx, sum);
         }
       } else {
         *reinterpret_cast<float4*>(a.part_o + ((size_t)slot * GR + r) * D + d) = v;
@@ -490,11 +493,11 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   griddep_wait();
   griddep_launch();
-  tile_list(a, KT, pre, warp_sum);
+  tile_list(a, KT, GR, pre, warp_sum);
   const int run = run_of(pre[a.B], a.ctas);
   // the first and last CTA that hold a part of an item, and the first part's slot (the others begin their CTA's run: 2 c)
-  auto parts = [&](int b, int h, int rg, int tiles, int& c0, int& c1, int& first) {
-    const int u0 = pre[b] + (h * a.rg + rg) * tiles;
+  auto parts = [&](const Seq& s, int b, int h, int rg, int tiles, int& c0, int& c1, int& first) {
+    const int u0 = pre[b] + (h * row_groups(a, s, GR) + rg) * tiles;
     c0 = u0 / run, c1 = (u0 + tiles - 1) / run;
     first = 2 * c0 + (u0 == c0 * run ? 0 : 1);
   };
@@ -519,7 +522,7 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
     const int row = rg * GR + r, tiles = (s.len + s.cnt + KT - 1) / KT;
     if (row >= s.cnt * a.G) return;
     int c0, c1, first;
-    parts(b, h, rg, tiles, c0, c1, first);
+    parts(s, b, h, rg, tiles, c0, c1, first);
     if (c0 == c1) return;
     float mx, sum;
     row_ml(c0, c1, first, r, mx, sum);
@@ -553,7 +556,7 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
   if (x % chunks * 512 >= T) return;
   for (int r = warp; r < rows; r += 4) {
     int c0, c1, first;
-    parts(b, h, r / GR, tiles, c0, c1, first);
+    parts(s, b, h, r / GR, tiles, c0, c1, first);
     float mx, sum;
     if (c0 == c1) {
       const float2 ml = a.full_ml[((size_t)bh * a.rg + r / GR) * GR + r % GR];
