@@ -292,7 +292,7 @@ int vt_attn_causal(cudaStream_t stream, const uint16_t* q, const uint16_t* kc, c
 
 /* Rotary embedding (vt_rope_qkv's: the first 32 dims of each q / k head) and quantised cache write of n new tokens for
  * each of B sequences: qkv bf16, row (b, i) at qkv + b*sx_b + i*sx_t = q [Hq][D] | k [H][D] | v [H][D]; cos_t / sin_t
- * fp32 [tab][16], row pos[b] + i (pos NULL: lens[b] + i); q rows to q + b*sq_b + i*sq_t + hq*sq_h; k (rounded to bf16) and v
+ * fp32 [tab][16], row pos[b] + i (pos NULL: lens[b] + i); q rows to q + b*sq_b + i*sq_t + hq*sq_h (not over qkv); k (rounded to bf16) and v
  * into slots lens[b] + i.  Strides multiples of 8 elements.  A block without tokens, or with zeros only (scale 0),
  * takes the scale max|x| / 127 of its new ones; a block that holds tokens keeps its scale, doubled as often as the
  * new ones need, its codes halved as often (rint): a value is then at most one step off however it arrived, half a

@@ -527,6 +527,26 @@ static bool overlap(const void* p, long long n, const void* q, long long m) {
   return a < b + (uintptr_t)m && b < a + (uintptr_t)n;
 }
 
+// Rows (b, t) of `w` elements at p + b sb + t st.
+struct Rows {
+  const uint16_t* p;
+  long long sb, st, w;
+};
+// Whether rows of x and y may share an element: by columns where both have the same strides, else by where they begin and end.
+static bool rows_meet(const Rows& x, const Rows& y, int B, int n) {
+  auto span = [&](const Rows& r, const uint16_t*& lo, const uint16_t*& hi) {
+    const long long b = (B - 1) * r.sb, t = (n - 1) * r.st;
+    lo = r.p + (b < 0 ? b : 0) + (t < 0 ? t : 0), hi = r.p + (b > 0 ? b : 0) + (t > 0 ? t : 0) + r.w;
+  };
+  const uint16_t *x0, *x1, *y0, *y1;
+  span(x, x0, x1), span(y, y0, y1);
+  if (x0 >= y1 || y0 >= x1) return false;
+  const long long pitch = n > 1 ? x.st : B > 1 ? x.sb : 0;
+  if (pitch <= 0 || (n > 1 && x.st != y.st) || (B > 1 && (x.sb != y.sb || x.sb % pitch))) return true;
+  const long long d = ((y.p - x.p) % pitch + pitch) % pitch;  // y's first column in x's rows
+  return d < x.w || d + y.w > pitch;
+}
+
 // Shared checks of a cache: C slots a multiple of 64, heads 64 or 128 wide, aligned pointers.
 static int check_cache(const char* what, const void* kc, const void* vc, const void* ks, const void* vs, int B, int H,
                        int C, int D) {
@@ -564,6 +584,8 @@ int vt_rope_kv8(cudaStream_t st, const uint16_t* qkv, long long sx_b, long long 
   long long qc = ((long long)B * n * Hq * (D / 8) + 127) / 128;
   if (qc > (1 << 20)) qc = 1 << 20;
   if (kv_units + qc > 0x7fffffffLL) return set_error(E_SHAPE, "vt_rope_kv8: grid too large (B=%d H=%d n=%d)", B, H, n);
+  if (kv8::rows_meet({qkv, sx_b, sx_t, (Hq + 2LL * H) * D}, {q, sq_b, sq_t, (Hq - 1) * sq_h + D}, B, n))
+    return set_error(E_SHAPE, "vt_rope_kv8: q overlaps qkv");
   kv8::AppendArgs a{qkv, sx_b, sx_t, B, n, Hq, H, C, tab, nb, cos_t, sin_t, lens, pos, counts, q, sq_b, sq_t, sq_h,
                     kc, vc, ks, vs, kv_units};
   if (D == 64) launch_k(kv8::rope_kv8_kernel<64>, (unsigned)(kv_units + qc), 128, 0, st, a);

@@ -37,10 +37,12 @@ int vt_attn_kv8(cudaStream_t st, const uint16_t* q, long long sq_b, long long sq
   const long long need = vt_attn_kv8_ws_bytes(B, n, Hq, H, D, C, weights != nullptr);
   if (need && (!ws || !aligned16(ws) || ws_bytes < need))
     return set_error(E_SHAPE, "vt_attn_kv8: workspace of %lld bytes, %lld needed (16-byte aligned)", ws ? ws_bytes : 0LL, need);
+  const bool meet = kv8::rows_meet({q, sq_b, sq_t, (Hq - 1) * sq_h + D}, {out, so_b, so_t, (Hq - 1) * so_h + D}, B, n);
   if (kv8::few_rows(n, Hq, H)) {
     const kv8::split::Plan p = kv8::split::make_plan(B, n, Hq, H, D, C, weights != nullptr, sm_count());
     if (B > kv8::split::MAXB || (long long)B * H * p.rg * (C / kv8::split::keys_per_tile(D)) > 0x40000000LL)
       return set_error(E_SHAPE, "vt_attn_kv8: B=%d (at most %d) or B * H * C too large", B, kv8::split::MAXB);
+    if (meet) return set_error(E_SHAPE, "vt_attn_kv8: out overlaps q");
     char* w8 = static_cast<char*>(ws);
     kv8::split::Args a{q, sq_b, sq_t, sq_h, kc, vc, ks, vs, lens, counts, B, n, Hq / H, H, C, causal, p.rows, p.rg, p.ctas,
                        scale * kv8::LOG2E, out, so_b, so_t, so_h, (float*)(w8 + p.o_off), (float2*)(w8 + p.ml_off),
@@ -52,6 +54,7 @@ int vt_attn_kv8(cudaStream_t st, const uint16_t* q, long long sq_b, long long sq
   const long long items = (p.rows + kv8::tc::ROWS - 1) / kv8::tc::ROWS;
   if (B > kv8::tc::MAXB || (long long)n * (Hq / H) > 0x3fffffffLL || B * items * H * (C / kv8::BLK) > 0x40000000LL)
     return set_error(E_SHAPE, "vt_attn_kv8: B=%d (at most %d) or B * H * n * C too large", B, kv8::tc::MAXB);
+  if (meet) return set_error(E_SHAPE, "vt_attn_kv8: out overlaps q");
   char* w8 = static_cast<char*>(ws);
   kv8::tc::Args a{q, sq_b, sq_t, sq_h, kc, vc, ks, vs, lens, counts, B, n, Hq / H, H, C, causal, p.rows, p.ctas,
                   p.whole ? (int)items : 0, scale * kv8::LOG2E,

@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 from strix_halo_maxx_b200 import ops
 from strix_halo_maxx_b200._lib import device_status
 from oracle import kv8_ref as R
-from test_kv8_gpu import BF, DEV, as_np, filled, i32, np_
+from test_kv8_gpu import BF, DEV, as_np, filled, i32, np_, tables
 
 
 @pytest.fixture(autouse=True)
@@ -273,3 +273,19 @@ def _attend(B, n, Hq, H, D, C, lens, counts, causal, weights):
     for b in range(B):
         m = n if counts is None else counts[b]
         assert (out[b, m:] == 3).all() and (w is None or (w[b, :, lens[b] + m:] == -1).all())
+
+
+@pytest.mark.parametrize("n", [1, 5, 70])
+def test_rows_side_by_side_in_one_buffer(n):
+    """q beside qkv, and out beside q, as columns of one matrix: the same numbers as in buffers of their own."""
+    B, Hq, H, D = 2, 4, 2, 64
+    g = torch.Generator(DEV).manual_seed(n)
+    wide = torch.randn(B, n, 1024, device=DEV, generator=g).to(BF)
+    qkv, q, out = wide[..., :512], wide[..., 512:768].view(B, n, Hq, D), wide[..., 768:]
+    cos, sin = tables()
+    a, b = (filled(B, H, 256, D, 4) for _ in range(2))
+    q2 = ops.rope_kv8(qkv.clone(), b, i32([3, 90]), cos, sin, torch.zeros(B, n, Hq, D, dtype=BF, device=DEV))
+    ops.rope_kv8(qkv, a, i32([3, 90]), cos, sin, q)
+    ops.attn_kv8(q, a, i32([3, 90]), out)
+    assert torch.equal(q, q2) and torch.equal(out, ops.attn_kv8(q2, b, i32([3, 90])))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
