@@ -16,8 +16,9 @@
 // moves, O through registers, when that has grown by P_MOVE (by 4 instead of 8: 319 against 275 us below).  So P' has f16's 11 bits
 // down to 2^-21 of the row's largest term and is off by 2^-32 of it below that; where one key is far above all before it and
 // beside it, such as a sink, m goes P_UP_SINK below it and these are 2^-27 and 2^-38.  (In bf16, with its 8 bits, an output's error
-// against 64 bits was 1.4 times its own rounding.)  V blocks with a scale below 2^-100 are zeros and take another block's scale
-// for P'.  The scales of a head's other blocks may differ by 2^64.
+// against 64 bits was 1.4 times its own rounding.)  V blocks with a scale below 2^-100 are zeros: their keys, with 1 for
+// the scale, count in the sum alone, so m may lie 2^116 below them (with 8 as for others, a sink among them took away the bits of
+// all other terms).  The scales of a head's other blocks may differ by 2^64.
 // A 2048-token chunk over 6001 slots (32 / 8 heads x 128, 236 GFLOP): 277 us, 850 TFLOP/s.  A tile takes about 2,040 cycles: the
 // exponentials occupy the MUFU for 1,024 (16 a clock and SM), the MMAs are issued over about 1,500, and P -> PV -> S of a
 // score buffer is a chain of which two are in flight.  128-key tiles with one score buffer were slower (346 us), so were
@@ -32,7 +33,7 @@ namespace tc {
 constexpr int ROWS = 256, KEYS = 64, THREADS = 16 * 32, ST = 3, MAXB = 2048;
 constexpr uint32_t TMEM_COLS = 512;  // S of M tile t, buffer f: columns 128 t + 64 f; O of tile t: 256 + 128 t
 constexpr long long kDrainCycles = 200000000LL;
-constexpr float P_TOP = 15.9f, P_MOVE = 8.f, P_UP = P_TOP - P_MOVE, P_UP_SINK = P_TOP - 2.f;  // log2 units
+constexpr float P_TOP = 15.9f, P_MOVE = 8.f, P_UP = P_TOP - P_MOVE, P_UP_SINK = P_TOP - 2.f, Z_TOP = 116.f;  // log2 units
 constexpr float L_SCALE = 0x1p-20f, L_LOG2 = -20.f;  // row sums are kept times 2^-20, so that 2^15 / vs does not overflow
 constexpr int SOFTMAX_REGS = 168, CONVERT_REGS = 96, MMA_REGS = 80;
 constexpr float kTinyScale = 0x1p-100f;
@@ -171,6 +172,12 @@ __device__ __forceinline__ void store_codes(uint8_t* tile, int row, int p, uint4
   auto hi = [](uint32_t x) { return two_codes<0x4342, F16>(x); };
   *reinterpret_cast<uint4*>(at) = make_uint4(lo(c.x), hi(c.x), lo(c.y), hi(c.y));
   *reinterpret_cast<uint4*>(at + CR * 16) = make_uint4(lo(c.z), hi(c.z), lo(c.w), hi(c.w));
+}
+// Two f16, numbers beyond its range as the largest one (they meet zeros only).
+__device__ __forceinline__ uint32_t pack_h2_finite(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 // The address of q row r of (b, h).
 __device__ __forceinline__ const uint16_t* q_row(const Args& a, int b, int h, int r) {
@@ -373,14 +380,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       float m = -INFINITY, l = 0.f;
       // of the tile: K's scale times the softmax scale, log2 and inverse (times L_SCALE) of V's scale (the approximations err by
       // 2^-22, both in the sum and in O); the next tile's are worked out while this one's scores arrive
-      float c, lvs, ivs, ks_next = ksp[0], vs_next = vsp[0], c_next, lvs_next, ivs_next, v = vs_next;
-      if (!(v >= kTinyScale)) {  // the first scale of the run that is one
-        v = 1.f;
-        for (int i = nt - 1; i >= 0; i--) v = vsp[i] >= kTinyScale ? vsp[i] : v;
-      }
+      // and how far terms may be above m
+      float c, lvs, ivs, top, ks_next = ksp[0], vs_next = vsp[0], c_next, lvs_next, ivs_next, top_next;
       auto next_scales = [&](int i) {
-        v = vs_next < kTinyScale ? v : vs_next;  // the converters made V zero
-        c_next = ks_next * a.scale_log2, lvs_next = __log2f(v), ivs_next = __frcp_rn(v) * L_SCALE;
+        const bool none = vs_next < kTinyScale;  // the converters made V zero
+        const float v = none ? 1.f : vs_next;
+        c_next = ks_next * a.scale_log2, lvs_next = __log2f(v), ivs_next = __frcp_rn(v) * L_SCALE, top_next = none ? Z_TOP : P_TOP;
         if (i + 1 < nt) ks_next = ksp[i + 1], vs_next = vsp[i + 1];
       };
       next_scales(0);
@@ -393,7 +398,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       for (int i = 0; i < nt; i++) {
         const int f = (js + i) & 1, key0 = (g.ta + i) * KEYS;
         const uint32_t t_s = tmem + 128 * t + 64 * f + lane_off;
-        c = c_next, lvs = lvs_next, ivs = ivs_next;
+        c = c_next, lvs = lvs_next, ivs = ivs_next, top = top_next;
         uint32_t r0[32], r1[32];
         float mx, sum;
         auto top32 = [&](const uint32_t (&r)[32]) {
@@ -416,7 +421,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
             f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), c2, sh2), x0, x1);
             const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
             sum2[e & 1] = f2_add(sum2[e & 1], f2_pack(p0, p1));
-            pk[e] = split::pack_h2(p0, p1);
+            pk[e] = pack_h2_finite(p0, p1);
           }
           tmem_st16(t_s + at, pk);
           float lo, hi;
@@ -440,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
           tmem_ld_wait();
           sum += exps(r1, 16, m);
           mx = fmaf(fmaxf(ma, top32(r1)), c, lvs);
-          again = __any_sync(0xffffffffu, mx > m + P_TOP);
+          again = __any_sync(0xffffffffu, mx > m + top);
         }
         if (again) {
           tmem_ld_wait();
@@ -453,15 +458,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
             }
           }
           mx = left > 0 ? fmaf(fmaxf(top32(r0), top32(r1)), c, lvs) : -INFINITY;
-          const bool need = mx > m + P_TOP;
-          const float mn = i == 0 ? mx - P_UP : need ? mx - (mx > m + (P_TOP + 12.f) ? P_UP_SINK : P_UP) : m;
+          const bool need = mx > m + top;
+          const float up = top - P_MOVE;
+          const float mn = i == 0 ? mx - up : need ? mx - (mx > m + (P_TOP + 12.f) ? fmaxf(up, P_UP_SINK) : up) : m;
           if (i > 0 && __any_sync(0xffffffffu, need)) {  // O through registers (warp-collective)
             // O must hold every product up to tile i - 1; the barrier's next arrival, ST tiles on, needs P of this row
             ok = wait(&kv_empty[(j + i - 1) % ST], ((j + i - 1) / ST) & 1);
             if (!ok) break;
             tc_fence_after();
-            const float alpha = need ? ex2_approx(m - mn) : 1.f;
-            l *= alpha;
+            const float half = need ? ex2_approx(0.5f * (m - mn)) : 1.f, alpha = half * half;
+            l = l * half * half;  // what zero blocks put there may be as large as alpha is small
 #pragma unroll
             for (int x = 0; x < D / 16; x++) {
               uint32_t r[16];
@@ -580,8 +586,8 @@ __global__ void __launch_bounds__(128) attn_kv8_tc_join_kernel(Args a) {
       const size_t p = (c == c0 ? first : 2 * (size_t)c) * ROWS + at;
       const float2 ml = a.part_ml[p];
       const float4 o = *reinterpret_cast<const float4*>(a.part_o + p * D + d);
-      const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - mx);
-      sum += ml.y * f, v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
+      const float half = ml.x == -INFINITY ? 0.f : ex2_approx(0.5f * (ml.x - mx)), f = half * half;
+      sum += ml.y * half * half, v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
     }
     const float inv = L_SCALE / sum;
     uint16_t* op = a.out + g.b * a.so_b + row / a.G * a.so_t + (size_t)(g.h * a.G + row % a.G) * a.so_h + d;

@@ -289,3 +289,24 @@ def test_rows_side_by_side_in_one_buffer(n):
     ops.attn_kv8(q, a, i32([3, 90]), out)
     assert torch.equal(q, q2) and torch.equal(out, ops.attn_kv8(q2, b, i32([3, 90])))
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("gap,at,e", [(12.0, 0, 0), (25.0, 0, 0), (40.0, 0, 0), (25.0, 200, 0), (40.0, 200, 0), (40.0, 129, 0), (12.0, 0, -85), (40.0, 0, 90), (40.0, 200, 90)])
+@pytest.mark.parametrize("n,D,T,Hq", [(64, 64, 730, 2), (200, 128, 1000, 4), (70, 64, 2500, 2), (300, 128, 2500, 2)])
+def test_attn_kv8_many_rows_beside_a_block_of_zero_values(n, D, T, Hq, gap, at, e):
+    """The key that takes the weight lies in a block whose values are all zero (scale 0): it counts in the sum alone, and what
+    the others add up to is as exact as without it, e^-40 of its weight or not, and with scales around 2^e."""
+    H, C = 2, (T + 63) // 64 * 64
+    cache = filled(1, H, C, D, n)
+    cache.k.zero_()
+    cache.ks.fill_(1 / 128)
+    cache.v.copy_(cache.v.abs() // 4 + 90)
+    cache.k[:, :, at, 0] = 127
+    cache.vs.mul_(2.0 ** e)
+    cache.vs[:, :, at // 64] = 0
+    cache.vs[:, :, 7] = 2.0 ** -90   # and one whose values are next to nothing
+    q = torch.randn(1, n, Hq, D, device=DEV, generator=torch.Generator(DEV).manual_seed(2)).to(BF)
+    q[..., 0] = 1
+    w = torch.zeros(1, H, C, device=DEV)
+    out = ops.attn_kv8(q, cache, i32([T - n]), causal=False, scale=gap * 128 / 127, weights=w)
+    check64(q, cache, [T - n], None, False, out, w, scale=gap * 128 / 127, random_v=False)
