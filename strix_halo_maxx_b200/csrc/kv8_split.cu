@@ -24,8 +24,8 @@
 //           of a tile's keys is which row of the MMA is free, so lane t takes keys t, 4 + t, 8 + t, 12 + t: its reads are
 //           free of bank conflicts (rows 64 B apart), and K's rows follow the same order;
 //   O       a tile's product is accumulated on its own and added as O = O * alpha + vs * (P V): V's scale stays fp32.
-// What bounds it: DRAM at long contexts (64 x 8 heads x 128 of 4k-8k slots, 818 MB: 137 us, 5.95 TB/s, issue slots 60 % busy;
-// three CTAs an SM with two stages each: 201 us), else the latency of one tile's chain and of the join.
+// What bounds it: DRAM at long contexts (64 x 8 heads x 128 of 4k-8k slots, 818 MB: 139 us, 5.89 TB/s, issue slots 57 % busy; under
+// the power cap, in loops of seconds, 159 us; three CTAs an SM with two stages each: 201 us), else the latency of one tile's chain and of the join.
 #include "vt_common.cuh"
 #include "vt_host.h"
 

@@ -19,7 +19,7 @@
 // against 64 bits was 1.4 times its own rounding.)  V blocks with a scale below 2^-100 are zeros: their keys, with 1 for
 // the scale, count in the sum alone, so m may lie 2^116 below them (with 8 as for others, a sink among them took away the bits of
 // all other terms).  The scales of a head's other blocks may differ by 2^64.
-// A 2048-token chunk over 6001 slots (32 / 8 heads x 128, 236 GFLOP): 277 us, 850 TFLOP/s.  A tile takes about 2,040 cycles: the
+// A 2048-token chunk over 6001 slots (32 / 8 heads x 128, 236 GFLOP): 276 us, 853 TFLOP/s (295 us under the power cap).  A tile takes about 2,040 cycles: the
 // exponentials occupy the MUFU for 1,024 (16 a clock and SM), the MMAs are issued over about 1,500, and P -> PV -> S of a
 // score buffer is a chain of which two are in flight.  128-key tiles with one score buffer were slower (346 us), so were
 // four stages (299) and P announced one tile late (294).
@@ -37,8 +37,9 @@ constexpr float P_TOP = 15.9f, P_MOVE = 8.f, P_UP = P_TOP - P_MOVE, P_UP_SINK = 
 constexpr float L_SCALE = 0x1p-20f, L_LOG2 = -20.f;  // row sums are kept times 2^-20, so that 2^15 / vs does not overflow
 constexpr int SOFTMAX_REGS = 168, CONVERT_REGS = 96, MMA_REGS = 80;
 constexpr float kTinyScale = 0x1p-100f;
-// With caches of up to so many blocks a CTA takes a whole item: equal runs for all SMs would cost more in parts to write and
-// join than they gain (the 730-token prefix, 96 items of 12 tiles: 20.5 us whole, 24.8 in runs and 12.4 to join them).
+// With caches of up to so many blocks a CTA takes a whole item, however few there are: equal runs for all SMs would cost more in
+// parts to write and join than they gain (whole / runs, us: 96 items of 12 tiles 20 / 34; 4 items of 16 22 / 30, 32 of them 23 / 25,
+// 128 24 / 41; 2 items of 23 tiles x 128 dims 25 / 54, 32 of them x 64 dims 22 / 24; 1 item of 7 tiles 10 / 16).
 constexpr int WHOLE_TILES = 24;
 
 template <int D>
@@ -230,8 +231,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, ST_KV8_WAIT)) != 0;
   };
 
-  // registers by role: 512 threads are launched with 128 each; the softmax holds 64 scores, and its spills cost 307 against
-  // 284 us for the 2048-token chunk
+  // registers by role: 512 threads are launched with 128 each; the softmax holds 64 scores (2048-token chunk 284 us with this
+  // split, 307 with 128 for all; the compiler, which sees 128, still spills 32 bytes a thread)
   static_assert(2 * SOFTMAX_REGS + CONVERT_REGS + MMA_REGS <= 4 * 128, "the split must come out of the launch's registers");
   if (warp >= 12) {
     set_regs_down<MMA_REGS>();  // one instruction for the whole warp group
