@@ -286,14 +286,15 @@ int vt_attn_causal(cudaStream_t stream, const uint16_t* q, const uint16_t* kc, c
  * (int, device memory, NULL: n for all) the number of its new tokens, 0 .. n; rows past counts[b] are padding: never
  * read into a result, and left as they were in every output.  Lengths on the device cannot be refused by the host: a
  * negative one, a count outside 0 .. n, tokens past C and positions past the rotary table are clamped and set bit 9
- * of the status word (vt_device_status; bit 10: a bounded wait of vt_attn_kv8 gave up).  Query head hq reads head hq / (Hq / H).  The reference has a bf16 cache only
- * (moondream/gpu/md2fast.py:186-191); these stand beside vt_rope_qkv and vt_attn_causal.
+ * of the status word (vt_device_status; bit 10: a bounded wait of vt_attn_kv8 gave up).  Query head hq reads head
+ * hq / (Hq / H).  The reference has a bf16 cache only (moondream/gpu/md2fast.py:186-191); these stand beside
+ * vt_rope_qkv and vt_attn_causal.
  * Limits: vt_attn_kv8 B <= 2048, 0 <= scale < 2^100; vt_kv8_evict C <= 262144. */
 
 /* Rotary embedding (vt_rope_qkv's: the first 32 dims of each q / k head) and quantised cache write of n new tokens for
  * each of B sequences: qkv bf16, row (b, i) at qkv + b*sx_b + i*sx_t = q [Hq][D] | k [H][D] | v [H][D]; cos_t / sin_t
- * fp32 [tab][16], row pos[b] + i (pos NULL: lens[b] + i); q rows to q + b*sq_b + i*sq_t + hq*sq_h (not over qkv); k (rounded to bf16) and v
- * into slots lens[b] + i.  Strides multiples of 8 elements.  A block without tokens, or with zeros only (scale 0),
+ * fp32 [tab][16], row pos[b] + i (pos NULL: lens[b] + i); q rows to q + b*sq_b + i*sq_t + hq*sq_h (not over qkv); k
+ * (rounded to bf16) and v into slots lens[b] + i.  Strides multiples of 8 elements.  A block without tokens, or with zeros only (scale 0),
  * takes the scale max|x| / 127 of its new ones; a block that holds tokens keeps its scale, doubled as often as the
  * new ones need, its codes halved as often (rint): a value is then at most one step off however it arrived, half a
  * step when its block was written in one call.  A NaN or an infinity makes its block's scale NaN.  A call may be
@@ -310,12 +311,14 @@ long long vt_attn_kv8_ws_bytes(int B, int n, int Hq, int H, int D, int C, int we
 
 /* Attention of the n new rows of each sequence over its cache, their own tokens already in it: row i of sequence b
  * sees slots 0 .. lens[b] + i (causal != 0) or 0 .. lens[b] + counts[b] - 1; softmax(scale q k^T) v, out
- * bf16 at out + b*so_b + i*so_t + hq*so_h (not over q).  Scores, maxima, sums, O and weights are fp32; before they meet V the
- * probabilities are rounded to f16's 11 bits, terms p * V scale below 2^-21 of the row's largest to 2^-32 of that.  With n Hq / H <= 32
- * q values below 2^-32 of their row's largest are rounded to 2^-40 of it; all else of q, k and v is exact.  V scales of 2^-100 .. 2^100,
- * those of a head within 2^64 of one another; smaller ones count as zero.  weights fp32 [B][H][C] (NULL: none) receives the attention weight of each
- * slot j < lens[b] + counts[b]: its probabilities summed over the sequence's rows and the group's query heads, plus
- * weights_in[b][h][j] (NULL: none; may be weights) for j < lens[b].  ws: vt_attn_kv8_ws_bytes bytes, 16-byte
+ * bf16 at out + b*so_b + i*so_t + hq*so_h (not over q).  weights fp32 [B][H][C] (NULL: none) receives the attention
+ * weight of each slot j < lens[b] + counts[b]: its probabilities summed over the sequence's rows and the group's query
+ * heads, plus weights_in[b][h][j] (NULL: none; may be weights) for j < lens[b].
+ * Scores, maxima, sums, O and weights are fp32.  Before they meet V the probabilities p are rounded to f16's 11 bits:
+ * with n Hq / H <= 32 those above 2^-29 of the row's largest, smaller ones to 2^-40 of it; else those whose p * V scale
+ * is above 2^-21 of the row's largest such product, smaller ones to 2^-32 of it.  q values below 2^-32 of their row's
+ * largest may be rounded to 2^-40 of it; all else of q, k and v is exact.  V scales of 2^-100 .. 2^100 (smaller ones
+ * may count as zero), those of a head within 2^64 of one another.  ws: vt_attn_kv8_ws_bytes bytes, 16-byte
  * aligned, one call at a time.  Results do not depend on the other sequences of the batch beyond the rounding of
  * how the keys are split, and are the same every time.
  * Replaces: nothing in the reference; the 8-bit form of the question's attention (md2fast.py:192-193). */
