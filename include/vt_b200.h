@@ -338,6 +338,55 @@ int vt_kv8_evict(cudaStream_t stream, const int8_t* kc, const int8_t* vc, const 
                  const float* weights, const int* lens, int B, int H, int D, int keep, int recent, int8_t* dst_kc,
                  int8_t* dst_vc, float* dst_ks, float* dst_vs, int dst_C, float* dst_weights, int* dst_lens, int* index);
 
+/* Bytes of the workspace of vt_attn_kv8_shared (0 for an empty problem or one that needs none), enough for fewer tokens and slots too;
+ * its contents need no initialisation. */
+long long vt_attn_kv8_shared_ws_bytes(int S, int B, int n, int Hq, int H, int D, int Cp, int C);
+
+/* Attention of sequences that share prefixes: S prefix caches pk, pv, pks, pvs ([S][H][Cp][D], plens [S] tokens each) and, for each of
+ * the B sequences (a multiple of S), a cache of its own with lens [B] tokens before the call; sequence b goes on behind prefix
+ * b / (B / S).  Row i of its n new ones (counts [B], NULL: n each; their own tokens already in its cache) sees its whole prefix
+ * and slots 0 .. lens[b] + i of its own cache; softmax(scale q k^T) v over both, out bf16 at out + b*so_b + i*so_t + hq*so_h (not
+ * over q).  Rows behind counts[b] are left as they were.  A prefix is read once for all of its sequences.  Lengths from 0 on;
+ * what does not fit in its cache is cut off and recorded in the status word (bit 9).
+ * Scores, maxima, sums and O are fp32; q and the probabilities are rounded as vt_attn_kv8 says, its last bounds for every number of
+ * rows.  V scales of 2^-100 .. 2^100 (smaller ones may count as zero), those of one head of a prefix or cache within 2^64 of one
+ * another.  ws: vt_attn_kv8_shared_ws_bytes bytes, 16-byte aligned, one call at a time.  The same results every time.
+ * Replaces: nothing in the reference, which asks one question of an image at a time (FastMD2._query, md2fast.py:208-212). */
+int vt_attn_kv8_shared(cudaStream_t stream, const uint16_t* q, long long sq_b, long long sq_t, long long sq_h, const int8_t* pk,
+                       const int8_t* pv, const float* pks, const float* pvs, int Cp, const int* plens, int S, const int8_t* kc,
+                       const int8_t* vc, const float* ks, const float* vs, int C, const int* lens, const int* counts, int B,
+                       int n, int Hq, int H, int D, float scale, uint16_t* out, long long so_b, long long so_t, long long so_h,
+                       void* ws, long long ws_bytes);
+
+/* Sequences become others.  The cache of `layers` layers ([layers][Bs][H][C][D]) and lens [Bs]; sequence b of B takes the first
+ * lens[parents[b]] slots of sequence parents[b] and the scales of their blocks, in every layer; what lies behind them stays as it was.
+ * In place (all four dst NULL, Bs = B): parents within the groups of `beams` (1 .. 64) sequences that follow one another; those with
+ * parents[b] = b cost nothing.  Else into another cache ([layers][B][H][dst_C][D], beams ignored), from any sequence.  new_lens [B]
+ * (NULL: none; not lens) receives the lengths.  A negative parent leaves its sequence as it is, with new_lens[b] = lens[b] in place and
+ * untouched otherwise; so does one outside the source or group, which is recorded in the status word (bit 9), as is a length beyond
+ * either cache, which is cut off.  The destination must not overlap the source.
+ * Replaces: nothing in the reference. */
+int vt_kv8_reorder(cudaStream_t stream, int8_t* kc, int8_t* vc, float* ks, float* vs, int layers, int Bs, int C, int8_t* dst_kc,
+                   int8_t* dst_vc, float* dst_ks, float* dst_vs, int dst_C, const int* parents, const int* lens, int B, int beams,
+                   int H, int D, int* new_lens);
+
+/* Bytes of the workspace of vt_beam_select; its contents need no initialisation. */
+long long vt_beam_select_ws_bytes(int S, int F, int V, int k);
+
+/* The choice of a beam search.  logits bf16 (f32 = 0) or fp32, S groups of F (1 .. 64) rows of V at a pitch of ld elements; scores fp32
+ * [S][F], done uint8 [S][F] (NULL: none).  Continuation (f, v) of a group has the total scores[f] + logits[f][v] - log sum_w
+ * exp(logits[f][w]); a finished beam (done) goes on with the word eos alone and the total scores[f].  The k (1 .. 128) continuations
+ * with the largest totals, in order, the lowest f V + v first where totals are equal: out_scores [S][k] the totals, out_parents the
+ * beams' rows s F + f, out_tokens the words, out_done whether they are finished (word eos, or a finished beam).  eos < 0: no word
+ * ends an answer (done must then be NULL).  Totals of -inf or NaN (banned words, beams with a score of -inf, rows with a NaN, an
+ * infinity or nothing but -inf) are no continuations; where fewer than k are left, entry j has score -inf, word -1, row s F + j mod F
+ * and counts as finished.  Sums are fp32 within at most 64 words and 64-bit beyond, totals 64-bit, rounded once to fp32.  Outputs must
+ * not overlap inputs.  ws: vt_beam_select_ws_bytes bytes, 16-byte aligned, one call at a time.
+ * Replaces: nothing in the reference, which answers yes or no (md2fast.py:210-212). */
+int vt_beam_select(cudaStream_t stream, const void* logits, long long ld, int f32, const float* scores, const uint8_t* done, int S,
+                   int F, int V, int k, int eos, float* out_scores, int* out_parents, int* out_tokens, uint8_t* out_done, void* ws,
+                   long long ws_bytes);
+
 /* One pass of the LANCZOS frame squash on 3-channel uint8 images: out[o, j, c] = clip(2^21 + sum_k
  * in[x0(o) + k, j, c] * w[o][k] >> 22) for o < n_out positions on the resampled axis and j < n_other along
  * the other, with bounds int32 [n_out][2] = (x0, count) and fixed-point weights int32 [n_out][ksize]

@@ -53,6 +53,11 @@ SIGNATURES = {
     "vt_attn_kv8_ws_bytes": (LL, [I, I, I, I, I, I, I]),
     "vt_attn_kv8": (I, [P, P, LL, LL, LL, P, P, P, P, I, P, P, I, I, I, I, I, I, F, P, LL, LL, LL, P, P, P, LL]),
     "vt_kv8_evict": (I, [P, P, P, P, P, I, P, P, I, I, I, I, I, P, P, P, P, I, P, P, P]),
+    "vt_attn_kv8_shared_ws_bytes": (LL, [I] * 8),
+    "vt_attn_kv8_shared": (I, [P, P, LL, LL, LL, P, P, P, P, I, P, I, P, P, P, P, I, P, P, I, I, I, I, I, F, P, LL, LL, LL, P, LL]),
+    "vt_kv8_reorder": (I, [P, P, P, P, P, I, I, I, P, P, P, P, I, P, P, I, I, I, I, P]),
+    "vt_beam_select_ws_bytes": (LL, [I] * 4),
+    "vt_beam_select": (I, [P, P, LL, I, P, P, I, I, I, I, I, P, P, P, P, P, LL]),
     "vt_resize_pass_u8": (I, [P, P, LL, LL, LL, P, LL, LL, LL, I, I, P, P, I]),
 }
 

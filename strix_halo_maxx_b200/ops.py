@@ -7,7 +7,8 @@
 * I8Lin  -- the `tlin_cls` of the reference's int8 text model, hgemm.HI8Lin (hgemm.py:95-137): W8A8 with
   quant(x) -> (q, s) and __call__(x, gelu=False, res=None, pre=None); quant_rows / layer_norm_quant / gemm_i8
   are its kernels.
-* Kv8 / kv8_cache -- the 8-bit KV cache, with rope_kv8 (rotary + quantised write), attn_kv8 and kv8_evict.
+* Kv8 / kv8_cache -- the 8-bit KV cache, with rope_kv8 (rotary + quantised write), attn_kv8 and kv8_evict; for many answers about
+  one context attn_kv8_shared, kv8_reorder and beam_select.
 * layer_norm / im2col / crop_combine / rglru -- thin wrappers of the remaining kernels.
 
 Every call launches on torch's current stream and raises VtError on a non-zero return code.
@@ -575,6 +576,119 @@ def kv8_evict(cache, weights, lens, keep, recent, dst, dst_weights, dst_lens, in
               _kv8_vec(what, "dst_lens", dst_lens, (B,), torch.int32, dev),
               _kv8_vec(what, "index", index, (B, H, keep), torch.int32, dev))
     return index
+
+
+def attn_kv8_shared_workspace(S, B, n, Hq, H, D, Cp, C, device):
+    """A workspace for attn_kv8_shared calls of these sizes, one call at a time (vt_attn_kv8_shared_ws_bytes)."""
+    return torch.empty(lib().vt_attn_kv8_shared_ws_bytes(S, B, n, Hq, H, D, Cp, C), dtype=torch.uint8, device=device)
+
+
+def attn_kv8_shared(q, prefix, plens, cache, lens, out=None, counts=None, scale=None, ws=None):
+    """vt_attn_kv8_shared: attention of B sequences that share S prefixes (B a multiple of S; sequence b goes on behind prefix
+    b // (B // S)).  prefix a Kv8 [S, H, Cp, D] with plens int32 [S] tokens, cache a Kv8 [B, H, C, D] of the sequences' own
+    tokens, lens int32 [B] before the call; q [B, n, Hq, D] bf16 the new rows (already in `cache` by rope_kv8 with
+    pos = plens[b // (B // S)] + lens[b]) -> out [B, n, Hq D] bf16; row i sees the whole prefix and its own slots
+    0 .. lens[b] + i.  counts int32 [B] (default n): the rows of a sequence, those behind are left as they were.
+    ws: attn_kv8_shared_workspace, else one is allocated."""
+    what, dev = "attn_kv8_shared", q.get_device()
+    S, H, Cp, D = _kv8_dims(what, prefix, dev)
+    B, Hc, C, Dc = _kv8_dims(what, cache, dev)
+    Bq, n, Hq, Dq = q.shape
+    if (Hc, Dc) != (H, D):
+        _kv8_fail(what, f"a cache of {tuple(cache.k.shape)} behind a prefix of {tuple(prefix.k.shape)}")
+    if out is None:
+        out = torch.empty(B, n, Hq * D, dtype=BF16, device=q.device)
+    sq, so = q.stride(), out.stride()
+    if (Bq, Dq) != (B, D) or out.shape != (B, n, Hq * D) or q.dtype is not BF16 or out.dtype is not BF16 or \
+            out.get_device() != dev or sq[3] != 1 or so[2] != 1:
+        _kv8_fail(what, f"q {tuple(q.shape)}, out {tuple(out.shape)} for a cache of B={B} H={H} D={D} (bf16, contiguous rows)")
+    if ws is None:
+        nb = lib().vt_attn_kv8_shared_ws_bytes(S, B, n, Hq, H, D, Cp, C)
+        if nb:  # held until the call is on the stream; its memory is reused on this stream only
+            ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
+    elif ws.get_device() != dev or not ws.is_contiguous():
+        _kv8_fail(what, "the workspace must be contiguous on the tensors' device")
+    _kv8_call(lib().vt_attn_kv8_shared, "vt_attn_kv8_shared", dev, q.data_ptr(), sq[0], sq[1], sq[2],
+              prefix.k.data_ptr(), prefix.v.data_ptr(), prefix.ks.data_ptr(), prefix.vs.data_ptr(), Cp,
+              _kv8_vec(what, "plens", plens, (S,), torch.int32, dev), S,
+              cache.k.data_ptr(), cache.v.data_ptr(), cache.ks.data_ptr(), cache.vs.data_ptr(), C,
+              _kv8_vec(what, "lens", lens, (B,), torch.int32, dev),
+              None if counts is None else _kv8_vec(what, "counts", counts, (B,), torch.int32, dev), B, n, Hq, H, D,
+              D ** -0.5 if scale is None else float(scale), out.data_ptr(), so[0], so[1], D,
+              None if ws is None else ws.data_ptr(), 0 if ws is None else ws.nbytes)
+    return out
+
+
+def _kv8_layers(what, cache, dev):
+    """layers, B, H, C, D of a cache of one layer (four dimensions) or of several ([layers, B, H, C, D], scales likewise)."""
+    if cache.k.dim() == 4:
+        return (1, *_kv8_dims(what, cache, dev))
+    if any(t.dim() != d or not t.is_contiguous() for t, d in zip(cache, (5, 5, 4, 4))):
+        _kv8_fail(what, "cache tensors must be contiguous, of one layer or of several")
+    layers, B = cache.k.shape[:2]
+    if any(t.shape[:2] != (layers, B) for t in cache):
+        _kv8_fail(what, f"cache shapes {[tuple(t.shape) for t in cache]}")
+    return (layers, B, *_kv8_dims(what, Kv8(*(t.view(layers * B, *t.shape[2:]) for t in cache)), dev)[1:])
+
+
+def kv8_reorder(cache, parents, lens, beams=None, dst=None, new_lens=None):
+    """vt_kv8_reorder: sequence b takes the first lens[parents[b]] slots of sequence parents[b] (int32 on the device; negative: it
+    stays as it is), in every layer of a cache [B, H, C, D] or [layers, B, H, C, D].  In place when dst is None: `beams`
+    sequences that follow one another are a group, and parents lie within it.  Else into the cache dst (a fork, or a batch
+    without its finished sequences), from any sequence.  new_lens int32 [B] (not lens) receives the lengths."""
+    what, dev = "kv8_reorder", cache.k.get_device()
+    layers, Bs, H, C, D = _kv8_layers(what, cache, dev)
+    B, Cd = Bs, C
+    if dst is None:
+        if beams is None:
+            _kv8_fail(what, "in place needs the number of beams of a group")
+    else:
+        if beams is not None:
+            _kv8_fail(what, "beams are groups of a cache that is reordered in place: no dst")
+        Ld, B, Hd, Cd, Dd = _kv8_layers(what, dst, dev)
+        if (Ld, Hd, Dd) != (layers, H, D):
+            _kv8_fail(what, f"dst {tuple(dst.k.shape)} for a cache of {tuple(cache.k.shape)}")
+    _kv8_call(lib().vt_kv8_reorder, "vt_kv8_reorder", dev, cache.k.data_ptr(), cache.v.data_ptr(), cache.ks.data_ptr(),
+              cache.vs.data_ptr(), layers, Bs, C, *((None,) * 4 if dst is None else (t.data_ptr() for t in dst)), Cd,
+              _kv8_vec(what, "parents", parents, (B,), torch.int32, dev), _kv8_vec(what, "lens", lens, (Bs,), torch.int32, dev), B,
+              0 if beams is None else int(beams), H, D,
+              None if new_lens is None else _kv8_vec(what, "new_lens", new_lens, (B,), torch.int32, dev))
+
+
+class Beams(NamedTuple):
+    """What beam_select chose, best first: totals fp32, rows of the batch int32, words int32, whether they are finished; each [S, k]."""
+    scores: torch.Tensor
+    parents: torch.Tensor
+    tokens: torch.Tensor
+    done: torch.Tensor
+
+
+def beam_select(logits, scores, beams, k=None, eos=-1, done=None, out=None, ws=None):
+    """vt_beam_select: of each group of `beams` rows of logits [S beams, V] (bf16 or fp32, any row pitch) the k (default beams)
+    continuations with the largest scores [S beams] + log softmax(logits), the lowest beam * V + word first where totals are equal.
+    A beam that is finished (done bool [S beams]) goes on with the word eos alone, as it is.  Returns Beams (out, where given); where
+    fewer than k are left their score is -inf, their word -1.  ws: a uint8 tensor of vt_beam_select_ws_bytes, else one is allocated."""
+    what, dev = "beam_select", logits.get_device()
+    if logits.dim() != 2 or logits.dtype not in (BF16, torch.float32) or logits.stride(1) != 1:
+        _kv8_fail(what, f"logits {tuple(logits.shape)} {logits.dtype} (bf16 or float32 rows)")
+    (B, V), beams = logits.shape, int(beams)
+    if beams <= 0 or B % beams:
+        _kv8_fail(what, f"{B} rows in groups of {beams}")
+    S, k = B // beams, beams if k is None else int(k)
+    if out is None:
+        out = Beams(*(torch.empty(S, max(k, 0), dtype=t, device=logits.device)
+                      for t in (torch.float32, torch.int32, torch.int32, torch.bool)))
+    nb = lib().vt_beam_select_ws_bytes(S, beams, V, k)
+    if ws is None:
+        ws = torch.empty(nb, dtype=torch.uint8, device=logits.device)
+    elif ws.get_device() != dev or not ws.is_contiguous():
+        _kv8_fail(what, "the workspace must be contiguous on the tensors' device")
+    _kv8_call(lib().vt_beam_select, "vt_beam_select", dev, logits.data_ptr(), logits.stride(0) if B > 1 else V,
+              int(logits.dtype is torch.float32), _kv8_vec(what, "scores", scores, (B,), torch.float32, dev),
+              None if done is None else _kv8_vec(what, "done", done, (B,), torch.bool, dev), S, beams, V, k, int(eos),
+              *(_kv8_vec(what, n, t, (S, k), d, dev) for n, t, d in zip(Beams._fields, out, (torch.float32, torch.int32, torch.int32, torch.bool))),
+              ws.data_ptr(), ws.nbytes)
+    return out
 
 
 def head_linear(x2, wt, bias, out):
