@@ -42,12 +42,12 @@ def totals(logits, scores, beams, eos=-1, done=None):
     res = np.full((B, V), -np.inf)
     for b in range(B):
         if done is not None and done[b]:
-            res[b, eos] = scores[b]
+            res[b, eos] = scores[b] if np.isfinite(scores[b]) else -np.inf
             continue
         with np.errstate(all="ignore"):
             top = x[b].max()
             t = float(scores[b]) + ((x[b] - top) - np.log(np.exp(x[b] - top).sum()))
-        res[b] = np.where(np.isnan(t), -np.inf, t)
+        res[b] = np.where(np.isfinite(t), t, -np.inf)
     return res.reshape(B // beams, beams * V)
 
 

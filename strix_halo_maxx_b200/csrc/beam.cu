@@ -1,95 +1,318 @@
 // The choice of a beam search: of a group of F beams the k continuations with the largest
 //   total(f, v) = score[f] + logit[f, v] - log sum_w exp(logit[f, w]),
-// in order, the lowest f V + v first where totals are equal.
+// in order, the lowest f V + v first where totals are equal.  Within a row totals follow its logits, so a row's k best words are found
+// without its sum, and the logits are read once:
+//   beam_words_kernel   a chunk of a row stays in registers: its largest logit, its sum of exponentials, and its k best words in order;
+//   beam_pick_kernel    a group: the rows' sums, the totals of the chunks' words, the k best of them.
+// The k best of many, in both: maxima of M >= 2 k parts (M = 4 k while it fits); the k'th largest of these maxima is a bound that k
+// values reach, and few others; those that reach it are gathered and each counts the ones ahead of it.  Everything is compared as (value,
+// place), so no two are equal: no order of arrival shows, and at most the k parts with a maximum that reaches the bound hold any.
 #include "vt_common.cuh"
 #include "vt_host.h"
 
 namespace vt {
 namespace beam {
 
-constexpr int MAX_BEAMS = 64, MAX_K = 128;
+constexpr int MAX_BEAMS = 64, MAX_K = 128, T = 256;  // threads of a CTA
+constexpr int CAP = 2048;                            // totals that beam_pick_kernel gathers; beyond, one by one
 
 struct Args {
   const void* logits;
   long long ld;
-  int f32;
   const float* scores;
   const uint8_t* done;
-  int F, V, k, eos;
+  int F, V, k, eos, chunks;
   float* out_scores;
   int *out_parents, *out_tokens;
   uint8_t* out_done;
-  double2* lse;  // of each row its largest logit and the log of the sum of exponentials above it
+  float2* sums;              // [rows][chunks] largest logit, sum of exponentials of the differences to it
+  unsigned long long* words; // [rows][chunks][k] (logit, place), best first; 0: none
 };
 
-__device__ __forceinline__ float logit(const Args& a, long long row, int v) {
-  return a.f32 ? static_cast<const float*>(a.logits)[row * a.ld + v] : bf2f(static_cast<const uint16_t*>(a.logits)[row * a.ld + v]);
-}
+// Parts whose maxima are compared: T threads in groups of T / parts.
+__host__ __device__ inline int parts_of(int k) { return k <= 8 ? 32 : k <= 16 ? 64 : k <= 32 ? 128 : 256; }
 
-__global__ void __launch_bounds__(256) beam_lse_kernel(Args a) {
-  __shared__ float red[8];
-  __shared__ double sum[8];
-  const int tid = threadIdx.x, lane = tid & 31;
-  griddep_wait();
-  griddep_launch();
-  float mx = -INFINITY;
-  for (int v = tid; v < a.V; v += 256) mx = fmaxf(mx, logit(a, blockIdx.x, v));
-  for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-  if (lane == 0) red[tid / 32] = mx;
-  __syncthreads();
-  for (int w = 0; w < 8; w++) mx = fmaxf(mx, red[w]);
-  double s = 0.;
-  for (int v = tid; v < a.V; v += 256) s += expf(logit(a, blockIdx.x, v) - mx);
-  for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-  if (lane == 0) sum[tid / 32] = s;
-  __syncthreads();
-  if (tid) return;
-  for (int w = 1; w < 8; w++) s += sum[w];
-  a.lse[blockIdx.x] = make_double2(mx, log(s));
+// A logit and its word as one number: larger logits first, of equal ones (zeros of both signs are) the lowest word; never 0.
+__device__ __forceinline__ unsigned long long key_of(float x, int v) {
+  const uint32_t u = __float_as_uint(x), o = u & 0x80000000u ? ~u : u | 0x80000000u;
+  return (unsigned long long)o << 32 | (uint32_t)~v;
 }
+__device__ __forceinline__ float key_logit(unsigned long long key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ unsigned long long shfl_xor(unsigned long long x, int d) { return __shfl_xor_sync(0xffffffffu, x, d); }
 
-// One group a CTA; round j takes the best candidate behind the one of round j - 1.
-__global__ void __launch_bounds__(256) beam_pick_kernel(Args a) {
-  __shared__ double top[8];
-  __shared__ long long top_at[8];
-  const int tid = threadIdx.x, g = blockIdx.x;
-  griddep_wait();
-  griddep_launch();
-  double last = INFINITY;
-  long long last_at = -1;
-  for (int j = 0; j < a.k; j++) {
-    double best = -INFINITY;
-    long long at = -1;
-    for (int f = 0; f < a.F; f++) {
-      const long long row = (long long)g * a.F + f;
-      const bool held = a.done && a.done[row];
-      for (int v = held ? a.eos + (tid ? a.V : 0) : tid; v < (held ? a.eos + 1 : a.V); v += 256) {
-        const double t = held ? a.scores[row] : a.scores[row] + (((double)logit(a, row, v) - a.lse[row].x) - a.lse[row].y);
-        const long long c = (long long)f * a.V + v;
-        if ((t < last || (t == last && c > last_at)) && t > best) best = t, at = c;
+template <typename Word, int VEC, int E>
+__device__ __forceinline__ void load_chunk(const Word* row, int v0, int V, float (&x)[E]) {
+#pragma unroll
+  for (int r = 0; r < E / VEC; r++) {
+    const int v = v0 + (r * T + (int)threadIdx.x) * VEC;
+    if (VEC > 1 && v + VEC <= V) {
+      const uint4 w = __ldcs(reinterpret_cast<const uint4*>(row + v));
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < VEC; e++)
+        x[r * VEC + e] = sizeof(Word) == 4 ? __uint_as_float(u[e % 4]) : __uint_as_float(e & 1 ? u[e / 2 % 4] & 0xffff0000u : u[e / 2 % 4] << 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        float y = -INFINITY;
+        if (v + e < V) {
+          if constexpr (sizeof(Word) == 4) y = __ldcs(reinterpret_cast<const float*>(row) + v + e);
+          else y = bf2f(__ldcs(reinterpret_cast<const unsigned short*>(row) + v + e));
+        }
+        x[r * VEC + e] = y;
       }
     }
-    for (int x = 16; x > 0; x >>= 1) {
-      const double t = __shfl_xor_sync(0xffffffffu, best, x);
-      const long long c = __shfl_xor_sync(0xffffffffu, at, x);
-      if (t > best || (t == best && t > -INFINITY && c < at)) best = t, at = c;
-    }
-    if (tid % 32 == 0) top[tid / 32] = best, top_at[tid / 32] = at;
-    __syncthreads();
-    for (int w = 0; w < 8; w++)
-      if (top[w] > best || (top[w] == best && best > -INFINITY && top_at[w] < at)) best = top[w], at = top_at[w];
-    __syncthreads();
-    if (tid == 0) {
-      const long long o = (long long)g * a.k + j;
-      const int f = at < 0 ? j % a.F : (int)(at / a.V), v = at < 0 ? -1 : (int)(at % a.V);
-      a.out_scores[o] = (float)best;
-      a.out_parents[o] = g * a.F + f;
-      a.out_tokens[o] = v;
-      a.out_done[o] = at < 0 || v == a.eos || (a.done && a.done[(long long)g * a.F + f]);
-    }
-    if (at >= 0) last = best, last_at = at;
-    else last = -INFINITY;
   }
+}
+
+// CTA = T E words of a row.  Bound: DRAM with many rows (MEASURED), the latency of one chunk with few.
+template <typename Word, int VEC, int E>
+__global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
+  __shared__ float sh_max[T / 32], sh_sum[T / 32];
+  __shared__ unsigned long long part[T], found[T * E / 2];
+  __shared__ unsigned long long bound;
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.k;
+  const long long row = blockIdx.x / a.chunks;
+  const int chunk = blockIdx.x % a.chunks, v0 = chunk * (T * E);
+  griddep_wait();
+  griddep_launch();
+  if (a.done && a.done[row]) return;  // its words are not looked at
+  float x[E];
+  load_chunk<Word, VEC, E>(static_cast<const Word*>(a.logits) + row * a.ld, v0, a.V, x);
+  auto word = [&](int e) { return v0 + ((e / VEC) * T + tid) * VEC + e % VEC; };
+  // ---- the largest logit, and the thread's best word
+  float mx = -INFINITY;
+  int at = 0;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    x[e] += 0.f;  // -0 is 0
+    if (x[e] > mx) mx = x[e], at = e;
+  }
+  unsigned long long best = mx == -INFINITY ? 0 : key_of(mx, word(at));
+  float top = mx;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  if (lane == 0) sh_max[warp] = top;
+  // ---- the parts' maxima
+  const int parts = parts_of(k), per = T / parts;
+  for (int d = 1; d < per; d <<= 1) best = max(best, shfl_xor(best, d));
+  if (tid % per == 0) part[tid / per] = best;
+  if (tid == 0) count = 0, bound = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < T / 32; w++) top = fmaxf(top, sh_max[w]);
+  // ---- a part's rank among the maxima, its threads taking a share of them each; the k'th is the bound
+  {
+    int ahead = 0;
+    for (int i = tid % per; i < parts; i += per) ahead += part[i] > best;
+    for (int d = 1; d < per; d <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
+    if (tid % per == 0 && ahead == k - 1 && best) bound = best;  // 0 where fewer than k parts have a word
+  }
+  // ---- sum of exponentials; a chunk of -inf adds nothing, a NaN or +inf makes it NaN
+  {
+    const float ref = top == -INFINITY ? 0.f : top;
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; e++) s += ex2_approx((x[e] - ref) * 1.4426950408889634f);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if (lane == 0) sh_sum[warp] = s;
+  }
+  __syncthreads();
+  // ---- gather: k parts at most have words that reach the bound, T / parts E each
+  const unsigned long long lim = bound;
+  const float lim_x = lim ? key_logit(lim) : -INFINITY;
+#pragma unroll
+  for (int e = 0; e < E; e++)
+    if (x[e] >= lim_x && x[e] > -INFINITY) {
+      const unsigned long long key = key_of(x[e], word(e));
+      if (key >= lim) found[atomicAdd(&count, 1)] = key;
+    }
+  if (tid == 0) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < T / 32; w++) s += sh_sum[w];
+    a.sums[blockIdx.x] = make_float2(top, s);
+  }
+  __syncthreads();
+  const int n = count;
+  unsigned long long* to = a.words + (long long)blockIdx.x * k;
+  for (int i = tid; i < n; i += T) {
+    const unsigned long long key = found[i];
+    int ahead = 0;
+    for (int j = 0; j < n; j++) ahead += found[j] > key;
+    if (ahead < k) to[ahead] = key;
+  }
+  for (int i = n + tid; i < k; i += T) to[i] = 0;
+}
+
+// A continuation: its total, and beam * V + word; -inf and INT_MAX for none.
+struct Total {
+  double t;
+  int at;
+};
+__device__ __forceinline__ bool ahead_of(const Total& x, const Total& y) { return x.t > y.t || (x.t == y.t && x.at < y.at); }
+
+// CTA = a group.  Bound: latency, of two trips to L2 and the rounds of comparisons.
+__global__ void __launch_bounds__(T) beam_pick_kernel(Args a) {
+  __shared__ double sh_top[MAX_BEAMS], sh_log[MAX_BEAMS], sh_score[MAX_BEAMS];
+  __shared__ double part_t[T], found_t[CAP];
+  __shared__ int part_at[T], found_at[CAP];
+  __shared__ uint8_t sh_done[MAX_BEAMS];
+  __shared__ Total bound;
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.k, F = a.F;
+  const long long row0 = (long long)blockIdx.x * F;
+  griddep_wait();
+  griddep_launch();
+  // ---- of each row the largest logit and the log of its sum, a warp a row
+  for (int f = warp; f < F; f += T / 32) {
+    const bool done = a.done && a.done[row0 + f];
+    double top = -INFINITY, sum = 0.;
+    if (!done) {
+      const float2* s = a.sums + (row0 + f) * a.chunks;
+      float m = -INFINITY;
+      for (int c = lane; c < a.chunks; c += 32) m = fmaxf(m, s[c].x);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      for (int c = lane; c < a.chunks; c += 32) sum += s[c].y == 0.f ? 0. : s[c].y * exp((double)s[c].x - m);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      top = m;
+    }
+    if (lane == 0) sh_top[f] = top, sh_log[f] = log(sum), sh_score[f] = a.scores[row0 + f], sh_done[f] = done;
+  }
+  if (tid == 0) count = 0, bound = {-INFINITY, 0x7fffffff};
+  __syncthreads();
+  const Total none{-INFINITY, 0x7fffffff};
+  // entry j of list l: l = a chunk of a row; a finished beam's only entry stands in its first list
+  auto entry = [&](int l, int j) {
+    const int f = l / a.chunks;
+    Total x = none;
+    if (sh_done[f]) {
+      if (l % a.chunks == 0 && j == 0) x = {sh_score[f], f * a.V + a.eos};
+    } else {
+      const unsigned long long key = a.words[(row0 * a.chunks + l) * k + j];
+      if (key) x = {sh_score[f] + (((double)key_logit(key) - sh_top[f]) - sh_log[f]), f * a.V + (int)~(uint32_t)key};
+    }
+    return isfinite(x.t) ? x : none;
+  };
+  // every list is dealt out to `deal` runs (entries j, j + deal, ..: in order too), so that there are enough of them; thread t takes
+  // runs t, t + T, ..
+  const int lists = F * a.chunks, parts = parts_of(k), per = T / parts;
+  int deal = 1;
+  while (lists * deal < parts && deal < k) deal <<= 1;
+  const int runs = lists * deal;
+  Total best = none;
+  for (int r = tid; r < runs; r += T)
+    if (r % deal < k) {
+      const Total x = entry(r / deal, r % deal);
+      if (ahead_of(x, best)) best = x;
+    }
+  const Total mine = best;
+  for (int d = 1; d < per; d <<= 1) {
+    const Total x{__shfl_xor_sync(0xffffffffu, best.t, d), __shfl_xor_sync(0xffffffffu, best.at, d)};
+    if (ahead_of(x, best)) best = x;
+  }
+  if (tid % per == 0) part_t[tid / per] = best.t, part_at[tid / per] = best.at;
+  __syncthreads();
+  {
+    int ahead = 0;
+    for (int i = tid % per; i < parts; i += per) ahead += ahead_of({part_t[i], part_at[i]}, best);
+    for (int d = 1; d < per; d <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
+    if (tid % per == 0 && ahead == k - 1 && best.t > -INFINITY) bound = best;
+  }
+  __syncthreads();
+  const Total lim = bound;  // none where fewer than k parts have a continuation
+  auto reaches = [&](const Total& x) { return x.t > -INFINITY && !ahead_of(lim, x); };
+  if (reaches(mine))
+    for (int r = tid; r < runs; r += T)
+      for (int j = r % deal; j < k; j += deal) {
+        const Total x = entry(r / deal, j);
+        if (!reaches(x)) break;
+        const int n = atomicAdd(&count, 1);
+        if (n < CAP) found_t[n] = x.t, found_at[n] = x.at;
+      }
+  __syncthreads();
+  const int n = count;
+  const long long o = (long long)blockIdx.x * k;
+  auto put = [&](int j, const Total& x) {
+    const int f = x.at / a.V, v = x.at % a.V;
+    a.out_scores[o + j] = (float)x.t;
+    a.out_parents[o + j] = (int)row0 + f;
+    a.out_tokens[o + j] = v;
+    a.out_done[o + j] = v == a.eos || sh_done[f];
+  };
+  auto put_none = [&](int j) {
+    a.out_scores[o + j] = -INFINITY;
+    a.out_parents[o + j] = (int)row0 + j % F;
+    a.out_tokens[o + j] = -1;
+    a.out_done[o + j] = 1;
+  };
+  if (n <= CAP) {
+    for (int i = tid; i < n; i += T) {
+      const Total x{found_t[i], found_at[i]};
+      int ahead = 0;
+      for (int j = 0; j < n; j++) ahead += ahead_of({found_t[j], found_at[j]}, x);
+      if (ahead < k) put(ahead, x);
+    }
+    for (int j = n + tid; j < k; j += T) put_none(j);
+    return;
+  }
+  // far more than k reach the bound (words that stand together in a few of many lists): one by one, the best behind the last
+  Total last{INFINITY, -1};
+  for (int j = 0; j < k; j++) {
+    best = none;
+    for (int r = tid; r < runs; r += T)
+      for (int i = r % deal; i < k; i += deal) {
+        const Total x = entry(r / deal, i);
+        if (!ahead_of(x, best)) break;
+        if (ahead_of(last, x)) {
+          best = x;
+          break;
+        }
+      }
+    for (int d = 1; d < 32; d <<= 1) {
+      const Total x{__shfl_xor_sync(0xffffffffu, best.t, d), __shfl_xor_sync(0xffffffffu, best.at, d)};
+      if (ahead_of(x, best)) best = x;
+    }
+    if (lane == 0) part_t[warp] = best.t, part_at[warp] = best.at;
+    __syncthreads();
+    for (int w = 0; w < T / 32; w++) {
+      const Total x{part_t[w], part_at[w]};
+      if (ahead_of(x, best)) best = x;
+    }
+    __syncthreads();
+    last = best;  // n > CAP >= k: there is one
+    if (tid == 0) put(j, best);
+  }
+}
+
+struct Plan {
+  int e, chunks;  // words of a thread, chunks of a row
+  long long words_off, bytes;
+};
+// Large chunks (32 words a thread) cost less in lists for the second kernel, small ones fill the GPU with few rows (MEASURED2).
+static Plan make_plan(int S, int F, int V, int k, int sms) {
+  Plan p;
+  const long long rows = (long long)S * F;
+  for (p.e = 32; p.e > 8; p.e >>= 1)
+    if (rows * ((V + T * p.e - 1) / (T * p.e)) >= 2LL * sms) break;
+  p.chunks = (int)(((long long)V + T * p.e - 1) / (T * p.e));
+  p.words_off = (rows * p.chunks * 8 + 255) / 256 * 256;
+  p.bytes = p.words_off + rows * p.chunks * k * 8;
+  return p;
+}
+
+template <typename Word, int VEC>
+static void launch_words(cudaStream_t st, const Args& a, const Plan& p, unsigned ctas) {
+  if (p.e == 32) launch_k(beam_words_kernel<Word, VEC, 32>, ctas, T, 0, st, a);
+  else if (p.e == 16) launch_k(beam_words_kernel<Word, VEC, 16>, ctas, T, 0, st, a);
+  else launch_k(beam_words_kernel<Word, VEC, 8>, ctas, T, 0, st, a);
 }
 
 }  // namespace beam
@@ -98,8 +321,9 @@ __global__ void __launch_bounds__(256) beam_pick_kernel(Args a) {
 extern "C" {
 
 long long vt_beam_select_ws_bytes(int S, int F, int V, int k) {
-  if (S <= 0 || F <= 0 || F > vt::beam::MAX_BEAMS || V <= 0 || k <= 0 || k > vt::beam::MAX_K) return 0;
-  return 16LL * S * F;
+  using namespace vt;
+  if (S <= 0 || F <= 0 || F > beam::MAX_BEAMS || V <= 0 || k <= 0 || k > beam::MAX_K) return 0;
+  return beam::make_plan(S, F, V, k, sm_count()).bytes;
 }
 
 int vt_beam_select(cudaStream_t st, const void* logits, long long ld, int f32, const float* scores, const uint8_t* done, int S, int F,
@@ -117,16 +341,23 @@ int vt_beam_select(cudaStream_t st, const void* logits, long long ld, int f32, c
   const long long need = vt_beam_select_ws_bytes(S, F, V, k);
   if (!ws || !aligned16(ws) || ws_bytes < need)
     return set_error(E_SHAPE, "%s: workspace of %lld bytes, %lld needed (16-byte aligned)", what, ws ? ws_bytes : 0LL, need);
-  if ((long long)S * F > 0xffffffLL) return set_error(E_SHAPE, "%s: S=%d too large", what, S);
+  const beam::Plan p = beam::make_plan(S, F, V, k, sm_count());
   const long long rows = (long long)S * F, n = (long long)S * k, es = f32 ? 4 : 2;
+  if (rows > 0xffffffLL || (long long)F * V > 0x7ffffffeLL || rows * p.chunks > 0x7fffffffLL)
+    return set_error(E_SHAPE, "%s: S=%d or F * V = %lld too large", what, S, (long long)F * V);
   const struct { const void* p; long long n; } in[] = {{logits, ((rows - 1) * ld + V) * es}, {scores, rows * 4}, {done, done ? rows : 0}, {ws, need}},
       outs[] = {{out_scores, n * 4}, {out_parents, n * 4}, {out_tokens, n * 4}, {out_done, n}};
   for (const auto& x : in)
     for (const auto& y : outs)
       if (x.n && kv8::overlap(x.p, x.n, y.p, y.n)) return set_error(E_SHAPE, "%s: an output overlaps an input", what);
-  beam::Args a{logits, ld, f32, scores, done, F, V, k, eos, out_scores, out_parents, out_tokens, out_done, (double2*)ws};
-  launch_k(beam::beam_lse_kernel, S * F, 256, 0, st, a);
-  launch_k(beam::beam_pick_kernel, S, 256, 0, st, a);
+  beam::Args a{logits, ld, scores, done, F, V, k, eos, p.chunks, out_scores, out_parents, out_tokens, out_done, (float2*)ws,
+               (unsigned long long*)((char*)ws + p.words_off)};
+  // rows that do not all begin on 16 bytes are read a word at a time: the words of a chunk must not depend on where its row begins
+  const bool wide = aligned16(logits) && (rows == 1 || ld * es % 16 == 0);
+  const unsigned ctas = (unsigned)(rows * p.chunks);
+  if (f32) wide ? beam::launch_words<float, 4>(st, a, p, ctas) : beam::launch_words<float, 1>(st, a, p, ctas);
+  else wide ? beam::launch_words<uint16_t, 8>(st, a, p, ctas) : beam::launch_words<uint16_t, 1>(st, a, p, ctas);
+  launch_k(beam::beam_pick_kernel, S, beam::T, 0, st, a);
   return check_launch(what);
 }
 

@@ -7,7 +7,7 @@ namespace kv8 {
 namespace reorder {
 
 constexpr int MAX_BEAMS = 64, THREADS = 128;
-constexpr int STAGE = 32768, MAX_CHUNK = 16384;  // bytes of the sources that are brought in together, of one of them at most
+constexpr int STAGE = 16384, MAX_CHUNK = 8192;  // bytes of the sources that are brought in together, of one of them at most
 constexpr long long kDrainCycles = 200000000LL;
 
 struct Args {
@@ -17,8 +17,8 @@ struct Args {
   float *dks, *dvs;
   const int *parents, *lens;
   int* new_lens;
-  int Bs, B, slots, H, C, Cd, D;  // slots: sequences that are brought in together
-  int chunk, splits;              // bytes of a sequence's codes at a time; CTAs that share an item
+  int layers, Bs, B, slots, H, C, Cd, D;  // slots: sequences that are brought in together
+  int chunk, ctas;                        // bytes of a sequence's codes at a time; CTAs of a group
 };
 
 // What sequence b becomes: -1 where it stays as it is.  Parents and lengths live on the device, where the host cannot refuse them:
@@ -38,10 +38,11 @@ __device__ __forceinline__ int len_of(const Args& a, int p, bool record) {
   return in;
 }
 
-// An item is one operand (K or V codes) of one head of a layer, of the `slots` sequences that are brought in together: in place a group's
-// beams, into another cache one source.  A CTA takes every splits'th chunk of an item: thread t brings the chunk of the t'th source in
-// if another sequence becomes it, all wait for all of them, then the threads of the sequences that become them write it out.  The
-// copies are bulk ones of up to 16 KB and take no registers; a chunk's loads run beside the stores of the one before.
+// The sequences that are brought in together are a group: in place its beams, into another cache one source.  A unit is a chunk of the
+// codes of one operand (K or V) of one head of a layer, of all sequences of a group; a group's CTAs take its units in turn.  Thread t
+// brings in the chunk of the t'th source, if another sequence becomes it; all wait for all of them, then the threads of the sequences
+// that become them write it out.  The copies are bulk ones of up to 16 KB, take no registers, and the next unit's loads run beside the
+// stores of this one.
 // Bound: DRAM, a read of every source that moves and a write of every sequence that changes (MEASURED).
 __global__ void __launch_bounds__(THREADS) kv8_reorder_kernel(Args a) {
   extern __shared__ __align__(128) uint8_t sm[];
@@ -50,14 +51,7 @@ __global__ void __launch_bounds__(THREADS) kv8_reorder_kernel(Args a) {
   volatile int* abort_flag = &sh_abort;
   const int tid = threadIdx.x, slots = a.slots;
   const bool in_place = a.dk == a.kc;
-  long long x = blockIdx.x;
-  const int split = (int)(x % a.splits);
-  x /= a.splits;
-  const bool v = x & 1;
-  x >>= 1;
-  const int h = (int)(x % a.H);
-  x /= a.H;
-  const int groups = a.Bs / slots, p0 = (int)(x % groups) * slots, layer = (int)(x / groups);
+  const int p0 = blockIdx.x / a.ctas * slots, cta = blockIdx.x % a.ctas;
   if (tid == 0) {
     mbar_init(&full[0], slots);
     mbar_init(&full[1], slots);
@@ -68,87 +62,98 @@ __global__ void __launch_bounds__(THREADS) kv8_reorder_kernel(Args a) {
   griddep_wait();
   griddep_launch();
   __syncthreads();
-  // the sequences that may become one of this item's sources: b_lo .., a thread each
+  // the sequences that may become one of the group's sources: b_lo .., a thread each
   const int b_lo = in_place ? p0 : 0, b_n = in_place ? slots : a.B;
-  const bool record = h == 0 && layer == 0 && !v && split == 0;
   for (int i = tid; i < b_n; i += THREADS) {
-    const int p = parent_of(a, b_lo + i, record);
-    if (p >= p0 && p < p0 + slots && !(in_place && p == b_lo + i)) need[p - p0] = 1;
-    if (record && (in_place || p0 == 0)) {
-      const int from = p >= 0 ? p : in_place ? b_lo + i : -1;
-      const int len = from >= 0 ? len_of(a, from, true) : 0;
-      if (a.new_lens && from >= 0) a.new_lens[b_lo + i] = len;
+    const int p = parent_of(a, b_lo + i, cta == 0);
+    const bool moves = p >= p0 && p < p0 + slots && !(in_place && p == b_lo + i);
+    const int from = p >= 0 ? p : b_lo + i;
+    const bool mine = cta == 0 && (in_place || (p0 == 0 && p >= 0));  // lengths are looked at once
+    if (moves || mine) {
+      const int len = len_of(a, from, mine);
+      if (moves) need[p - p0] = len;
+      if (mine && a.new_lens) a.new_lens[b_lo + i] = len;
     }
   }
   __syncthreads();
+  int longest = 0;
+  for (int i = 0; i < slots; i++) longest = max(longest, need[i]);
+  const int chunks = (int)(((long long)longest * a.D + a.chunk - 1) / a.chunk);
+  const long long units = 2LL * a.layers * a.H * chunks;  // chunk by chunk, K and V, head by head, layer by layer
   const size_t row = (size_t)a.C * a.D, drow = (size_t)a.Cd * a.D;  // bytes of a head
-  const int8_t* src = (v ? a.vc : a.kc) + ((size_t)layer * a.Bs * a.H + h) * row;  // of sequence p: + p H row
-  int8_t* dst = (v ? a.dv : a.dk) + ((size_t)layer * a.B * a.H + h) * drow;
-  // ---- scales, by the first CTA of an item: values of a few columns of all sequences are read before the first is written
-  if (split == 0) {
-    const float* ss = (v ? a.vs : a.ks) + ((size_t)layer * a.Bs * a.H + h) * (a.C / BLK);
-    float* ds = (v ? a.dvs : a.dks) + ((size_t)layer * a.B * a.H + h) * (a.Cd / BLK);
-    const int nb = min(a.C, a.Cd) / BLK;
-    if (in_place) {
-      constexpr int PER = 4;
-      const int cols = THREADS * PER / slots;
-      for (int c0 = 0; c0 < nb; c0 += cols) {
-        float val[PER];
-        size_t to[PER];
+  const int mine = tid < slots ? need[tid] * a.D : 0;               // bytes of this thread's source
+  auto load = [&](long long u, int st) {
+    if (tid >= slots) return;
+    const int at = (int)(u % chunks) * a.chunk, bytes = min(a.chunk, mine - at);
+    const long long x = u / chunks, lh = x >> 1;
+    mbar_arrive_expect_tx(&full[st], bytes > 0 ? bytes : 0);
+    if (bytes > 0)
+      bulk_load(sm + (size_t)(st * slots + tid) * a.chunk,
+                (x & 1 ? a.vc : a.kc) + ((lh / a.H * a.Bs + p0 + tid) * a.H + lh % a.H) * row + at, bytes, &full[st]);
+  };
+  if (cta < units) load(cta, 0);
+  // ---- scales, while the first unit arrives
+  const int heads2 = 2 * a.layers * a.H, sb = a.C / BLK, db = a.Cd / BLK;
+  auto scale_at = [&](int x, int B, int b, int blocks) { return ((size_t)(x >> 1) / a.H * B + b) * a.H * blocks + (size_t)((x >> 1) % a.H) * blocks; };
+  if (in_place) {  // columns of one block of all sequences: they are read before the first of them is written
+    constexpr int PER = 4;
+    const int nb = (longest + BLK - 1) / BLK, cols = THREADS * PER / slots;
+    const long long all = (long long)heads2 * nb;
+    for (long long c0 = (long long)cta * cols; c0 < all; c0 += (long long)a.ctas * cols) {
+      float val[PER];
+      float* to[PER];
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-          const int e = tid + THREADS * k, i = e / cols, c = c0 + e % cols;
-          to[k] = (size_t)-1;
-          if (i >= slots || c >= nb) continue;
-          const int p = parent_of(a, p0 + i, false);
-          if (p < 0 || p == p0 + i || c * BLK >= len_of(a, p, false)) continue;
-          val[k] = ss[(size_t)p * a.H * (a.C / BLK) + c];
-          to[k] = (size_t)(p0 + i) * a.H * (a.C / BLK) + c;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < PER; k++)
-          if (to[k] != (size_t)-1) ds[to[k]] = val[k];
+      for (int k = 0; k < PER; k++) {
+        const int e = tid + THREADS * k, i = e / cols;
+        const long long c = c0 + e % cols;
+        to[k] = nullptr;
+        if (i >= slots || c >= all) continue;
+        const int p = parent_of(a, p0 + i, false), x = (int)(c / nb), blk = (int)(c % nb);
+        if (p < 0 || p == p0 + i || blk * BLK >= need[p - p0]) continue;
+        val[k] = (x & 1 ? a.vs : a.ks)[scale_at(x, a.Bs, p, sb) + blk];
+        to[k] = (x & 1 ? a.dvs : a.dks) + scale_at(x, a.B, p0 + i, db) + blk;
       }
-    } else {  // shared among the sources' CTAs, whatever they bring in
-      for (int b = p0; b < a.B; b += a.Bs) {
-        const int p = parent_of(a, b, false);
-        if (p < 0) continue;
-        const int blocks = (len_of(a, p, false) + BLK - 1) / BLK;
-        for (int c = tid; c < blocks; c += THREADS) ds[(size_t)b * a.H * (a.Cd / BLK) + c] = ss[(size_t)p * a.H * (a.C / BLK) + c];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < PER; k++)
+        if (to[k]) *to[k] = val[k];
+    }
+  } else {  // the sequences are dealt out to the groups, whatever they become
+    for (int b = p0; b < a.B; b += a.Bs) {
+      const int p = parent_of(a, b, false);
+      if (p < 0) continue;
+      const int nb = (len_of(a, p, false) + BLK - 1) / BLK;
+      const long long all = (long long)heads2 * nb;
+      for (long long e = (long long)cta * THREADS + tid; e < all; e += (long long)a.ctas * THREADS) {
+        const int x = (int)(e / nb), blk = (int)(e % nb);
+        (x & 1 ? a.dvs : a.dks)[scale_at(x, a.B, b, db) + blk] = (x & 1 ? a.vs : a.ks)[scale_at(x, a.Bs, p, sb) + blk];
       }
     }
   }
   // ---- codes
-  const int mine = tid < slots && need[tid] ? len_of(a, p0 + tid, false) * a.D : 0;  // bytes of this thread's source
-  int longest = 0;
-  for (int i = 0; i < slots; i++) longest = max(longest, need[i] ? len_of(a, p0 + i, false) : 0);
-  const int chunks = (int)(((long long)longest * a.D + a.chunk - 1) / a.chunk);
-  auto load = [&](int c, int st) {
-    if (tid >= slots) return;
-    const int at = c * a.chunk, bytes = min(a.chunk, mine - at);
-    mbar_arrive_expect_tx(&full[st], bytes > 0 ? bytes : 0);
-    if (bytes > 0) bulk_load(sm + (size_t)(st * slots + tid) * a.chunk, src + (size_t)(p0 + tid) * a.H * row + at, bytes, &full[st]);
-  };
-  if (split < chunks) load(split, 0);
-  for (int c = split, n = 0; c < chunks; c += a.splits, n++) {
+  int n = 0;
+  for (long long u = cta; u < units; u += a.ctas, n++) {
     const int st = n & 1;
-    if (c + a.splits < chunks) {  // the other stage: its stores have been read out
+    if (u + a.ctas < units) {  // the other stage: its stores have been read out
       bulk_wait_read<0>();
       __syncthreads();
-      load(c + a.splits, st ^ 1);
+      load(u + a.ctas, st ^ 1);
     }
     const bool ok = mbar_wait(&full[st], (n >> 1) & 1, abort_flag, ST_KV8_WAIT);
     if (!ok) {  // copies in flight land before the CTA ends
       mbar_wait_drain(&full[st], (n >> 1) & 1, kDrainCycles);
-      if (c + a.splits < chunks) mbar_wait_drain(&full[st ^ 1], ((n + 1) >> 1) & 1, kDrainCycles);
+      if (u + a.ctas < units) mbar_wait_drain(&full[st ^ 1], ((n + 1) >> 1) & 1, kDrainCycles);
       break;
     }
+    const int at = (int)(u % chunks) * a.chunk;
+    const long long x = u / chunks, lh = x >> 1;
     for (int i = tid; i < b_n; i += THREADS) {
       const int p = parent_of(a, b_lo + i, false);
       if (p < p0 || p >= p0 + slots || (in_place && p == b_lo + i)) continue;
-      const int at = c * a.chunk, bytes = min(a.chunk, len_of(a, p, false) * a.D - at);
-      if (bytes > 0) bulk_store(dst + (size_t)(b_lo + i) * a.H * drow + at, sm + (size_t)(st * slots + p - p0) * a.chunk, bytes);
+      const int bytes = min(a.chunk, need[p - p0] * a.D - at);
+      if (bytes > 0)
+        bulk_store((x & 1 ? a.dv : a.dk) + ((lh / a.H * a.B + b_lo + i) * a.H + lh % a.H) * drow + at,
+                   sm + (size_t)(st * slots + p - p0) * a.chunk, bytes);
     }
     bulk_commit();
   }
@@ -193,16 +198,18 @@ extern "C" int vt_kv8_reorder(cudaStream_t st, int8_t* kc, int8_t* vc, float* ks
   int chunk = kv8::reorder::STAGE / slots / 128 * 128;
   if (chunk > kv8::reorder::MAX_CHUNK) chunk = kv8::reorder::MAX_CHUNK;
   if (chunk > top) chunk = top;
-  // items of two operands; split so that there are about eight CTAs for each SM, where the caches are long enough
-  const long long items = 2LL * layers * H * (Bs / slots), chunks = (top + chunk - 1) / chunk;
-  long long splits = (8LL * sm_count() + items - 1) / items;
-  if (splits > chunks) splits = chunks;
-  if (items * splits > 0x7fffffffLL) return set_error(E_SHAPE, "%s: grid too large (layers=%d H=%d B=%d)", what, layers, H, B);
+  // CTAs for every SM to hold as many as fit, or several times as many where each still has many units (lengths may differ)
+  const long long groups = Bs / slots, units = 2LL * layers * H * ((top + chunk - 1) / chunk);
+  const int fit = 225 * 1024 / (2 * slots * chunk + 2048), per_sm = fit > 16 ? 16 : fit;
+  const long long one = (long long)per_sm * sm_count(), want = units * groups > 16 * one ? 4 * one : one;
+  long long ctas = (want + groups - 1) / groups;
+  if (ctas > units) ctas = units;
+  if (groups * ctas > 0x7fffffffLL) return set_error(E_SHAPE, "%s: grid too large (B=%d)", what, B);
   kv8::reorder::Args a{kc, vc, ks, vs, in_place ? kc : dst_kc, in_place ? vc : dst_vc, in_place ? ks : dst_ks, in_place ? vs : dst_vs,
-                       parents, lens, new_lens, Bs, B, slots, H, C, in_place ? C : dst_C, D, chunk, (int)splits};
-  const int smem = (chunks > splits ? 2 : 1) * slots * chunk;  // one stage where a CTA has one chunk
+                       parents, lens, new_lens, layers, Bs, B, slots, H, C, in_place ? C : dst_C, D, chunk, (int)ctas};
+  const int smem = (units > ctas ? 2 : 1) * slots * chunk;  // one stage where a CTA has one unit
   rc = smem_attr_once((const void*)kv8::reorder::kv8_reorder_kernel, 2 * kv8::reorder::STAGE, what);
   if (rc) return rc;
-  launch_k(kv8::reorder::kv8_reorder_kernel, (unsigned)(items * splits), kv8::reorder::THREADS, smem, st, a);
+  launch_k(kv8::reorder::kv8_reorder_kernel, (unsigned)(groups * ctas), kv8::reorder::THREADS, smem, st, a);
   return check_launch(what);
 }

@@ -621,14 +621,22 @@ def attn_kv8_shared(q, prefix, plens, cache, lens, out=None, counts=None, scale=
 
 def _kv8_layers(what, cache, dev):
     """layers, B, H, C, D of a cache of one layer (four dimensions) or of several ([layers, B, H, C, D], scales likewise)."""
-    if cache.k.dim() == 4:
+    k, v, ks, vs = cache
+    shape = k.shape
+    if len(shape) == 4:
         return (1, *_kv8_dims(what, cache, dev))
-    if any(t.dim() != d or not t.is_contiguous() for t, d in zip(cache, (5, 5, 4, 4))):
-        _kv8_fail(what, "cache tensors must be contiguous, of one layer or of several")
-    layers, B = cache.k.shape[:2]
-    if any(t.shape[:2] != (layers, B) for t in cache):
+    if len(shape) != 5:
+        _kv8_fail(what, f"cache shape {tuple(shape)}")
+    layers, B, H, C, D = shape
+    scales = (layers, B, H, C // KV8_BLOCK)
+    if k.dtype is not torch.int8 or v.dtype is not torch.int8 or ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
+        _kv8_fail(what, "codes are int8, scales float32")
+    if v.shape != shape or ks.shape != scales or vs.shape != scales or C % KV8_BLOCK:
         _kv8_fail(what, f"cache shapes {[tuple(t.shape) for t in cache]}")
-    return (layers, B, *_kv8_dims(what, Kv8(*(t.view(layers * B, *t.shape[2:]) for t in cache)), dev)[1:])
+    for t in cache:
+        if t.get_device() != dev or not t.is_contiguous():
+            _kv8_fail(what, "cache tensors must be contiguous on one device")
+    return layers, B, H, C, D
 
 
 def kv8_reorder(cache, parents, lens, beams=None, dst=None, new_lens=None):
@@ -648,8 +656,9 @@ def kv8_reorder(cache, parents, lens, beams=None, dst=None, new_lens=None):
         Ld, B, Hd, Cd, Dd = _kv8_layers(what, dst, dev)
         if (Ld, Hd, Dd) != (layers, H, D):
             _kv8_fail(what, f"dst {tuple(dst.k.shape)} for a cache of {tuple(cache.k.shape)}")
+    dk, dv, dks, dvs = (None,) * 4 if dst is None else (t.data_ptr() for t in dst)
     _kv8_call(lib().vt_kv8_reorder, "vt_kv8_reorder", dev, cache.k.data_ptr(), cache.v.data_ptr(), cache.ks.data_ptr(),
-              cache.vs.data_ptr(), layers, Bs, C, *((None,) * 4 if dst is None else (t.data_ptr() for t in dst)), Cd,
+              cache.vs.data_ptr(), layers, Bs, C, dk, dv, dks, dvs, Cd,
               _kv8_vec(what, "parents", parents, (B,), torch.int32, dev), _kv8_vec(what, "lens", lens, (Bs,), torch.int32, dev), B,
               0 if beams is None else int(beams), H, D,
               None if new_lens is None else _kv8_vec(what, "new_lens", new_lens, (B,), torch.int32, dev))
