@@ -4,8 +4,8 @@
 // without its sum, and the logits are read once:
 //   beam_words_kernel   a chunk of a row stays in registers: its largest logit, its sum of exponentials, and its k best words in order;
 //   beam_pick_kernel    a group: the rows' sums, the totals of the chunks' words, the k best of them.
-// The k best of many, in both: maxima of M >= 2 k parts (M = 4 k while it fits); the k'th largest of these maxima is a bound that k
-// values reach, and few others; those that reach it are gathered and each counts the ones ahead of it.  Everything is compared as (value,
+// The k best of many, in both: maxima of parts, more than k of them; the k'th largest of these maxima is a bound that k values
+// reach, and few others; those that reach it are gathered and each counts the ones ahead of it.  Everything is compared as (value,
 // place), so no two are equal: no order of arrival shows, and at most the k parts with a maximum that reaches the bound hold any.
 #include "vt_common.cuh"
 #include "vt_host.h"
@@ -13,7 +13,7 @@
 namespace vt {
 namespace beam {
 
-constexpr int MAX_BEAMS = 64, MAX_K = 128, T = 256;  // threads of a CTA
+constexpr int MAX_BEAMS = 64, MAX_K = 128, T = 256, TP = 512;  // threads of a CTA of the two kernels
 constexpr int CAP = 2048;                            // totals that beam_pick_kernel gathers; beyond, one by one
 
 struct Args {
@@ -29,12 +29,13 @@ struct Args {
   unsigned long long* words; // [rows][chunks][k] (logit, place), best first; 0: none
 };
 
-// Parts whose maxima are compared: T threads in groups of T / parts.
-__host__ __device__ inline int parts_of(int k) { return k <= 8 ? 32 : k <= 16 ? 64 : k <= 32 ? 128 : 256; }
+// Parts of a chunk whose maxima are compared, T / parts threads each: 2 k or more.  The best k of 2 k parts leave about 1.4 k words to
+// gather, and as many comparisons as parts squared (MEASURED3).
+__host__ __device__ inline int parts_of(int k) { return k <= 16 ? 32 : k <= 32 ? 64 : k <= 64 ? 128 : 256; }
 
 // A logit and its word as one number: larger logits first, of equal ones (zeros of both signs are) the lowest word; never 0.
 __device__ __forceinline__ unsigned long long key_of(float x, int v) {
-  const uint32_t u = __float_as_uint(x), o = u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(x + 0.f), o = u & 0x80000000u ? ~u : u | 0x80000000u;
   return (unsigned long long)o << 32 | (uint32_t)~v;
 }
 __device__ __forceinline__ float key_logit(unsigned long long key) {
@@ -43,27 +44,27 @@ __device__ __forceinline__ float key_logit(unsigned long long key) {
 }
 __device__ __forceinline__ unsigned long long shfl_xor(unsigned long long x, int d) { return __shfl_xor_sync(0xffffffffu, x, d); }
 
+template <typename Word>
+__device__ __forceinline__ float load_word(const Word* p) {
+  if constexpr (sizeof(Word) == 4) return __ldg(p);
+  else return bf2f(__ldg(p));
+}
+// Words v0 + (r T + thread) VEC ..; -inf behind the row's end.
 template <typename Word, int VEC, int E>
 __device__ __forceinline__ void load_chunk(const Word* row, int v0, int V, float (&x)[E]) {
+  const Word* p = row + v0 + (int)threadIdx.x * VEC;
+  const int left = V - v0 - (int)threadIdx.x * VEC;
 #pragma unroll
   for (int r = 0; r < E / VEC; r++) {
-    const int v = v0 + (r * T + (int)threadIdx.x) * VEC;
-    if (VEC > 1 && v + VEC <= V) {
-      const uint4 w = __ldcs(reinterpret_cast<const uint4*>(row + v));
+    if (VEC > 1 && r * T * VEC + VEC <= left) {
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(p + r * T * VEC));
       const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int e = 0; e < VEC; e++)
         x[r * VEC + e] = sizeof(Word) == 4 ? __uint_as_float(u[e % 4]) : __uint_as_float(e & 1 ? u[e / 2 % 4] & 0xffff0000u : u[e / 2 % 4] << 16);
     } else {
 #pragma unroll
-      for (int e = 0; e < VEC; e++) {
-        float y = -INFINITY;
-        if (v + e < V) {
-          if constexpr (sizeof(Word) == 4) y = __ldcs(reinterpret_cast<const float*>(row) + v + e);
-          else y = bf2f(__ldcs(reinterpret_cast<const unsigned short*>(row) + v + e));
-        }
-        x[r * VEC + e] = y;
-      }
+      for (int e = 0; e < VEC; e++) x[r * VEC + e] = r * T * VEC + e < left ? load_word(p + r * T * VEC + e) : -INFINITY;
     }
   }
 }
@@ -82,16 +83,15 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
   griddep_launch();
   if (a.done && a.done[row]) return;  // its words are not looked at
   float x[E];
-  load_chunk<Word, VEC, E>(static_cast<const Word*>(a.logits) + row * a.ld, v0, a.V, x);
+  const Word* words = static_cast<const Word*>(a.logits) + row * a.ld;
+  load_chunk<Word, VEC, E>(words, v0, a.V, x);
   auto word = [&](int e) { return v0 + ((e / VEC) * T + tid) * VEC + e % VEC; };
   // ---- the largest logit, and the thread's best word
   float mx = -INFINITY;
   int at = 0;
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    x[e] += 0.f;  // -0 is 0
+  for (int e = 0; e < E; e++)
     if (x[e] > mx) mx = x[e], at = e;
-  }
   unsigned long long best = mx == -INFINITY ? 0 : key_of(mx, word(at));
   float top = mx;
 #pragma unroll
@@ -115,23 +115,33 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
   // ---- sum of exponentials; a chunk of -inf adds nothing, a NaN or +inf makes it NaN
   {
     const float ref = top == -INFINITY ? 0.f : top;
-    float s = 0.f;
+    const unsigned long long ref2 = f2_pack(-ref, -ref), log2e = f2_pack(1.4426950408889634f, 1.4426950408889634f);
+    unsigned long long s2 = 0ull;
 #pragma unroll
-    for (int e = 0; e < E; e++) s += ex2_approx((x[e] - ref) * 1.4426950408889634f);
+    for (int e = 0; e < E; e += 2) {
+      float y0, y1;
+      f2_unpack(f2_mul(f2_add(f2_pack(x[e], x[e + 1]), ref2), log2e), y0, y1);
+      s2 = f2_add(s2, f2_pack(ex2_approx(y0), ex2_approx(y1)));
+    }
+    float s, s_odd;
+    f2_unpack(s2, s, s_odd);
+    s += s_odd;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
     if (lane == 0) sh_sum[warp] = s;
   }
   __syncthreads();
-  // ---- gather: k parts at most have words that reach the bound, T / parts E each
+  // ---- gather: k parts at most have words that reach the bound, T / parts E each.  They are few: the others' only cost is a bit
   const unsigned long long lim = bound;
-  const float lim_x = lim ? key_logit(lim) : -INFINITY;
+  const float lim_x = lim ? key_logit(lim) : -3.402823466e38f;
+  uint32_t hits = 0;
 #pragma unroll
-  for (int e = 0; e < E; e++)
-    if (x[e] >= lim_x && x[e] > -INFINITY) {
-      const unsigned long long key = key_of(x[e], word(e));
-      if (key >= lim) found[atomicAdd(&count, 1)] = key;
-    }
+  for (int e = 0; e < E; e++) hits |= x[e] >= lim_x ? 1u << e : 0u;
+  for (; hits; hits &= hits - 1) {
+    const int v = word(__ffs(hits) - 1);
+    const unsigned long long key = key_of(load_word(words + v), v);
+    if (key >= lim) found[atomicAdd(&count, 1)] = key;
+  }
   if (tid == 0) {
     float s = 0.f;
 #pragma unroll
@@ -158,10 +168,10 @@ struct Total {
 __device__ __forceinline__ bool ahead_of(const Total& x, const Total& y) { return x.t > y.t || (x.t == y.t && x.at < y.at); }
 
 // CTA = a group.  Bound: latency, of two trips to L2 and the rounds of comparisons.
-__global__ void __launch_bounds__(T) beam_pick_kernel(Args a) {
+__global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
   __shared__ double sh_top[MAX_BEAMS], sh_log[MAX_BEAMS], sh_score[MAX_BEAMS];
-  __shared__ double part_t[T], found_t[CAP];
-  __shared__ int part_at[T], found_at[CAP];
+  __shared__ double part_t[TP], found_t[CAP];
+  __shared__ int part_at[TP], found_at[CAP];
   __shared__ uint8_t sh_done[MAX_BEAMS];
   __shared__ Total bound;
   __shared__ int count;
@@ -170,7 +180,7 @@ __global__ void __launch_bounds__(T) beam_pick_kernel(Args a) {
   griddep_wait();
   griddep_launch();
   // ---- of each row the largest logit and the log of its sum, a warp a row
-  for (int f = warp; f < F; f += T / 32) {
+  for (int f = warp; f < F; f += TP / 32) {
     const bool done = a.done && a.done[row0 + f];
     double top = -INFINITY, sum = 0.;
     if (!done) {
@@ -201,26 +211,31 @@ __global__ void __launch_bounds__(T) beam_pick_kernel(Args a) {
     }
     return isfinite(x.t) ? x : none;
   };
-  // every list is dealt out to `deal` runs (entries j, j + deal, ..: in order too), so that there are enough of them; thread t takes
-  // runs t, t + T, ..
-  const int lists = F * a.chunks, parts = parts_of(k), per = T / parts;
+  // every list is dealt out to `deal` runs (entries j, j + deal, ..: in order too); run r is of list r % lists, thread t takes runs
+  // t, t + TP, .., and threads p, p + parts, .. are a part: the best words of one beam stand in many parts
+  const int lists = F * a.chunks, parts = k <= 16 ? 64 : k <= 32 ? 128 : 256, per = TP / parts;
   int deal = 1;
-  while (lists * deal < parts && deal < k) deal <<= 1;
+  while (lists * deal < 2 * TP && deal < k) deal <<= 1;
   const int runs = lists * deal;
   Total best = none;
-  for (int r = tid; r < runs; r += T)
-    if (r % deal < k) {
-      const Total x = entry(r / deal, r % deal);
+  for (int r = tid; r < runs; r += TP)
+    if (r / lists < k) {
+      const Total x = entry(r % lists, r / lists);
       if (ahead_of(x, best)) best = x;
     }
   const Total mine = best;
-  for (int d = 1; d < per; d <<= 1) {
-    const Total x{__shfl_xor_sync(0xffffffffu, best.t, d), __shfl_xor_sync(0xffffffffu, best.at, d)};
-    if (ahead_of(x, best)) best = x;
-  }
-  if (tid % per == 0) part_t[tid / per] = best.t, part_at[tid / per] = best.at;
+  part_t[tid] = best.t, part_at[tid] = best.at;
   __syncthreads();
   {
+    const int from = tid / per + tid % per * parts;  // of this thread's part, TP / per of them
+    best = {part_t[from], part_at[from]};
+    for (int d = 1; d < per; d <<= 1) {
+      const Total x{__shfl_xor_sync(0xffffffffu, best.t, d), __shfl_xor_sync(0xffffffffu, best.at, d)};
+      if (ahead_of(x, best)) best = x;
+    }
+    __syncthreads();
+    if (tid % per == 0) part_t[tid / per] = best.t, part_at[tid / per] = best.at;
+    __syncthreads();
     int ahead = 0;
     for (int i = tid % per; i < parts; i += per) ahead += ahead_of({part_t[i], part_at[i]}, best);
     for (int d = 1; d < per; d <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
@@ -230,9 +245,9 @@ __global__ void __launch_bounds__(T) beam_pick_kernel(Args a) {
   const Total lim = bound;  // none where fewer than k parts have a continuation
   auto reaches = [&](const Total& x) { return x.t > -INFINITY && !ahead_of(lim, x); };
   if (reaches(mine))
-    for (int r = tid; r < runs; r += T)
-      for (int j = r % deal; j < k; j += deal) {
-        const Total x = entry(r / deal, j);
+    for (int r = tid; r < runs; r += TP)
+      for (int j = r / lists; j < k; j += deal) {
+        const Total x = entry(r % lists, j);
         if (!reaches(x)) break;
         const int n = atomicAdd(&count, 1);
         if (n < CAP) found_t[n] = x.t, found_at[n] = x.at;
@@ -254,22 +269,22 @@ __global__ void __launch_bounds__(T) beam_pick_kernel(Args a) {
     a.out_done[o + j] = 1;
   };
   if (n <= CAP) {
-    for (int i = tid; i < n; i += T) {
+    for (int i = tid; i < n; i += TP) {
       const Total x{found_t[i], found_at[i]};
       int ahead = 0;
       for (int j = 0; j < n; j++) ahead += ahead_of({found_t[j], found_at[j]}, x);
       if (ahead < k) put(ahead, x);
     }
-    for (int j = n + tid; j < k; j += T) put_none(j);
+    for (int j = n + tid; j < k; j += TP) put_none(j);
     return;
   }
   // far more than k reach the bound (words that stand together in a few of many lists): one by one, the best behind the last
   Total last{INFINITY, -1};
   for (int j = 0; j < k; j++) {
     best = none;
-    for (int r = tid; r < runs; r += T)
-      for (int i = r % deal; i < k; i += deal) {
-        const Total x = entry(r / deal, i);
+    for (int r = tid; r < runs; r += TP)
+      for (int i = r / lists; i < k; i += deal) {
+        const Total x = entry(r % lists, i);
         if (!ahead_of(x, best)) break;
         if (ahead_of(last, x)) {
           best = x;
@@ -282,7 +297,7 @@ __global__ void __launch_bounds__(T) beam_pick_kernel(Args a) {
     }
     if (lane == 0) part_t[warp] = best.t, part_at[warp] = best.at;
     __syncthreads();
-    for (int w = 0; w < T / 32; w++) {
+    for (int w = 0; w < TP / 32; w++) {
       const Total x{part_t[w], part_at[w]};
       if (ahead_of(x, best)) best = x;
     }
@@ -357,7 +372,7 @@ int vt_beam_select(cudaStream_t st, const void* logits, long long ld, int f32, c
   const unsigned ctas = (unsigned)(rows * p.chunks);
   if (f32) wide ? beam::launch_words<float, 4>(st, a, p, ctas) : beam::launch_words<float, 1>(st, a, p, ctas);
   else wide ? beam::launch_words<uint16_t, 8>(st, a, p, ctas) : beam::launch_words<uint16_t, 1>(st, a, p, ctas);
-  launch_k(beam::beam_pick_kernel, S, beam::T, 0, st, a);
+  launch_k(beam::beam_pick_kernel, S, beam::TP, 0, st, a);
   return check_launch(what);
 }
 
