@@ -5,8 +5,8 @@
 //   beam_words_kernel   a chunk of a row stays in registers: its largest logit, its sum of exponentials, and its k best words in order;
 //   beam_pick_kernel    a group: the rows' sums, the totals of the chunks' words, the k best of them.
 // The k best of many, in both: maxima of parts, more than k of them; the k'th largest of these maxima is a bound that k values
-// reach, and few others; those that reach it are gathered and each counts the ones ahead of it.  Everything is compared as (value,
-// place), so no two are equal: no order of arrival shows, and at most the k parts with a maximum that reaches the bound hold any.
+// reach, and few others; those that reach it are gathered and each counts the ones ahead of it.  The gathered are compared
+// as (value, place), no two of them equal, so no order of arrival shows; fewer than k parts have any above the bound.
 #include "vt_common.cuh"
 #include "vt_host.h"
 
@@ -42,7 +42,6 @@ __device__ __forceinline__ float key_logit(unsigned long long key) {
   const uint32_t o = (uint32_t)(key >> 32);
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
-__device__ __forceinline__ unsigned long long shfl_xor(unsigned long long x, int d) { return __shfl_xor_sync(0xffffffffu, x, d); }
 
 template <typename Word>
 __device__ __forceinline__ float load_word(const Word* p) {
@@ -53,10 +52,16 @@ __device__ __forceinline__ float load_word(const Word* p) {
 template <typename Word, int VEC, int E>
 __device__ __forceinline__ void load_chunk(const Word* row, int v0, int V, float (&x)[E]) {
   const Word* p = row + v0 + (int)threadIdx.x * VEC;
+  const bool whole = v0 + T * E <= V;
   const int left = V - v0 - (int)threadIdx.x * VEC;
+  if (VEC == 1 && whole) {
+#pragma unroll
+    for (int r = 0; r < E; r++) x[r] = load_word(p + r * T);
+    return;
+  }
 #pragma unroll
   for (int r = 0; r < E / VEC; r++) {
-    if (VEC > 1 && r * T * VEC + VEC <= left) {
+    if (VEC > 1 && (whole || r * T * VEC + VEC <= left)) {
       const uint4 w = __ldg(reinterpret_cast<const uint4*>(p + r * T * VEC));
       const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -69,12 +74,13 @@ __device__ __forceinline__ void load_chunk(const Word* row, int v0, int V, float
   }
 }
 
-// CTA = T E words of a row.  Bound: DRAM with many rows (MEASURED), the latency of one chunk with few.
+// CTA = T E words of a row.  Bound: issue slots and DRAM with many rows (MEASURED), the latency of one chunk with few.
 template <typename Word, int VEC, int E>
 __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
-  __shared__ float sh_max[T / 32], sh_sum[T / 32];
-  __shared__ unsigned long long part[T], found[T * E / 2];
-  __shared__ unsigned long long bound;
+  constexpr int FOUND = T * E / 2;  // words above the bound are of fewer than k of 2 k parts or more
+  __shared__ float sh_max[T / 32], sh_sum[T / 32], part[T];
+  __shared__ unsigned long long found[FOUND];
+  __shared__ float bound;
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.k;
   const long long row = blockIdx.x / a.chunks;
@@ -86,31 +92,34 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
   const Word* words = static_cast<const Word*>(a.logits) + row * a.ld;
   load_chunk<Word, VEC, E>(words, v0, a.V, x);
   auto word = [&](int e) { return v0 + ((e / VEC) * T + tid) * VEC + e % VEC; };
-  // ---- the largest logit, and the thread's best word
-  float mx = -INFINITY;
-  int at = 0;
+  // ---- the largest logit of the thread, its part and the chunk
+  float mx = x[0];
 #pragma unroll
-  for (int e = 0; e < E; e++)
-    if (x[e] > mx) mx = x[e], at = e;
-  unsigned long long best = mx == -INFINITY ? 0 : key_of(mx, word(at));
-  float top = mx;
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  if (lane == 0) sh_max[warp] = top;
-  // ---- the parts' maxima
+  for (int e = 1; e + 1 < E; e += 2) mx = max3f(mx, x[e], x[e + 1]);
+  mx = fmaxf(fmaxf(mx, x[E - 1]), -INFINITY);  // NaN only where the thread has nothing else
   const int parts = parts_of(k), per = T / parts;
-  for (int d = 1; d < per; d <<= 1) best = max(best, shfl_xor(best, d));
+  float top = mx, best = mx;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if (2 * d == per) best = top;
+  }
+  if (lane == 0) sh_max[warp] = top;
   if (tid % per == 0) part[tid / per] = best;
-  if (tid == 0) count = 0, bound = 0;
+  if (tid == 0) count = 0, bound = -INFINITY;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < T / 32; w++) top = fmaxf(top, sh_max[w]);
   // ---- a part's rank among the maxima, its threads taking a share of them each; the k'th is the bound
   {
     int ahead = 0;
-    for (int i = tid % per; i < parts; i += per) ahead += part[i] > best;
+    const int me = tid / per;
+    for (int i = tid % per; i < parts; i += per) {
+      const float y = part[i];
+      ahead += y > best || (y == best && i < me);
+    }
     for (int d = 1; d < per; d <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
-    if (tid % per == 0 && ahead == k - 1 && best) bound = best;  // 0 where fewer than k parts have a word
+    if (tid % per == 0 && ahead == k - 1) bound = best;  // -inf where fewer than k parts have a word
   }
   // ---- sum of exponentials; a chunk of -inf adds nothing, a NaN or +inf makes it NaN
   {
@@ -131,16 +140,15 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
     if (lane == 0) sh_sum[warp] = s;
   }
   __syncthreads();
-  // ---- gather: k parts at most have words that reach the bound, T / parts E each.  They are few: the others' only cost is a bit
-  const unsigned long long lim = bound;
-  const float lim_x = lim ? key_logit(lim) : -3.402823466e38f;
+  // ---- gather the words that reach the bound.  They are few: the others' only cost is a bit
+  const float lim = bound == -INFINITY ? -3.402823466e38f : bound;
   uint32_t hits = 0;
 #pragma unroll
-  for (int e = 0; e < E; e++) hits |= x[e] >= lim_x ? 1u << e : 0u;
+  for (int e = 0; e < E; e++)
+    asm("{\n\t.reg .pred p;\n\tsetp.ge.f32 p, %1, %2;\n\t@p or.b32 %0, %0, %3;\n\t}" : "+r"(hits) : "f"(x[e]), "f"(lim), "r"(1u << e));
   for (; hits; hits &= hits - 1) {
-    const int v = word(__ffs(hits) - 1);
-    const unsigned long long key = key_of(load_word(words + v), v);
-    if (key >= lim) found[atomicAdd(&count, 1)] = key;
+    const int v = word(__ffs(hits) - 1), n = atomicAdd(&count, 1);
+    if (n < FOUND) found[n] = key_of(load_word(words + v), v);
   }
   if (tid == 0) {
     float s = 0.f;
@@ -149,7 +157,30 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
     a.sums[blockIdx.x] = make_float2(top, s);
   }
   __syncthreads();
-  const int n = count;
+  int n = count;
+  if (n > FOUND) {  // equal logits in crowds (words banned by the lowest value): those above the bound, then its first words
+    __syncthreads();
+    if (tid == 0) count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      if (x[e] > lim) found[atomicAdd(&count, 1)] = key_of(x[e], word(e));
+    __syncthreads();
+    n = count;
+    if (warp == 0) {
+      int got = n;
+      for (int v = v0 + lane; got < k; v += 32) {
+        const bool is = v < a.V && load_word(words + v) == lim;
+        const uint32_t all = __ballot_sync(0xffffffffu, is);
+        const int at = got + __popc(all & ((1u << lane) - 1));
+        if (is && at < k) found[at] = key_of(lim, v);
+        got += __popc(all);
+        if (__all_sync(0xffffffffu, v >= min(a.V, v0 + T * E))) break;
+      }
+    }
+    n = k;
+    __syncthreads();
+  }
   unsigned long long* to = a.words + (long long)blockIdx.x * k;
   for (int i = tid; i < n; i += T) {
     const unsigned long long key = found[i];
