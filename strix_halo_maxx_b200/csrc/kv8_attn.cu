@@ -47,8 +47,7 @@ int vt_attn_kv8(cudaStream_t st, const uint16_t* q, long long sq_b, long long sq
     kv8::split::Args a{q, sq_b, sq_t, sq_h, kc, vc, ks, vs, lens, counts, B, n, Hq / H, H, C, causal, p.rows, p.rg, p.ctas,
                        scale * kv8::LOG2E, out, so_b, so_t, so_h, (float*)(w8 + p.o_off), (float2*)(w8 + p.ml_off),
                        (float2*)(w8 + p.full_off), weights ? (float*)(w8 + p.s_off) : nullptr, weights, weights_in};
-    if (D == 64) return p.nt == 1 ? kv8::split::launch<64, 1>(st, a, p.whole) : p.nt == 2 ? kv8::split::launch<64, 2>(st, a, p.whole) : kv8::split::launch<64, 4>(st, a, p.whole);
-    return p.nt == 1 ? kv8::split::launch<128, 1>(st, a, p.whole) : kv8::split::launch<128, 2>(st, a, p.whole);
+    return kv8::split::launch_any<kv8::split::PLAIN>(st, a, D, p.nt, p.whole, "vt_attn_kv8");
   }
   const kv8::tc::Plan p = kv8::tc::make_plan(B, n, Hq, H, D, C, weights != nullptr, sm_count());
   const long long items = (p.rows + kv8::tc::ROWS - 1) / kv8::tc::ROWS;

@@ -26,12 +26,19 @@
 //   O       a tile's product is accumulated on its own and added as O = O * alpha + vs * (P V): V's scale stays fp32.
 // What bounds it: DRAM at long contexts (64 x 8 heads x 128 of 4k-8k slots, 818 MB: 139 us, 5.89 TB/s, issue slots 57 % busy; under
 // the power cap, in loops of seconds, 159 us; three CTAs an SM with two stages each: 201 us), else the latency of one tile's chain and of the join.
+// For sequences that share a prefix the same kernel takes one of two more forms:
+//   SHARED   the rows of all F sequences on a prefix (F n G <= 32) are one item per head, whose tiles are the prefix's and then
+//            each sequence's own; a row sees the prefix and its own sequence's slots;
+//   OWN      only the sequences' own slots, each row's normalised output, maximum and sum in fp32, for
+//            attn_kv8_shared_join_kernel.
 #include "vt_common.cuh"
 #include "vt_host.h"
 
 namespace vt {
 namespace kv8 {
 namespace split {
+
+enum : int { PLAIN = 0, SHARED = 1, OWN = 2 };
 
 constexpr int ST = 3, FEW_ROWS = 32;                // stages; rows of a kv head that this kernel takes
 constexpr int TILE = 4096;                         // bytes of K (or V) codes in a tile
@@ -56,15 +63,17 @@ struct Plan {       // fixed on the host from sizes alone
 
 __host__ __device__ inline int keys_per_tile(int D) { return TILE / D; }
 
-static Plan make_plan(int B, int n, int Hq, int H, int D, int C, bool weights, int sms) {
+// tiles: of an item at most; those of C slots unless told otherwise.
+static Plan make_plan(int B, int n, int Hq, int H, int D, int C, bool weights, int sms, long long tiles = -1, int whole_tiles = WHOLE_TILES) {
   Plan p;
+  if (tiles < 0) tiles = C / keys_per_tile(D);
   p.rows = n * (Hq / H);
   // rows of a group: registers hold O [D][rows] of a warp (D rows / 32 a lane) beside q and P: 32 rows for D = 64,
   // 16 for D = 128
   p.nt = p.rows <= 8 ? 1 : (p.rows <= 16 || D == 128) ? 2 : 4;
   p.rg = (p.rows + 8 * p.nt - 1) / (8 * p.nt);
   p.ctas = 2 * sms;
-  p.whole = C / keys_per_tile(D) <= WHOLE_TILES && (p.rg == 1 || !weights) && (long long)B * H * p.rg <= 4LL * sms;
+  p.whole = tiles <= whole_tiles && (p.rg == 1 || !weights) && (long long)B * H * p.rg <= 4LL * sms;
   const long long slots = 2LL * p.ctas, gr = 8LL * p.nt;
   auto up = [](long long x) { return (x + 255) / 256 * 256; };
   p.o_off = 0;
@@ -90,19 +99,49 @@ struct Args {
   float* scores;  // [B][H][rows][C], or null
   float* w;
   const float* w_in;
+  // SHARED: the prefixes (B counts them, not the sequences), F sequences on each; OWN: where rows go
+  const int8_t *pk, *pv;
+  const float *pks, *pvs;
+  const int* plens;
+  int Cp, F;
+  float* own_o;  // [B][H][rows][D], [B][H][rows]
+  float2* own_ml;
 };
+
+// Tokens of prefix s: what does not fit is cut off and recorded.
+__device__ __forceinline__ int prefix_len(const int* plens, int s, int Cp, bool record) {
+  const int len = plens[s], in = min(max(len, 0), Cp);
+  if (in != len && record) atomicOr(&g_status, (unsigned int)ST_KV8_RANGE);
+  return in;
+}
+// Tiles of a head's item over prefix s and the sequences on it: none where no sequence has a row.
+__device__ __forceinline__ int shared_tiles(const Args& a, int kt, int s, bool record) {
+  const int P = prefix_len(a.plens, s, a.Cp, record);
+  int t = 0;
+  for (int f = 0; f < a.F; f++) {
+    const Seq q = seq_of(a.lens, a.counts, s * a.F + f, a.n, a.C, record);
+    if (q.cnt) t += (q.len + q.cnt + kt - 1) / kt;
+  }
+  return t ? t + (P + kt - 1) / kt : 0;
+}
 
 // Row groups of gr rows that a sequence's new tokens fill (rg of the plan at most).
 __device__ __forceinline__ int row_groups(const Args& a, const Seq& s, int gr) { return (s.cnt * a.G + gr - 1) / gr; }
 // First tile of each sequence in the list of all tiles, pre[0 .. B]; a sequence's tiles are those of its (head, row group)
 // items one after another.  Every CTA computes it for itself.
+template <int MODE = PLAIN>
 __device__ __forceinline__ void tile_list(const Args& a, int kt, int gr, int* pre, int* warp_sum) {
   const int tid = threadIdx.x, nth = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.B + nth - 1) / nth, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
   int sum = 0;
   for (int b = b0; b < b1; b++) {
-    const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C, blockIdx.x == 0);  // those without work are looked at here only
-    const int t = (s.len + s.cnt + kt - 1) / kt * a.H * row_groups(a, s, gr);
+    int t;
+    if constexpr (MODE == SHARED) {
+      t = shared_tiles(a, kt, b, blockIdx.x == 0) * a.H;
+    } else {
+      const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C, blockIdx.x == 0);  // those without work are looked at here only
+      t = (s.len + s.cnt + kt - 1) / kt * a.H * row_groups(a, s, gr);
+    }
     pre[b] = t;
     sum += t;
   }
@@ -158,7 +197,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 }
 constexpr uint32_t H1152 = 0x64806480u;  // 1152 in both halves
 
-template <int D, int NT, bool WHOLE>
+template <int D, int NT, bool WHOLE, int MODE = PLAIN>
 __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 : 2) attn_kv8_split_kernel(Args a) {
   constexpr int WARPS = WHOLE ? WHOLE_WARPS : split::WARPS;
   constexpr int KT = TILE / D, GR = 8 * NT, WQ = D / 16, MT = KT / 16, OM = D / 16;
@@ -166,6 +205,7 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
   __shared__ int pre[WHOLE ? 1 : MAXB + 1], warp_sum[WARPS];
   __shared__ __align__(8) uint64_t full[WARPS * ST];
   __shared__ float sh_m[WARPS][GR], sh_l[WARPS][GR], sh_lse[WHOLE ? GR : 1];
+  __shared__ int sh_cnt[MODE == SHARED ? 32 : 1];  // rows of the sequences on a prefix
   __shared__ int sh_abort;
   volatile int* abort_flag = &sh_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -183,7 +223,7 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
   if (WHOLE) {
     __syncthreads();
   } else {
-    tile_list(a, KT, GR, pre, warp_sum);  // its barriers also publish the mbarriers
+    tile_list<MODE>(a, KT, GR, pre, warp_sum);  // its barriers also publish the mbarriers
     total = pre[a.B];
     const int run = run_of(total, a.ctas);
     u_begin = (long long)blockIdx.x * run;
@@ -193,43 +233,92 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
   bool ok = true;
   for (int u = (int)min(u_begin, (long long)total); u < u_end;) {
     const int b = WHOLE ? blockIdx.x / (a.H * a.rg) : find_seq(pre, a.B, u);
-    const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C);
-    const int T = s.len + s.cnt, tiles = (T + KT - 1) / KT;
-    const int rgs = WHOLE ? a.rg : row_groups(a, s, GR);
+    Seq s{0, 0};
+    int T = 0, tiles, P = 0, ptiles = 0, own_end = 0;  // own_end: of lane f's sequence on a prefix, its last tile's end among all own ones
+    if constexpr (MODE == SHARED) {
+      if (lane < a.F) s = seq_of(a.lens, a.counts, b * a.F + lane, a.n, a.C, WHOLE && warp == 0 && blockIdx.x % a.H == 0);
+      const int own = s.cnt ? (s.len + s.cnt + KT - 1) / KT : 0;
+      own_end = own;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, own_end, d);
+        if (lane >= d) own_end += y;
+      }
+      P = prefix_len(a.plens, b, a.Cp, WHOLE && tid == 0);
+      tiles = __shfl_sync(0xffffffffu, own_end, 31);
+      if (tiles) ptiles = (P + KT - 1) / KT, tiles += ptiles;
+      if (warp == 0) sh_cnt[lane] = s.cnt;
+    } else {
+      s = seq_of(a.lens, a.counts, b, a.n, a.C);
+      T = s.len + s.cnt, tiles = (T + KT - 1) / KT;
+    }
+    const int rgs = MODE == SHARED ? 1 : WHOLE ? a.rg : row_groups(a, s, GR);
     const int item = WHOLE ? blockIdx.x % (a.H * rgs) : (u - pre[b]) / tiles, ta = WHOLE ? 0 : (u - pre[b]) % tiles;
     const int h = item / rgs, rg = item % rgs, r0 = rg * GR;
     // this CTA's tiles of the item: [ta, tb)
-    const int tb = WHOLE ? (r0 < s.cnt * a.G ? tiles : 0) : min(tiles, ta + (u_end - u));
+    const int tb = WHOLE ? (MODE == SHARED || r0 < s.cnt * a.G ? tiles : 0) : min(tiles, ta + (u_end - u));
     const size_t bh = (size_t)b * a.H + h;
     const int8_t *kp = a.kc + bh * a.C * D, *vp = a.vc + bh * a.C * D;
     const float *ksp = a.ks + bh * (a.C / BLK), *vsp = a.vs + bh * (a.C / BLK);
     const int mine = tb - ta > warp ? (tb - ta - warp + WARPS - 1) / WARPS : 0;  // tiles ta + warp + WARPS j
     const int base = consumed;                        // tile j of them goes to slot (base + j) % ST
+    // SHARED: a tile's cache (f: the sequence's, -1: the prefix) and first key; the whole warp asks
+    struct Where {
+      int f, key0;
+    };
+    auto locate = [&](int j) {
+      const int x = ta + warp + WARPS * j;
+      if (x < ptiles) return Where{-1, x * KT};
+      const int own = x - ptiles, f = __popc(__ballot_sync(0xffffffffu, own_end <= own));
+      const int from = __shfl_sync(0xffffffffu, own_end, f > 0 ? f - 1 : 0);
+      return Where{f, (own - (f > 0 ? from : 0)) * KT};
+    };
+    auto head_of = [&](const Where& w) { return w.f < 0 ? bh : ((size_t)b * a.F + w.f) * a.H + h; };
+    auto k_scale = [&](const Where& w) { return w.f < 0 ? a.pks[head_of(w) * (a.Cp / BLK) + w.key0 / BLK] : a.ks[head_of(w) * (a.C / BLK) + w.key0 / BLK]; };
+    auto v_scale = [&](const Where& w) { return w.f < 0 ? a.pvs[head_of(w) * (a.Cp / BLK) + w.key0 / BLK] : a.vs[head_of(w) * (a.C / BLK) + w.key0 / BLK]; };
     auto load = [&](int j) {
       const int slot = (base + j) % ST;
-      const size_t off = (size_t)(ta + warp + WARPS * j) * TILE;
-      mbar_arrive_expect_tx(&bar[slot], 2 * TILE);
-      bulk_load(ring + slot * 2 * TILE, kp + off, TILE, &bar[slot]);
-      bulk_load(ring + slot * 2 * TILE + TILE, vp + off, TILE, &bar[slot]);
+      const int8_t *kt, *vt_;
+      bool one = true;
+      if constexpr (MODE == SHARED) {
+        const Where w = locate(j);
+        const size_t off = (head_of(w) * (w.f < 0 ? a.Cp : a.C) + w.key0) * D;
+        kt = (w.f < 0 ? a.pk : a.kc) + off, vt_ = (w.f < 0 ? a.pv : a.vc) + off;
+        one = lane == 0;
+      } else {
+        const size_t off = (size_t)(ta + warp + WARPS * j) * TILE;
+        kt = kp + off, vt_ = vp + off;
+      }
+      if (one) {
+        mbar_arrive_expect_tx(&bar[slot], 2 * TILE);
+        bulk_load(ring + slot * 2 * TILE, kt, TILE, &bar[slot]);
+        bulk_load(ring + slot * 2 * TILE + TILE, vt_, TILE, &bar[slot]);
+      }
     };
-    if (lane == 0 && ok)
+    if ((MODE == SHARED || lane == 0) && ok)
       for (int j = 0; j < min(mine, ST); j++) load(j);
     float ks_next = 0.f, vs_next = 0.f;  // scales of the next tile
-    if (mine > 0) ks_next = ksp[(ta + warp) * KT / BLK], vs_next = vsp[(ta + warp) * KT / BLK];
+    Where at_next{-1, 0};
+    if (mine > 0) {
+      if constexpr (MODE == SHARED) at_next = locate(0), ks_next = k_scale(at_next), vs_next = v_scale(at_next);
+      else ks_next = ksp[(ta + warp) * KT / BLK], vs_next = vsp[(ta + warp) * KT / BLK];
+    }
     // q of rows r0 + 8 nt + g, this lane's dims t D/4 .. as f16 pairs, scaled to a largest value of 2^15 .. 2^16
     uint32_t qf[NT][WQ][2];
     float cq[NT][2];  // scale of columns 2t, 2t + 1: scale * log2 e * the row's power of two
-    int lim[NT][2];   // keys that they see
+    int lim[NT][2];   // keys that they see (SHARED: of their own sequence)
+    int seq[NT][2];   // SHARED: that sequence
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const int r = r0 + 8 * nt + g, i = r / a.G;
+      const int r = r0 + 8 * nt + g, fr = MODE == SHARED ? r / (a.n * a.G) : 0, i = r / a.G - fr * a.n;
+      const int cnt = MODE == SHARED ? __shfl_sync(0xffffffffu, s.cnt, fr) : s.cnt;  // at most 32 rows: fr < 32; none behind F
       uint32_t x[WQ][2];
       uint32_t top = 0;
-      const uint16_t* qp = a.q + b * a.sq_b + i * a.sq_t + (size_t)(h * a.G + r % a.G) * a.sq_h + t * (D / 4);
+      const uint16_t* qp = a.q + (MODE == SHARED ? (long long)b * a.F + fr : b) * a.sq_b + i * a.sq_t + (size_t)(h * a.G + r % a.G) * a.sq_h + t * (D / 4);
 #pragma unroll
       for (int w = 0; w < WQ; w += 2) {
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (i < s.cnt) v = *reinterpret_cast<const uint4*>(qp + 4 * w);
+        if (i < cnt) v = *reinterpret_cast<const uint4*>(qp + 4 * w);
         x[w][0] = v.x, x[w][1] = v.y, x[w + 1][0] = v.z, x[w + 1][1] = v.w;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
@@ -252,12 +341,19 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
 #pragma unroll
       for (int k = 0; k < 2; k++) {
         cq[nt][k] = __shfl_sync(0xffffffffu, back, (2 * t + k) * 4);  // lane of row 2t + k
-        const int ic = (r0 + 8 * nt + 2 * t + k) / a.G;
-        lim[nt][k] = ic >= s.cnt ? 0 : a.causal ? s.len + ic + 1 : T;
+        const int rc = r0 + 8 * nt + 2 * t + k;
+        if constexpr (MODE == SHARED) {
+          const int fc = rc / (a.n * a.G), ic = rc / a.G - fc * a.n;
+          const int len = __shfl_sync(0xffffffffu, s.len, fc), cnt_c = __shfl_sync(0xffffffffu, s.cnt, fc);
+          seq[nt][k] = fc, lim[nt][k] = ic >= cnt_c ? 0 : len + ic + 1;
+        } else {
+          const int ic = rc / a.G;
+          seq[nt][k] = 0, lim[nt][k] = ic >= s.cnt ? 0 : a.causal ? s.len + ic + 1 : T;
+        }
       }
     }
-    const int sees_all = a.causal ? s.len + r0 / a.G + 1 : T;  // keys that every row of the group sees
-    const bool all_rows = r0 + GR <= s.cnt * a.G;
+    const int sees_all = MODE == SHARED ? P : a.causal ? s.len + r0 / a.G + 1 : T;  // keys that every row of the group sees
+    const bool all_rows = MODE == SHARED ? a.rows == GR && __all_sync(0xffffffffu, lane >= a.F || s.cnt == a.n) : r0 + GR <= s.cnt * a.G;
     float m[NT][2], l[NT][2], o[OM][NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -269,9 +365,13 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
         for (int e = 0; e < 4; e++) o[x][nt][e] = 0.f;
     }
     for (int j = 0; j < mine && ok; j++) {
-      const int slot = consumed % ST, key0 = (ta + warp + WARPS * j) * KT;
+      const int slot = consumed % ST, key0 = MODE == SHARED ? at_next.key0 : (ta + warp + WARPS * j) * KT;
+      const int of = at_next.f;  // SHARED: whose tile it is
       const float ks = ks_next, vs = vs_next;
-      if (j + 1 < mine) ks_next = ksp[(key0 + WARPS * KT) / BLK], vs_next = vsp[(key0 + WARPS * KT) / BLK];
+      if (j + 1 < mine) {
+        if constexpr (MODE == SHARED) at_next = locate(j + 1), ks_next = k_scale(at_next), vs_next = v_scale(at_next);
+        else ks_next = ksp[(key0 + WARPS * KT) / BLK], vs_next = vsp[(key0 + WARPS * KT) / BLK];
+      }
       ok = __all_sync(0xffffffffu, mbar_wait(&bar[slot], (consumed / ST) & 1, abort_flag, ST_KV8_WAIT));
       if (!ok) {
         if (lane == 0)  // the copies in flight land before the CTA ends
@@ -307,20 +407,22 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
         }
       }
       // ---- scores in log2 units; keys out of sight -inf
-      const bool edge = !all_rows || key0 + KT > sees_all;
+      const bool edge = !all_rows || (MODE == SHARED && of >= 0) || key0 + KT > sees_all;
+      auto sees = [&](int nt, int k) { return MODE != SHARED ? lim[nt][k] : of < 0 ? (lim[nt][k] ? P : 0) : seq[nt][k] == of ? lim[nt][k] : 0; };
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
         const float c[2] = {cq[nt][0] * ks, cq[nt][1] * ks};
+        const int see[2] = {sees(nt, 0), sees(nt, 1)};
 #pragma unroll
         for (int x = 0; x < MT; x++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             float v = sc[x][nt][e] * c[e & 1];
-            if (edge && key0 + 16 * x + (g >> 1) + 4 * (g & 1) + 8 * (e >> 1) >= lim[nt][e & 1]) v = -INFINITY;
+            if (edge && key0 + 16 * x + (g >> 1) + 4 * (g & 1) + 8 * (e >> 1) >= see[e & 1]) v = -INFINITY;
             sc[x][nt][e] = v;
           }
       }
-      if (a.scores) {
+      if (MODE == PLAIN && a.scores) {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -375,7 +477,7 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int k = 0; k < 2; k++) vc[nt][k] = edge && key0 >= lim[nt][k] ? 0.f : vs * (1.f / P_SCALE);
+        for (int k = 0; k < 2; k++) vc[nt][k] = edge && key0 >= sees(nt, k) ? 0.f : vs * (1.f / P_SCALE);
 #pragma unroll
       for (int w = 0; w < D / 32; w++) {
         float acc[2][NT][4];
@@ -412,7 +514,7 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
       }
       consumed++;
       __syncwarp();  // every lane has read the slot before it is filled again
-      if (lane == 0 && j + ST < mine) load(j + ST);
+      if ((MODE == SHARED || lane == 0) && j + ST < mine) load(j + ST);
     }
     // ---- the warps' parts of the item, merged over their rings (all their copies have landed)
 #pragma unroll
@@ -436,7 +538,9 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
     const int slot = 2 * blockIdx.x + (u == u_begin ? 0 : 1);  // of a part; a run has two at most: its first and its last
     for (int e = tid; e < GR * D / 4; e += WARPS * 32) {
       const int r = e / (D / 4), d = e % (D / 4) * 4, row = r0 + r;
-      if (row >= s.cnt * a.G) break;
+      const int f = MODE == SHARED ? row / (a.n * a.G) : 0, i = row / a.G - f * a.n;  // the row's sequence and token
+      if (MODE == SHARED && (row >= a.rows || i >= sh_cnt[f])) continue;
+      if (MODE != SHARED && row >= s.cnt * a.G) break;
       float mx = -INFINITY;
 #pragma unroll
       for (int w = 0; w < WARPS; w++) mx = fmaxf(mx, sh_m[w][r]);
@@ -451,9 +555,14 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
       }
       if (whole) {
         const float inv = P_SCALE / sum;
-        uint16_t* op = a.out + b * a.so_b + row / a.G * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
+        if constexpr (MODE == OWN) {
+          *reinterpret_cast<float4*>(a.own_o + (bh * a.rows + row) * D + d) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+          if (d == 0) a.own_ml[bh * a.rows + row] = make_float2(mx, sum);
+          continue;
+        }
+        uint16_t* op = a.out + (MODE == SHARED ? (long long)b * a.F + f : b) * a.so_b + i * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
         *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
-        if (d == 0 && a.w) {
+        if (MODE == PLAIN && d == 0 && a.w) {
           if (WHOLE) sh_lse[r] = mx + log2f(sum);
           else a.full_ml[(bh * a.rg + rg) * GR + r] = make_float2(mx, sum);
         }
@@ -463,7 +572,7 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
       }
     }
     if (WHOLE) {
-      if (a.w) {  // one row group: the item's rows are all the rows of (b, h)
+      if (MODE == PLAIN && a.w) {  // one row group: the item's rows are all the rows of (b, h)
         __syncthreads();
         for (int j = tid; j < T; j += WARPS * 32) {
           const size_t at = bh * a.C + j;
@@ -484,7 +593,7 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
 // CTAs [0, merge_ctas): one row of an item; each of 128 * 4 / D groups of threads (thread = 4 dims) takes every so many'th
 // part, the groups' sums are added in order.  The others: 512 keys of one (sequence, head):
 // weight = (key before len ? weights_in : 0) + sum over rows of 2^(score - m - log2 l), a row's (m, l) by a warp.
-template <int D, int NT>
+template <int D, int NT, int MODE = PLAIN>
 __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ctas) {
   constexpr int KT = TILE / D, GR = 8 * NT, GROUPS = 128 * 4 / D;
   __shared__ int pre[MAXB + 1], warp_sum[4];
@@ -493,11 +602,11 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   griddep_wait();
   griddep_launch();
-  tile_list(a, KT, GR, pre, warp_sum);
+  tile_list<MODE>(a, KT, GR, pre, warp_sum);
   const int run = run_of(pre[a.B], a.ctas);
   // the first and last CTA that hold a part of an item, and the first part's slot (the others begin their CTA's run: 2 c)
   auto parts = [&](const Seq& s, int b, int h, int rg, int tiles, int& c0, int& c1, int& first) {
-    const int u0 = pre[b] + (h * row_groups(a, s, GR) + rg) * tiles;
+    const int u0 = pre[b] + (MODE == SHARED ? h : h * row_groups(a, s, GR) + rg) * tiles;
     c0 = u0 / run, c1 = (u0 + tiles - 1) / run;
     first = 2 * c0 + (u0 == c0 * run ? 0 : 1);
   };
@@ -518,9 +627,10 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
   if ((int)blockIdx.x < merge_ctas) {
     const int rows = min(GR, a.rows), item = blockIdx.x / rows, r = blockIdx.x % rows;
     const int rg = item % a.rg, h = item / a.rg % a.H, b = item / a.rg / a.H;
-    const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C);
-    const int row = rg * GR + r, tiles = (s.len + s.cnt + KT - 1) / KT;
-    if (row >= s.cnt * a.G) return;
+    const int row = rg * GR + r, f = MODE == SHARED ? row / (a.n * a.G) : 0, i = row / a.G - f * a.n;
+    const Seq s = seq_of(a.lens, a.counts, MODE == SHARED ? b * a.F + f : b, a.n, a.C, false);
+    const int tiles = MODE == SHARED ? (pre[b + 1] - pre[b]) / a.H : (s.len + s.cnt + KT - 1) / KT;
+    if (i >= s.cnt) return;
     int c0, c1, first;
     parts(s, b, h, rg, tiles, c0, c1, first);
     if (c0 == c1) return;
@@ -544,11 +654,12 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
         v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
       }
       const float inv = P_SCALE / sum;
-      uint16_t* op = a.out + b * a.so_b + row / a.G * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
+      uint16_t* op = a.out + (MODE == SHARED ? (long long)b * a.F + f : b) * a.so_b + i * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
       *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
     }
     return;
   }
+  if (MODE != PLAIN) return;
   const int chunks = (a.C + 511) / 512, x = blockIdx.x - merge_ctas;
   const int bh = x / chunks, j = x % chunks * 512 + tid * 4, h = bh % a.H, b = bh / a.H;
   const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C);
@@ -584,24 +695,32 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
     if (j + e < T) a.w[at + e] = acc[e];
 }
 
-template <int D, int NT>
-static int launch(cudaStream_t st, const Args& a, bool whole) {
+// what: the entry point, for its errors.  OWN's parts are joined elsewhere.
+template <int D, int NT, int MODE = PLAIN>
+static int launch(cudaStream_t st, const Args& a, bool whole, const char* what = "vt_attn_kv8") {
   if (whole) {
     constexpr int SMEM = WHOLE_WARPS * RING;
-    const int rc = smem_attr_once((const void*)attn_kv8_split_kernel<D, NT, true>, SMEM, "vt_attn_kv8");
+    const int rc = smem_attr_once((const void*)attn_kv8_split_kernel<D, NT, true, MODE>, SMEM, what);
     if (rc) return rc;
-    launch_k(attn_kv8_split_kernel<D, NT, true>, (unsigned)(a.B * a.H * a.rg), WHOLE_WARPS * 32, SMEM, st, a);
-    return check_launch("vt_attn_kv8");
+    launch_k(attn_kv8_split_kernel<D, NT, true, MODE>, (unsigned)(a.B * a.H * a.rg), WHOLE_WARPS * 32, SMEM, st, a);
+    return check_launch(what);
   }
   constexpr int SMEM = WARPS * RING;
-  const int rc = smem_attr_once((const void*)attn_kv8_split_kernel<D, NT, false>, SMEM, "vt_attn_kv8");
+  const int rc = smem_attr_once((const void*)attn_kv8_split_kernel<D, NT, false, MODE>, SMEM, what);
   if (rc) return rc;
-  launch_k(attn_kv8_split_kernel<D, NT, false>, a.ctas, WARPS * 32, SMEM, st, a);
-  const int rows = 8 * NT < a.rows ? 8 * NT : a.rows;
-  const int merge = a.B * a.H * a.rg * rows;
-  const int chunks = a.w ? a.B * a.H * ((a.C + 511) / 512) : 0;
-  launch_k(attn_kv8_join_kernel<D, NT>, merge + chunks, 128, 0, st, a, merge);
-  return check_launch("vt_attn_kv8");
+  launch_k(attn_kv8_split_kernel<D, NT, false, MODE>, a.ctas, WARPS * 32, SMEM, st, a);
+  if constexpr (MODE != OWN) {
+    const int rows = 8 * NT < a.rows ? 8 * NT : a.rows;
+    const int merge = a.B * a.H * a.rg * rows;
+    const int chunks = a.w ? a.B * a.H * ((a.C + 511) / 512) : 0;
+    launch_k(attn_kv8_join_kernel<D, NT, MODE>, merge + chunks, 128, 0, st, a, merge);
+  }
+  return check_launch(what);
+}
+template <int MODE>
+static int launch_any(cudaStream_t st, const Args& a, int D, int nt, bool whole, const char* what) {
+  if (D == 64) return nt == 1 ? launch<64, 1, MODE>(st, a, whole, what) : nt == 2 ? launch<64, 2, MODE>(st, a, whole, what) : launch<64, 4, MODE>(st, a, whole, what);
+  return nt == 1 ? launch<128, 1, MODE>(st, a, whole, what) : launch<128, 2, MODE>(st, a, whole, what);
 }
 
 }  // namespace split

@@ -54,6 +54,9 @@ SHARED = [  # S, F, n, Hq, H, D, plens, lens, counts
     (2, 3, 1, 4, 2, 64, [1, 1000], [5, 0, 70, 127, 1, 300], [1, 1, 0, 1, 0, 1]), (1, 8, 4, 2, 2, 64, [200], [0, 9, 60, 61, 62, 63, 64, 65], [4, 0, 1, 2, 4, 4, 3, 4]),
     (3, 2, 3, 5, 1, 128, [64, 0, 129], [0, 1, 2, 0, 100, 64], [3, 2, 0, 0, 1, 3]), (5, 1, 2, 8, 1, 64, [0, 63, 64, 65, 400], [0, 0, 0, 0, 0], None),
     (1, 16, 1, 4, 2, 64, [5000], [3] * 16, None), (1, 4, 1, 8, 1, 128, [9000], [700, 0, 3, 64], None),
+    # a short prefix and many sequences' own slots, over many CTAs
+    (2, 12, 1, 2, 2, 64, [730, 100], [i * 5 for i in range(24)], None), (1, 16, 2, 1, 1, 64, [60], [i * 31 for i in range(16)], [i % 3 for i in range(16)]),
+    (3, 4, 1, 4, 1, 128, [500, 0, 64], [300, 0, 64, 1, 290, 17, 33, 32, 31, 64, 65, 200], None), (1, 32, 1, 1, 1, 64, [64], [(i * 37) % 200 for i in range(32)], None),
     # many rows on a prefix, few of each sequence
     (1, 40, 1, 3, 3, 64, [500], [i * 7 for i in range(40)], None), (2, 17, 1, 8, 2, 128, [300, 0], [0] * 17 + [i * 13 for i in range(17)], [i % 3 % 2 for i in range(34)]),
     (1, 9, 8, 4, 4, 64, [700], [0] * 9, [8, 1, 0, 3, 8, 7, 2, 5, 0]), (1, 33, 2, 4, 1, 128, [64], [i for i in range(33)], None),
