@@ -338,8 +338,8 @@ int vt_kv8_evict(cudaStream_t stream, const int8_t* kc, const int8_t* vc, const 
                  const float* weights, const int* lens, int B, int H, int D, int keep, int recent, int8_t* dst_kc,
                  int8_t* dst_vc, float* dst_ks, float* dst_vs, int dst_C, float* dst_weights, int* dst_lens, int* index);
 
-/* Bytes of the workspace of vt_attn_kv8_shared (0 for an empty problem or one that needs none), enough for fewer tokens and slots too;
- * its contents need no initialisation. */
+/* Bytes of the workspace of vt_attn_kv8_shared (0 for an empty problem or one that needs none), enough for fewer tokens over the
+ * same caches too; its contents need no initialisation. */
 long long vt_attn_kv8_shared_ws_bytes(int S, int B, int n, int Hq, int H, int D, int Cp, int C);
 
 /* Attention of sequences that share prefixes: S prefix caches pk, pv, pks, pvs ([S][H][Cp][D], plens [S] tokens each) and, for each of

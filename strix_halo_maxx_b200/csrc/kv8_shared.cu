@@ -1,10 +1,18 @@
 // Attention over the 8-bit cache for sequences that share a prefix: S prefix caches, F = B / S sequences on each, every sequence
-// with a cache of its own behind it.  A prefix is read once for the rows of all of its sequences; softmax over the two caches comes
-// apart into parts with a maximum and a sum each, which are put together by weight:  out = sum w o / sum w,  w = l 2^(m - max m).
+// with a cache of its own behind it.  A prefix is read once for the rows of all of its sequences.
 //
-// Few rows on a prefix (F n G <= 32; 16 heads' dims of 128): one item per head with all keys in its list of tiles (kv8_split.cu).
-// More: the rows of all sequences over the prefix on tcgen05 (kv8_tc.cu), each sequence's rows over its own slots by either, then
-// attn_kv8_shared_join_kernel.
+//   few rows on a prefix   F n G <= 32 (16 where heads are 128 wide): one item per head with the prefix's tiles and all own ones (kv8_split.cu)
+//   more                   attn_kv8_shared_tc_kernel below.  Where each sequence's own slots are few beside the prefix, or its rows
+//                          many, it takes them too; else it takes the prefix alone and leaves each row's output, maximum and sum, and
+//                          kv8_split.cu adds the own slots, whose reading then is what costs
+//
+// The kernel is the one of kv8_tc.cu (its comment says how codes, scales and P are held, and what bounds a tile) with other lists.  A head's
+// rows over prefix s are r = t G + g, t numbering the new tokens of all of its sequences without gaps: idle and short sequences cost
+// nothing.  An item is ROWS of them; its tiles of 64 keys are the prefix's, then those of each sequence that has rows in it, in order.
+//   two M tiles of 128 rows  share every converted tile; own tiles that concern the rows of one M tile are passed over by the other;
+//   ALT, up to 128 rows      both M tiles hold the same rows and take the key tiles in turn, so that two are in flight all the same; in
+//                            the end each pair of threads puts its row's two halves together (MEASURED).
+// Items' tiles form one list cut into equal runs, one for each SM; what spans CTAs leaves parts for attn_kv8_shared_join_kernel.
 #include "vt_common.cuh"
 #include "vt_host.h"
 
@@ -12,124 +20,728 @@ namespace vt {
 namespace kv8 {
 namespace shared {
 
+using tc::KEYS;
+using tc::kDrainCycles;
+using tc::kTinyScale;
+using tc::L_LOG2;
+using tc::L_SCALE;
+using tc::P_MOVE;
+using tc::P_TOP;
+using tc::P_UP;
+using tc::P_UP_SINK;
+using tc::THREADS;
+using tc::Z_TOP;
 constexpr int MAXB = 2048;
+constexpr uint32_t TMEM_COLS = 512;  // S of M tile t, buffer f: columns 128 t + 64 f; O of tile t: 256 + 128 t
 
-struct JoinArgs {
-  tc::Args p;     // the prefixes' call
-  split::Args s;  // the sequences' own slots, by whichever of the two
-  tc::Args t;
-  bool own_tc, own_whole;
-  int B, nt;
+template <int D, bool ALT>
+struct Smem {
+  static constexpr int ROWS = ALT ? 128 : 256, ST = ALT ? 4 : 3;
+  static constexpr int QT = 128 * D * 2;   // bytes of one M tile of q
+  static constexpr int KT = KEYS * D * 2;  // of a converted K or V tile
+  static constexpr int K = (ALT ? 1 : 2) * QT, V = K + ST * KT, BYTES = V + ST * KT;
 };
 
-// Thread = 4 dims of a row of the output; 16 rows a CTA.  A part is a whole row (its kernel left it normalised) or one CTA's share.
-template <int D>
-__global__ void __launch_bounds__(128) attn_kv8_shared_join_kernel(const __grid_constant__ JoinArgs j) {
-  __shared__ int tok[MAXB + 1], ppre[MAXB + 1], opre[MAXB + 1], scratch[4];
+struct Args {
+  const uint16_t* q;
+  long long sq_b, sq_t, sq_h;
+  const int8_t *pk, *pv;
+  const float *pks, *pvs;
+  int Cp, S, F;
+  const int* plens;
+  const int8_t *kc, *vc;
+  const float *ks, *vs;
+  int C;
+  const int *lens, *counts;
+  int n, G, H, ctas;
+  int items;  // > 0: items of a head, and a CTA for each item (no runs, nothing to join)
+  int own;    // whether the sequences' own slots are in the lists
+  float scale_log2;
+  uint16_t* out;
+  long long so_b, so_t, so_h;
+  float* row_o;      // [B][n][Hq][D] and [B][n][Hq]: where rows go without own slots
+  float2* row_ml;
+  float* part_o;     // [2 ctas][ROWS][D]
+  float2* part_ml;   // [2 ctas][ROWS]
+  int4* unfinished;  // [ctas] the item that a CTA begins and others go on with: last CTA (-1: none), slot of the first part, head, first row
+  int* row_at;       // [ctas][ROWS] where that item's rows are: b n + i, -1 for none
+};
+
+// What every CTA works out for itself.
+struct Lists {
+  int *tok, *len;  // new tokens before each sequence, [B + 1]; tokens that it held before the call
+  int *own, *pre;  // own tiles of the items before each sequence's, [B + 1]; tiles before each prefix's heads, [S + 1]
+};
+__device__ __forceinline__ int seq_of_token(const Args& a, const Lists& l, int s, int t) {  // t: of the prefix's sequences
+  return s * a.F + split::find_seq(l.tok + s * a.F, a.F, l.tok[s * a.F] + t);
+}
+// Own tiles that rows [q ROWS, q ROWS + ROWS) of its prefix need of sequence x, which has rows among them or none at all.
+template <int ROWS>
+__device__ __forceinline__ int own_tiles(const Args& a, const Lists& l, int s, int x, int q) {
+  const int cnt = l.tok[x + 1] - l.tok[x];
+  if (!a.own || cnt == 0) return 0;
+  const int last = min(cnt - 1, (q * ROWS + ROWS - 1) / a.G - (l.tok[x] - l.tok[s * a.F]));
+  return (l.len[x] + last + KEYS) / KEYS;
+}
+template <int ROWS>
+__device__ __forceinline__ void make_lists(const Args& a, const Lists& l, int* scratch) {
+  const bool record = blockIdx.x == 0;
+  split::sums_before(l.tok, a.S * a.F, scratch, [&](int b) {
+    const Seq q = seq_of(a.lens, a.counts, b, a.n, a.C, record);
+    l.len[b] = q.len;
+    return q.cnt;
+  });
+  if (a.own)
+    split::sums_before(l.own, a.S * a.F, scratch, [&](int x) {
+      const int s = x / a.F, first = (l.tok[x] - l.tok[s * a.F]) * a.G, rows = (l.tok[x + 1] - l.tok[x]) * a.G;
+      int t = 0;
+      if (rows)
+        for (int q = first / ROWS; q <= (first + rows - 1) / ROWS; q++) t += own_tiles<ROWS>(a, l, s, x, q);
+      return t;
+    });
+  if (a.items > 0) return;
+  split::sums_before(l.pre, a.S, scratch, [&](int s) {
+    const int P = split::prefix_len(a.plens, s, a.Cp, record), rows = (l.tok[(s + 1) * a.F] - l.tok[s * a.F]) * a.G;
+    return ((rows + ROWS - 1) / ROWS * ((P + KEYS - 1) / KEYS) + (a.own ? l.own[(s + 1) * a.F] - l.own[s * a.F] : 0)) * a.H;
+  });
+}
+
+// A CTA's share of an item: rows q ROWS .. of prefix s, head h; key tiles [ta, tb) of `tiles`, the first pt of them the prefix's.
+struct Seg {
+  int s, h, q, rows, P, pt, x0, x1, t0, tiles, ta, tb;  // x0, x1: first and last sequence of the item; t0: own tiles of x0
+  struct Part {
+    int oa, ob;  // own tiles that concern the M tile: [oa, ob) of the item's
+    bool act;    // whether it has any tile here
+  } m0, m1;
+  __device__ __forceinline__ Part of(int t) const { return t ? m1 : m0; }
+};
+template <int ROWS>
+__device__ __forceinline__ int own_before(const Args& a, const Lists& l, const Seg& g, int x) {  // own tiles of the item before x's
+  return !a.own || x == g.x0 ? 0 : g.t0 + l.own[x] - l.own[g.x0 + 1];
+}
+// Tiles of items 0 .. q - 1 of a head.
+template <int ROWS>
+__device__ __forceinline__ int tiles_before(const Args& a, const Lists& l, int s, int q, int pt) {
+  if (q == 0) return 0;
+  int t = q * pt;
+  if (a.own) {
+    const int x = seq_of_token(a, l, s, q * ROWS / a.G), first = (l.tok[x] - l.tok[s * a.F]) * a.G;
+    t += l.own[x] - l.own[s * a.F];
+    for (int i = first / ROWS; i < q; i++) t += own_tiles<ROWS>(a, l, s, x, i);
+  }
+  return t;
+}
+template <int D, bool ALT>
+__device__ __forceinline__ Seg segment(const Args& a, const Lists& l, int u, int u_end, bool record) {
+  constexpr int ROWS = Smem<D, ALT>::ROWS;
+  Seg g;
+  int at = 0;
+  if (a.items > 0) {
+    const int sh = blockIdx.x / a.items;
+    g.s = sh / a.H, g.h = sh % a.H, g.q = blockIdx.x % a.items;
+  } else {
+    g.s = split::find_seq(l.pre, a.S, u);
+    const int head = (l.pre[g.s + 1] - l.pre[g.s]) / a.H;
+    g.h = (u - l.pre[g.s]) / head, at = (u - l.pre[g.s]) % head;
+  }
+  g.rows = (l.tok[(g.s + 1) * a.F] - l.tok[g.s * a.F]) * a.G;
+  g.P = split::prefix_len(a.plens, g.s, a.Cp, record);
+  g.pt = (g.P + KEYS - 1) / KEYS;
+  if (a.items == 0) {  // the last item that begins at `at` or before
+    int lo = 0, hi = (g.rows + ROWS - 1) / ROWS;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (tiles_before<ROWS>(a, l, g.s, mid, g.pt) <= at) lo = mid; else hi = mid;
+    }
+    g.q = lo;
+    at -= tiles_before<ROWS>(a, l, g.s, lo, g.pt);
+  }
+  const int r0 = g.q * ROWS;
+  g.tiles = 0, g.ta = at;
+  if (r0 < g.rows) {
+    g.x0 = seq_of_token(a, l, g.s, r0 / a.G), g.x1 = seq_of_token(a, l, g.s, (min(r0 + ROWS, g.rows) - 1) / a.G);
+    g.t0 = own_tiles<ROWS>(a, l, g.s, g.x0, g.q);
+    g.tiles = g.pt + own_before<ROWS>(a, l, g, g.x1) + own_tiles<ROWS>(a, l, g.s, g.x1, g.q);
+  }
+  g.tb = a.items > 0 ? g.tiles : min(g.tiles, g.ta + (u_end - u));
+  auto part = [&](int t) {
+    Seg::Part p{g.pt, g.tiles, g.ta < g.tb};
+    if (ALT) {
+      p.act = g.tb - g.ta >= 2 || (g.ta < g.tb && (g.ta & 1) == t);
+    } else if (r0 + 128 * t >= g.rows) {
+      p.act = false;
+    } else if (a.own) {
+      const int xa = seq_of_token(a, l, g.s, (r0 + 128 * t) / a.G), xb = seq_of_token(a, l, g.s, (min(r0 + 128 * t + 128, g.rows) - 1) / a.G);
+      p.oa = g.pt + own_before<ROWS>(a, l, g, xa);
+      p.ob = g.pt + own_before<ROWS>(a, l, g, xb) + own_tiles<ROWS>(a, l, g.s, xb, g.q);
+      p.act = g.ta < g.tb && (g.ta < g.pt || max(g.ta, p.oa) < min(g.tb, p.ob));
+    }
+    return p;
+  };
+  g.m0 = part(0), g.m1 = part(1);
+  return g;
+}
+// The first tile from j on that M tile t takes part in; tb where there is none.
+template <bool ALT>
+__device__ __forceinline__ int tile_from(const Seg& g, int t, int j) {
+  if (ALT) return min(j + ((j ^ t) & 1), g.tb);
+  const Seg::Part p = g.of(t);
+  if (j >= g.pt) j = max(j, p.oa);
+  return j >= g.tb || (j >= g.pt && j >= p.ob) ? g.tb : j;
+}
+
+// Where tile j of an item lies: sequence x (-1: the prefix) and block kt of its cache, of n that the item needs.
+struct Cursor {
+  int x, kt, n;
+};
+template <int ROWS>
+__device__ __forceinline__ Cursor cursor_at(const Args& a, const Lists& l, const Seg& g, int j) {
+  if (j < g.pt) return {-1, j, g.pt};
+  int lo = g.x0, hi = g.x1 + 1;  // the last sequence whose tiles begin at j or before
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (own_before<ROWS>(a, l, g, mid) <= j - g.pt) lo = mid; else hi = mid;
+  }
+  return {lo, j - g.pt - own_before<ROWS>(a, l, g, lo), own_tiles<ROWS>(a, l, g.s, lo, g.q)};
+}
+template <int ROWS>
+__device__ __forceinline__ void advance(const Args& a, const Lists& l, const Seg& g, Cursor& c) {  // there is a next tile
+  if (++c.kt < c.n) return;
+  c.x = c.x < 0 ? g.x0 : c.x + 1, c.kt = 0;
+  while ((c.n = own_tiles<ROWS>(a, l, g.s, c.x, g.q)) == 0) c.x++;
+}
+// Of the tile's cache: block number among all of its heads and sequences.
+__device__ __forceinline__ size_t block_of(const Args& a, const Seg& g, const Cursor& c) {
+  return c.x < 0 ? ((size_t)g.s * a.H + g.h) * (a.Cp / BLK) + c.kt : ((size_t)c.x * a.H + g.h) * (a.C / BLK) + c.kt;
+}
+
+template <int D, bool ALT>
+__global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __grid_constant__ Args a) {
+  using L = Smem<D, ALT>;
+  constexpr int ROWS = L::ROWS, ST = L::ST;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  __shared__ int tok[MAXB + 1], len[MAXB], own[MAXB + 1], pre[MAXB + 1], scratch[THREADS / 32];
+  __shared__ float2 halves[ALT ? 2 : 1][2][128];  // ALT: (m, l) of a row's two halves
+  __shared__ __align__(8) uint64_t bars[2 + 2 * ST + 4 + 4 + 4 + 2 + 2 + 1];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int sh_abort;
+  volatile int* abort_flag = &sh_abort;
+  uint64_t *q_full = bars, *kv_full = bars + 2, *kv_empty = kv_full + ST;
+  uint64_t *s_full = kv_empty + ST, *p_full = s_full + 4, *o_full = p_full + 4, *o_empty = o_full + 2, *pv_done = o_empty + 2, *drain = pv_done + 2, *halves_full = drain + 2;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Lists l{tok, len, own, pre};
+  if (tid == 0) {
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&q_full[i], ALT ? 8 : 4);  // ALT: one q, which all eight warps bring in
+      mbar_init(&o_full[i], 1), mbar_init(&o_empty[i], ALT ? 8 : 4), mbar_init(&pv_done[i], 1), mbar_init(&drain[i], 1);
+    }
+    for (int i = 0; i < ST; i++) mbar_init(&kv_full[i], 4), mbar_init(&kv_empty[i], 2);
+    for (int i = 0; i < 4; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4);
+    mbar_init(halves_full, 8);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(&tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  griddep_wait();  // programmatic dependent launch: the previous kernel has completed
+  griddep_launch();
+  make_lists<ROWS>(a, l, scratch);
+  int u_begin = 0, u_end, run = 1;  // this CTA's run of tiles
+  if (a.items > 0) {
+    u_end = segment<D, ALT>(a, l, 0, 0, tid == 0).tiles;
+  } else {
+    const int total = pre[a.S];
+    run = max((total + a.ctas - 1) / a.ctas, 1);
+    u_begin = (int)min((long long)blockIdx.x * run, (long long)total);
+    u_end = (int)min((long long)u_begin + run, (long long)total);
+  }
+  // a wait of the whole warp: every lane gives up when one does
+  auto wait = [&](uint64_t* bar, int parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, ST_KV8_WAIT)) != 0;
+  };
+
+  static_assert(2 * tc::SOFTMAX_REGS + tc::CONVERT_REGS + tc::MMA_REGS <= 4 * 128, "the split must come out of the launch's registers");
+  if (warp >= 12) {
+    set_regs_down<tc::MMA_REGS>();
+    // ---------------- MMA issuer of M tile t, one warp each.  The whole warp walks the loop, one lane issues
+    const int t = warp - 12, end = t < 2 ? u_end : u_begin;  // warps 14 and 15 are idle
+    const uint32_t leader = elect_one();
+    constexpr uint32_t IDESC_S = idesc_bf16(128, KEYS), IDESC_O = idesc_f16(128, D) | (1u << 16);  // V MN-major
+    const uint64_t dq = sdesc_noswz(smem_u32(sm) + (ALT ? 0 : t * L::QT), 2048, 128), dk = sdesc_noswz(smem_u32(sm + L::K), 1024, 128);
+    const uint64_t dv = sdesc_noswz(smem_u32(sm + L::V), 128, 1024);
+    const uint32_t t_s = tmem + 128 * t, t_o = tmem + 256 + 128 * t;
+    bool ok = true;
+    int base = 0, js = 0, so = 0, sq = 0;  // tiles of the segments before; tiles and segments that t took part in; q's that came in
+    for (int u = u_begin; u < end && ok;) {
+      const Seg g = segment<D, ALT>(a, l, u, u_end, false);
+      const int nt = g.tb - g.ta;
+      u += nt;
+      auto stage = [&](int j) { return (base + j - g.ta) % ST; };
+      auto phase = [&](int j) { return ((base + j - g.ta) / ST) & 1; };
+      auto pass = [&](int j, int to) {  // tiles [j, to) are the other M tile's: only the barriers
+        for (; j < to && ok; j++) {
+          ok = wait(&kv_full[stage(j)], phase(j));
+          mbar_arrive_if(&kv_empty[stage(j)], leader != 0);
+        }
+      };
+      auto issue_s = [&](int j, int f) {
+        ok = ok && wait(&kv_full[stage(j)], phase(j));
+        if (!ok) return;
+        tc_fence_after();
+        if (leader) {
+          const uint64_t b = dk + stage(j) * (L::KT >> 4);
+#pragma unroll
+          for (int k = 0; k < D / 16; k++) umma_f16(t_s + 64 * f, dq + k * (4096 >> 4), b + k * (2048 >> 4), IDESC_S, k > 0 ? 1u : 0u);
+          umma_commit(&s_full[2 * t + f]);
+        }
+        __syncwarp();
+      };
+      const bool q_here = ALT ? nt > 0 : g.of(t).act;
+      if (!g.of(t).act) {
+        pass(g.ta, g.tb);
+      } else {
+        int j = tile_from<ALT>(g, t, g.ta);
+        pass(g.ta, j);
+        ok = ok && wait(&q_full[ALT ? 0 : t], sq & 1);
+        issue_s(j, js & 1);
+        bool first = true;
+        while (j < g.tb && ok) {
+          const int f = js & 1, nx = tile_from<ALT>(g, t, j + 1);
+          // S of the next tile goes ahead of this one's P V, unless that needs a stage that is freed by this one
+          const bool ahead = nx < g.tb && nx - j < ST;
+          if (ahead) pass(j + 1, nx), issue_s(nx, f ^ 1);
+          ok = ok && (!first || so == 0 || wait(&o_empty[t], (so - 1) & 1)) && wait(&p_full[2 * t + f], (js >> 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+            const uint64_t b = dv + stage(j) * (L::KT >> 4);
+#pragma unroll
+            for (int k = 0; k < KEYS / 16; k++) umma_f16_ts(t_o, t_s + 64 * f + k * 8, b + k * (256 >> 4), IDESC_O, !first || k > 0 ? 1u : 0u);
+            umma_commit(&kv_empty[stage(j)]);
+            umma_commit(&pv_done[t]);
+            if (nx >= g.tb) umma_commit(&o_full[t]);
+          }
+          __syncwarp();
+          if (!ahead) {
+            pass(j + 1, nx);
+            if (nx < g.tb) issue_s(nx, f ^ 1);
+          }
+          first = false, j = nx, js++;
+        }
+        so++;
+      }
+      sq += q_here ? 1 : 0;
+      base += nt;
+    }
+    if (leader && t < 2) {
+      umma_commit(&drain[t]);
+      mbar_wait_drain(&drain[t], 0, kDrainCycles);
+    }
+  } else if (warp >= 8) {
+    set_regs_down<tc::CONVERT_REGS>();
+    // ---------------- converters: warp w rows 16 w .. of a block, 8 lanes = 8 rows of one 16-byte piece.  K's and V's codes of
+    // the next tile are fetched as soon as this tile's are out of the registers
+    constexpr int PER = D / 32;  // pieces of a K or V block that a lane takes
+    const int w = warp - 8;
+    bool ok = true;
+    int j = 0;
+    for (int u = u_begin; u < u_end && ok;) {
+      const Seg g = segment<D, ALT>(a, l, u, u_end, false);
+      const int nt = g.tb - g.ta;
+      u += nt;
+      const int row = 16 * w + (lane & 7), piece = lane >> 3;
+      Cursor c = cursor_at<ROWS>(a, l, g, g.ta);
+      uint4 kr[PER], vr[PER];
+      float vs;
+      auto fetch = [&](uint4 (&to)[PER], const int8_t* from) {
+#pragma unroll
+        for (int x = 0; x < PER; x++)
+          to[x] = *reinterpret_cast<const uint4*>(from + (row + 8 * (x & 1)) * D + 16 * (piece + 4 * (x >> 1)));
+      };
+      size_t blk = block_of(a, g, c);
+      fetch(kr, (c.x < 0 ? a.pk : a.kc) + blk * (KEYS * D));
+      fetch(vr, (c.x < 0 ? a.pv : a.vc) + blk * (KEYS * D));
+      vs = (c.x < 0 ? a.pvs : a.vs)[blk];
+      for (int i = 0; i < nt; i++, j++) {
+        const int st = j % ST;
+        if (j >= ST) ok = wait(&kv_empty[st], (j / ST - 1) & 1);
+        if (!ok) break;
+        if (i + 1 < nt) advance<ROWS>(a, l, g, c), blk = block_of(a, g, c);
+#pragma unroll
+        for (int x = 0; x < PER; x++) tc::store_codes<KEYS, false>(sm + L::K + st * L::KT, row + 8 * (x & 1), piece + 4 * (x >> 1), kr[x]);
+        if (i + 1 < nt) fetch(kr, (c.x < 0 ? a.pk : a.kc) + blk * (KEYS * D));
+#pragma unroll
+        for (int x = 0; x < PER; x++)
+          tc::store_codes<KEYS, true>(sm + L::V + st * L::KT, row + 8 * (x & 1), piece + 4 * (x >> 1), vs < kTinyScale ? make_uint4(0, 0, 0, 0) : vr[x]);
+        if (i + 1 < nt) fetch(vr, (c.x < 0 ? a.pv : a.vc) + blk * (KEYS * D)), vs = (c.x < 0 ? a.pvs : a.vs)[blk];
+        fence_proxy_async_smem();
+        __syncwarp();
+        mbar_arrive_if(&kv_full[st], lane == 0);
+      }
+    }
+  } else {
+    set_regs_up<tc::SOFTMAX_REGS>();
+    // ---------------- softmax of M tile t: thread = row.  It brings in its row of q itself (ALT: half of it)
+    const int t = warp >> 2;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, t_o = tmem + 256 + 128 * t + lanes;
+    bool ok = true;
+    int js = 0, so = 0, so1 = 0, segs = 0;  // tiles that t took part in; outputs stored (ALT: of M tile 0 and 1); segments
+    int4 open = make_int4(-1, 0, 0, 0);
+    auto row_of = [&](const Seg& g) { return g.q * ROWS + (ALT ? 0 : 128 * t) + (warp & 3) * 32 + lane; };
+    auto load_q = [&](const Seg& g) {  // every product with the q before it is done: its last scores have been read
+      if (!ALT && !g.of(t).act) return;
+      const int row = min(row_of(g), g.rows - 1);  // rows past the last are copies of it
+      const int x = seq_of_token(a, l, g.s, row / a.G), i = row / a.G - (tok[x] - tok[g.s * a.F]);
+      const uint16_t* src = a.q + x * a.sq_b + i * a.sq_t + (size_t)(g.h * a.G + row % a.G) * a.sq_h;
+      uint8_t* dst = sm + (ALT ? 0 : t * L::QT) + ((warp & 3) * 32 + lane) * 16;
+      constexpr int CH = ALT ? D / 16 : D / 8;  // 16-byte pieces of this thread
+      const int from = ALT ? t * CH : 0;
+#pragma unroll
+      for (int c0 = 0; c0 < CH; c0 += 4) {
+        uint4 v[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) v[c] = *reinterpret_cast<const uint4*>(src + 8 * (from + c0 + c));
+#pragma unroll
+        for (int c = 0; c < 4; c++) *reinterpret_cast<uint4*>(dst + (from + c0 + c) * 2048) = v[c];
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      mbar_arrive_if(&q_full[ALT ? 0 : t], lane == 0);
+    };
+    Seg g;
+    if (u_begin < u_end) load_q(g = segment<D, ALT>(a, l, u_begin, u_end, false));
+    for (int u = u_begin; u < u_end && ok; segs++) {
+      const int nt = g.tb - g.ta, row = row_of(g), valid = g.rows;
+      const bool first_of_run = u == u_begin, whole = g.ta == 0 && g.tb == g.tiles;
+      const int u0 = u;
+      u += nt;
+      const int rr = min(row, valid - 1), rx = seq_of_token(a, l, g.s, rr / a.G), ri = rr / a.G - (tok[rx] - tok[g.s * a.F]);
+      const int own_lim = len[rx] + ri + 1;
+      const int warp_x0 = __shfl_sync(0xffffffffu, rx, 0), warp_x1 = __shfl_sync(0xffffffffu, rx, 31);
+      float m = -INFINITY, sum_l = 0.f;
+      if (g.of(t).act) {
+        int j = tile_from<ALT>(g, t, g.ta);
+        Cursor cur = cursor_at<ROWS>(a, l, g, j);
+        // of the tile: K's scale times the softmax scale, log2 and inverse (times L_SCALE) of V's scale (the approximations err by
+        // 2^-22, both in the sum and in O), and how far terms may be above m; the next tile's are fetched while this one is worked on
+        float ks_next, vs_next;
+        auto fetch_scales = [&](const Cursor& c) {
+          const size_t blk = block_of(a, g, c);
+          ks_next = (c.x < 0 ? a.pks : a.ks)[blk], vs_next = (c.x < 0 ? a.pvs : a.vs)[blk];
+        };
+        fetch_scales(cur);
+        auto announce = [&](int f) {  // P in buffer f is complete
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          mbar_arrive_if(&p_full[2 * t + f], lane == 0);
+        };
+        bool first = true, fresh = true;  // fresh: a row of the warp has seen no key yet
+        while (j < g.tb) {
+          const int f = js & 1, key0 = cur.kt * KEYS, x = cur.x, nx = tile_from<ALT>(g, t, j + 1);
+          const uint32_t t_s = tmem + 128 * t + 64 * f + lanes;
+          const bool none = vs_next < kTinyScale;  // the converters made V zero
+          const float v1 = none ? 1.f : vs_next;
+          float c = ks_next * a.scale_log2, lvs = __log2f(v1), ivs = __frcp_rn(v1) * L_SCALE;
+          const float top = none ? Z_TOP : P_TOP;
+          if (nx < g.tb) {
+            if (nx == j + 1 || cur.kt + nx - j < cur.n) {
+              for (int k = j; k < nx; k++) advance<ROWS>(a, l, g, cur);
+            } else {
+              cur = cursor_at<ROWS>(a, l, g, nx);
+            }
+            fetch_scales(cur);
+          }
+          const bool mine = x < 0 || (x >= warp_x0 && x <= warp_x1);  // whether the warp has rows that see this cache
+          const int lim = x < 0 ? g.P : x == rx ? own_lim : 0;
+          uint32_t r0[32], r1[32];
+          float mx, sum = 0.f;
+          auto top32 = [&](const uint32_t (&r)[32]) {
+            float y[11];
+#pragma unroll
+            for (int e = 0; e < 10; e++) y[e] = max3f(__uint_as_float(r[3 * e]), __uint_as_float(r[3 * e + 1]), __uint_as_float(r[3 * e + 2]));
+            y[10] = fmaxf(__uint_as_float(r[30]), __uint_as_float(r[31]));
+#pragma unroll
+            for (int e = 0; e < 3; e++) y[e] = max3f(y[3 * e], y[3 * e + 1], y[3 * e + 2]);
+            return max3f(max3f(y[0], y[1], y[2]), y[9], y[10]);
+          };
+          // P' = 2^(s c + log2 vs - m) of 32 scores into columns `at` of P; returns their sum
+          auto exps = [&](const uint32_t (&r)[32], uint32_t at, float mu) {
+            const unsigned long long c2 = f2_pack(c, c), sh2 = f2_pack(lvs - mu, lvs - mu);
+            unsigned long long sum2[2] = {0ull, 0ull};
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+              float x0, x1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), c2, sh2), x0, x1);
+              const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+              sum2[e & 1] = f2_add(sum2[e & 1], f2_pack(p0, p1));
+              pk[e] = tc::pack_h2_finite(p0, p1);
+            }
+            tmem_st16(t_s + at, pk);
+            float lo, hi;
+            f2_unpack(f2_add(sum2[0], sum2[1]), lo, hi);
+            return lo + hi;
+          };
+          ok = wait(&s_full[2 * t + f], (js >> 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (!mine) {  // no row of the warp: P is zero
+            uint32_t zero[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) zero[e] = 0u;
+            tmem_st16(t_s, zero);
+            tmem_st16(t_s + 16, zero);
+            announce(f);
+            first = false, js++, j = nx;
+            continue;
+          }
+          tmem_ld32(t_s, r0);
+          // the fewest keys that a row of this warp sees: tiles up to there need no mask
+          const bool edge = key0 + KEYS > (x < 0 ? g.P : __reduce_min_sync(0xffffffffu, lim));
+          tmem_ld_wait();
+          tmem_ld32(t_s + 32, r1);
+          // a tile that every row sees whole, once rows have a maximum: P with the maximum so far, while the second half of
+          // the scores arrives and the new maximum is found beside the exponentials; they stand unless it grew too far
+          bool again = fresh || edge;
+          if (!again) {
+            sum = exps(r0, 0, m);
+            const float ma = top32(r0);
+            tmem_ld_wait();
+            sum += exps(r1, 16, m);
+            mx = fmaf(fmaxf(ma, top32(r1)), c, lvs);
+            again = __any_sync(0xffffffffu, mx > m + top);
+          }
+          if (again) {
+            tmem_ld_wait();
+            const int left = lim - key0;  // keys of the tile that the row sees
+            if (edge) {
+#pragma unroll
+              for (int e = 0; e < 32; e++) {
+                if (e >= left) r0[e] = 0xff800000u;
+                if (32 + e >= left) r1[e] = 0xff800000u;
+              }
+            }
+            const bool begins = m == -INFINITY;  // the row's first keys
+            mx = left > 0 ? fmaf(fmaxf(top32(r0), top32(r1)), c, lvs) : -INFINITY;
+            const bool need = mx > m + top;
+            const float up = top - P_MOVE;
+            const float mn = begins ? mx - up : need ? mx - (mx > m + (P_TOP + 12.f) ? fmaxf(up, P_UP_SINK) : up) : m;
+            if (!first && __any_sync(0xffffffffu, need && !begins)) {  // O through registers (warp-collective)
+              // O must hold every product up to this M tile's last tile; the barrier's next arrival needs P of this row
+              ok = wait(&pv_done[t], (js - 1) & 1);
+              if (!ok) break;
+              tc_fence_after();
+              const float half = need && !begins ? ex2_approx(0.5f * (m - mn)) : 1.f, alpha = half * half;
+              sum_l = sum_l * half * half;  // what zero blocks put there may be as large as alpha is small
+#pragma unroll
+              for (int y = 0; y < D / 16; y++) {
+                uint32_t r[16];
+                tmem_ld16(t_o + y * 16, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
+                tmem_st16(t_o + y * 16, r);
+              }
+            }
+            m = mn;
+            // a row that sees nothing of the tile takes no part in its scales, which may be NaN; scores out of sight are -inf,
+            // and -inf * 0 of a zero scale must not be NaN
+            const float mu = m == -INFINITY ? 0.f : m;
+            if (edge) {
+              if (left <= 0) c = 1.f, lvs = 0.f, ivs = 1.f;
+              if (c == 0.f) {
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                  r0[e] = e < left ? 0u : r0[e];
+                  r1[e] = 32 + e < left ? 0u : r1[e];
+                }
+                c = 1.f;
+              }
+            }
+            sum = exps(r0, 0, mu) + exps(r1, 16, mu);
+            const bool sink = begins && m != -INFINITY && sum < 1.05f * exp2f(P_UP);  // its other keys add up to a twentieth of its largest one
+            if (__any_sync(0xffffffffu, sink)) {
+              m -= sink ? P_UP_SINK - P_UP : 0.f;
+              const float ms = m == -INFINITY ? 0.f : m;
+              sum = exps(r0, 0, ms) + exps(r1, 16, ms);
+            }
+            fresh = __any_sync(0xffffffffu, m == -INFINITY);
+          }
+          sum_l += sum * ivs;
+          announce(f);
+          first = false, js++, j = nx;
+        }
+        if (!ok) break;
+      }
+      const Seg done = g;
+      if (!ALT && u < u_end) load_q(g = segment<D, ALT>(a, l, u, u_end, false));  // the next item's products start before this one's O is stored
+      const int r = row - done.q * ROWS;
+      const size_t slot = (2 * (size_t)blockIdx.x + (first_of_run ? 0 : 1)) * ROWS + r;
+      const int hq = done.h * a.G + rr % a.G;
+      const size_t out_row = ((size_t)rx * a.n + ri) * (a.G * a.H) + hq;
+      uint16_t* op = a.out + rx * a.so_b + ri * a.so_t + hq * a.so_h;
+      if (done.ta == 0 && !whole) open = make_int4((u0 + done.tiles - 1) / run, 2 * blockIdx.x + (first_of_run ? 0 : 1), done.h, done.q * ROWS);
+      if (done.ta == 0 && !whole && (!ALT || t == 0)) a.row_at[(size_t)blockIdx.x * ROWS + r] = row < valid ? rx * a.n + ri : -1;
+      // dims y16 .. y16 + 15 of the row, o = O / l where it is whole
+      auto put = [&](int y16, const float (&o)[16]) {
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(a.part_o + slot * D + y16 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        } else if (!a.own) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(a.row_o + out_row * D + y16 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; e += 8)
+            *reinterpret_cast<uint4*>(op + y16 + e) = make_uint4(pack_bf2(o[e], o[e + 1]), pack_bf2(o[e + 2], o[e + 3]), pack_bf2(o[e + 4], o[e + 5]), pack_bf2(o[e + 6], o[e + 7]));
+        }
+      };
+      auto put_ml = [&](float mm, float ll) {
+        if (!whole) a.part_ml[slot] = make_float2(mm, ll);
+        else if (!a.own) a.row_ml[out_row] = make_float2(mm, ll / L_SCALE);
+      };
+      if (ALT) {
+        float2(&hv)[2][128] = halves[segs & 1];
+        hv[t][r] = make_float2(m, sum_l);
+        __syncwarp();
+        mbar_arrive_if(halves_full, lane == 0);
+        ok = wait(halves_full, segs & 1);
+        ok = ok && (!done.m0.act || wait(&o_full[0], so & 1)) && (!done.m1.act || wait(&o_full[1], so1 & 1));
+        if (!ok) break;
+        tc_fence_after();
+        if (u < u_end) load_q(g = segment<D, ALT>(a, l, u, u_end, false));  // both M tiles' scores have been read
+        const float2 h0 = hv[0][r], h1 = hv[1][r];
+        const float mm = fmaxf(h0.x, h1.x);
+        auto weigh = [&](const float2& h, float& w) {  // factor of O; l's is the same, by halves
+          const float half = h.x == -INFINITY ? 0.f : ex2_approx(0.5f * (h.x - mm));
+          w = half * half;
+          return h.y * half * half;
+        };
+        float w0, w1;
+        const float ll = weigh(h0, w0) + weigh(h1, w1), inv = whole ? L_SCALE / ll : 1.f;
+        w0 *= inv, w1 *= inv;
+#pragma unroll
+        for (int y = 0; y < D / 32; y++) {  // this thread's half of the dims
+          const int y16 = 16 * (t * (D / 32) + y);
+          uint32_t a0[16], a1[16];
+          if (done.m0.act) tmem_ld16(tmem + 256 + lanes + y16, a0);
+          if (done.m1.act) tmem_ld16(tmem + 384 + lanes + y16, a1);
+          tmem_ld_wait();
+          float o[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) o[e] = (done.m0.act ? __uint_as_float(a0[e]) * w0 : 0.f) + (done.m1.act ? __uint_as_float(a1[e]) * w1 : 0.f);
+          if (row < valid) put(y16, o);
+        }
+        if (t == 0 && row < valid) put_ml(mm, ll);
+        tc_fence_before();
+        __syncwarp();
+        if (done.m0.act) mbar_arrive_if(&o_empty[0], lane == 0), so++;
+        if (done.m1.act) mbar_arrive_if(&o_empty[1], lane == 0), so1++;
+      } else if (!done.of(t).act) {
+        if (row < valid && !whole) a.part_ml[slot] = make_float2(-INFINITY, 0.f);
+      } else {
+        ok = wait(&o_full[t], so & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const float inv = whole ? L_SCALE / sum_l : 1.f;
+#pragma unroll
+        for (int y = 0; y < D / 16; y++) {
+          uint32_t x[16];
+          tmem_ld16(t_o + y * 16, x);
+          tmem_ld_wait();
+          float o[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) o[e] = __uint_as_float(x[e]) * inv;
+          if (row < valid) put(16 * y, o);
+        }
+        if (row < valid) put_ml(m, sum_l);
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_if(&o_empty[t], lane == 0);
+        so++;
+      }
+    }
+    if (a.items == 0 && tid == 0) a.unfinished[blockIdx.x] = open;
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// Merges the parts of an item, in the CTAs' order.  blockIdx.x = c: the item that CTA c began and did not finish; blockIdx.y: 16 of its
+// rows; thread = 4 dims of a row.
+template <int D, int ROWS>
+__global__ void __launch_bounds__(128) attn_kv8_shared_join_kernel(const __grid_constant__ Args a) {
   constexpr int PER = 128 * 4 / D;
-  const tc::Args& p = j.p;
-  const int n = p.n, G = p.G, H = p.H, Hq = G * H, F = p.F;
   griddep_wait();
   griddep_launch();
-  tc::token_list(p, tok, scratch);
-  int prun = 0, orun = 0;
-  if (p.items == 0) {
-    prun = tc::tile_list<tc::SHARED>(p, ppre, scratch, tok);
-    __syncthreads();
-  }
-  if (!j.own_whole) {
-    if (j.own_tc) {
-      orun = tc::tile_list(j.t, opre, scratch);
-    } else {
-      split::tile_list(j.s, split::keys_per_tile(D), 8 * j.nt, opre, scratch);
-      orun = split::run_of(opre[j.B], j.s.ctas);
-    }
-  }
-  const int d = threadIdx.x % (D / 4) * 4;
-  const long long rows = (long long)j.B * n * Hq;
-  for (int x = threadIdx.x / (D / 4); x < 16; x += PER) {
-    const long long at = (long long)blockIdx.x * 16 + x;
-    if (at >= rows) break;
-    const int hq = (int)(at % Hq), i = (int)(at / Hq % n), b = (int)(at / Hq / n), s = b / F, h = hq / G;
-    if (i >= tok[b + 1] - tok[b]) continue;
-    // the row's parts: of the prefix, then of its own slots; [c0, c1] are the CTAs that share it, first the slot of c0's
-    const int P = split::prefix_len(p.plens, s, p.C, false), rp = (tok[b] - tok[s * F] + i) * G + hq % G;
-    const int pt = (P + tc::KEYS - 1) / tc::KEYS;
-    int pc0 = 0, pc1 = pt ? 0 : -1, oc0 = 0, oc1 = 0;
-    size_t pfirst = 0, ofirst = 0;
-    if (pt && p.items == 0) {
-      const int items = ((tok[(s + 1) * F] - tok[s * F]) * G + tc::ROWS - 1) / tc::ROWS;
-      const int u0 = ppre[s] + (h * items + rp / tc::ROWS) * pt;
-      pc0 = u0 / prun, pc1 = (u0 + pt - 1) / prun, pfirst = 2 * (size_t)pc0 + (u0 == pc0 * prun ? 0 : 1);
-    }
-    const Seq q = seq_of(p.lens, p.counts, b, n, p.Co, false);
-    const int ro = i * G + hq % G;
-    int group = 1 << 30;  // rows of an item of the own slots
-    if (!j.own_whole) {
-      int u0, tiles;
-      if (j.own_tc) {
-        group = tc::ROWS;
-        u0 = opre[b] + (opre[b + 1] - opre[b]) / H * h;
-        int qt = 0;
-        for (; qt < ro / tc::ROWS; qt++) u0 += tc::item_tiles(j.t, q, qt);
-        tiles = tc::item_tiles(j.t, q, qt);
-      } else {
-        group = 8 * j.nt;
-        tiles = (q.len + q.cnt + split::keys_per_tile(D) - 1) / split::keys_per_tile(D);
-        u0 = opre[b] + (h * split::row_groups(j.s, q, group) + ro / group) * tiles;
-      }
-      oc0 = u0 / orun, oc1 = (u0 + tiles - 1) / orun, ofirst = 2 * (size_t)oc0 + (u0 == oc0 * orun ? 0 : 1);
-    }
-    const float2* prow = p.row_ml + ((size_t)s * H + h) * p.rows + rp;
-    const float2* orow = (j.own_tc ? j.t.row_ml : j.s.own_ml) + ((size_t)b * H + h) * (n * G) + ro;
-    auto pslot = [&](int c) { return (c == pc0 ? pfirst : 2 * (size_t)c) * tc::ROWS + rp % tc::ROWS; };
-    auto oslot = [&](int c) { return (c == oc0 ? ofirst : 2 * (size_t)c) * group + ro % group; };
-    auto pml = [&](int c) {
-      if (pc0 == pc1) return *prow;
-      const float2 v = p.part_ml[pslot(c)];
-      return make_float2(v.x, v.y * (1.f / tc::L_SCALE));
-    };
-    auto oml = [&](int c) {
-      if (oc0 == oc1) return *orow;
-      if (!j.own_tc) return j.s.part_ml[oslot(c)];
-      const float2 v = j.t.part_ml[oslot(c)];
-      return make_float2(v.x, v.y * (1.f / tc::L_SCALE));
-    };
+  const int4 open = a.unfinished[blockIdx.x];
+  if (open.x < 0) return;
+  const int c0 = blockIdx.x, c1 = open.x, d = threadIdx.x % (D / 4) * 4;
+  for (int y = threadIdx.x / (D / 4); y < 16; y += PER) {
+    const int r = blockIdx.y * 16 + y, at = a.row_at[(size_t)c0 * ROWS + r];
+    if (at < 0) break;
+    auto part = [&](int c) { return (size_t)(c == c0 ? open.y : 2 * c) * ROWS + r; };
     float mx = -INFINITY;
-    for (int c = pc0; c <= pc1; c++) mx = fmaxf(mx, pml(c).x);
-    for (int c = oc0; c <= oc1; c++) mx = fmaxf(mx, oml(c).x);
+    for (int c = c0; c <= c1; c++) mx = fmaxf(mx, a.part_ml[part(c)].x);
     float sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    // a part adds f (its O as it stands) and l 2^(m - mx) to the sum; the halves keep 2^(m - mx) l from vanishing where l is large
-    auto add = [&](const float2& ml, const float4& o, bool normal, float unit) {
-      const float half = ml.x == -INFINITY ? 0.f : ex2_approx(0.5f * (ml.x - mx)), w = ml.y * half * half, f = normal ? w : half * half * unit;
-      sum += w, v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
-    };
-    if (pc0 == pc1) add(*prow, *reinterpret_cast<const float4*>(p.row_o + (((size_t)s * H + h) * p.rows + rp) * D + d), true, 0.f);
-    else
-#pragma unroll 2
-      for (int c = pc0; c <= pc1; c++) add(pml(c), *reinterpret_cast<const float4*>(p.part_o + pslot(c) * D + d), false, 1.f);
-    if (oc0 == oc1)
-      add(*orow, *reinterpret_cast<const float4*>((j.own_tc ? j.t.row_o : j.s.own_o) + (((size_t)b * H + h) * (n * G) + ro) * D + d), true, 0.f);
-    else
-#pragma unroll 2
-      for (int c = oc0; c <= oc1; c++)
-        add(oml(c), *reinterpret_cast<const float4*>((j.own_tc ? j.t.part_o : j.s.part_o) + oslot(c) * D + d), false, j.own_tc ? 1.f : split::P_SCALE);
-    const float inv = 1.f / sum;
-    *reinterpret_cast<uint2*>(p.out + b * p.so_b + i * p.so_t + hq * p.so_h + d) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
+#pragma unroll 4
+    for (int c = c0; c <= c1; c++) {
+      const float2 ml = a.part_ml[part(c)];
+      if (ml.x == -INFINITY) {  // its M tile took part in nothing, or all scores were NaN
+        sum += 0.f * ml.y;
+        continue;
+      }
+      const float4 o = *reinterpret_cast<const float4*>(a.part_o + part(c) * D + d);
+      const float half = ex2_approx(0.5f * (ml.x - mx)), f = half * half;
+      sum += ml.y * half * half, v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
+    }
+    const float inv = L_SCALE / sum;
+    const int hq = open.z * a.G + (open.w + r) % a.G, b = at / a.n, i = at % a.n;
+    if (a.own) {
+      uint16_t* op = a.out + b * a.so_b + i * a.so_t + hq * a.so_h + d;
+      *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
+    } else {
+      const size_t out_row = (size_t)at * (a.G * a.H) + hq;
+      *reinterpret_cast<float4*>(a.row_o + out_row * D + d) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+      if (d == 0) a.row_ml[out_row] = make_float2(mx, sum / L_SCALE);
+    }
   }
+}
+
+template <int D, bool ALT>
+static int launch(cudaStream_t st, const Args& a, const char* what) {
+  using L = Smem<D, ALT>;
+  const int rc = smem_attr_once((const void*)attn_kv8_shared_tc_kernel<D, ALT>, L::BYTES, what);
+  if (rc) return rc;
+  launch_k(attn_kv8_shared_tc_kernel<D, ALT>, (unsigned)(a.items > 0 ? a.S * a.H * a.items : a.ctas), THREADS, L::BYTES, st, a);
+  if (a.items == 0) launch_k(attn_kv8_shared_join_kernel<D, L::ROWS>, dim3(a.ctas, L::ROWS / 16), 128, 0, st, a);
+  return check_launch(what);
 }
 
 // Fixed on the host from sizes alone.
 struct Plan {
-  bool few;           // one item per head with all rows and keys
-  bool own_tc;
-  split::Plan s;      // of few, or of the sequences' own slots
-  tc::Plan p, t;
-  long long p_row, p_ml, o_off, o_row, o_ml, bytes;  // workspace: the prefixes' call and rows, the own slots' call and rows
+  bool few, alt, own;  // one item per head with all rows and keys; rows of an item; whether the tcgen05 kernel takes the own slots too
+  bool whole;          // a CTA for each item of it
+  int items, ctas;
+  split::Plan s;       // of few, or of the sequences' own slots
+  long long o_off, ml_off, un_off, at_off, row_off, rml_off, s_off, bytes;  // workspace
 };
-// With F n G rows up to which one kernel takes all; a CTA of eight warps takes a whole item where it has at most so many tiles (MEASURED)
-constexpr int FEW_TILES = 32;
+// Rows up to which one kernel takes all; tiles up to which a CTA takes a whole item (MEASURED); tiles of own slots (times two, beside
+// the prefix's) up to which the tcgen05 kernel takes them (MEASURED)
+constexpr int FEW_TILES = 32, WHOLE_TILES = 24, OWN_TILES = 24;
 static int few_rows(int D) { return D == 64 ? split::FEW_ROWS : 16; }
 
 static Plan make_plan(int S, int B, int n, int Hq, int H, int D, int Cp, int C, int sms) {
@@ -144,12 +756,20 @@ static Plan make_plan(int S, int B, int n, int Hq, int H, int D, int Cp, int C, 
     x.bytes = x.s.full_off;
     return x;
   }
-  x.own_tc = n * G > split::FEW_ROWS;
-  x.p = tc::make_plan(S, F * n, Hq, H, D, Cp, false, sms);
-  x.p_row = up(x.p.lse_off), x.p_ml = x.p_row + up((long long)B * n * Hq * D * 4), x.o_off = x.p_ml + up((long long)B * n * Hq * 8);
-  if (x.own_tc) x.t = tc::make_plan(B, n, Hq, H, D, C, false, sms), x.o_row = x.o_off + up(x.t.lse_off);
-  else x.s = split::make_plan(B, n, Hq, H, D, C, false, sms), x.o_row = x.o_off + x.s.full_off;
-  x.o_ml = x.o_row + up((long long)B * n * Hq * D * 4), x.bytes = x.o_ml + up((long long)B * n * Hq * 8);
+  x.alt = all <= 128;
+  const int rows = x.alt ? 128 : 256;
+  x.items = (int)((all + rows - 1) / rows), x.ctas = sms;
+  // sequences with rows in an item, and their tiles
+  const long long seqs = (long long)n * G >= rows ? 2 : rows / ((long long)n * G) + 2, own = (seqs < F ? seqs : F) * (C / BLK);
+  x.own = (long long)n * G > split::FEW_ROWS || own <= OWN_TILES || own <= Cp / BLK / 2;
+  x.whole = Cp / BLK + (x.own ? own : 0) <= WHOLE_TILES;
+  x.ml_off = x.whole ? 0 : up(2LL * sms * rows * D * 4);
+  x.un_off = x.ml_off + (x.whole ? 0 : up(2LL * sms * rows * 8));
+  x.at_off = x.un_off + (x.whole ? 0 : up(sms * 16LL));
+  x.row_off = x.at_off + (x.whole ? 0 : up((long long)sms * rows * 4));
+  x.rml_off = x.row_off + (x.own ? 0 : up((long long)B * n * Hq * D * 4));
+  x.s_off = x.bytes = x.rml_off + (x.own ? 0 : up((long long)B * n * Hq * 8));
+  if (!x.own) x.s = split::make_plan(B, n, Hq, H, D, C, false, sms), x.bytes += x.s.full_off;
   return x;
 }
 
@@ -162,12 +782,10 @@ extern "C" {
 long long vt_attn_kv8_shared_ws_bytes(int S, int B, int n, int Hq, int H, int D, int Cp, int C) {
   using namespace vt::kv8;
   if (S <= 0 || B <= 0 || B % S || n <= 0 || Hq <= 0 || H <= 0 || Hq % H || Cp <= 0 || C <= 0 || (D != 64 && D != 128)) return 0;
-  // what n tokens need, and any fewer that may follow with the same workspace: at the largest n of each plan
-  const int sms = vt::sm_count(), G = Hq / H, F = B / S;
-  long long most = shared::make_plan(S, B, n, Hq, H, D, Cp, C, sms).bytes;
-  for (const int rows : {shared::few_rows(D) / F, split::FEW_ROWS}) {
-    const int m = rows / G;
-    if (m <= 0 || m >= n) continue;
+  // what n tokens need, and any fewer that may follow with the same workspace: a plan for few rows needs most at its largest n
+  const int sms = vt::sm_count();
+  long long most = 0;
+  for (int m = n; m > 0; m = m > 64 ? (m + 1) / 2 : m - 1) {
     const long long x = shared::make_plan(S, B, m, Hq, H, D, Cp, C, sms).bytes;
     if (x > most) most = x;
   }
@@ -197,38 +815,24 @@ int vt_attn_kv8_shared(cudaStream_t st, const uint16_t* q, long long sq_b, long 
   if (kv8::rows_meet({q, sq_b, sq_t, (Hq - 1) * sq_h + D}, {out, so_b, so_t, (Hq - 1) * so_h + D}, B, n))
     return set_error(E_SHAPE, "%s: out overlaps q", what);
   const int G = Hq / H, F = B / S, sms = sm_count();
-  const long long most = 0x20000000LL;  // tiles of a list, four rows
-  if ((long long)B * n * Hq > most / 4 || (long long)S * H * (Cp / kv8::BLK) * ((long long)F * n * G / 32 + 1) > most ||
-      (long long)B * H * (C / kv8::BLK) * ((long long)n * G / 8 + 1) > most)
+  const long long most = 0x20000000LL;  // tiles of a list, rows
+  if ((long long)B * n * Hq > most / 4 || (long long)S * H * (Cp / kv8::BLK) * ((long long)F * n * G / 128 + 1) > most ||
+      (long long)B * H * (C / kv8::BLK) * ((long long)n * G / 8 + 2) > most)
     return set_error(E_SHAPE, "%s: B * Hq * n or B * H * C too large", what);
   const kv8::shared::Plan x = kv8::shared::make_plan(S, B, n, Hq, H, D, Cp, C, sms);
   char* w8 = static_cast<char*>(ws);
   const float c = scale * kv8::LOG2E;
   kv8::split::Args sa{q, sq_b, sq_t, sq_h, kc, vc, ks, vs, lens, counts, x.few ? S : B, n, G, H, C, 1, x.few ? F * n * G : n * G, x.few ? 1 : x.s.rg, x.s.ctas, c,
-                      out, so_b, so_t, so_h, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, pk, pv, pks, pvs, plens, Cp, F, nullptr, nullptr};
-  if (x.few) {
-    sa.part_o = (float*)(w8 + x.s.o_off), sa.part_ml = (float2*)(w8 + x.s.ml_off);
-    return kv8::split::launch_any<kv8::split::SHARED>(st, sa, D, x.s.nt, x.s.whole, what);
-  }
-  kv8::tc::Args pa{q, sq_b, sq_t, sq_h, pk, pv, pks, pvs, lens, counts, S, n, G, H, Cp, 0, F * n * G, x.p.ctas,
-                   x.p.whole ? (int)(((long long)F * n * G + kv8::tc::ROWS - 1) / kv8::tc::ROWS) : 0, c, out, so_b, so_t, so_h,
-                   (float*)w8, (float2*)(w8 + x.p.ml_off), nullptr, nullptr, nullptr, plens, F, C, (float*)(w8 + x.p_row), (float2*)(w8 + x.p_ml)};
-  kv8::tc::Args ta{q, sq_b, sq_t, sq_h, kc, vc, ks, vs, lens, counts, B, n, G, H, C, 1, n * G, x.t.ctas,
-                   x.own_tc && x.t.whole ? (n * G + kv8::tc::ROWS - 1) / kv8::tc::ROWS : 0, c, out, so_b, so_t, so_h,
-                   (float*)(w8 + x.o_off), (float2*)(w8 + x.o_off + x.t.ml_off), nullptr, nullptr, nullptr, nullptr, 1, C,
-                   (float*)(w8 + x.o_row), (float2*)(w8 + x.o_ml)};
-  sa.part_o = (float*)(w8 + x.o_off + x.s.o_off), sa.part_ml = (float2*)(w8 + x.o_off + x.s.ml_off);
-  sa.own_o = (float*)(w8 + x.o_row), sa.own_ml = (float2*)(w8 + x.o_ml);
-  rc = D == 64 ? kv8::tc::launch<64, kv8::tc::SHARED>(st, pa, what) : kv8::tc::launch<128, kv8::tc::SHARED>(st, pa, what);
-  if (rc) return rc;
-  if (!x.own_tc) rc = kv8::split::launch_any<kv8::split::OWN>(st, sa, D, x.s.nt, x.s.whole, what);
-  else rc = D == 64 ? kv8::tc::launch<64, kv8::tc::OWN>(st, ta, what) : kv8::tc::launch<128, kv8::tc::OWN>(st, ta, what);
-  if (rc) return rc;
-  kv8::shared::JoinArgs j{pa, sa, ta, x.own_tc, x.own_tc ? x.t.whole : x.s.whole, B, x.s.nt};
-  const unsigned ctas = (unsigned)(((long long)B * n * Hq + 15) / 16);
-  if (D == 64) launch_k(kv8::shared::attn_kv8_shared_join_kernel<64>, ctas, 128, 0, st, j);
-  else launch_k(kv8::shared::attn_kv8_shared_join_kernel<128>, ctas, 128, 0, st, j);
-  return check_launch(what);
+                      out, so_b, so_t, so_h, (float*)(w8 + x.s_off + x.s.o_off), (float2*)(w8 + x.s_off + x.s.ml_off), nullptr, nullptr, nullptr, nullptr,
+                      pk, pv, pks, pvs, plens, Cp, F, (const float*)(w8 + x.row_off), (const float2*)(w8 + x.rml_off)};
+  if (x.few) return kv8::split::launch_any<kv8::split::SHARED>(st, sa, D, x.s.nt, x.s.whole, what);
+  const kv8::shared::Args a{q, sq_b, sq_t, sq_h, pk, pv, pks, pvs, Cp, S, F, plens, kc, vc, ks, vs, C, lens, counts, n, G, H, x.ctas,
+                            x.whole ? x.items : 0, x.own, c, out, so_b, so_t, so_h, (float*)(w8 + x.row_off), (float2*)(w8 + x.rml_off), (float*)w8,
+                            (float2*)(w8 + x.ml_off), (int4*)(w8 + x.un_off), (int*)(w8 + x.at_off)};
+  rc = D == 64 ? (x.alt ? kv8::shared::launch<64, true>(st, a, what) : kv8::shared::launch<64, false>(st, a, what))
+               : (x.alt ? kv8::shared::launch<128, true>(st, a, what) : kv8::shared::launch<128, false>(st, a, what));
+  if (rc || x.own) return rc;
+  return kv8::split::launch_any<kv8::split::OWN>(st, sa, D, x.s.nt, x.s.whole, what);
 }
 
 }  // extern "C"

@@ -29,8 +29,8 @@
 // For sequences that share a prefix the same kernel takes one of two more forms:
 //   SHARED   the rows of all F sequences on a prefix (F n G <= 32) are one item per head, whose tiles are the prefix's and then
 //            each sequence's own; a row sees the prefix and its own sequence's slots;
-//   OWN      only the sequences' own slots, each row's normalised output, maximum and sum in fp32, for
-//            attn_kv8_shared_join_kernel.
+//   OWN      the sequences' own slots, to which each row adds what it has of the prefix (its normalised output, maximum and sum
+//            in fp32, from the kernels of kv8_shared.cu).
 #include "vt_common.cuh"
 #include "vt_host.h"
 
@@ -104,9 +104,24 @@ struct Args {
   const float *pks, *pvs;
   const int* plens;
   int Cp, F;
-  float* own_o;  // [B][H][rows][D], [B][H][rows]
-  float2* own_ml;
+  const float* row_o;  // OWN: [B][n][Hq][D] and [B][n][Hq], of prefixes that are not empty
+  const float2* row_ml;
 };
+
+// OWN: what row (b, i, hq) has of the prefix, joined to (mx, sum, v): dims d .. of its own slots, 2^15 too small as the kernel holds them.
+template <int D>
+__device__ __forceinline__ void add_prefix(const Args& a, int b, int i, int hq, int d, float& mx, float& sum, float4& v) {
+  if (a.plens[b / a.F] <= 0) return;
+  const size_t at = ((size_t)b * a.n + i) * ((size_t)a.H * a.G) + hq;
+  const float2 ml = a.row_ml[at];
+  const float4 o = *reinterpret_cast<const float4*>(a.row_o + at * D + d);
+  const float top = fmaxf(mx, ml.x);
+  // l may be as large as 2^(m - top) is small: the halves keep the product
+  const float f = ex2_approx(mx - top), half = ml.x == -INFINITY ? 0.f : ex2_approx(0.5f * (ml.x - top)), w = ml.y * half * half;
+  constexpr float DOWN = 1.f / P_SCALE;
+  mx = top, sum = sum * f + w;
+  v.x = v.x * f + o.x * w * DOWN, v.y = v.y * f + o.y * w * DOWN, v.z = v.z * f + o.z * w * DOWN, v.w = v.w * f + o.w * w * DOWN;
+}
 
 // Tokens of prefix s: what does not fit is cut off and recorded.
 __device__ __forceinline__ int prefix_len(const int* plens, int s, int Cp, bool record) {
@@ -114,35 +129,19 @@ __device__ __forceinline__ int prefix_len(const int* plens, int s, int Cp, bool 
   if (in != len && record) atomicOr(&g_status, (unsigned int)ST_KV8_RANGE);
   return in;
 }
-// Tiles of a head's item over prefix s and the sequences on it: none where no sequence has a row.
-__device__ __forceinline__ int shared_tiles(const Args& a, int kt, int s, bool record) {
-  const int P = prefix_len(a.plens, s, a.Cp, record);
-  int t = 0;
-  for (int f = 0; f < a.F; f++) {
-    const Seq q = seq_of(a.lens, a.counts, s * a.F + f, a.n, a.C, record);
-    if (q.cnt) t += (q.len + q.cnt + kt - 1) / kt;
-  }
-  return t ? t + (P + kt - 1) / kt : 0;
-}
-
 // Row groups of gr rows that a sequence's new tokens fill (rg of the plan at most).
 __device__ __forceinline__ int row_groups(const Args& a, const Seq& s, int gr) { return (s.cnt * a.G + gr - 1) / gr; }
 // First tile of each sequence in the list of all tiles, pre[0 .. B]; a sequence's tiles are those of its (head, row group)
 // items one after another.  Every CTA computes it for itself.
-template <int MODE = PLAIN>
-__device__ __forceinline__ void tile_list(const Args& a, int kt, int gr, int* pre, int* warp_sum) {
+// list[0 .. n] becomes the sums before each of its n numbers; count(i) gives them, each thread takes some that follow one another.
+template <typename Count>
+__device__ __forceinline__ void sums_before(int* list, int n, int* warp_sum, const Count& count) {
   const int tid = threadIdx.x, nth = blockDim.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (a.B + nth - 1) / nth, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
+  const int per = (n + nth - 1) / nth, b0 = min(tid * per, n), b1 = min(b0 + per, n);
   int sum = 0;
   for (int b = b0; b < b1; b++) {
-    int t;
-    if constexpr (MODE == SHARED) {
-      t = shared_tiles(a, kt, b, blockIdx.x == 0) * a.H;
-    } else {
-      const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C, blockIdx.x == 0);  // those without work are looked at here only
-      t = (s.len + s.cnt + kt - 1) / kt * a.H * row_groups(a, s, gr);
-    }
-    pre[b] = t;
+    const int t = count(b);
+    list[b] = t;
     sum += t;
   }
   int inc = sum;
@@ -156,12 +155,31 @@ __device__ __forceinline__ void tile_list(const Args& a, int kt, int gr, int* pr
   int at = inc - sum;
   for (int i = 0; i < warp; i++) at += warp_sum[i];
   for (int b = b0; b < b1; b++) {
-    const int t = pre[b];
-    pre[b] = at;
+    const int t = list[b];
+    list[b] = at;
     at += t;
   }
-  if (tid == nth - 1) pre[a.B] = at;
+  if (tid == nth - 1) list[n] = at;
   __syncthreads();
+}
+template <int MODE = PLAIN>
+__device__ __forceinline__ void tile_list(const Args& a, int kt, int gr, int* pre, int* warp_sum, int* own = nullptr) {
+  const bool record = blockIdx.x == 0;  // lengths of those without work are looked at here only
+  if constexpr (MODE == SHARED) {  // a head's item over prefix s and the sequences on it: nothing where no sequence has a row
+    sums_before(own, a.B * a.F, warp_sum, [&](int b) {
+      const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C, record);
+      return s.cnt ? (s.len + s.cnt + kt - 1) / kt : 0;
+    });
+    sums_before(pre, a.B, warp_sum, [&](int s) {
+      const int P = prefix_len(a.plens, s, a.Cp, record), t = own[(s + 1) * a.F] - own[s * a.F];
+      return t ? (t + (P + kt - 1) / kt) * a.H : 0;
+    });
+  } else {
+    sums_before(pre, a.B, warp_sum, [&](int b) {
+      const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C, record);
+      return (s.len + s.cnt + kt - 1) / kt * a.H * row_groups(a, s, gr);
+    });
+  }
 }
 __device__ __forceinline__ int find_seq(const int* pre, int B, int u) {  // largest b with pre[b] <= u
   int lo = 0, hi = B;
@@ -206,6 +224,7 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
   __shared__ __align__(8) uint64_t full[WARPS * ST];
   __shared__ float sh_m[WARPS][GR], sh_l[WARPS][GR], sh_lse[WHOLE ? GR : 1];
   __shared__ int sh_cnt[MODE == SHARED ? 32 : 1];  // rows of the sequences on a prefix
+  __shared__ int own[MODE == SHARED && !WHOLE ? MAXB + 1 : 1];
   __shared__ int sh_abort;
   volatile int* abort_flag = &sh_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -223,7 +242,7 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
   if (WHOLE) {
     __syncthreads();
   } else {
-    tile_list<MODE>(a, KT, GR, pre, warp_sum);  // its barriers also publish the mbarriers
+    tile_list<MODE>(a, KT, GR, pre, warp_sum, own);  // its barriers also publish the mbarriers
     total = pre[a.B];
     const int run = run_of(total, a.ctas);
     u_begin = (long long)blockIdx.x * run;
@@ -554,12 +573,8 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
         sum += sh_l[w][r] * f, v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
       }
       if (whole) {
+        if constexpr (MODE == OWN) add_prefix<D>(a, b, i, h * a.G + row % a.G, d, mx, sum, v);
         const float inv = P_SCALE / sum;
-        if constexpr (MODE == OWN) {
-          *reinterpret_cast<float4*>(a.own_o + (bh * a.rows + row) * D + d) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-          if (d == 0) a.own_ml[bh * a.rows + row] = make_float2(mx, sum);
-          continue;
-        }
         uint16_t* op = a.out + (MODE == SHARED ? (long long)b * a.F + f : b) * a.so_b + i * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
         *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
         if (MODE == PLAIN && d == 0 && a.w) {
@@ -602,7 +617,8 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   griddep_wait();
   griddep_launch();
-  tile_list<MODE>(a, KT, GR, pre, warp_sum);
+  __shared__ int own[MODE == SHARED ? MAXB + 1 : 1];
+  tile_list<MODE>(a, KT, GR, pre, warp_sum, own);
   const int run = run_of(pre[a.B], a.ctas);
   // the first and last CTA that hold a part of an item, and the first part's slot (the others begin their CTA's run: 2 c)
   auto parts = [&](const Seq& s, int b, int h, int rg, int tiles, int& c0, int& c1, int& first) {
@@ -653,6 +669,7 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
         const float4 x = sh_o[tid + k * (D / 4)];
         v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
       }
+      if constexpr (MODE == OWN) add_prefix<D>(a, b, i, h * a.G + row % a.G, d, mx, sum, v);
       const float inv = P_SCALE / sum;
       uint16_t* op = a.out + (MODE == SHARED ? (long long)b * a.F + f : b) * a.so_b + i * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
       *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
@@ -695,7 +712,7 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
     if (j + e < T) a.w[at + e] = acc[e];
 }
 
-// what: the entry point, for its errors.  OWN's parts are joined elsewhere.
+// what: the entry point, for its errors.
 template <int D, int NT, int MODE = PLAIN>
 static int launch(cudaStream_t st, const Args& a, bool whole, const char* what = "vt_attn_kv8") {
   if (whole) {
@@ -709,12 +726,10 @@ static int launch(cudaStream_t st, const Args& a, bool whole, const char* what =
   const int rc = smem_attr_once((const void*)attn_kv8_split_kernel<D, NT, false, MODE>, SMEM, what);
   if (rc) return rc;
   launch_k(attn_kv8_split_kernel<D, NT, false, MODE>, a.ctas, WARPS * 32, SMEM, st, a);
-  if constexpr (MODE != OWN) {
-    const int rows = 8 * NT < a.rows ? 8 * NT : a.rows;
-    const int merge = a.B * a.H * a.rg * rows;
-    const int chunks = a.w ? a.B * a.H * ((a.C + 511) / 512) : 0;
-    launch_k(attn_kv8_join_kernel<D, NT, MODE>, merge + chunks, 128, 0, st, a, merge);
-  }
+  const int rows = 8 * NT < a.rows ? 8 * NT : a.rows;
+  const int merge = a.B * a.H * a.rg * rows;
+  const int chunks = a.w ? a.B * a.H * ((a.C + 511) / 512) : 0;
+  launch_k(attn_kv8_join_kernel<D, NT, MODE>, merge + chunks, 128, 0, st, a, merge);
   return check_launch(what);
 }
 template <int MODE>

@@ -23,21 +23,12 @@
 // exponentials occupy the MUFU for 1,024 (16 a clock and SM), the MMAs are issued over about 1,500, and P -> PV -> S of a
 // score buffer is a chain of which two are in flight.  128-key tiles with one score buffer were slower (346 us), so were
 // four stages (299) and P announced one tile late (294).
-// For sequences that share a prefix the same kernel takes one of two more forms, both of which leave each row's normalised output,
-// maximum and sum in fp32 for attn_kv8_shared_join_kernel:
-//   SHARED   the rows of all F sequences on a prefix over its slots.  A head's rows are r = t * G + g, t numbering the group's new
-//            tokens without gaps, so idle and short sequences cost nothing;
-//   OWN      the sequences' own slots.
 #include "vt_common.cuh"
 #include "vt_host.h"
 
 namespace vt {
 namespace kv8 {
 namespace tc {
-
-using split::OWN;
-using split::PLAIN;
-using split::SHARED;
 
 constexpr int ROWS = 256, KEYS = 64, THREADS = 16 * 32, ST = 3, MAXB = 2048;
 constexpr uint32_t TMEM_COLS = 512;  // S of M tile t, buffer f: columns 128 t + 64 f; O of tile t: 256 + 128 t
@@ -74,11 +65,6 @@ struct Args {
   float* lse;        // [B][H][rows] minus log2 of the row's sum, or null
   float* w;
   const float* w_in;
-  // SHARED: B counts the prefixes (kc .. C and plens are theirs), F sequences on each with caches of Co slots
-  const int* plens;
-  int F, Co;
-  float* row_o;  // [B][H][rows][D], [B][H][rows]: where rows go (SHARED, OWN)
-  float2* row_ml;
 };
 
 struct Plan {
@@ -98,59 +84,23 @@ static Plan make_plan(int B, int n, int Hq, int H, int D, int C, bool weights, i
   return p;
 }
 
-// SHARED: new tokens before each sequence, tok[0 .. B F]; every CTA computes it for itself.
-__device__ __forceinline__ void token_list(const Args& a, int* tok, int* scratch) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.B * a.F;
-  const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x, b0 = min(tid * per, n), b1 = min(b0 + per, n);
-  int sum = 0;
-  for (int b = b0; b < b1; b++) sum += tok[b] = seq_of(a.lens, a.counts, b, a.n, a.Co, blockIdx.x == 0 && blockIdx.y == 0).cnt;
-  int inc = sum;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, inc, d);
-    if (lane >= d) inc += y;
-  }
-  if (lane == 31) scratch[warp] = inc;
-  __syncthreads();
-  int at = inc - sum;
-  for (int i = 0; i < warp; i++) at += scratch[i];
-  for (int b = b0; b < b1; b++) {
-    const int t = tok[b];
-    tok[b] = at;
-    at += t;
-  }
-  if (tid == (int)blockDim.x - 1) tok[n] = at;
-  __syncthreads();
-}
-// Sequence b; SHARED: prefix b with the new tokens of all sequences on it.
-template <int MODE>
-__device__ __forceinline__ Seq seq_at(const Args& a, const int* tok, int b, bool record) {
-  if constexpr (MODE == SHARED) return {split::prefix_len(a.plens, b, a.C, record), tok[(b + 1) * a.F] - tok[b * a.F]};
-  return seq_of(a.lens, a.counts, b, a.n, a.C, record);
-}
-
 // Key tiles of rows [ROWS qt, ROWS qt + ROWS) of one head: up to the last key that the last of them sees.
-template <int MODE = PLAIN>
 __device__ __forceinline__ int item_tiles(const Args& a, const Seq& s, int qt) {
-  if constexpr (MODE == SHARED) return (s.len + KEYS - 1) / KEYS;
   const int last = min((qt * ROWS + ROWS - 1) / a.G, s.cnt - 1);
   return ((a.causal ? s.len + last + 1 : s.len + s.cnt) + KEYS - 1) / KEYS;
 }
 __device__ __forceinline__ int seq_items(const Args& a, const Seq& s) { return (s.cnt * a.G + ROWS - 1) / ROWS; }
 
 // The list of all tiles, sequence by sequence, head by head, item by item: pre[b] first tile of sequence b; and the run.
-template <int MODE = PLAIN>
-__device__ __forceinline__ int tile_list(const Args& a, int* pre, int* scratch, const int* tok = nullptr) {
+__device__ __forceinline__ int tile_list(const Args& a, int* pre, int* scratch) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.B + (int)blockDim.x - 1) / (int)blockDim.x, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
   int sum = 0;
   for (int b = b0; b < b1; b++) {
-    const Seq s = seq_at<MODE>(a, tok, b, blockIdx.x == 0 && blockIdx.y == 0);  // those without work are looked at here only
+    const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C, blockIdx.x == 0 && blockIdx.y == 0);  // those without work are looked at here only
     int t = 0;
     const int items = seq_items(a, s);
-    if (MODE == SHARED)
-      t = items * item_tiles<MODE>(a, s, 0);
-    else if (a.causal)
+    if (a.causal)
       for (int q = 0; q < items; q++) t += item_tiles(a, s, q);
     else if (items)
       t = items * item_tiles(a, s, 0);
@@ -183,23 +133,21 @@ struct Seg {
   int b, h, r0, ta, tb, tiles;
   Seq s;
 };
-template <int MODE = PLAIN>
-__device__ __forceinline__ Seg segment(const Args& a, const int* pre, int u, int u_end, const int* tok = nullptr) {
+__device__ __forceinline__ Seg segment(const Args& a, const int* pre, int u, int u_end) {
   Seg g;
   if (a.items > 0) {  // CTA = item
     const int bh = blockIdx.x / a.items, qt = blockIdx.x % a.items;
     g.b = bh / a.H, g.h = bh % a.H, g.r0 = qt * ROWS, g.ta = 0;
-    g.s = seq_at<MODE>(a, tok, g.b, threadIdx.x == 0);
-    g.tb = g.tiles = g.r0 < g.s.cnt * a.G ? item_tiles<MODE>(a, g.s, qt) : 0;
+    g.s = seq_of(a.lens, a.counts, g.b, a.n, a.C);
+    g.tb = g.tiles = g.r0 < g.s.cnt * a.G ? item_tiles(a, g.s, qt) : 0;
     return g;
   }
   g.b = split::find_seq(pre, a.B, u);
-  g.s = seq_at<MODE>(a, tok, g.b, threadIdx.x == 0);
+  g.s = seq_of(a.lens, a.counts, g.b, a.n, a.C);
   const int head = (pre[g.b + 1] - pre[g.b]) / a.H;  // tiles of one head
   g.h = (u - pre[g.b]) / head;
   int at = (u - pre[g.b]) % head, qt = 0;
-  if (MODE == SHARED) g.tiles = item_tiles<MODE>(a, g.s, 0), qt = at / g.tiles, at %= g.tiles;
-  else for (g.tiles = item_tiles(a, g.s, 0); at >= g.tiles; g.tiles = item_tiles(a, g.s, ++qt)) at -= g.tiles;
+  for (g.tiles = item_tiles(a, g.s, 0); at >= g.tiles; g.tiles = item_tiles(a, g.s, ++qt)) at -= g.tiles;
   g.r0 = qt * ROWS, g.ta = at, g.tb = min(g.tiles, at + (u_end - u));
   return g;
 }
@@ -237,17 +185,11 @@ __device__ __forceinline__ const uint16_t* q_row(const Args& a, int b, int h, in
   return a.q + b * a.sq_b + r / a.G * a.sq_t + (size_t)(h * a.G + r % a.G) * a.sq_h;
 }
 
-// SHARED: of row r of prefix b.
-__device__ __forceinline__ const uint16_t* q_row(const Args& a, const int* tok, int b, int h, int r) {
-  const int t = tok[b * a.F] + r / a.G, x = b * a.F + split::find_seq(tok + b * a.F, a.F, t);
-  return a.q + x * a.sq_b + (t - tok[x]) * a.sq_t + (size_t)(h * a.G + r % a.G) * a.sq_h;
-}
-
-template <int D, int MODE = PLAIN>
+template <int D>
 __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
   using L = Smem<D>;
   extern __shared__ __align__(1024) uint8_t sm[];
-  __shared__ int pre[MAXB + 1], scratch[THREADS / 32], tok[MODE == SHARED ? MAXB + 1 : 1];
+  __shared__ int pre[MAXB + 1], scratch[THREADS / 32];
   __shared__ __align__(8) uint64_t bars[2 + 2 * ST + 4 + 4 + 4 + 2];
   __shared__ uint32_t tmem_slot;
   __shared__ int sh_abort;
@@ -276,12 +218,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
   const uint32_t tmem = tmem_slot;
   griddep_wait();  // programmatic dependent launch: the previous kernel has completed
   griddep_launch();
-  if constexpr (MODE == SHARED) token_list(a, tok, scratch);
   int u_begin = 0, u_end;  // this CTA's run of tiles
   if (a.items > 0) {
-    u_end = segment<MODE>(a, pre, 0, 0, tok).tiles;
+    u_end = segment(a, pre, 0, 0).tiles;
   } else {
-    const int run = tile_list<MODE>(a, pre, scratch, tok), total = pre[a.B];
+    const int run = tile_list(a, pre, scratch), total = pre[a.B];
     u_begin = (int)min((long long)blockIdx.x * run, (long long)total);
     u_end = (int)min((long long)u_begin + run, (long long)total);
   }
@@ -307,7 +248,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
     int st = 0, ph = 0, js = 0, so = 0;  // stage and phase of the next tile's operands; tiles, segments in which t had rows
     auto next = [](int& x, int& y) { if (++x == ST) x = 0, y ^= 1; };
     for (int u = u_begin; u < end && ok;) {
-      const Seg g = segment<MODE>(a, pre, u, u_end, tok);
+      const Seg g = segment(a, pre, u, u_end);
       const int nt = g.tb - g.ta;
       u += nt;
       if (g.r0 + 128 * t >= g.s.cnt * a.G) {  // no rows in this M tile: only the barriers
@@ -363,7 +304,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
     bool ok = true;
     int j = 0;
     for (int u = u_begin; u < u_end && ok;) {
-      const Seg g = segment<MODE>(a, pre, u, u_end, tok);
+      const Seg g = segment(a, pre, u, u_end);
       const int nt = g.tb - g.ta;
       u += nt;
       const size_t bh = (size_t)g.b * a.H + g.h;
@@ -407,8 +348,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
     auto load_q = [&](const Seg& g) {  // every product with the q before it is done: its last scores have been read
       const int r = (warp & 3) * 32 + lane, row = g.r0 + 128 * t + r;
       if (g.r0 + 128 * t >= g.s.cnt * a.G) return;
-      const int from = min(row, g.s.cnt * a.G - 1);  // rows past the last are copies of it
-      const uint16_t* src = MODE == SHARED ? q_row(a, tok, g.b, g.h, from) : q_row(a, g.b, g.h, from);
+      const uint16_t* src = q_row(a, g.b, g.h, min(row, g.s.cnt * a.G - 1));  // rows past the last are copies of it
       uint8_t* dst = sm + t * L::QT + r * 16;
 #pragma unroll
       for (int c0 = 0; c0 < D / 8; c0 += 8) {
@@ -423,19 +363,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       mbar_arrive_if(&q_full[t], lane == 0);
     };
     Seg g;
-    if (u_begin < u_end) load_q(g = segment<MODE>(a, pre, u_begin, u_end, tok));
+    if (u_begin < u_end) load_q(g = segment(a, pre, u_begin, u_end));
     for (int u = u_begin; u < u_end && ok;) {
       const int nt = g.tb - g.ta, row = g.r0 + 128 * t + (warp & 3) * 32 + lane, valid = g.s.cnt * a.G;
       const bool first = u == u_begin;
       u += nt;
       if (g.r0 + 128 * t >= valid) {  // no rows: the MMA issuer skips this M tile too
         j += nt;
-        if (u < u_end) load_q(g = segment<MODE>(a, pre, u, u_end, tok));
+        if (u < u_end) load_q(g = segment(a, pre, u, u_end));
         continue;
       }
       const size_t bh = (size_t)g.b * a.H + g.h;
       const float *ksp = a.ks + bh * (a.C / BLK) + g.ta, *vsp = a.vs + bh * (a.C / BLK) + g.ta;
-      const int lim = MODE == SHARED ? g.s.len : a.causal ? g.s.len + min(row / a.G, g.s.cnt - 1) + 1 : g.s.len + g.s.cnt;
+      const int lim = a.causal ? g.s.len + min(row / a.G, g.s.cnt - 1) + 1 : g.s.len + g.s.cnt;
       // the fewest keys that a row of this warp sees: tiles up to there need no mask
       const int lim_min = __reduce_min_sync(0xffffffffu, lim);
       float m = -INFINITY, l = 0.f;
@@ -569,7 +509,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       }
       if (!ok) break;
       const Seg done = g;
-      if (u < u_end) load_q(g = segment<MODE>(a, pre, u, u_end, tok));  // the next item's products start before this one's O is stored
+      if (u < u_end) load_q(g = segment(a, pre, u, u_end));  // the next item's products start before this one's O is stored
       ok = wait(&o_full[t], so & 1);
       if (!ok) break;
       tc_fence_after();
@@ -584,12 +524,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
         tmem_ld16(t_o + x16 * 16, r);
         tmem_ld_wait();
         if (row < valid) {
-          if (MODE != PLAIN && whole) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<float4*>(a.row_o + (bh * a.rows + row) * D + 16 * x16 + e) =
-                  make_float4(__uint_as_float(r[e]) * inv, __uint_as_float(r[e + 1]) * inv, __uint_as_float(r[e + 2]) * inv, __uint_as_float(r[e + 3]) * inv);
-          } else if (whole) {
+          if (whole) {
 #pragma unroll
             for (int e = 0; e < 16; e += 8)
               *reinterpret_cast<uint4*>(op + 16 * x16 + e) =
@@ -606,7 +541,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(Args a) {
       }
       if (row < valid) {
         if (!whole) a.part_ml[slot] = make_float2(m, l);
-        else if (MODE != PLAIN) a.row_ml[bh * a.rows + row] = make_float2(m, l / L_SCALE);
         else if (a.lse) a.lse[bh * a.rows + row] = -(m - L_LOG2 + log2f(l));
       }
       tc_fence_before();
@@ -851,20 +785,19 @@ __global__ void __launch_bounds__(WTHREADS, 2) kv8_weights_tc_kernel(Args a) {
   }
 }
 
-// what: the entry point, for its errors.  SHARED's and OWN's parts are joined elsewhere.
-template <int D, int MODE = PLAIN>
-static int launch(cudaStream_t st, const Args& a, const char* what = "vt_attn_kv8") {
-  int rc = smem_attr_once((const void*)attn_kv8_tc_kernel<D, MODE>, Smem<D>::BYTES, what);
-  if (!rc) rc = smem_attr_once((const void*)kv8_weights_tc_kernel<D>, WSmem<D>::BYTES, what);
+template <int D>
+static int launch(cudaStream_t st, const Args& a) {
+  int rc = smem_attr_once((const void*)attn_kv8_tc_kernel<D>, Smem<D>::BYTES, "vt_attn_kv8");
+  if (!rc) rc = smem_attr_once((const void*)kv8_weights_tc_kernel<D>, WSmem<D>::BYTES, "vt_attn_kv8");
   if (rc) return rc;
   if (a.items > 0) {
-    launch_k(attn_kv8_tc_kernel<D, MODE>, (unsigned)(a.B * a.H * a.items), THREADS, Smem<D>::BYTES, st, a);
+    launch_k(attn_kv8_tc_kernel<D>, (unsigned)(a.B * a.H * a.items), THREADS, Smem<D>::BYTES, st, a);
   } else {
-    launch_k(attn_kv8_tc_kernel<D, MODE>, a.ctas, THREADS, Smem<D>::BYTES, st, a);
-    if constexpr (MODE == PLAIN) launch_k(attn_kv8_tc_join_kernel<D>, dim3(a.ctas, ROWS / 16), 128, 0, st, a);
+    launch_k(attn_kv8_tc_kernel<D>, a.ctas, THREADS, Smem<D>::BYTES, st, a);
+    launch_k(attn_kv8_tc_join_kernel<D>, dim3(a.ctas, ROWS / 16), 128, 0, st, a);
   }
-  if (MODE == PLAIN && a.w) launch_k(kv8_weights_tc_kernel<D>, (unsigned)(a.B * a.H * ((a.C + WK - 1) / WK)), WTHREADS, WSmem<D>::BYTES, st, a);
-  return check_launch(what);
+  if (a.w) launch_k(kv8_weights_tc_kernel<D>, (unsigned)(a.B * a.H * ((a.C + WK - 1) / WK)), WTHREADS, WSmem<D>::BYTES, st, a);
+  return check_launch("vt_attn_kv8");
 }
 
 }  // namespace tc
