@@ -39,8 +39,12 @@ struct Smem {
   static constexpr int ROWS = ALT ? 128 : 256, ST = ALT ? 4 : 3;
   static constexpr int QT = 128 * D * 2;   // bytes of one M tile of q
   static constexpr int KT = KEYS * D * 2;  // of a converted K or V tile
-  static constexpr int K = (ALT ? 1 : 2) * QT, V = K + ST * KT, BYTES = V + ST * KT;
+  static constexpr int K = (ALT ? 1 : 2) * QT, V = K + ST * KT, RAW = V + ST * KT;
+  static constexpr int RAW_TILE = 2 * KEYS * D;  // bytes of a tile's codes, K and V
+  static constexpr int BUDGET = (ALT ? 220 : 223) * 1024;  // with the lists behind them, and beside the static arrays
 };
+constexpr int MAX_RAW = 6;  // tiles of codes in flight
+__host__ __device__ inline int list_bytes(int S, int B) { return (3 * B + S + 3) * 4; }
 
 struct Args {
   const uint16_t* q;
@@ -56,6 +60,7 @@ struct Args {
   int n, G, H, ctas;
   int items;  // > 0: items of a head, and a CTA for each item (no runs, nothing to join)
   int own;    // whether the sequences' own slots are in the lists
+  int raw;    // tiles of codes in flight
   float scale_log2;
   uint16_t* out;
   long long so_b, so_t, so_h;
@@ -215,21 +220,37 @@ __device__ __forceinline__ size_t block_of(const Args& a, const Seg& g, const Cu
   return c.x < 0 ? ((size_t)g.s * a.H + g.h) * (a.Cp / BLK) + c.kt : ((size_t)c.x * a.H + g.h) * (a.C / BLK) + c.kt;
 }
 
+// A tile as its consumers need it: whose slots (x, -1: the prefix's) from which key on, K's scale times the softmax scale, log2 and inverse
+// (times L_SCALE) of V's scale (the approximations err by 2^-22, both in the sum and in O), and how far terms may be above m.
+struct Tile {
+  int x, key0;
+  float c, lvs, ivs, top;
+};
+
+// Warps 0-3, 4-7: softmax of M tile 0 / 1, thread = row; 8-11: codes -> operands; 12, 13: MMAs of M tile 0 / 1; 14: brings in codes and
+// scales, `raw` tiles ahead (with the converters' registers as the only stage, one tile ahead, 16 rows x 4 heads over 131,007 slots
+// took 131 us).
 template <int D, bool ALT>
 __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __grid_constant__ Args a) {
   using L = Smem<D, ALT>;
   constexpr int ROWS = L::ROWS, ST = L::ST;
   extern __shared__ __align__(1024) uint8_t sm[];
-  __shared__ int tok[MAXB + 1], len[MAXB], own[MAXB + 1], pre[MAXB + 1], scratch[THREADS / 32];
+  __shared__ int scratch[THREADS / 32];
+  __shared__ Seg segs_of[2][15];                // by segment and warp: what a warp works on
+  __shared__ Tile tiles[ST];
+  __shared__ float2 raw_scale[MAX_RAW];         // K's and V's
+  __shared__ int2 raw_at[MAX_RAW];              // x and key0
   __shared__ float2 halves[ALT ? 2 : 1][2][128];  // ALT: (m, l) of a row's two halves
-  __shared__ __align__(8) uint64_t bars[2 + 2 * ST + 4 + 4 + 4 + 2 + 2 + 1];
+  __shared__ __align__(8) uint64_t bars[2 + 2 * ST + 4 + 4 + 4 + 2 + 2 + 1 + 2 * MAX_RAW];
   __shared__ uint32_t tmem_slot;
   __shared__ int sh_abort;
   volatile int* abort_flag = &sh_abort;
   uint64_t *q_full = bars, *kv_full = bars + 2, *kv_empty = kv_full + ST;
   uint64_t *s_full = kv_empty + ST, *p_full = s_full + 4, *o_full = p_full + 4, *o_empty = o_full + 2, *pv_done = o_empty + 2, *drain = pv_done + 2, *halves_full = drain + 2;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const Lists l{tok, len, own, pre};
+  uint64_t *raw_full = halves_full + 1, *raw_empty = raw_full + MAX_RAW;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, B = a.S * a.F;
+  int* lists = reinterpret_cast<int*>(sm + L::RAW + a.raw * L::RAW_TILE);
+  const Lists l{lists, lists + B + 1, lists + 2 * B + 1, lists + 3 * B + 2};
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
       mbar_init(&q_full[i], ALT ? 8 : 4);  // ALT: one q, which all eight warps bring in
@@ -237,6 +258,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
     }
     for (int i = 0; i < ST; i++) mbar_init(&kv_full[i], 4), mbar_init(&kv_empty[i], 2);
     for (int i = 0; i < 4; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4);
+    for (int i = 0; i < MAX_RAW; i++) mbar_init(&raw_full[i], 2), mbar_init(&raw_empty[i], 4);  // the bulk copies' bytes, the scales
     mbar_init(halves_full, 8);
     *abort_flag = 0;
     fence_mbar_init();
@@ -256,7 +278,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
   if (a.items > 0) {
     u_end = segment<D, ALT>(a, l, 0, 0, tid == 0).tiles;
   } else {
-    const int total = pre[a.S];
+    const int total = l.pre[a.S];
     run = max((total + a.ctas - 1) / a.ctas, 1);
     u_begin = (int)min((long long)blockIdx.x * run, (long long)total);
     u_end = (int)min((long long)u_begin + run, (long long)total);
@@ -266,11 +288,20 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, ST_KV8_WAIT)) != 0;
   };
 
+  // this warp's share of the next item, in shared memory: it is looked at often and would take registers
+  auto next_segment = [&](int i, int u) -> const Seg& {
+    const Seg g = segment<D, ALT>(a, l, u, u_end, false);
+    __syncwarp();
+    if (lane == 0) segs_of[i & 1][warp] = g;
+    __syncwarp();
+    return segs_of[i & 1][warp];
+  };
+
   static_assert(2 * tc::SOFTMAX_REGS + tc::CONVERT_REGS + tc::MMA_REGS <= 4 * 128, "the split must come out of the launch's registers");
   if (warp >= 12) {
     set_regs_down<tc::MMA_REGS>();
     // ---------------- MMA issuer of M tile t, one warp each.  The whole warp walks the loop, one lane issues
-    const int t = warp - 12, end = t < 2 ? u_end : u_begin;  // warps 14 and 15 are idle
+    const int t = warp - 12, end = t < 2 ? u_end : u_begin;  // warp 15 is idle
     const uint32_t leader = elect_one();
     constexpr uint32_t IDESC_S = idesc_bf16(128, KEYS), IDESC_O = idesc_f16(128, D) | (1u << 16);  // V MN-major
     const uint64_t dq = sdesc_noswz(smem_u32(sm) + (ALT ? 0 : t * L::QT), 2048, 128), dk = sdesc_noswz(smem_u32(sm + L::K), 1024, 128);
@@ -278,8 +309,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
     const uint32_t t_s = tmem + 128 * t, t_o = tmem + 256 + 128 * t;
     bool ok = true;
     int base = 0, js = 0, so = 0, sq = 0;  // tiles of the segments before; tiles and segments that t took part in; q's that came in
-    for (int u = u_begin; u < end && ok;) {
-      const Seg g = segment<D, ALT>(a, l, u, u_end, false);
+    for (int u = u_begin, i = 0; u < end && ok; i++) {
+      const Seg& g = next_segment(i, u);
       const int nt = g.tb - g.ta;
       u += nt;
       auto stage = [&](int j) { return (base + j - g.ta) % ST; };
@@ -343,47 +374,80 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
       umma_commit(&drain[t]);
       mbar_wait_drain(&drain[t], 0, kDrainCycles);
     }
+    if (warp == 14) {
+      // ---------------- codes and scales of every tile, in order, as far ahead as there is room
+      int j = 0;
+      for (int u = u_begin, i = 0; u < u_end && ok; i++) {
+        const Seg& g = next_segment(i, u);
+        const int nt = g.tb - g.ta;
+        u += nt;
+        Cursor c = cursor_at<ROWS>(a, l, g, g.ta);
+        for (int k = 0; k < nt; k++, j++) {
+          const int st = j % a.raw;
+          if (j >= a.raw) ok = wait(&raw_empty[st], (j / a.raw - 1) & 1);
+          if (!ok) break;
+          if (lane == 0) {
+            const size_t blk = block_of(a, g, c);
+            uint8_t* to = sm + L::RAW + st * L::RAW_TILE;
+            raw_at[st] = make_int2(c.x, c.kt * KEYS);
+            mbar_arrive_expect_tx(&raw_full[st], L::RAW_TILE);
+            bulk_load(to, (c.x < 0 ? a.pk : a.kc) + blk * (KEYS * D), KEYS * D, &raw_full[st]);
+            bulk_load(to + KEYS * D, (c.x < 0 ? a.pv : a.vc) + blk * (KEYS * D), KEYS * D, &raw_full[st]);
+            const float *ks = (c.x < 0 ? a.pks : a.ks) + blk, *vs = (c.x < 0 ? a.pvs : a.vs) + blk;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&raw_scale[st].x)), "l"(ks) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&raw_scale[st].y)), "l"(vs) : "memory");
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&raw_full[st])) : "memory");
+          }
+          __syncwarp();
+          if (k + 1 < nt) advance<ROWS>(a, l, g, c);
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      for (int k = max(j - a.raw, 0); k < j; k++) mbar_wait_drain(&raw_full[k % a.raw], (k / a.raw) & 1, kDrainCycles);  // copies in flight land, whatever the others do
+    }
   } else if (warp >= 8) {
     set_regs_down<tc::CONVERT_REGS>();
-    // ---------------- converters: warp w rows 16 w .. of a block, 8 lanes = 8 rows of one 16-byte piece.  K's and V's codes of
-    // the next tile are fetched as soon as this tile's are out of the registers
-    constexpr int PER = D / 32;  // pieces of a K or V block that a lane takes
+    // ---------------- converters: warp w rows 16 w .. of a block.  A lane's 16-byte pieces lie on a diagonal: eight lanes read eight
+    // pieces of different banks, and write eight rows
+    constexpr int PER = D / 32, PIECES = D / 16;  // pieces of a K or V block that a lane takes, of a row
     const int w = warp - 8;
     bool ok = true;
-    int j = 0;
-    for (int u = u_begin; u < u_end && ok;) {
-      const Seg g = segment<D, ALT>(a, l, u, u_end, false);
-      const int nt = g.tb - g.ta;
-      u += nt;
-      const int row = 16 * w + (lane & 7), piece = lane >> 3;
-      Cursor c = cursor_at<ROWS>(a, l, g, g.ta);
-      uint4 kr[PER], vr[PER];
-      float vs;
-      auto fetch = [&](uint4 (&to)[PER], const int8_t* from) {
-#pragma unroll
-        for (int x = 0; x < PER; x++)
-          to[x] = *reinterpret_cast<const uint4*>(from + (row + 8 * (x & 1)) * D + 16 * (piece + 4 * (x >> 1)));
+    for (int j = 0; j < u_end - u_begin; j++) {
+      const int st = j % ST, rs = j % a.raw;
+      ok = wait(&raw_full[rs], (j / a.raw) & 1) && (j < ST || wait(&kv_empty[st], (j / ST - 1) & 1));
+      if (!ok) break;
+      const uint8_t* raw = sm + L::RAW + rs * L::RAW_TILE;
+      const float2 scale = raw_scale[rs];
+      const bool none = scale.y < kTinyScale;  // V becomes zero
+      auto piece = [&](int x, int& row, int& p) {
+        row = 16 * w + 8 * (x & 1) + (lane & 7);
+        p = ((D == 64 ? (lane & 7) >> 1 : lane & 7) + (lane >> 3) + 4 * (x >> 1)) % PIECES;
+        return row * D + 16 * p;
       };
-      size_t blk = block_of(a, g, c);
-      fetch(kr, (c.x < 0 ? a.pk : a.kc) + blk * (KEYS * D));
-      fetch(vr, (c.x < 0 ? a.pv : a.vc) + blk * (KEYS * D));
-      vs = (c.x < 0 ? a.pvs : a.vs)[blk];
-      for (int i = 0; i < nt; i++, j++) {
-        const int st = j % ST;
-        if (j >= ST) ok = wait(&kv_empty[st], (j / ST - 1) & 1);
-        if (!ok) break;
-        if (i + 1 < nt) advance<ROWS>(a, l, g, c), blk = block_of(a, g, c);
+      uint4 kr[PER], vr[PER];
 #pragma unroll
-        for (int x = 0; x < PER; x++) tc::store_codes<KEYS, false>(sm + L::K + st * L::KT, row + 8 * (x & 1), piece + 4 * (x >> 1), kr[x]);
-        if (i + 1 < nt) fetch(kr, (c.x < 0 ? a.pk : a.kc) + blk * (KEYS * D));
-#pragma unroll
-        for (int x = 0; x < PER; x++)
-          tc::store_codes<KEYS, true>(sm + L::V + st * L::KT, row + 8 * (x & 1), piece + 4 * (x >> 1), vs < kTinyScale ? make_uint4(0, 0, 0, 0) : vr[x]);
-        if (i + 1 < nt) fetch(vr, (c.x < 0 ? a.pv : a.vc) + blk * (KEYS * D)), vs = (c.x < 0 ? a.pvs : a.vs)[blk];
-        fence_proxy_async_smem();
-        __syncwarp();
-        mbar_arrive_if(&kv_full[st], lane == 0);
+      for (int x = 0; x < PER; x++) {
+        int row, p;
+        const int at = piece(x, row, p);
+        kr[x] = *reinterpret_cast<const uint4*>(raw + at), vr[x] = *reinterpret_cast<const uint4*>(raw + KEYS * D + at);
       }
+      if (w == 0 && lane == 0) {
+        const float v1 = none ? 1.f : scale.y;
+        const int2 at = raw_at[rs];
+        tiles[st] = {at.x, at.y, scale.x * a.scale_log2, __log2f(v1), __frcp_rn(v1) * L_SCALE, none ? Z_TOP : P_TOP};
+      }
+      __syncwarp();
+      mbar_arrive_if(&raw_empty[rs], lane == 0);
+#pragma unroll
+      for (int x = 0; x < PER; x++) {
+        int row, p;
+        piece(x, row, p);
+        tc::store_codes<KEYS, false>(sm + L::K + st * L::KT, row, p, kr[x]);
+        tc::store_codes<KEYS, true>(sm + L::V + st * L::KT, row, p, none ? make_uint4(0, 0, 0, 0) : vr[x]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      mbar_arrive_if(&kv_full[st], lane == 0);
     }
   } else {
     set_regs_up<tc::SOFTMAX_REGS>();
@@ -391,13 +455,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
     const int t = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, t_o = tmem + 256 + 128 * t + lanes;
     bool ok = true;
-    int js = 0, so = 0, so1 = 0, segs = 0;  // tiles that t took part in; outputs stored (ALT: of M tile 0 and 1); segments
+    int base = 0, js = 0, so = 0, so1 = 0, segs = 0;  // tiles of the segments before; tiles that t took part in; outputs stored (ALT: of M tile 0 and 1); segments
     int4 open = make_int4(-1, 0, 0, 0);
     auto row_of = [&](const Seg& g) { return g.q * ROWS + (ALT ? 0 : 128 * t) + (warp & 3) * 32 + lane; };
     auto load_q = [&](const Seg& g) {  // every product with the q before it is done: its last scores have been read
       if (!ALT && !g.of(t).act) return;
       const int row = min(row_of(g), g.rows - 1);  // rows past the last are copies of it
-      const int x = seq_of_token(a, l, g.s, row / a.G), i = row / a.G - (tok[x] - tok[g.s * a.F]);
+      const int x = seq_of_token(a, l, g.s, row / a.G), i = row / a.G - (l.tok[x] - l.tok[g.s * a.F]);
       const uint16_t* src = a.q + x * a.sq_b + i * a.sq_t + (size_t)(g.h * a.G + row % a.G) * a.sq_h;
       uint8_t* dst = sm + (ALT ? 0 : t * L::QT) + ((warp & 3) * 32 + lane) * 16;
       constexpr int CH = ALT ? D / 16 : D / 8;  // 16-byte pieces of this thread
@@ -414,28 +478,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
       __syncwarp();
       mbar_arrive_if(&q_full[ALT ? 0 : t], lane == 0);
     };
-    Seg g;
-    if (u_begin < u_end) load_q(g = segment<D, ALT>(a, l, u_begin, u_end, false));
+    if (u_begin < u_end) load_q(next_segment(0, u_begin));
     for (int u = u_begin; u < u_end && ok; segs++) {
+      const Seg& g = segs_of[segs & 1][warp];
       const int nt = g.tb - g.ta, row = row_of(g), valid = g.rows;
       const bool first_of_run = u == u_begin, whole = g.ta == 0 && g.tb == g.tiles;
       const int u0 = u;
       u += nt;
-      const int rr = min(row, valid - 1), rx = seq_of_token(a, l, g.s, rr / a.G), ri = rr / a.G - (tok[rx] - tok[g.s * a.F]);
-      const int own_lim = len[rx] + ri + 1;
+      const int rr = min(row, valid - 1), rx = seq_of_token(a, l, g.s, rr / a.G), ri = rr / a.G - (l.tok[rx] - l.tok[g.s * a.F]);
+      const int own_lim = l.len[rx] + ri + 1;
       const int warp_x0 = __shfl_sync(0xffffffffu, rx, 0), warp_x1 = __shfl_sync(0xffffffffu, rx, 31);
       float m = -INFINITY, sum_l = 0.f;
       if (g.of(t).act) {
         int j = tile_from<ALT>(g, t, g.ta);
-        Cursor cur = cursor_at<ROWS>(a, l, g, j);
-        // of the tile: K's scale times the softmax scale, log2 and inverse (times L_SCALE) of V's scale (the approximations err by
-        // 2^-22, both in the sum and in O), and how far terms may be above m; the next tile's are fetched while this one is worked on
-        float ks_next, vs_next;
-        auto fetch_scales = [&](const Cursor& c) {
-          const size_t blk = block_of(a, g, c);
-          ks_next = (c.x < 0 ? a.pks : a.ks)[blk], vs_next = (c.x < 0 ? a.pvs : a.vs)[blk];
-        };
-        fetch_scales(cur);
         auto announce = [&](int f) {  // P in buffer f is complete
           tmem_st_wait();
           tc_fence_before();
@@ -444,23 +499,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
         };
         bool first = true, fresh = true;  // fresh: a row of the warp has seen no key yet
         while (j < g.tb) {
-          const int f = js & 1, key0 = cur.kt * KEYS, x = cur.x, nx = tile_from<ALT>(g, t, j + 1);
+          const int f = js & 1, at = base + j - g.ta;
           const uint32_t t_s = tmem + 128 * t + 64 * f + lanes;
-          const bool none = vs_next < kTinyScale;  // the converters made V zero
-          const float v1 = none ? 1.f : vs_next;
-          float c = ks_next * a.scale_log2, lvs = __log2f(v1), ivs = __frcp_rn(v1) * L_SCALE;
-          const float top = none ? Z_TOP : P_TOP;
-          if (nx < g.tb) {
-            if (nx == j + 1 || cur.kt + nx - j < cur.n) {
-              for (int k = j; k < nx; k++) advance<ROWS>(a, l, g, cur);
-            } else {
-              cur = cursor_at<ROWS>(a, l, g, nx);
-            }
-            fetch_scales(cur);
-          }
+          uint32_t r0[32], r1[32];
+          // the scores, and with them the tile: its operands' phase (before the scores are there, it might be an earlier one's)
+          ok = wait(&s_full[2 * t + f], (js >> 1) & 1) && wait(&kv_full[at % ST], (at / ST) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          tmem_ld32(t_s, r0);
+          const int x = tiles[at % ST].x, key0 = tiles[at % ST].key0;
+          float c = tiles[at % ST].c, lvs = tiles[at % ST].lvs, ivs = tiles[at % ST].ivs;
+          const float top = tiles[at % ST].top;
           const bool mine = x < 0 || (x >= warp_x0 && x <= warp_x1);  // whether the warp has rows that see this cache
           const int lim = x < 0 ? g.P : x == rx ? own_lim : 0;
-          uint32_t r0[32], r1[32];
           float mx, sum = 0.f;
           auto top32 = [&](const uint32_t (&r)[32]) {
             float y[11];
@@ -489,20 +540,17 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
             f2_unpack(f2_add(sum2[0], sum2[1]), lo, hi);
             return lo + hi;
           };
-          ok = wait(&s_full[2 * t + f], (js >> 1) & 1);
-          if (!ok) break;
-          tc_fence_after();
           if (!mine) {  // no row of the warp: P is zero
             uint32_t zero[16];
 #pragma unroll
             for (int e = 0; e < 16; e++) zero[e] = 0u;
+            tmem_ld_wait();
             tmem_st16(t_s, zero);
             tmem_st16(t_s + 16, zero);
             announce(f);
-            first = false, js++, j = nx;
+            first = false, js++, j = tile_from<ALT>(g, t, j + 1);
             continue;
           }
-          tmem_ld32(t_s, r0);
           // the fewest keys that a row of this warp sees: tiles up to there need no mask
           const bool edge = key0 + KEYS > (x < 0 ? g.P : __reduce_min_sync(0xffffffffu, lim));
           tmem_ld_wait();
@@ -576,12 +624,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
           }
           sum_l += sum * ivs;
           announce(f);
-          first = false, js++, j = nx;
+          first = false, js++, j = tile_from<ALT>(g, t, j + 1);
         }
         if (!ok) break;
       }
-      const Seg done = g;
-      if (!ALT && u < u_end) load_q(g = segment<D, ALT>(a, l, u, u_end, false));  // the next item's products start before this one's O is stored
+      base += nt;
+      const Seg& done = g;
+      if (!ALT && u < u_end) load_q(next_segment(segs + 1, u));  // the next item's products start before this one's O is stored
       const int r = row - done.q * ROWS;
       const size_t slot = (2 * (size_t)blockIdx.x + (first_of_run ? 0 : 1)) * ROWS + r;
       const int hq = done.h * a.G + rr % a.G;
@@ -616,7 +665,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
         ok = ok && (!done.m0.act || wait(&o_full[0], so & 1)) && (!done.m1.act || wait(&o_full[1], so1 & 1));
         if (!ok) break;
         tc_fence_after();
-        if (u < u_end) load_q(g = segment<D, ALT>(a, l, u, u_end, false));  // both M tiles' scores have been read
+        if (u < u_end) load_q(next_segment(segs + 1, u));  // both M tiles' scores have been read
         const float2 h0 = hv[0][r], h1 = hv[1][r];
         const float mm = fmaxf(h0.x, h1.x);
         auto weigh = [&](const float2& h, float& w) {  // factor of O; l's is the same, by halves
@@ -679,55 +728,70 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
   }
 }
 
-// Merges the parts of an item, in the CTAs' order.  blockIdx.x = c: the item that CTA c began and did not finish; blockIdx.y: 16 of its
-// rows; thread = 4 dims of a row.
+// Merges the parts of an item, always in the same order.  blockIdx.x = c: the item that CTA c began and did not finish; blockIdx.y: two of its
+// rows, 64 threads each: thread = 4 dims, of every 256 / D'th part.
 template <int D, int ROWS>
 __global__ void __launch_bounds__(128) attn_kv8_shared_join_kernel(const __grid_constant__ Args a) {
-  constexpr int PER = 128 * 4 / D;
+  constexpr int SHARE = 256 / D;
+  __shared__ __align__(16) float4 sh_o[128];
   griddep_wait();
   griddep_launch();
   const int4 open = a.unfinished[blockIdx.x];
   if (open.x < 0) return;
-  const int c0 = blockIdx.x, c1 = open.x, d = threadIdx.x % (D / 4) * 4;
-  for (int y = threadIdx.x / (D / 4); y < 16; y += PER) {
-    const int r = blockIdx.y * 16 + y, at = a.row_at[(size_t)c0 * ROWS + r];
-    if (at < 0) break;
-    auto part = [&](int c) { return (size_t)(c == c0 ? open.y : 2 * c) * ROWS + r; };
-    float mx = -INFINITY;
-    for (int c = c0; c <= c1; c++) mx = fmaxf(mx, a.part_ml[part(c)].x);
-    float sum = 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = c0; c <= c1; c++) {
+  const int c0 = blockIdx.x, c1 = open.x, lane = threadIdx.x & 31, x = threadIdx.x & 63, share = x / (D / 4), d = x % (D / 4) * 4;
+  const int r = blockIdx.y * 2 + threadIdx.x / 64, at = a.row_at[(size_t)c0 * ROWS + r];
+  auto part = [&](int c) { return (size_t)(c == c0 ? open.y : 2 * c) * ROWS + r; };
+  float mx = -INFINITY, sum = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (at >= 0) {  // whole warps: a row's threads are two of them
+    for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, a.part_ml[part(c)].x);
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+    for (int c = c0 + lane; c <= c1; c += 32) {
       const float2 ml = a.part_ml[part(c)];
-      if (ml.x == -INFINITY) {  // its M tile took part in nothing, or all scores were NaN
-        sum += 0.f * ml.y;
-        continue;
-      }
+      const float half = ml.x == -INFINITY ? 0.f : ex2_approx(0.5f * (ml.x - mx));
+      sum += ml.y * half * half;
+    }
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+#pragma unroll 4
+    for (int c = c0 + share; c <= c1; c += SHARE) {
+      const float m = a.part_ml[part(c)].x;
       const float4 o = *reinterpret_cast<const float4*>(a.part_o + part(c) * D + d);
-      const float half = ex2_approx(0.5f * (ml.x - mx)), f = half * half;
-      sum += ml.y * half * half, v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
+      const float half = ex2_approx(0.5f * (m - mx)), f = half * half;
+      if (m != -INFINITY) v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;  // else its M tile took part in nothing, or all scores were NaN
     }
-    const float inv = L_SCALE / sum;
-    const int hq = open.z * a.G + (open.w + r) % a.G, b = at / a.n, i = at % a.n;
-    if (a.own) {
-      uint16_t* op = a.out + b * a.so_b + i * a.so_t + hq * a.so_h + d;
-      *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
-    } else {
-      const size_t out_row = (size_t)at * (a.G * a.H) + hq;
-      *reinterpret_cast<float4*>(a.row_o + out_row * D + d) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-      if (d == 0) a.row_ml[out_row] = make_float2(mx, sum / L_SCALE);
-    }
+  }
+  sh_o[threadIdx.x] = v;
+  __syncthreads();
+  if (at < 0 || share) return;
+#pragma unroll
+  for (int k = 1; k < SHARE; k++) {
+    const float4 o = sh_o[threadIdx.x + k * (D / 4)];
+    v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+  }
+  const float inv = L_SCALE / sum;
+  const int hq = open.z * a.G + (open.w + r) % a.G, b = at / a.n, i = at % a.n;
+  if (a.own) {
+    uint16_t* op = a.out + b * a.so_b + i * a.so_t + hq * a.so_h + d;
+    *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
+  } else {
+    const size_t out_row = (size_t)at * (a.G * a.H) + hq;
+    *reinterpret_cast<float4*>(a.row_o + out_row * D + d) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    if (d == 0) a.row_ml[out_row] = make_float2(mx, sum / L_SCALE);
   }
 }
 
 template <int D, bool ALT>
-static int launch(cudaStream_t st, const Args& a, const char* what) {
+static int launch(cudaStream_t st, Args a, const char* what) {
   using L = Smem<D, ALT>;
-  const int rc = smem_attr_once((const void*)attn_kv8_shared_tc_kernel<D, ALT>, L::BYTES, what);
+  const int rc = smem_attr_once((const void*)attn_kv8_shared_tc_kernel<D, ALT>, L::BUDGET, what);
   if (rc) return rc;
-  launch_k(attn_kv8_shared_tc_kernel<D, ALT>, (unsigned)(a.items > 0 ? a.S * a.H * a.items : a.ctas), THREADS, L::BYTES, st, a);
-  if (a.items == 0) launch_k(attn_kv8_shared_join_kernel<D, L::ROWS>, dim3(a.ctas, L::ROWS / 16), 128, 0, st, a);
+  const int lists = list_bytes(a.S, a.S * a.F), room = (L::BUDGET - L::RAW - lists) / L::RAW_TILE;
+  static_assert((L::BUDGET - L::RAW - (4 * MAXB + 3) * 4) / L::RAW_TILE >= 1, "codes in flight beside the longest lists");
+  a.raw = room < MAX_RAW ? room : MAX_RAW;
+  launch_k(attn_kv8_shared_tc_kernel<D, ALT>, (unsigned)(a.items > 0 ? a.S * a.H * a.items : a.ctas), THREADS, L::RAW + a.raw * L::RAW_TILE + lists, st, a);
+  if (a.items == 0) launch_k(attn_kv8_shared_join_kernel<D, L::ROWS>, dim3(a.ctas, L::ROWS / 2), 128, 0, st, a);
   return check_launch(what);
 }
 
@@ -827,7 +891,7 @@ int vt_attn_kv8_shared(cudaStream_t st, const uint16_t* q, long long sq_b, long 
                       pk, pv, pks, pvs, plens, Cp, F, (const float*)(w8 + x.row_off), (const float2*)(w8 + x.rml_off)};
   if (x.few) return kv8::split::launch_any<kv8::split::SHARED>(st, sa, D, x.s.nt, x.s.whole, what);
   const kv8::shared::Args a{q, sq_b, sq_t, sq_h, pk, pv, pks, pvs, Cp, S, F, plens, kc, vc, ks, vs, C, lens, counts, n, G, H, x.ctas,
-                            x.whole ? x.items : 0, x.own, c, out, so_b, so_t, so_h, (float*)(w8 + x.row_off), (float2*)(w8 + x.rml_off), (float*)w8,
+                            x.whole ? x.items : 0, x.own, 0, c, out, so_b, so_t, so_h, (float*)(w8 + x.row_off), (float2*)(w8 + x.rml_off), (float*)w8,
                             (float2*)(w8 + x.ml_off), (int4*)(w8 + x.un_off), (int*)(w8 + x.at_off)};
   rc = D == 64 ? (x.alt ? kv8::shared::launch<64, true>(st, a, what) : kv8::shared::launch<64, false>(st, a, what))
                : (x.alt ? kv8::shared::launch<128, true>(st, a, what) : kv8::shared::launch<128, false>(st, a, what));
