@@ -31,7 +31,7 @@ using tc::P_UP;
 using tc::P_UP_SINK;
 using tc::THREADS;
 using tc::Z_TOP;
-constexpr int MAXB = 2048;
+constexpr int MAXB = 2048, MAX_CTAS = 512;  // sequences and runs (one for each SM) of a call
 constexpr uint32_t TMEM_COLS = 512;  // S of M tile t, buffer f: columns 128 t + 64 f; O of tile t: 256 + 128 t
 
 template <int D, bool ALT>
@@ -41,10 +41,10 @@ struct Smem {
   static constexpr int KT = KEYS * D * 2;  // of a converted K or V tile
   static constexpr int K = (ALT ? 1 : 2) * QT, V = K + ST * KT, RAW = V + ST * KT;
   static constexpr int RAW_TILE = 2 * KEYS * D;  // bytes of a tile's codes, K and V
-  static constexpr int BUDGET = (ALT ? 220 : 223) * 1024;  // with the lists behind them, and beside the static arrays
+  static constexpr int BUDGET = (ALT ? 217 : 221) * 1024;  // with the lists behind them, and beside the static arrays
 };
 constexpr int MAX_RAW = 6;  // tiles of codes in flight
-__host__ __device__ inline int list_bytes(int S, int B) { return (3 * B + S + 3) * 4; }
+__host__ __device__ inline int list_bytes(int S, int B) { return (3 * B + 2 * S + 3) * 4; }
 
 struct Args {
   const uint16_t* q;
@@ -76,6 +76,7 @@ struct Args {
 struct Lists {
   int *tok, *len;  // new tokens before each sequence, [B + 1]; tokens that it held before the call
   int *own, *pre;  // own tiles of the items before each sequence's, [B + 1]; tiles before each prefix's heads, [S + 1]
+  int* plen;       // tokens of each prefix
 };
 __device__ __forceinline__ int seq_of_token(const Args& a, const Lists& l, int s, int t) {  // t: of the prefix's sequences
   return s * a.F + split::find_seq(l.tok + s * a.F, a.F, l.tok[s * a.F] + t);
@@ -104,9 +105,8 @@ __device__ __forceinline__ void make_lists(const Args& a, const Lists& l, int* s
         for (int q = first / ROWS; q <= (first + rows - 1) / ROWS; q++) t += own_tiles<ROWS>(a, l, s, x, q);
       return t;
     });
-  if (a.items > 0) return;
   split::sums_before(l.pre, a.S, scratch, [&](int s) {
-    const int P = split::prefix_len(a.plens, s, a.Cp, record), rows = (l.tok[(s + 1) * a.F] - l.tok[s * a.F]) * a.G;
+    const int P = l.plen[s] = split::prefix_len(a.plens, s, a.Cp, record), rows = (l.tok[(s + 1) * a.F] - l.tok[s * a.F]) * a.G;
     return ((rows + ROWS - 1) / ROWS * ((P + KEYS - 1) / KEYS) + (a.own ? l.own[(s + 1) * a.F] - l.own[s * a.F] : 0)) * a.H;
   });
 }
@@ -114,15 +114,16 @@ __device__ __forceinline__ void make_lists(const Args& a, const Lists& l, int* s
 // A CTA's share of an item: rows q ROWS .. of prefix s, head h; key tiles [ta, tb) of `tiles`, the first pt of them the prefix's.
 struct Seg {
   int s, h, q, rows, P, pt, x0, x1, t0, tiles, ta, tb;  // x0, x1: first and last sequence of the item; t0: own tiles of x0
+  int u;                                                // of its first tile in the list
   struct Part {
     int oa, ob;  // own tiles that concern the M tile: [oa, ob) of the item's
     bool act;    // whether it has any tile here
   } m0, m1;
   __device__ __forceinline__ Part of(int t) const { return t ? m1 : m0; }
 };
-template <int ROWS>
-__device__ __forceinline__ int own_before(const Args& a, const Lists& l, const Seg& g, int x) {  // own tiles of the item before x's
-  return !a.own || x == g.x0 ? 0 : g.t0 + l.own[x] - l.own[g.x0 + 1];
+// Own tiles of an item before those of sequence x.
+__device__ __forceinline__ int own_before(const Args& a, const Lists& l, int x0, int t0, int x) {
+  return !a.own || x == x0 ? 0 : t0 + l.own[x] - l.own[x0 + 1];
 }
 // Tiles of items 0 .. q - 1 of a head.
 template <int ROWS>
@@ -136,54 +137,63 @@ __device__ __forceinline__ int tiles_before(const Args& a, const Lists& l, int s
   }
   return t;
 }
+// The largest i < n with value(i) <= u (value(0) is), and its value: the whole warp looks at 32 places at a time.
+template <typename Value>
+__device__ __forceinline__ int warp_search(int n, int u, int& found, const Value& value) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0;
+  found = 0;
+  while (n > 0) {
+    const int step = (n + 31) / 32;
+    const int v = lane * step < n ? value(lo + lane * step) : 0x7fffffff;
+    const int k = 31 - __clz(__ballot_sync(0xffffffffu, v <= u) | 1u);
+    found = __shfl_sync(0xffffffffu, v, k);
+    lo += k * step, n = step > 1 ? min(step, n - k * step) : 0;
+  }
+  return lo;
+}
+// The share that begins at place u of the list (of whole items: this CTA's), worked out by a warp.
 template <int D, bool ALT>
-__device__ __forceinline__ Seg segment(const Args& a, const Lists& l, int u, int u_end, bool record) {
+__device__ __forceinline__ Seg segment(const Args& a, const Lists& l, int u, int u_end) {
   constexpr int ROWS = Smem<D, ALT>::ROWS;
+  const int lane = threadIdx.x & 31;
   Seg g;
   int at = 0;
   if (a.items > 0) {
     const int sh = blockIdx.x / a.items;
     g.s = sh / a.H, g.h = sh % a.H, g.q = blockIdx.x % a.items;
   } else {
-    g.s = split::find_seq(l.pre, a.S, u);
+    int before = 0;
+    g.s = a.S > 1 ? warp_search(a.S, u, before, [&](int s) { return l.pre[s]; }) : 0;
     const int head = (l.pre[g.s + 1] - l.pre[g.s]) / a.H;
-    g.h = (u - l.pre[g.s]) / head, at = (u - l.pre[g.s]) % head;
+    g.h = (u - before) / head, at = (u - before) % head;
   }
   g.rows = (l.tok[(g.s + 1) * a.F] - l.tok[g.s * a.F]) * a.G;
-  g.P = split::prefix_len(a.plens, g.s, a.Cp, record);
+  g.P = l.plen[g.s];
   g.pt = (g.P + KEYS - 1) / KEYS;
   if (a.items == 0) {  // the last item that begins at `at` or before
-    int lo = 0, hi = (g.rows + ROWS - 1) / ROWS;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (tiles_before<ROWS>(a, l, g.s, mid, g.pt) <= at) lo = mid; else hi = mid;
-    }
-    g.q = lo;
-    at -= tiles_before<ROWS>(a, l, g.s, lo, g.pt);
+    int before = 0;
+    g.q = warp_search((g.rows + ROWS - 1) / ROWS, at, before, [&](int q) { return tiles_before<ROWS>(a, l, g.s, q, g.pt); });
+    at -= before;
   }
   const int r0 = g.q * ROWS;
-  g.tiles = 0, g.ta = at;
+  g.tiles = 0, g.ta = at, g.u = u, g.x0 = g.x1 = g.t0 = 0;
+  int oa1 = 0, ob0 = 0;
   if (r0 < g.rows) {
-    g.x0 = seq_of_token(a, l, g.s, r0 / a.G), g.x1 = seq_of_token(a, l, g.s, (min(r0 + ROWS, g.rows) - 1) / a.G);
-    g.t0 = own_tiles<ROWS>(a, l, g.s, g.x0, g.q);
-    g.tiles = g.pt + own_before<ROWS>(a, l, g, g.x1) + own_tiles<ROWS>(a, l, g.s, g.x1, g.q);
+    // lanes 0 .. 3: the first row of the item, the last one of M tile 0, the first one of M tile 1, the last one of the item
+    const int row = min(lane == 0 ? r0 : lane == 1 ? r0 + 127 : lane == 2 ? r0 + 128 : r0 + ROWS - 1, g.rows - 1);
+    const int x = seq_of_token(a, l, g.s, row / a.G), own = own_tiles<ROWS>(a, l, g.s, x, g.q);
+    g.x0 = __shfl_sync(0xffffffffu, x, 0), g.t0 = __shfl_sync(0xffffffffu, own, 0), g.x1 = __shfl_sync(0xffffffffu, x, 3);
+    const int from = g.pt + own_before(a, l, g.x0, g.t0, x), to = from + own;
+    ob0 = __shfl_sync(0xffffffffu, to, 1), oa1 = __shfl_sync(0xffffffffu, from, 2), g.tiles = __shfl_sync(0xffffffffu, to, 3);
   }
   g.tb = a.items > 0 ? g.tiles : min(g.tiles, g.ta + (u_end - u));
-  auto part = [&](int t) {
-    Seg::Part p{g.pt, g.tiles, g.ta < g.tb};
-    if (ALT) {
-      p.act = g.tb - g.ta >= 2 || (g.ta < g.tb && (g.ta & 1) == t);
-    } else if (r0 + 128 * t >= g.rows) {
-      p.act = false;
-    } else if (a.own) {
-      const int xa = seq_of_token(a, l, g.s, (r0 + 128 * t) / a.G), xb = seq_of_token(a, l, g.s, (min(r0 + 128 * t + 128, g.rows) - 1) / a.G);
-      p.oa = g.pt + own_before<ROWS>(a, l, g, xa);
-      p.ob = g.pt + own_before<ROWS>(a, l, g, xb) + own_tiles<ROWS>(a, l, g.s, xb, g.q);
-      p.act = g.ta < g.tb && (g.ta < g.pt || max(g.ta, p.oa) < min(g.tb, p.ob));
-    }
-    return p;
+  const int nt = g.tb - g.ta;
+  auto part = [&](int t, int oa, int ob) {
+    if (ALT) return Seg::Part{g.pt, g.tiles, nt >= 2 || (nt == 1 && (g.ta & 1) == t)};
+    return Seg::Part{oa, ob, nt > 0 && r0 + 128 * t < g.rows && (g.ta < g.pt || max(g.ta, oa) < min(g.tb, ob))};
   };
-  g.m0 = part(0), g.m1 = part(1);
+  g.m0 = part(0, g.pt, ob0), g.m1 = part(1, oa1, g.tiles);
   return g;
 }
 // The first tile from j on that M tile t takes part in; tb where there is none.
@@ -205,9 +215,9 @@ __device__ __forceinline__ Cursor cursor_at(const Args& a, const Lists& l, const
   int lo = g.x0, hi = g.x1 + 1;  // the last sequence whose tiles begin at j or before
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (own_before<ROWS>(a, l, g, mid) <= j - g.pt) lo = mid; else hi = mid;
+    if (own_before(a, l, g.x0, g.t0, mid) <= j - g.pt) lo = mid; else hi = mid;
   }
-  return {lo, j - g.pt - own_before<ROWS>(a, l, g, lo), own_tiles<ROWS>(a, l, g.s, lo, g.q)};
+  return {lo, j - g.pt - own_before(a, l, g.x0, g.t0, lo), own_tiles<ROWS>(a, l, g.s, lo, g.q)};
 }
 template <int ROWS>
 __device__ __forceinline__ void advance(const Args& a, const Lists& l, const Seg& g, Cursor& c) {  // there is a next tile
@@ -227,8 +237,8 @@ struct Tile {
   float c, lvs, ivs, top;
 };
 
-// Warps 0-3, 4-7: softmax of M tile 0 / 1, thread = row; 8-11: codes -> operands; 12, 13: MMAs of M tile 0 / 1; 14: brings in codes and
-// scales, `raw` tiles ahead (with the converters' registers as the only stage, one tile ahead, 16 rows x 4 heads over 131,007 slots
+// Warps 0-3, 4-7: softmax of M tile 0 / 1, thread = row; 8-11: codes -> operands; 12, 13: MMAs of M tile 0 / 1; 15: works out the CTA's
+// shares of items, for all (each warp for itself took 6 us before the first tile); 14: brings in codes and scales, `raw` tiles ahead (with the converters' registers as the only stage, one tile ahead, 16 rows x 4 heads over 131,007 slots
 // took 131 us).
 template <int D, bool ALT>
 __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __grid_constant__ Args a) {
@@ -236,25 +246,27 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
   constexpr int ROWS = L::ROWS, ST = L::ST;
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ int scratch[THREADS / 32];
-  __shared__ Seg segs_of[2][15];                // by segment and warp: what a warp works on
+  __shared__ Seg segs[2];                       // shares of items, in turn; an empty one ends
+  __shared__ int2 row_at[2][256];               // of a thread's row: its sequence and token
   __shared__ Tile tiles[ST];
   __shared__ float2 raw_scale[MAX_RAW];         // K's and V's
   __shared__ int2 raw_at[MAX_RAW];              // x and key0
   __shared__ float2 halves[ALT ? 2 : 1][2][128];  // ALT: (m, l) of a row's two halves
-  __shared__ __align__(8) uint64_t bars[2 + 2 * ST + 4 + 4 + 4 + 2 + 2 + 1 + 2 * MAX_RAW];
+  __shared__ __align__(8) uint64_t bars[2 + 2 * ST + 4 + 4 + 4 + 2 + 2 + 1 + 2 * MAX_RAW + 4];
   __shared__ uint32_t tmem_slot;
   __shared__ int sh_abort;
   volatile int* abort_flag = &sh_abort;
   uint64_t *q_full = bars, *kv_full = bars + 2, *kv_empty = kv_full + ST;
   uint64_t *s_full = kv_empty + ST, *p_full = s_full + 4, *o_full = p_full + 4, *o_empty = o_full + 2, *pv_done = o_empty + 2, *drain = pv_done + 2, *halves_full = drain + 2;
-  uint64_t *raw_full = halves_full + 1, *raw_empty = raw_full + MAX_RAW;
+  uint64_t *raw_full = halves_full + 1, *raw_empty = raw_full + MAX_RAW, *seg_full = raw_empty + MAX_RAW, *seg_empty = seg_full + 2;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, B = a.S * a.F;
   int* lists = reinterpret_cast<int*>(sm + L::RAW + a.raw * L::RAW_TILE);
-  const Lists l{lists, lists + B + 1, lists + 2 * B + 1, lists + 3 * B + 2};
+  const Lists l{lists, lists + B + 1, lists + 2 * B + 1, lists + 3 * B + 2, lists + 3 * B + a.S + 3};
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
       mbar_init(&q_full[i], ALT ? 8 : 4);  // ALT: one q, which all eight warps bring in
       mbar_init(&o_full[i], 1), mbar_init(&o_empty[i], ALT ? 8 : 4), mbar_init(&pv_done[i], 1), mbar_init(&drain[i], 1);
+      mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 15);
     }
     for (int i = 0; i < ST; i++) mbar_init(&kv_full[i], 4), mbar_init(&kv_empty[i], 2);
     for (int i = 0; i < 4; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4);
@@ -274,34 +286,24 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
   griddep_wait();  // programmatic dependent launch: the previous kernel has completed
   griddep_launch();
   make_lists<ROWS>(a, l, scratch);
-  int u_begin = 0, u_end, run = 1;  // this CTA's run of tiles
-  if (a.items > 0) {
-    u_end = segment<D, ALT>(a, l, 0, 0, tid == 0).tiles;
-  } else {
-    const int total = l.pre[a.S];
-    run = max((total + a.ctas - 1) / a.ctas, 1);
-    u_begin = (int)min((long long)blockIdx.x * run, (long long)total);
-    u_end = (int)min((long long)u_begin + run, (long long)total);
-  }
+  const int run = a.items > 0 ? 1 : max((l.pre[a.S] + a.ctas - 1) / a.ctas, 1);
   // a wait of the whole warp: every lane gives up when one does
   auto wait = [&](uint64_t* bar, int parity) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, ST_KV8_WAIT)) != 0;
   };
 
-  // this warp's share of the next item, in shared memory: it is looked at often and would take registers
-  auto next_segment = [&](int i, int u) -> const Seg& {
-    const Seg g = segment<D, ALT>(a, l, u, u_end, false);
+  // the i'th share: for the warps that work on it
+  auto take = [&](int i) { return wait(&seg_full[i & 1], (i >> 1) & 1); };
+  auto leave = [&](int i) {
     __syncwarp();
-    if (lane == 0) segs_of[i & 1][warp] = g;
-    __syncwarp();
-    return segs_of[i & 1][warp];
+    mbar_arrive_if(&seg_empty[i & 1], lane == 0);
   };
 
   static_assert(2 * tc::SOFTMAX_REGS + tc::CONVERT_REGS + tc::MMA_REGS <= 4 * 128, "the split must come out of the launch's registers");
   if (warp >= 12) {
     set_regs_down<tc::MMA_REGS>();
     // ---------------- MMA issuer of M tile t, one warp each.  The whole warp walks the loop, one lane issues
-    const int t = warp - 12, end = t < 2 ? u_end : u_begin;  // warp 15 is idle
+    const int t = warp - 12;
     const uint32_t leader = elect_one();
     constexpr uint32_t IDESC_S = idesc_bf16(128, KEYS), IDESC_O = idesc_f16(128, D) | (1u << 16);  // V MN-major
     const uint64_t dq = sdesc_noswz(smem_u32(sm) + (ALT ? 0 : t * L::QT), 2048, 128), dk = sdesc_noswz(smem_u32(sm + L::K), 1024, 128);
@@ -309,10 +311,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
     const uint32_t t_s = tmem + 128 * t, t_o = tmem + 256 + 128 * t;
     bool ok = true;
     int base = 0, js = 0, so = 0, sq = 0;  // tiles of the segments before; tiles and segments that t took part in; q's that came in
-    for (int u = u_begin, i = 0; u < end && ok; i++) {
-      const Seg& g = next_segment(i, u);
+    for (int i = 0; t < 2 && ok; i++) {
+      ok = take(i);
+      const Seg& g = segs[i & 1];
       const int nt = g.tb - g.ta;
-      u += nt;
+      if (!ok || nt == 0) break;
       auto stage = [&](int j) { return (base + j - g.ta) % ST; };
       auto phase = [&](int j) { return ((base + j - g.ta) / ST) & 1; };
       auto pass = [&](int j, int to) {  // tiles [j, to) are the other M tile's: only the barriers
@@ -369,6 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
       }
       sq += q_here ? 1 : 0;
       base += nt;
+      leave(i);
     }
     if (leader && t < 2) {
       umma_commit(&drain[t]);
@@ -377,10 +381,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
     if (warp == 14) {
       // ---------------- codes and scales of every tile, in order, as far ahead as there is room
       int j = 0;
-      for (int u = u_begin, i = 0; u < u_end && ok; i++) {
-        const Seg& g = next_segment(i, u);
+      for (int i = 0; ok; i++) {
+        ok = take(i);
+        const Seg& g = segs[i & 1];
         const int nt = g.tb - g.ta;
-        u += nt;
+        if (!ok || nt == 0) break;
         Cursor c = cursor_at<ROWS>(a, l, g, g.ta);
         for (int k = 0; k < nt; k++, j++) {
           const int st = j % a.raw;
@@ -401,9 +406,28 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
           __syncwarp();
           if (k + 1 < nt) advance<ROWS>(a, l, g, c);
         }
+        leave(i);
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       for (int k = max(j - a.raw, 0); k < j; k++) mbar_wait_drain(&raw_full[k % a.raw], (k / a.raw) & 1, kDrainCycles);  // copies in flight land, whatever the others do
+    }
+    if (warp == 15) {
+      // ---------------- the shares
+      const int total = a.items > 0 ? 1 : l.pre[a.S], u_begin = a.items > 0 ? 0 : (int)min((long long)blockIdx.x * run, (long long)total);
+      const int u_end = (int)min((long long)u_begin + run, (long long)total);
+      for (int u = u_begin, i = 0; ok; i++) {
+        Seg g;
+        g.ta = g.tb = 0;
+        if (u < u_end) g = segment<D, ALT>(a, l, u, u_end);
+        ok = i < 2 || wait(&seg_empty[i & 1], ((i >> 1) - 1) & 1);
+        if (!ok) break;
+        const int nt = g.tb - g.ta;
+        if (lane == 0) segs[i & 1] = g;
+        __syncwarp();
+        mbar_arrive_if(&seg_full[i & 1], lane == 0);
+        if (nt == 0) break;
+        u = a.items > 0 ? u_end : u + nt;
+      }
     }
   } else if (warp >= 8) {
     set_regs_down<tc::CONVERT_REGS>();
@@ -412,7 +436,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
     constexpr int PER = D / 32, PIECES = D / 16;  // pieces of a K or V block that a lane takes, of a row
     const int w = warp - 8;
     bool ok = true;
-    for (int j = 0; j < u_end - u_begin; j++) {
+    for (int j = 0, i = -1, left = 0; ok; j++, left--) {
+      if (left == 0) {
+        if (i >= 0) leave(i);
+        ok = take(++i);
+        left = segs[i & 1].tb - segs[i & 1].ta;
+        if (!ok || left == 0) break;
+      }
       const int st = j % ST, rs = j % a.raw;
       ok = wait(&raw_full[rs], (j / a.raw) & 1) && (j < ST || wait(&kv_empty[st], (j / ST - 1) & 1));
       if (!ok) break;
@@ -455,38 +485,37 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
     const int t = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, t_o = tmem + 256 + 128 * t + lanes;
     bool ok = true;
-    int base = 0, js = 0, so = 0, so1 = 0, segs = 0;  // tiles of the segments before; tiles that t took part in; outputs stored (ALT: of M tile 0 and 1); segments
+    int base = 0, js = 0, so = 0, so1 = 0, segs_done = 0;  // tiles of the shares before; tiles that t took part in; outputs stored (ALT: of M tile 0 and 1); shares
+    int known = -1;  // the last tile whose scores were seen: every one up to it was in place
     int4 open = make_int4(-1, 0, 0, 0);
-    auto row_of = [&](const Seg& g) { return g.q * ROWS + (ALT ? 0 : 128 * t) + (warp & 3) * 32 + lane; };
-    auto load_q = [&](const Seg& g) {  // every product with the q before it is done: its last scores have been read
+    const int mine_r = (ALT ? 0 : 128 * t) + (warp & 3) * 32 + lane, me = 128 * t + (warp & 3) * 32 + lane;  // this thread's row of an item
+    auto load_q = [&](int i) {  // of the i'th share; every product with the q before it is done: its last scores have been read
+      const Seg& g = segs[i & 1];
+      const int row = min(g.q * ROWS + mine_r, g.rows - 1);  // rows past the last are copies of it
+      const int x = seq_of_token(a, l, g.s, row / a.G), token = row / a.G - (l.tok[x] - l.tok[g.s * a.F]);
+      row_at[i & 1][me] = make_int2(x, token);
       if (!ALT && !g.of(t).act) return;
-      const int row = min(row_of(g), g.rows - 1);  // rows past the last are copies of it
-      const int x = seq_of_token(a, l, g.s, row / a.G), i = row / a.G - (l.tok[x] - l.tok[g.s * a.F]);
-      const uint16_t* src = a.q + x * a.sq_b + i * a.sq_t + (size_t)(g.h * a.G + row % a.G) * a.sq_h;
-      uint8_t* dst = sm + (ALT ? 0 : t * L::QT) + ((warp & 3) * 32 + lane) * 16;
+      const uint16_t* src = a.q + x * a.sq_b + token * a.sq_t + (size_t)(g.h * a.G + row % a.G) * a.sq_h;
+      const uint32_t dst = smem_u32(sm + (ALT ? 0 : t * L::QT) + ((warp & 3) * 32 + lane) * 16);
       constexpr int CH = ALT ? D / 16 : D / 8;  // 16-byte pieces of this thread
       const int from = ALT ? t * CH : 0;
 #pragma unroll
-      for (int c0 = 0; c0 < CH; c0 += 4) {
-        uint4 v[4];
-#pragma unroll
-        for (int c = 0; c < 4; c++) v[c] = *reinterpret_cast<const uint4*>(src + 8 * (from + c0 + c));
-#pragma unroll
-        for (int c = 0; c < 4; c++) *reinterpret_cast<uint4*>(dst + (from + c0 + c) * 2048) = v[c];
-      }
+      for (int c = 0; c < CH; c++)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (from + c) * 2048), "l"(src + 8 * (from + c)) : "memory");
+      asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async_smem();
       __syncwarp();
       mbar_arrive_if(&q_full[ALT ? 0 : t], lane == 0);
     };
-    if (u_begin < u_end) load_q(next_segment(0, u_begin));
-    for (int u = u_begin; u < u_end && ok; segs++) {
-      const Seg& g = segs_of[segs & 1][warp];
-      const int nt = g.tb - g.ta, row = row_of(g), valid = g.rows;
-      const bool first_of_run = u == u_begin, whole = g.ta == 0 && g.tb == g.tiles;
-      const int u0 = u;
-      u += nt;
-      const int rr = min(row, valid - 1), rx = seq_of_token(a, l, g.s, rr / a.G), ri = rr / a.G - (l.tok[rx] - l.tok[g.s * a.F]);
-      const int own_lim = l.len[rx] + ri + 1;
+    ok = take(0);
+    if (ok && segs[0].tb > segs[0].ta) load_q(0);
+    for (; ok; segs_done++) {
+      const Seg& g = segs[segs_done & 1];
+      const int nt = g.tb - g.ta, row = g.q * ROWS + mine_r, valid = g.rows;
+      if (nt == 0) break;
+      const bool whole = g.ta == 0 && g.tb == g.tiles;
+      const int2 rat = row_at[segs_done & 1][me];
+      const int rx = rat.x, ri = rat.y, own_lim = l.len[rx] + ri + 1;
       const int warp_x0 = __shfl_sync(0xffffffffu, rx, 0), warp_x1 = __shfl_sync(0xffffffffu, rx, 31);
       float m = -INFINITY, sum_l = 0.f;
       if (g.of(t).act) {
@@ -502,11 +531,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
           const int f = js & 1, at = base + j - g.ta;
           const uint32_t t_s = tmem + 128 * t + 64 * f + lanes;
           uint32_t r0[32], r1[32];
-          // the scores, and with them the tile: its operands' phase (before the scores are there, it might be an earlier one's)
-          ok = wait(&s_full[2 * t + f], (js >> 1) & 1) && wait(&kv_full[at % ST], (at / ST) & 1);
+          // what the tile is, before its scores are there; where others lie between, with them: only then is the stage's phase surely its own
+          const bool near = at - known < ST;
+          ok = (near || wait(&s_full[2 * t + f], (js >> 1) & 1)) && wait(&kv_full[at % ST], (at / ST) & 1);
           if (!ok) break;
-          tc_fence_after();
-          tmem_ld32(t_s, r0);
+          known = at;
           const int x = tiles[at % ST].x, key0 = tiles[at % ST].key0;
           float c = tiles[at % ST].c, lvs = tiles[at % ST].lvs, ivs = tiles[at % ST].ivs;
           const float top = tiles[at % ST].top;
@@ -540,6 +569,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
             f2_unpack(f2_add(sum2[0], sum2[1]), lo, hi);
             return lo + hi;
           };
+          ok = !near || wait(&s_full[2 * t + f], (js >> 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          tmem_ld32(t_s, r0);
           if (!mine) {  // no row of the warp: P is zero
             uint32_t zero[16];
 #pragma unroll
@@ -629,20 +662,27 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
         if (!ok) break;
       }
       base += nt;
-      const Seg& done = g;
-      if (!ALT && u < u_end) load_q(next_segment(segs + 1, u));  // the next item's products start before this one's O is stored
-      const int r = row - done.q * ROWS;
-      const size_t slot = (2 * (size_t)blockIdx.x + (first_of_run ? 0 : 1)) * ROWS + r;
-      const int hq = done.h * a.G + rr % a.G;
+      // the next item's products start before this one's O is stored (ALT: both M tiles' scores must have been read)
+      auto load_next = [&] {
+        ok = take(segs_done + 1);
+        if (ok && segs[(segs_done + 1) & 1].tb > segs[(segs_done + 1) & 1].ta) load_q(segs_done + 1);
+        return ok;
+      };
+      if (!ALT && !load_next()) break;
+      const size_t slot = 2 * (size_t)blockIdx.x + (segs_done ? 1 : 0);
+      const int hq = g.h * a.G + min(row, valid - 1) % a.G;
       const size_t out_row = ((size_t)rx * a.n + ri) * (a.G * a.H) + hq;
       uint16_t* op = a.out + rx * a.so_b + ri * a.so_t + hq * a.so_h;
-      if (done.ta == 0 && !whole) open = make_int4((u0 + done.tiles - 1) / run, 2 * blockIdx.x + (first_of_run ? 0 : 1), done.h, done.q * ROWS);
-      if (done.ta == 0 && !whole && (!ALT || t == 0)) a.row_at[(size_t)blockIdx.x * ROWS + r] = row < valid ? rx * a.n + ri : -1;
-      // dims y16 .. y16 + 15 of the row, o = O / l where it is whole
+      if (g.ta == 0 && !whole) {
+        open = make_int4((g.u + g.tiles - 1) / run, (int)slot, g.h, g.q * ROWS);
+        if (!ALT || t == 0) a.row_at[(size_t)blockIdx.x * ROWS + mine_r] = row < valid ? rx * a.n + ri : -1;
+      }
+      // dims y16 .. y16 + 15 of the row, o = O / l where it is whole.  Parts lie as [dims / 4][row][4]: a warp writes whole lines
       auto put = [&](int y16, const float (&o)[16]) {
         if (!whole) {
 #pragma unroll
-          for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(a.part_o + slot * D + y16 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<float4*>(a.part_o + ((slot * (D / 4) + (y16 + e) / 4) * ROWS + mine_r) * 4) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         } else if (!a.own) {
 #pragma unroll
           for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(a.row_o + out_row * D + y16 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
@@ -653,20 +693,20 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
         }
       };
       auto put_ml = [&](float mm, float ll) {
-        if (!whole) a.part_ml[slot] = make_float2(mm, ll);
+        if (!whole) a.part_ml[slot * ROWS + mine_r] = make_float2(mm, ll);
         else if (!a.own) a.row_ml[out_row] = make_float2(mm, ll / L_SCALE);
       };
       if (ALT) {
-        float2(&hv)[2][128] = halves[segs & 1];
-        hv[t][r] = make_float2(m, sum_l);
+        float2(&hv)[2][128] = halves[segs_done & 1];
+        hv[t][mine_r] = make_float2(m, sum_l);
         __syncwarp();
         mbar_arrive_if(halves_full, lane == 0);
-        ok = wait(halves_full, segs & 1);
-        ok = ok && (!done.m0.act || wait(&o_full[0], so & 1)) && (!done.m1.act || wait(&o_full[1], so1 & 1));
+        ok = wait(halves_full, segs_done & 1);
+        ok = ok && (!g.m0.act || wait(&o_full[0], so & 1)) && (!g.m1.act || wait(&o_full[1], so1 & 1));
         if (!ok) break;
         tc_fence_after();
-        if (u < u_end) load_q(next_segment(segs + 1, u));  // both M tiles' scores have been read
-        const float2 h0 = hv[0][r], h1 = hv[1][r];
+        if (!load_next()) break;
+        const float2 h0 = hv[0][mine_r], h1 = hv[1][mine_r];
         const float mm = fmaxf(h0.x, h1.x);
         auto weigh = [&](const float2& h, float& w) {  // factor of O; l's is the same, by halves
           const float half = h.x == -INFINITY ? 0.f : ex2_approx(0.5f * (h.x - mm));
@@ -680,21 +720,21 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
         for (int y = 0; y < D / 32; y++) {  // this thread's half of the dims
           const int y16 = 16 * (t * (D / 32) + y);
           uint32_t a0[16], a1[16];
-          if (done.m0.act) tmem_ld16(tmem + 256 + lanes + y16, a0);
-          if (done.m1.act) tmem_ld16(tmem + 384 + lanes + y16, a1);
+          if (g.m0.act) tmem_ld16(tmem + 256 + lanes + y16, a0);
+          if (g.m1.act) tmem_ld16(tmem + 384 + lanes + y16, a1);
           tmem_ld_wait();
           float o[16];
 #pragma unroll
-          for (int e = 0; e < 16; e++) o[e] = (done.m0.act ? __uint_as_float(a0[e]) * w0 : 0.f) + (done.m1.act ? __uint_as_float(a1[e]) * w1 : 0.f);
+          for (int e = 0; e < 16; e++) o[e] = (g.m0.act ? __uint_as_float(a0[e]) * w0 : 0.f) + (g.m1.act ? __uint_as_float(a1[e]) * w1 : 0.f);
           if (row < valid) put(y16, o);
         }
         if (t == 0 && row < valid) put_ml(mm, ll);
         tc_fence_before();
         __syncwarp();
-        if (done.m0.act) mbar_arrive_if(&o_empty[0], lane == 0), so++;
-        if (done.m1.act) mbar_arrive_if(&o_empty[1], lane == 0), so1++;
-      } else if (!done.of(t).act) {
-        if (row < valid && !whole) a.part_ml[slot] = make_float2(-INFINITY, 0.f);
+        if (g.m0.act) mbar_arrive_if(&o_empty[0], lane == 0), so++;
+        if (g.m1.act) mbar_arrive_if(&o_empty[1], lane == 0), so1++;
+      } else if (!g.of(t).act) {
+        if (row < valid && !whole) a.part_ml[slot * ROWS + mine_r] = make_float2(-INFINITY, 0.f);
       } else {
         ok = wait(&o_full[t], so & 1);
         if (!ok) break;
@@ -716,6 +756,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
         mbar_arrive_if(&o_empty[t], lane == 0);
         so++;
       }
+      leave(segs_done);
     }
     if (a.items == 0 && tid == 0) a.unfinished[blockIdx.x] = open;
   }
@@ -728,58 +769,48 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
   }
 }
 
-// Merges the parts of an item, always in the same order.  blockIdx.x = c: the item that CTA c began and did not finish; blockIdx.y: two of its
-// rows, 64 threads each: thread = 4 dims, of every 256 / D'th part.
+// Merges the parts of an item, always in the same order.  blockIdx.x = c: the item that CTA c began and did not finish; blockIdx.y: eight of
+// its rows; thread = a row's dims 4 (thread / 8) .. and, where heads are 128 wide, those 64 on.
 template <int D, int ROWS>
 __global__ void __launch_bounds__(128) attn_kv8_shared_join_kernel(const __grid_constant__ Args a) {
-  constexpr int SHARE = 256 / D;
-  __shared__ __align__(16) float4 sh_o[128];
+  __shared__ float2 sh_ml[MAX_CTAS][8];
   griddep_wait();
   griddep_launch();
   const int4 open = a.unfinished[blockIdx.x];
   if (open.x < 0) return;
-  const int c0 = blockIdx.x, c1 = open.x, lane = threadIdx.x & 31, x = threadIdx.x & 63, share = x / (D / 4), d = x % (D / 4) * 4;
-  const int r = blockIdx.y * 2 + threadIdx.x / 64, at = a.row_at[(size_t)c0 * ROWS + r];
-  auto part = [&](int c) { return (size_t)(c == c0 ? open.y : 2 * c) * ROWS + r; };
-  float mx = -INFINITY, sum = 0.f;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (at >= 0) {  // whole warps: a row's threads are two of them
-    for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, a.part_ml[part(c)].x);
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-    for (int c = c0 + lane; c <= c1; c += 32) {
-      const float2 ml = a.part_ml[part(c)];
-      const float half = ml.x == -INFINITY ? 0.f : ex2_approx(0.5f * (ml.x - mx));
-      sum += ml.y * half * half;
-    }
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-#pragma unroll 4
-    for (int c = c0 + share; c <= c1; c += SHARE) {
-      const float m = a.part_ml[part(c)].x;
-      const float4 o = *reinterpret_cast<const float4*>(a.part_o + part(c) * D + d);
-      const float half = ex2_approx(0.5f * (m - mx)), f = half * half;
-      if (m != -INFINITY) v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;  // else its M tile took part in nothing, or all scores were NaN
-    }
-  }
-  sh_o[threadIdx.x] = v;
+  const int c0 = blockIdx.x, parts = open.x - c0 + 1, r = threadIdx.x & 7, row = blockIdx.y * 8 + r;
+  const int at = a.row_at[(size_t)c0 * ROWS + row];
+  auto slot = [&](int p) { return (size_t)(p == 0 ? open.y : 2 * (c0 + p)); };
+  for (int p = threadIdx.x >> 3; p < parts; p += 16) sh_ml[p][r] = at < 0 ? make_float2(0.f, 1.f) : a.part_ml[slot(p) * ROWS + row];
   __syncthreads();
-  if (at < 0 || share) return;
+  if (at < 0) return;
+  float mx = -INFINITY, sum = 0.f;
+  for (int p = 0; p < parts; p++) mx = fmaxf(mx, sh_ml[p][r].x);
+  float4 v[D / 64];
 #pragma unroll
-  for (int k = 1; k < SHARE; k++) {
-    const float4 o = sh_o[threadIdx.x + k * (D / 4)];
-    v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+  for (int y = 0; y < D / 64; y++) v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int chunk = threadIdx.x >> 3;
+#pragma unroll 4
+  for (int p = 0; p < parts; p++) {
+    const float2 ml = sh_ml[p][r];
+    const float half = ml.x == -INFINITY ? 0.f : ex2_approx(0.5f * (ml.x - mx)), f = half * half;
+    sum += ml.y * half * half;
+#pragma unroll
+    for (int y = 0; y < D / 64; y++) {
+      const float4 o = *reinterpret_cast<const float4*>(a.part_o + ((slot(p) * (D / 4) + chunk + 16 * y) * ROWS + row) * 4);
+      if (ml.x != -INFINITY) v[y].x += o.x * f, v[y].y += o.y * f, v[y].z += o.z * f, v[y].w += o.w * f;  // else the part is empty, or all its scores were NaN
+    }
   }
   const float inv = L_SCALE / sum;
-  const int hq = open.z * a.G + (open.w + r) % a.G, b = at / a.n, i = at % a.n;
-  if (a.own) {
-    uint16_t* op = a.out + b * a.so_b + i * a.so_t + hq * a.so_h + d;
-    *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
-  } else {
-    const size_t out_row = (size_t)at * (a.G * a.H) + hq;
-    *reinterpret_cast<float4*>(a.row_o + out_row * D + d) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-    if (d == 0) a.row_ml[out_row] = make_float2(mx, sum / L_SCALE);
+  const int hq = open.z * a.G + (open.w + row) % a.G, b = at / a.n, i = at % a.n;
+  const size_t out_row = (size_t)at * (a.G * a.H) + hq;
+#pragma unroll
+  for (int y = 0; y < D / 64; y++) {
+    const int d = 4 * chunk + 64 * y;
+    if (a.own) *reinterpret_cast<uint2*>(a.out + b * a.so_b + i * a.so_t + hq * a.so_h + d) = make_uint2(pack_bf2(v[y].x * inv, v[y].y * inv), pack_bf2(v[y].z * inv, v[y].w * inv));
+    else *reinterpret_cast<float4*>(a.row_o + out_row * D + d) = make_float4(v[y].x * inv, v[y].y * inv, v[y].z * inv, v[y].w * inv);
   }
+  if (!a.own && chunk == 0) a.row_ml[out_row] = make_float2(mx, sum / L_SCALE);
 }
 
 template <int D, bool ALT>
@@ -788,10 +819,10 @@ static int launch(cudaStream_t st, Args a, const char* what) {
   const int rc = smem_attr_once((const void*)attn_kv8_shared_tc_kernel<D, ALT>, L::BUDGET, what);
   if (rc) return rc;
   const int lists = list_bytes(a.S, a.S * a.F), room = (L::BUDGET - L::RAW - lists) / L::RAW_TILE;
-  static_assert((L::BUDGET - L::RAW - (4 * MAXB + 3) * 4) / L::RAW_TILE >= 1, "codes in flight beside the longest lists");
+  static_assert((L::BUDGET - L::RAW - (5 * MAXB + 3) * 4) / L::RAW_TILE >= 1, "codes in flight beside the longest lists");
   a.raw = room < MAX_RAW ? room : MAX_RAW;
   launch_k(attn_kv8_shared_tc_kernel<D, ALT>, (unsigned)(a.items > 0 ? a.S * a.H * a.items : a.ctas), THREADS, L::RAW + a.raw * L::RAW_TILE + lists, st, a);
-  if (a.items == 0) launch_k(attn_kv8_shared_join_kernel<D, L::ROWS>, dim3(a.ctas, L::ROWS / 2), 128, 0, st, a);
+  if (a.items == 0) launch_k(attn_kv8_shared_join_kernel<D, L::ROWS>, dim3(a.ctas, L::ROWS / 8), 128, 0, st, a);
   return check_launch(what);
 }
 
@@ -822,15 +853,15 @@ static Plan make_plan(int S, int B, int n, int Hq, int H, int D, int Cp, int C, 
   }
   x.alt = all <= 128;
   const int rows = x.alt ? 128 : 256;
-  x.items = (int)((all + rows - 1) / rows), x.ctas = sms;
+  x.items = (int)((all + rows - 1) / rows), x.ctas = sms < MAX_CTAS ? sms : MAX_CTAS;
   // sequences with rows in an item, and their tiles
   const long long seqs = (long long)n * G >= rows ? 2 : rows / ((long long)n * G) + 2, own = (seqs < F ? seqs : F) * (C / BLK);
   x.own = (long long)n * G > split::FEW_ROWS || own <= OWN_TILES || own <= Cp / BLK / 2;
   x.whole = Cp / BLK + (x.own ? own : 0) <= WHOLE_TILES;
-  x.ml_off = x.whole ? 0 : up(2LL * sms * rows * D * 4);
-  x.un_off = x.ml_off + (x.whole ? 0 : up(2LL * sms * rows * 8));
-  x.at_off = x.un_off + (x.whole ? 0 : up(sms * 16LL));
-  x.row_off = x.at_off + (x.whole ? 0 : up((long long)sms * rows * 4));
+  x.ml_off = x.whole ? 0 : up(2LL * x.ctas * rows * D * 4);
+  x.un_off = x.ml_off + (x.whole ? 0 : up(2LL * x.ctas * rows * 8));
+  x.at_off = x.un_off + (x.whole ? 0 : up(x.ctas * 16LL));
+  x.row_off = x.at_off + (x.whole ? 0 : up((long long)x.ctas * rows * 4));
   x.rml_off = x.row_off + (x.own ? 0 : up((long long)B * n * Hq * D * 4));
   x.s_off = x.bytes = x.rml_off + (x.own ? 0 : up((long long)B * n * Hq * 8));
   if (!x.own) x.s = split::make_plan(B, n, Hq, H, D, C, false, sms), x.bytes += x.s.full_off;
