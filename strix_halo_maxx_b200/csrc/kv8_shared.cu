@@ -92,6 +92,7 @@ __device__ __forceinline__ int own_tiles(const Args& a, const Lists& l, int s, i
 template <int ROWS>
 __device__ __forceinline__ void make_lists(const Args& a, const Lists& l, int* scratch) {
   const bool record = blockIdx.x == 0;
+  for (int s = threadIdx.x; s < a.S; s += blockDim.x) l.plen[s] = split::prefix_len(a.plens, s, a.Cp, record);
   split::sums_before(l.tok, a.S * a.F, scratch, [&](int b) {
     const Seq q = seq_of(a.lens, a.counts, b, a.n, a.C, record);
     l.len[b] = q.len;
@@ -106,7 +107,7 @@ __device__ __forceinline__ void make_lists(const Args& a, const Lists& l, int* s
       return t;
     });
   split::sums_before(l.pre, a.S, scratch, [&](int s) {
-    const int P = l.plen[s] = split::prefix_len(a.plens, s, a.Cp, record), rows = (l.tok[(s + 1) * a.F] - l.tok[s * a.F]) * a.G;
+    const int P = l.plen[s], rows = (l.tok[(s + 1) * a.F] - l.tok[s * a.F]) * a.G;
     return ((rows + ROWS - 1) / ROWS * ((P + KEYS - 1) / KEYS) + (a.own ? l.own[(s + 1) * a.F] - l.own[s * a.F] : 0)) * a.H;
   });
 }
@@ -495,13 +496,18 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
       const int x = seq_of_token(a, l, g.s, row / a.G), token = row / a.G - (l.tok[x] - l.tok[g.s * a.F]);
       row_at[i & 1][me] = make_int2(x, token);
       if (!ALT && !g.of(t).act) return;
-      const uint16_t* src = a.q + x * a.sq_b + token * a.sq_t + (size_t)(g.h * a.G + row % a.G) * a.sq_h;
-      const uint32_t dst = smem_u32(sm + (ALT ? 0 : t * L::QT) + ((warp & 3) * 32 + lane) * 16);
-      constexpr int CH = ALT ? D / 16 : D / 8;  // 16-byte pieces of this thread
-      const int from = ALT ? t * CH : 0;
+      const uint16_t* mine = a.q + x * a.sq_b + token * a.sq_t + (size_t)(g.h * a.G + row % a.G) * a.sq_h;
+      const uint32_t dst = smem_u32(sm + (ALT ? 0 : t * L::QT) + (warp & 3) * 32 * 16);
+      // four lanes bring 64 bytes of a row, whole sectors, eight rows at a time (a lane a row took 4 us); rows side by side in a bank line
+      constexpr int CH = ALT ? D / 16 : D / 8;  // 16-byte pieces of this M tile's threads
+      const int piece = (ALT ? t * CH : 0) + (lane >> 3);
 #pragma unroll
-      for (int c = 0; c < CH; c++)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (from + c) * 2048), "l"(src + 8 * (from + c)) : "memory");
+      for (int rg = 0; rg < 32; rg += 8) {
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), rg + (lane & 7)));
+#pragma unroll
+        for (int c = 0; c < CH; c += 4)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (piece + c) * 2048 + (rg + (lane & 7)) * 16), "l"(src + 8 * (piece + c)) : "memory");
+      }
       asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async_smem();
       __syncwarp();
@@ -832,7 +838,7 @@ struct Plan {
   bool whole;          // a CTA for each item of it
   int items, ctas;
   split::Plan s;       // of few, or of the sequences' own slots
-  long long o_off, ml_off, un_off, at_off, row_off, rml_off, s_off, bytes;  // workspace
+  long long o_off, ml_off, un_off, at_off, row_off, rml_off, s_off, sun_off, bytes;  // workspace
 };
 // Rows up to which one kernel takes all; tiles up to which a CTA takes a whole item (MEASURED); tiles of own slots (times two, beside
 // the prefix's) up to which the tcgen05 kernel takes them (MEASURED)
@@ -847,8 +853,9 @@ static Plan make_plan(int S, int B, int n, int Hq, int H, int D, int Cp, int C, 
   x.few = all <= few_rows(D);
   if (x.few) {
     const int kt = split::keys_per_tile(D);
-    x.s = split::make_plan(S, F * n, Hq, H, D, Cp, false, sms, Cp / kt + (long long)F * (C / kt), FEW_TILES);
-    x.bytes = x.s.full_off;
+    x.s = split::make_plan(S, F * n, Hq, H, D, Cp, false, sms, Cp / kt + (long long)F * (C / kt), 2LL * S * H >= sms ? 4 * FEW_TILES : FEW_TILES);
+    x.sun_off = x.s.full_off;
+    x.bytes = x.sun_off + (x.s.whole ? 0 : up(x.s.ctas * 16LL));
     return x;
   }
   x.alt = all <= 128;
@@ -857,14 +864,15 @@ static Plan make_plan(int S, int B, int n, int Hq, int H, int D, int Cp, int C, 
   // sequences with rows in an item, and their tiles
   const long long seqs = (long long)n * G >= rows ? 2 : rows / ((long long)n * G) + 2, own = (seqs < F ? seqs : F) * (C / BLK);
   x.own = (long long)n * G > split::FEW_ROWS || own <= OWN_TILES || own <= Cp / BLK / 2;
-  x.whole = Cp / BLK + (x.own ? own : 0) <= WHOLE_TILES;
+  const long long tiles = Cp / BLK + (x.own ? own : 0);
+  x.whole = tiles <= WHOLE_TILES || (tiles <= 4 * WHOLE_TILES && 2LL * S * H * x.items >= sms);
   x.ml_off = x.whole ? 0 : up(2LL * x.ctas * rows * D * 4);
   x.un_off = x.ml_off + (x.whole ? 0 : up(2LL * x.ctas * rows * 8));
   x.at_off = x.un_off + (x.whole ? 0 : up(x.ctas * 16LL));
   x.row_off = x.at_off + (x.whole ? 0 : up((long long)x.ctas * rows * 4));
   x.rml_off = x.row_off + (x.own ? 0 : up((long long)B * n * Hq * D * 4));
   x.s_off = x.bytes = x.rml_off + (x.own ? 0 : up((long long)B * n * Hq * 8));
-  if (!x.own) x.s = split::make_plan(B, n, Hq, H, D, C, false, sms), x.bytes += x.s.full_off;
+  if (!x.own) x.s = split::make_plan(B, n, Hq, H, D, C, false, sms), x.sun_off = x.s_off + x.s.full_off, x.bytes = x.sun_off + (x.s.whole ? 0 : up(x.s.ctas * 16LL));
   return x;
 }
 
@@ -919,7 +927,7 @@ int vt_attn_kv8_shared(cudaStream_t st, const uint16_t* q, long long sq_b, long 
   const float c = scale * kv8::LOG2E;
   kv8::split::Args sa{q, sq_b, sq_t, sq_h, kc, vc, ks, vs, lens, counts, x.few ? S : B, n, G, H, C, 1, x.few ? F * n * G : n * G, x.few ? 1 : x.s.rg, x.s.ctas, c,
                       out, so_b, so_t, so_h, (float*)(w8 + x.s_off + x.s.o_off), (float2*)(w8 + x.s_off + x.s.ml_off), nullptr, nullptr, nullptr, nullptr,
-                      pk, pv, pks, pvs, plens, Cp, F, (const float*)(w8 + x.row_off), (const float2*)(w8 + x.rml_off)};
+                      pk, pv, pks, pvs, plens, Cp, F, (const float*)(w8 + x.row_off), (const float2*)(w8 + x.rml_off), (int4*)(w8 + x.sun_off)};
   if (x.few) return kv8::split::launch_any<kv8::split::SHARED>(st, sa, D, x.s.nt, x.s.whole, what);
   const kv8::shared::Args a{q, sq_b, sq_t, sq_h, pk, pv, pks, pvs, Cp, S, F, plens, kc, vc, ks, vs, C, lens, counts, n, G, H, x.ctas,
                             x.whole ? x.items : 0, x.own, 0, c, out, so_b, so_t, so_h, (float*)(w8 + x.row_off), (float2*)(w8 + x.rml_off), (float*)w8,

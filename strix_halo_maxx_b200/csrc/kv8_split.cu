@@ -106,6 +106,7 @@ struct Args {
   int Cp, F;
   const float* row_o;  // OWN: [B][n][Hq][D] and [B][n][Hq], of prefixes that are not empty
   const float2* row_ml;
+  int4* unfinished;  // SHARED, OWN: [ctas] the item that a CTA begins and others go on with: last CTA (-1: none), slot of the first part, b, h rg + row group
 };
 
 // OWN: what row (b, i, hq) has of the prefix, joined to (mx, sum, v): dims d .. of its own slots, 2^15 too small as the kernel holds them.
@@ -238,13 +239,14 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
   griddep_wait();  // programmatic dependent launch: the previous kernel has completed
   griddep_launch();
   long long u_begin = 0;
-  int total = 1, u_end = 1;  // this CTA's run of tiles (a whole item: one round)
+  int total = 1, u_end = 1, run = 1;  // this CTA's run of tiles (a whole item: one round)
+  int4 open = make_int4(-1, 0, 0, 0);
   if (WHOLE) {
     __syncthreads();
   } else {
     tile_list<MODE>(a, KT, GR, pre, warp_sum, own);  // its barriers also publish the mbarriers
     total = pre[a.B];
-    const int run = run_of(total, a.ctas);
+    run = run_of(total, a.ctas);
     u_begin = (long long)blockIdx.x * run;
     u_end = (int)min(u_begin + run, (long long)total);
   }
@@ -554,6 +556,9 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
       }
     __syncthreads();
     const bool whole = WHOLE || (ta == 0 && tb == tiles);
+    if constexpr (MODE != PLAIN && !WHOLE) {
+      if (ta == 0 && !whole) open = make_int4((u + tiles - 1) / run, 2 * blockIdx.x + (u == u_begin ? 0 : 1), b, h * a.rg + rg);
+    }
     const int slot = 2 * blockIdx.x + (u == u_begin ? 0 : 1);  // of a part; a run has two at most: its first and its last
     for (int e = tid; e < GR * D / 4; e += WARPS * 32) {
       const int r = e / (D / 4), d = e % (D / 4) * 4, row = r0 + r;
@@ -602,13 +607,61 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
     __syncthreads();
     u += tb - ta;
   }
+  if (MODE != PLAIN && !WHOLE && tid == 0) a.unfinished[blockIdx.x] = open;
+}
+
+// SHARED, OWN: merges the parts of an item, always in the same order.  blockIdx.x = c: the item that CTA c began and did not finish (it said
+// so: the lists are not needed again), blockIdx.y: one of its rows; threads as in attn_kv8_join_kernel.
+template <int D, int NT, int MODE>
+__global__ void __launch_bounds__(128) attn_kv8_open_join_kernel(Args a) {
+  constexpr int GR = 8 * NT, GROUPS = 128 * 4 / D;
+  __shared__ __align__(16) float4 sh_o[128];
+  const int tid = threadIdx.x, lane = tid & 31, r = blockIdx.y;
+  griddep_wait();
+  griddep_launch();
+  const int4 open = a.unfinished[blockIdx.x];
+  if (open.x < 0) return;
+  const int c0 = blockIdx.x, c1 = open.x, b = open.z, h = open.w / a.rg, row = open.w % a.rg * GR + r;
+  const int f = MODE == SHARED ? row / (a.n * a.G) : 0, i = row / a.G - f * a.n, seq = MODE == SHARED ? b * a.F + f : b;
+  if (row >= a.rows || i >= seq_of(a.lens, a.counts, seq, a.n, a.C, false).cnt) return;
+  auto part = [&](int c) { return (size_t)(c == c0 ? open.y : 2 * c) * GR + r; };
+  float mx = -INFINITY, sum = 0.f;
+  for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, a.part_ml[part(c)].x);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+  for (int c = c0 + lane; c <= c1; c += 32) {
+    const float2 ml = a.part_ml[part(c)];
+    sum += ml.x == -INFINITY ? 0.f * ml.y : ml.y * ex2_approx(ml.x - mx);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  const int grp = tid / (D / 4), d = tid % (D / 4) * 4;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int c = c0 + grp; c <= c1; c += GROUPS) {
+    const float m = a.part_ml[part(c)].x;
+    const float4 x = *reinterpret_cast<const float4*>(a.part_o + part(c) * D + d);
+    const float w = m == -INFINITY ? 0.f : ex2_approx(m - mx);
+    v.x += x.x * w, v.y += x.y * w, v.z += x.z * w, v.w += x.w * w;
+  }
+  sh_o[tid] = v;
+  __syncthreads();
+  if (grp) return;
+  for (int k = 1; k < GROUPS; k++) {
+    const float4 x = sh_o[tid + k * (D / 4)];
+    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+  }
+  if constexpr (MODE == OWN) add_prefix<D>(a, b, i, h * a.G + row % a.G, d, mx, sum, v);
+  const float inv = P_SCALE / sum;
+  uint16_t* op = a.out + seq * a.so_b + i * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
+  *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
 }
 
 // Merges the parts of items that span CTAs and turns scores into weights.
 // CTAs [0, merge_ctas): one row of an item; each of 128 * 4 / D groups of threads (thread = 4 dims) takes every so many'th
 // part, the groups' sums are added in order.  The others: 512 keys of one (sequence, head):
 // weight = (key before len ? weights_in : 0) + sum over rows of 2^(score - m - log2 l), a row's (m, l) by a warp.
-template <int D, int NT, int MODE = PLAIN>
+template <int D, int NT>
 __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ctas) {
   constexpr int KT = TILE / D, GR = 8 * NT, GROUPS = 128 * 4 / D;
   __shared__ int pre[MAXB + 1], warp_sum[4];
@@ -617,12 +670,11 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   griddep_wait();
   griddep_launch();
-  __shared__ int own[MODE == SHARED ? MAXB + 1 : 1];
-  tile_list<MODE>(a, KT, GR, pre, warp_sum, own);
+  tile_list(a, KT, GR, pre, warp_sum);
   const int run = run_of(pre[a.B], a.ctas);
   // the first and last CTA that hold a part of an item, and the first part's slot (the others begin their CTA's run: 2 c)
   auto parts = [&](const Seq& s, int b, int h, int rg, int tiles, int& c0, int& c1, int& first) {
-    const int u0 = pre[b] + (MODE == SHARED ? h : h * row_groups(a, s, GR) + rg) * tiles;
+    const int u0 = pre[b] + (h * row_groups(a, s, GR) + rg) * tiles;
     c0 = u0 / run, c1 = (u0 + tiles - 1) / run;
     first = 2 * c0 + (u0 == c0 * run ? 0 : 1);
   };
@@ -643,10 +695,9 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
   if ((int)blockIdx.x < merge_ctas) {
     const int rows = min(GR, a.rows), item = blockIdx.x / rows, r = blockIdx.x % rows;
     const int rg = item % a.rg, h = item / a.rg % a.H, b = item / a.rg / a.H;
-    const int row = rg * GR + r, f = MODE == SHARED ? row / (a.n * a.G) : 0, i = row / a.G - f * a.n;
-    const Seq s = seq_of(a.lens, a.counts, MODE == SHARED ? b * a.F + f : b, a.n, a.C, false);
-    const int tiles = MODE == SHARED ? (pre[b + 1] - pre[b]) / a.H : (s.len + s.cnt + KT - 1) / KT;
-    if (i >= s.cnt) return;
+    const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C);
+    const int row = rg * GR + r, tiles = (s.len + s.cnt + KT - 1) / KT;
+    if (row >= s.cnt * a.G) return;
     int c0, c1, first;
     parts(s, b, h, rg, tiles, c0, c1, first);
     if (c0 == c1) return;
@@ -669,14 +720,12 @@ __global__ void __launch_bounds__(128) attn_kv8_join_kernel(Args a, int merge_ct
         const float4 x = sh_o[tid + k * (D / 4)];
         v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
       }
-      if constexpr (MODE == OWN) add_prefix<D>(a, b, i, h * a.G + row % a.G, d, mx, sum, v);
       const float inv = P_SCALE / sum;
-      uint16_t* op = a.out + (MODE == SHARED ? (long long)b * a.F + f : b) * a.so_b + i * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
+      uint16_t* op = a.out + b * a.so_b + row / a.G * a.so_t + (size_t)(h * a.G + row % a.G) * a.so_h + d;
       *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
     }
     return;
   }
-  if (MODE != PLAIN) return;
   const int chunks = (a.C + 511) / 512, x = blockIdx.x - merge_ctas;
   const int bh = x / chunks, j = x % chunks * 512 + tid * 4, h = bh % a.H, b = bh / a.H;
   const Seq s = seq_of(a.lens, a.counts, b, a.n, a.C);
@@ -727,9 +776,13 @@ static int launch(cudaStream_t st, const Args& a, bool whole, const char* what =
   if (rc) return rc;
   launch_k(attn_kv8_split_kernel<D, NT, false, MODE>, a.ctas, WARPS * 32, SMEM, st, a);
   const int rows = 8 * NT < a.rows ? 8 * NT : a.rows;
-  const int merge = a.B * a.H * a.rg * rows;
-  const int chunks = a.w ? a.B * a.H * ((a.C + 511) / 512) : 0;
-  launch_k(attn_kv8_join_kernel<D, NT, MODE>, merge + chunks, 128, 0, st, a, merge);
+  if constexpr (MODE == PLAIN) {
+    const int merge = a.B * a.H * a.rg * rows;
+    const int chunks = a.w ? a.B * a.H * ((a.C + 511) / 512) : 0;
+    launch_k(attn_kv8_join_kernel<D, NT>, merge + chunks, 128, 0, st, a, merge);
+  } else {
+    launch_k(attn_kv8_open_join_kernel<D, NT, MODE>, dim3(a.ctas, rows), 128, 0, st, a);
+  }
   return check_launch(what);
 }
 template <int MODE>
