@@ -433,52 +433,64 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
   } else if (warp >= 8) {
     set_regs_down<tc::CONVERT_REGS>();
     // ---------------- converters: warp w rows 16 w .. of a block.  A lane's 16-byte pieces lie on a diagonal: eight lanes read eight
-    // pieces of different banks, and write eight rows
+    // pieces of different banks, and write eight rows.  K's and V's codes of the next tile, if they are there, are fetched as soon as
+    // this tile's are out of the registers: a tile is mostly waiting, not work
     constexpr int PER = D / 32, PIECES = D / 16;  // pieces of a K or V block that a lane takes, of a row
     const int w = warp - 8;
-    bool ok = true;
-    for (int j = 0, i = -1, left = 0; ok; j++, left--) {
+    int at[PER];  // of a piece in a tile's codes
+    uint8_t* to[PER];  // and of its operand
+#pragma unroll
+    for (int x = 0; x < PER; x++) {
+      const int row = 16 * w + 8 * (x & 1) + (lane & 7), p = ((D == 64 ? (lane & 7) >> 1 : lane & 7) + (lane >> 3) + 4 * (x >> 1)) % PIECES;
+      at[x] = row * D + 16 * p, to[x] = sm + L::K + (2 * p * KEYS + row) * 16;
+    }
+    uint4 kr[PER], vr[PER];
+    float2 scale, scale_next;
+    int2 where, where_next;
+    bool ok = true, have = false;  // have: the next tile's codes are in the registers
+    for (int j = 0, i = -1, left = 0, rs = 0, rph = 0, st = 0, sph = 0; ok; j++, left--) {
       if (left == 0) {
         if (i >= 0) leave(i);
         ok = take(++i);
         left = segs[i & 1].tb - segs[i & 1].ta;
         if (!ok || left == 0) break;
       }
-      const int st = j % ST, rs = j % a.raw;
-      ok = wait(&raw_full[rs], (j / a.raw) & 1) && (j < ST || wait(&kv_empty[st], (j / ST - 1) & 1));
-      if (!ok) break;
-      const uint8_t* raw = sm + L::RAW + rs * L::RAW_TILE;
-      const float2 scale = raw_scale[rs];
-      const bool none = scale.y < kTinyScale;  // V becomes zero
-      auto piece = [&](int x, int& row, int& p) {
-        row = 16 * w + 8 * (x & 1) + (lane & 7);
-        p = ((D == 64 ? (lane & 7) >> 1 : lane & 7) + (lane >> 3) + 4 * (x >> 1)) % PIECES;
-        return row * D + 16 * p;
-      };
-      uint4 kr[PER], vr[PER];
+      auto fetch = [&](uint4 (&r)[PER], int from) {
 #pragma unroll
-      for (int x = 0; x < PER; x++) {
-        int row, p;
-        const int at = piece(x, row, p);
-        kr[x] = *reinterpret_cast<const uint4*>(raw + at), vr[x] = *reinterpret_cast<const uint4*>(raw + KEYS * D + at);
+        for (int x = 0; x < PER; x++) r[x] = *reinterpret_cast<const uint4*>(sm + L::RAW + rs * L::RAW_TILE + from + at[x]);
+      };
+      auto fetched = [&] {  // the stage of codes is free again
+        __syncwarp();
+        mbar_arrive_if(&raw_empty[rs], lane == 0);
+        if (++rs == a.raw) rs = 0, rph ^= 1;
+      };
+      if (!have) {
+        ok = wait(&raw_full[rs], rph);
+        if (!ok) break;
+        fetch(kr, 0), fetch(vr, KEYS * D);
+        scale_next = raw_scale[rs], where_next = raw_at[rs];
+        fetched();
       }
+      scale = scale_next, where = where_next;
+      const bool none = scale.y < kTinyScale;  // V becomes zero
+      ok = j < ST || wait(&kv_empty[st], sph ^ 1);
+      if (!ok) break;
       if (w == 0 && lane == 0) {
         const float v1 = none ? 1.f : scale.y;
-        const int2 at = raw_at[rs];
-        tiles[st] = {at.x, at.y, scale.x * a.scale_log2, __log2f(v1), __frcp_rn(v1) * L_SCALE, none ? Z_TOP : P_TOP};
+        tiles[st] = {where.x, where.y, scale.x * a.scale_log2, __log2f(v1), __frcp_rn(v1) * L_SCALE, none ? Z_TOP : P_TOP};
       }
-      __syncwarp();
-      mbar_arrive_if(&raw_empty[rs], lane == 0);
+      have = left > 1 && __all_sync(0xffffffffu, mbar_try_wait(&raw_full[rs], rph));
 #pragma unroll
-      for (int x = 0; x < PER; x++) {
-        int row, p;
-        piece(x, row, p);
-        tc::store_codes<KEYS, false>(sm + L::K + st * L::KT, row, p, kr[x]);
-        tc::store_codes<KEYS, true>(sm + L::V + st * L::KT, row, p, none ? make_uint4(0, 0, 0, 0) : vr[x]);
-      }
+      for (int x = 0; x < PER; x++) tc::store_codes<KEYS, false>(to[x] + st * L::KT, 0, 0, kr[x]);
+      if (have) fetch(kr, 0), scale_next = raw_scale[rs], where_next = raw_at[rs];
+#pragma unroll
+      for (int x = 0; x < PER; x++) tc::store_codes<KEYS, true>(to[x] + (L::V - L::K) + st * L::KT, 0, 0, none ? make_uint4(0, 0, 0, 0) : vr[x]);
+      if (have) fetch(vr, KEYS * D);
       fence_proxy_async_smem();
       __syncwarp();
       mbar_arrive_if(&kv_full[st], lane == 0);
+      if (have) fetched();
+      if (++st == ST) st = 0, sph ^= 1;
     }
   } else {
     set_regs_up<tc::SOFTMAX_REGS>();
