@@ -13,6 +13,7 @@
 
 Every call launches on torch's current stream and raises VtError on a non-zero return code.
 """
+import functools
 import os
 from typing import NamedTuple
 
@@ -578,6 +579,11 @@ def kv8_evict(cache, weights, lens, keep, recent, dst, dst_weights, dst_lens, in
     return index
 
 
+@functools.lru_cache(maxsize=1024)
+def _shared_ws_bytes(dev, *sizes):
+    return lib().vt_attn_kv8_shared_ws_bytes(*sizes)
+
+
 def attn_kv8_shared_workspace(S, B, n, Hq, H, D, Cp, C, device):
     """A workspace for attn_kv8_shared calls of these sizes, one call at a time (vt_attn_kv8_shared_ws_bytes)."""
     return torch.empty(lib().vt_attn_kv8_shared_ws_bytes(S, B, n, Hq, H, D, Cp, C), dtype=torch.uint8, device=device)
@@ -590,7 +596,7 @@ def attn_kv8_shared(q, prefix, plens, cache, lens, out=None, counts=None, scale=
     pos = plens[b // (B // S)] + lens[b]) -> out [B, n, Hq D] bf16; row i sees the whole prefix and its own slots
     0 .. lens[b] + i.  counts int32 [B] (default n): the rows of a sequence, those behind are left as they were.
     ws: attn_kv8_shared_workspace, else one is allocated."""
-    what, dev = "attn_kv8_shared", q.get_device()
+    what, dev, i32 = "attn_kv8_shared", q.get_device(), torch.int32
     S, H, Cp, D = _kv8_dims(what, prefix, dev)
     B, Hc, C, Dc = _kv8_dims(what, cache, dev)
     Bq, n, Hq, Dq = q.shape
@@ -603,19 +609,21 @@ def attn_kv8_shared(q, prefix, plens, cache, lens, out=None, counts=None, scale=
             out.get_device() != dev or sq[3] != 1 or so[2] != 1:
         _kv8_fail(what, f"q {tuple(q.shape)}, out {tuple(out.shape)} for a cache of B={B} H={H} D={D} (bf16, contiguous rows)")
     if ws is None:
-        nb = lib().vt_attn_kv8_shared_ws_bytes(S, B, n, Hq, H, D, Cp, C)
+        nb = _shared_ws_bytes(dev, S, B, n, Hq, H, D, Cp, C)
         if nb:  # held until the call is on the stream; its memory is reused on this stream only
             ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
-    elif ws.get_device() != dev or not ws.is_contiguous():
-        _kv8_fail(what, "the workspace must be contiguous on the tensors' device")
+        wp = ws.data_ptr() if nb else None
+    else:
+        if ws.get_device() != dev or not ws.is_contiguous():
+            _kv8_fail(what, "the workspace must be contiguous on the tensors' device")
+        nb, wp = ws.nbytes, ws.data_ptr()
+    pk, pv, pks, pvs = prefix
+    k, v, ks, vs = cache
     _kv8_call(lib().vt_attn_kv8_shared, "vt_attn_kv8_shared", dev, q.data_ptr(), sq[0], sq[1], sq[2],
-              prefix.k.data_ptr(), prefix.v.data_ptr(), prefix.ks.data_ptr(), prefix.vs.data_ptr(), Cp,
-              _kv8_vec(what, "plens", plens, (S,), torch.int32, dev), S,
-              cache.k.data_ptr(), cache.v.data_ptr(), cache.ks.data_ptr(), cache.vs.data_ptr(), C,
-              _kv8_vec(what, "lens", lens, (B,), torch.int32, dev),
-              None if counts is None else _kv8_vec(what, "counts", counts, (B,), torch.int32, dev), B, n, Hq, H, D,
-              D ** -0.5 if scale is None else float(scale), out.data_ptr(), so[0], so[1], D,
-              None if ws is None else ws.data_ptr(), 0 if ws is None else ws.nbytes)
+              pk.data_ptr(), pv.data_ptr(), pks.data_ptr(), pvs.data_ptr(), Cp, _kv8_vec(what, "plens", plens, (S,), i32, dev), S,
+              k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), C, _kv8_vec(what, "lens", lens, (B,), i32, dev),
+              None if counts is None else _kv8_vec(what, "counts", counts, (B,), i32, dev), B, n, Hq, H, D,
+              D ** -0.5 if scale is None else float(scale), out.data_ptr(), so[0], so[1], D, wp, nb)
     return out
 
 
@@ -672,31 +680,41 @@ class Beams(NamedTuple):
     done: torch.Tensor
 
 
+@functools.lru_cache(maxsize=1024)
+def _beam_ws_bytes(dev, *sizes):
+    return lib().vt_beam_select_ws_bytes(*sizes)
+
+
 def beam_select(logits, scores, beams, k=None, eos=-1, done=None, out=None, ws=None):
     """vt_beam_select: of each group of `beams` rows of logits [S beams, V] (bf16 or fp32, any row pitch) the k (default beams)
     continuations with the largest scores [S beams] + log softmax(logits), the lowest beam * V + word first where totals are equal.
     A beam that is finished (done bool [S beams]) goes on with the word eos alone, as it is.  Returns Beams (out, where given); where
     fewer than k are left their score is -inf, their word -1.  ws: a uint8 tensor of vt_beam_select_ws_bytes, else one is allocated."""
-    what, dev = "beam_select", logits.get_device()
-    if logits.dim() != 2 or logits.dtype not in (BF16, torch.float32) or logits.stride(1) != 1:
+    what, dev, f32, i32, flag = "beam_select", logits.get_device(), torch.float32, torch.int32, torch.bool
+    wide = logits.dtype is f32
+    if logits.dim() != 2 or not (wide or logits.dtype is BF16) or logits.stride(1) != 1:
         _kv8_fail(what, f"logits {tuple(logits.shape)} {logits.dtype} (bf16 or float32 rows)")
-    (B, V), beams = logits.shape, int(beams)
+    (B, V), beams, device = logits.shape, int(beams), logits.device
     if beams <= 0 or B % beams:
         _kv8_fail(what, f"{B} rows in groups of {beams}")
     S, k = B // beams, beams if k is None else int(k)
     if out is None:
-        out = Beams(*(torch.empty(S, max(k, 0), dtype=t, device=logits.device)
-                      for t in (torch.float32, torch.int32, torch.int32, torch.bool)))
-    nb = lib().vt_beam_select_ws_bytes(S, beams, V, k)
+        n = max(k, 0)
+        out = Beams(torch.empty(S, n, dtype=f32, device=device), torch.empty(S, n, dtype=i32, device=device),
+                    torch.empty(S, n, dtype=i32, device=device), torch.empty(S, n, dtype=flag, device=device))
+        to = out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr()
+    else:
+        to = [_kv8_vec(what, name, x, (S, k), d, dev) for name, x, d in zip(Beams._fields, out, (f32, i32, i32, flag))]
     if ws is None:
-        ws = torch.empty(nb, dtype=torch.uint8, device=logits.device)
+        nb = _beam_ws_bytes(dev, S, beams, V, k)
+        ws = torch.empty(nb, dtype=torch.uint8, device=device)  # held until the call is on the stream; its memory is reused on this stream only
     elif ws.get_device() != dev or not ws.is_contiguous():
         _kv8_fail(what, "the workspace must be contiguous on the tensors' device")
-    _kv8_call(lib().vt_beam_select, "vt_beam_select", dev, logits.data_ptr(), logits.stride(0) if B > 1 else V,
-              int(logits.dtype is torch.float32), _kv8_vec(what, "scores", scores, (B,), torch.float32, dev),
-              None if done is None else _kv8_vec(what, "done", done, (B,), torch.bool, dev), S, beams, V, k, int(eos),
-              *(_kv8_vec(what, n, t, (S, k), d, dev) for n, t, d in zip(Beams._fields, out, (torch.float32, torch.int32, torch.int32, torch.bool))),
-              ws.data_ptr(), ws.nbytes)
+    else:
+        nb = ws.nbytes
+    _kv8_call(lib().vt_beam_select, "vt_beam_select", dev, logits.data_ptr(), logits.stride(0) if B > 1 else V, int(wide),
+              _kv8_vec(what, "scores", scores, (B,), f32, dev), None if done is None else _kv8_vec(what, "done", done, (B,), flag, dev),
+              S, beams, V, k, int(eos), *to, ws.data_ptr(), nb)
     return out
 
 
