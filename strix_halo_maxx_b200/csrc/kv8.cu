@@ -18,13 +18,15 @@ constexpr float LOG2E = 1.4426950408889634f;
 struct Seq {
   int len, cnt;
 };
-__device__ __forceinline__ Seq seq_of(const int* lens, const int* counts, int b, int n, int C, bool record) {
-  int len = lens[b], cnt = counts ? counts[b] : n;
+__device__ __forceinline__ Seq clip_seq(int len, int cnt, int n, int C, bool record) {
   const bool bad = len < 0 || len > C || cnt < 0 || cnt > n || cnt > C - len;
   len = min(max(len, 0), C);
   cnt = min(min(max(cnt, 0), n), C - len);
   if (bad && record) atomicOr(&g_status, (unsigned int)ST_KV8_RANGE);
   return {len, cnt};
+}
+__device__ __forceinline__ Seq seq_of(const int* lens, const int* counts, int b, int n, int C, bool record) {
+  return clip_seq(lens[b], counts ? counts[b] : n, n, C, record);
 }
 __device__ __forceinline__ Seq seq_of(const int* lens, const int* counts, int b, int n, int C) {
   return seq_of(lens, counts, b, n, C, threadIdx.x == 0);

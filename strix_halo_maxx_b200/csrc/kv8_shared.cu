@@ -32,6 +32,7 @@ using tc::P_UP_SINK;
 using tc::THREADS;
 using tc::Z_TOP;
 constexpr int MAXB = 2048, MAX_CTAS = 512;  // sequences and runs (one for each SM) of a call
+constexpr float SINK_SUM = 238.856f;   // 2^P_UP: what the largest term of a row's first tile is
 constexpr uint32_t TMEM_COLS = 512;  // S of M tile t, buffer f: columns 128 t + 64 f; O of tile t: 256 + 128 t
 
 template <int D, bool ALT>
@@ -89,24 +90,57 @@ __device__ __forceinline__ int own_tiles(const Args& a, const Lists& l, int s, i
   const int last = min(cnt - 1, (q * ROWS + ROWS - 1) / a.G - (l.tok[x] - l.tok[s * a.F]));
   return (l.len[x] + last + KEYS) / KEYS;
 }
+// list[0 .. n] becomes the sums before each of n numbers, count(i) gives them: a warp, 32 at a time.
+template <typename Count>
+__device__ __forceinline__ void warp_sums(int* list, int n, const Count& count) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int x = i0 + lane < n ? count(i0 + lane) : 0;
+    int inc = x;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += y;
+    }
+    if (i0 + lane < n) list[i0 + lane] = before + inc - x;
+    before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (lane == 0) list[n] = before;
+  __syncwarp();
+}
+// By one warp (block-wide sums took 2 us with their barriers).
 template <int ROWS>
-__device__ __forceinline__ void make_lists(const Args& a, const Lists& l, int* scratch) {
+__device__ __forceinline__ void make_lists(const Args& a, const Lists& l) {
   const bool record = blockIdx.x == 0;
-  for (int s = threadIdx.x; s < a.S; s += blockDim.x) l.plen[s] = split::prefix_len(a.plens, s, a.Cp, record);
-  split::sums_before(l.tok, a.S * a.F, scratch, [&](int b) {
-    const Seq q = seq_of(a.lens, a.counts, b, a.n, a.C, record);
-    l.len[b] = q.len;
-    return q.cnt;
-  });
+  const int lane = threadIdx.x & 31, B = a.S * a.F;
+  for (int s = lane; s < a.S; s += 32) l.plen[s] = split::prefix_len(a.plens, s, a.Cp, record);
+  for (int i0 = 0; i0 < B; i0 += 128) {  // the loads of four at a time side by side
+    int len[4], cnt[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int b = i0 + 32 * k + lane;
+      len[k] = b < B ? a.lens[b] : 0, cnt[k] = b < B && a.counts ? a.counts[b] : a.n;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int b = i0 + 32 * k + lane;
+      if (b >= B) continue;
+      const Seq q = clip_seq(len[k], cnt[k], a.n, a.C, record);
+      l.len[b] = q.len, l.tok[b] = q.cnt;
+    }
+  }
+  __syncwarp();
+  warp_sums(l.tok, B, [&](int b) { return l.tok[b]; });
   if (a.own)
-    split::sums_before(l.own, a.S * a.F, scratch, [&](int x) {
+    warp_sums(l.own, B, [&](int x) {
       const int s = x / a.F, first = (l.tok[x] - l.tok[s * a.F]) * a.G, rows = (l.tok[x + 1] - l.tok[x]) * a.G;
       int t = 0;
       if (rows)
         for (int q = first / ROWS; q <= (first + rows - 1) / ROWS; q++) t += own_tiles<ROWS>(a, l, s, x, q);
       return t;
     });
-  split::sums_before(l.pre, a.S, scratch, [&](int s) {
+  warp_sums(l.pre, a.S, [&](int s) {
     const int P = l.plen[s], rows = (l.tok[(s + 1) * a.F] - l.tok[s * a.F]) * a.G;
     return ((rows + ROWS - 1) / ROWS * ((P + KEYS - 1) / KEYS) + (a.own ? l.own[(s + 1) * a.F] - l.own[s * a.F] : 0)) * a.H;
   });
@@ -115,7 +149,7 @@ __device__ __forceinline__ void make_lists(const Args& a, const Lists& l, int* s
 // A CTA's share of an item: rows q ROWS .. of prefix s, head h; key tiles [ta, tb) of `tiles`, the first pt of them the prefix's.
 struct Seg {
   int s, h, q, rows, P, pt, x0, x1, t0, tiles, ta, tb;  // x0, x1: first and last sequence of the item; t0: own tiles of x0
-  int u;                                                // of its first tile in the list
+  int last;                                             // the CTA with the item's last tile
   struct Part {
     int oa, ob;  // own tiles that concern the M tile: [oa, ob) of the item's
     bool act;    // whether it has any tile here
@@ -178,7 +212,7 @@ __device__ __forceinline__ Seg segment(const Args& a, const Lists& l, int u, int
     at -= before;
   }
   const int r0 = g.q * ROWS;
-  g.tiles = 0, g.ta = at, g.u = u, g.x0 = g.x1 = g.t0 = 0;
+  g.tiles = 0, g.ta = at, g.x0 = g.x1 = g.t0 = 0;
   int oa1 = 0, ob0 = 0;
   if (r0 < g.rows) {
     // lanes 0 .. 3: the first row of the item, the last one of M tile 0, the first one of M tile 1, the last one of the item
@@ -246,7 +280,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
   using L = Smem<D, ALT>;
   constexpr int ROWS = L::ROWS, ST = L::ST;
   extern __shared__ __align__(1024) uint8_t sm[];
-  __shared__ int scratch[THREADS / 32];
   __shared__ Seg segs[2];                       // shares of items, in turn; an empty one ends
   __shared__ int2 row_at[2][256];               // of a thread's row: its sequence and token
   __shared__ Tile tiles[ST];
@@ -286,8 +319,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
   const uint32_t tmem = tmem_slot;
   griddep_wait();  // programmatic dependent launch: the previous kernel has completed
   griddep_launch();
-  make_lists<ROWS>(a, l, scratch);
-  const int run = a.items > 0 ? 1 : max((l.pre[a.S] + a.ctas - 1) / a.ctas, 1);
   // a wait of the whole warp: every lane gives up when one does
   auto wait = [&](uint64_t* bar, int parity) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, ST_KV8_WAIT)) != 0;
@@ -414,12 +445,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
     }
     if (warp == 15) {
       // ---------------- the shares
-      const int total = a.items > 0 ? 1 : l.pre[a.S], u_begin = a.items > 0 ? 0 : (int)min((long long)blockIdx.x * run, (long long)total);
+      make_lists<ROWS>(a, l);
+      const int total = a.items > 0 ? 1 : l.pre[a.S], run = max((total + a.ctas - 1) / a.ctas, 1), u_begin = a.items > 0 ? 0 : (int)min((long long)blockIdx.x * run, (long long)total);
       const int u_end = (int)min((long long)u_begin + run, (long long)total);
       for (int u = u_begin, i = 0; ok; i++) {
         Seg g;
         g.ta = g.tb = 0;
-        if (u < u_end) g = segment<D, ALT>(a, l, u, u_end);
+        if (u < u_end) g = segment<D, ALT>(a, l, u, u_end), g.last = (u - g.ta + g.tiles - 1) / run;
         ok = i < 2 || wait(&seg_empty[i & 1], ((i >> 1) - 1) & 1);
         if (!ok) break;
         const int nt = g.tb - g.ta;
@@ -560,6 +592,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
           const bool mine = x < 0 || (x >= warp_x0 && x <= warp_x1);  // whether the warp has rows that see this cache
           const int lim = x < 0 ? g.P : x == rx ? own_lim : 0;
           float mx, sum = 0.f;
+          bool look = false;  // whether the row's first keys are in this tile
           auto top32 = [&](const uint32_t (&r)[32]) {
             float y[11];
 #pragma unroll
@@ -607,72 +640,79 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
           tmem_ld_wait();
           tmem_ld32(t_s + 32, r1);
           // a tile that every row sees whole, once rows have a maximum: P with the maximum so far, while the second half of
-          // the scores arrives and the new maximum is found beside the exponentials; they stand unless it grew too far
-          bool again = fresh || edge;
-          if (!again) {
-            sum = exps(r0, 0, m);
-            const float ma = top32(r0);
-            tmem_ld_wait();
-            sum += exps(r1, 16, m);
-            mx = fmaf(fmaxf(ma, top32(r1)), c, lvs);
-            again = __any_sync(0xffffffffu, mx > m + top);
-          }
-          if (again) {
-            tmem_ld_wait();
-            const int left = lim - key0;  // keys of the tile that the row sees
-            if (edge) {
-#pragma unroll
-              for (int e = 0; e < 32; e++) {
-                if (e >= left) r0[e] = 0xff800000u;
-                if (32 + e >= left) r1[e] = 0xff800000u;
-              }
-            }
-            const bool begins = m == -INFINITY;  // the row's first keys
-            mx = left > 0 ? fmaf(fmaxf(top32(r0), top32(r1)), c, lvs) : -INFINITY;
-            const bool need = mx > m + top;
-            const float up = top - P_MOVE;
-            const float mn = begins ? mx - up : need ? mx - (mx > m + (P_TOP + 12.f) ? fmaxf(up, P_UP_SINK) : up) : m;
-            if (!first && __any_sync(0xffffffffu, need && !begins)) {  // O through registers (warp-collective)
-              // O must hold every product up to this M tile's last tile; the barrier's next arrival needs P of this row
-              ok = wait(&pv_done[t], (js - 1) & 1);
-              if (!ok) break;
-              tc_fence_after();
-              const float half = need && !begins ? ex2_approx(0.5f * (m - mn)) : 1.f, alpha = half * half;
-              sum_l = sum_l * half * half;  // what zero blocks put there may be as large as alpha is small
-#pragma unroll
-              for (int y = 0; y < D / 16; y++) {
-                uint32_t r[16];
-                tmem_ld16(t_o + y * 16, r);
-                tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 16; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
-                tmem_st16(t_o + y * 16, r);
-              }
-            }
-            m = mn;
-            // a row that sees nothing of the tile takes no part in its scales, which may be NaN; scores out of sight are -inf,
-            // and -inf * 0 of a zero scale must not be NaN
-            const float mu = m == -INFINITY ? 0.f : m;
-            if (edge) {
-              if (left <= 0) c = 1.f, lvs = 0.f, ivs = 1.f;
-              if (c == 0.f) {
+          // the scores arrives and the new maximum is found beside the exponentials; they stand unless it grew too far.  Else the maximum
+          // comes first.  One copy of the exponentials for all (the cold instruction cache cost 3 us before the second tile)
+          bool guess = !(fresh || edge), sink_looked = false;
+          float mu = m;
+#pragma unroll 1
+          while (true) {
+            if (!guess && !sink_looked) {  // the row's maximum, O and the sum brought to it
+              tmem_ld_wait();
+              const int left = lim - key0;  // keys of the tile that the row sees
+              if (edge) {
 #pragma unroll
                 for (int e = 0; e < 32; e++) {
-                  r0[e] = e < left ? 0u : r0[e];
-                  r1[e] = 32 + e < left ? 0u : r1[e];
+                  if (e >= left) r0[e] = 0xff800000u;
+                  if (32 + e >= left) r1[e] = 0xff800000u;
                 }
-                c = 1.f;
+              }
+              const bool begins = m == -INFINITY;  // the row's first keys
+              mx = left > 0 ? fmaf(fmaxf(top32(r0), top32(r1)), c, lvs) : -INFINITY;
+              const bool need = mx > m + top;
+              const float up = top - P_MOVE;
+              const float mn = begins ? mx - up : need ? mx - (mx > m + (P_TOP + 12.f) ? fmaxf(up, P_UP_SINK) : up) : m;
+              if (!first && __any_sync(0xffffffffu, need && !begins)) {  // O through registers (warp-collective)
+                // O must hold every product up to this M tile's last tile; the barrier's next arrival needs P of this row
+                ok = wait(&pv_done[t], (js - 1) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const float half = need && !begins ? ex2_approx(0.5f * (m - mn)) : 1.f, alpha = half * half;
+                sum_l = sum_l * half * half;  // what zero blocks put there may be as large as alpha is small
+#pragma unroll
+                for (int y = 0; y < D / 16; y++) {
+                  uint32_t r[16];
+                  tmem_ld16(t_o + y * 16, r);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int e = 0; e < 16; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
+                  tmem_st16(t_o + y * 16, r);
+                }
+              }
+              m = mn;
+              look = begins && m != -INFINITY;
+              // a row that sees nothing of the tile takes no part in its scales, which may be NaN; scores out of sight are -inf,
+              // and -inf * 0 of a zero scale must not be NaN
+              mu = m == -INFINITY ? 0.f : m;
+              if (edge) {
+                if (left <= 0) c = 1.f, lvs = 0.f, ivs = 1.f;
+                if (c == 0.f) {
+#pragma unroll
+                  for (int e = 0; e < 32; e++) {
+                    r0[e] = e < left ? 0u : r0[e];
+                    r1[e] = 32 + e < left ? 0u : r1[e];
+                  }
+                  c = 1.f;
+                }
               }
             }
-            sum = exps(r0, 0, mu) + exps(r1, 16, mu);
-            const bool sink = begins && m != -INFINITY && sum < 1.05f * exp2f(P_UP);  // its other keys add up to a twentieth of its largest one
-            if (__any_sync(0xffffffffu, sink)) {
-              m -= sink ? P_UP_SINK - P_UP : 0.f;
-              const float ms = m == -INFINITY ? 0.f : m;
-              sum = exps(r0, 0, ms) + exps(r1, 16, ms);
+            sum = exps(r0, 0, mu);
+            const float ma = guess ? top32(r0) : 0.f;
+            tmem_ld_wait();
+            sum += exps(r1, 16, mu);
+            if (guess) {
+              mx = fmaf(fmaxf(ma, top32(r1)), c, lvs);
+              if (!__any_sync(0xffffffffu, mx > m + top)) break;
+              guess = false;
+              continue;
             }
-            fresh = __any_sync(0xffffffffu, m == -INFINITY);
+            const bool sink = look && sum < 1.05f * SINK_SUM;  // a row's first tile whose other keys add up to a twentieth of its largest one
+            if (sink_looked || !__any_sync(0xffffffffu, sink)) break;
+            m -= sink ? P_UP_SINK - P_UP : 0.f;
+            mu = m == -INFINITY ? 0.f : m;
+            sink_looked = true;
           }
+          if (!ok) break;
+          fresh = fresh && __any_sync(0xffffffffu, m == -INFINITY);
           sum_l += sum * ivs;
           announce(f);
           first = false, js++, j = tile_from<ALT>(g, t, j + 1);
@@ -692,7 +732,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
       const size_t out_row = ((size_t)rx * a.n + ri) * (a.G * a.H) + hq;
       uint16_t* op = a.out + rx * a.so_b + ri * a.so_t + hq * a.so_h;
       if (g.ta == 0 && !whole) {
-        open = make_int4((g.u + g.tiles - 1) / run, (int)slot, g.h, g.q * ROWS);
+        open = make_int4(g.last, (int)slot, g.h, g.q * ROWS);
         if (!ALT || t == 0) a.row_at[(size_t)blockIdx.x * ROWS + mine_r] = row < valid ? rx * a.n + ri : -1;
       }
       // dims y16 .. y16 + 15 of the row, o = O / l where it is whole.  Parts lie as [dims / 4][row][4]: a warp writes whole lines
