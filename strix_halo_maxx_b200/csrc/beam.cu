@@ -33,15 +33,15 @@ struct Args {
 // gather, and as many comparisons as parts squared (MEASURED3).
 __host__ __device__ inline int parts_of(int k) { return k <= 16 ? 32 : k <= 32 ? 64 : k <= 64 ? 128 : 256; }
 
-// A logit and its word as one number: larger logits first, of equal ones (zeros of both signs are) the lowest word; never 0.
-__device__ __forceinline__ unsigned long long key_of(float x, int v) {
-  const uint32_t u = __float_as_uint(x + 0.f), o = u & 0x80000000u ? ~u : u | 0x80000000u;
-  return (unsigned long long)o << 32 | (uint32_t)~v;
+// Numbers in the order of floats (zeros of both signs are one), and back.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float key_logit(unsigned long long key) {
-  const uint32_t o = (uint32_t)(key >> 32);
-  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
-}
+__device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+// A logit and its word as one number: larger logits first, of equal ones the lowest word; never 0.
+__device__ __forceinline__ unsigned long long key_of(float x, int v) { return (unsigned long long)ordered(x) << 32 | (uint32_t)~v; }
+__device__ __forceinline__ float key_logit(unsigned long long key) { return unordered((uint32_t)(key >> 32)); }
 
 template <typename Word>
 __device__ __forceinline__ float load_word(const Word* p) {
@@ -77,8 +77,9 @@ __device__ __forceinline__ void load_chunk(const Word* row, int v0, int V, float
 // CTA = T E words of a row.  Bound: issue slots and DRAM with many rows (MEASURED), the latency of one chunk with few.
 template <typename Word, int VEC, int E>
 __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
-  constexpr int FOUND = T * E / 2;  // words above the bound are of fewer than k of 2 k parts or more
-  __shared__ float sh_max[T / 32], sh_sum[T / 32], part[T];
+  constexpr int FOUND = T * E / 2;  // words above the bound are of at most k of 2 k parts or more
+  __shared__ float sh_max[T / 32], sh_sum[T / 32];
+  __shared__ __align__(16) uint32_t part[T];
   __shared__ unsigned long long found[FOUND];
   __shared__ float bound;
   __shared__ int count;
@@ -105,7 +106,9 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
     if (2 * d == per) best = top;
   }
   if (lane == 0) sh_max[warp] = top;
-  if (tid % per == 0) part[tid / per] = best;
+  // a part's maximum with its number in the lowest bits: no two are equal, and the bound is at most 2^-15 of a value low
+  const uint32_t number = parts - 1, mine = (ordered(best) & ~number) | (number - tid / per);
+  if (tid % per == 0) part[tid / per] = mine;
   if (tid == 0) count = 0, bound = -INFINITY;
   __syncthreads();
 #pragma unroll
@@ -113,13 +116,12 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
   // ---- a part's rank among the maxima, its threads taking a share of them each; the k'th is the bound
   {
     int ahead = 0;
-    const int me = tid / per;
-    for (int i = tid % per; i < parts; i += per) {
-      const float y = part[i];
-      ahead += y > best || (y == best && i < me);
+    for (int i = tid % per; i < parts / 4; i += per) {
+      const uint4 y = reinterpret_cast<const uint4*>(part)[i];
+      ahead += (y.x > mine) + (y.y > mine) + (y.z > mine) + (y.w > mine);
     }
     for (int d = 1; d < per; d <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
-    if (tid % per == 0 && ahead == k - 1) bound = best;  // -inf where fewer than k parts have a word
+    if (tid % per == 0 && ahead == k - 1 && best > -INFINITY) bound = unordered(mine & ~number);  // -inf where fewer than k parts have a word
   }
   // ---- sum of exponentials; a chunk of -inf adds nothing, a NaN or +inf makes it NaN
   {
@@ -143,6 +145,7 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
   // ---- gather the words that reach the bound.  They are few: the others' only cost is a bit
   const float lim = bound == -INFINITY ? -3.402823466e38f : bound;
   uint32_t hits = 0;
+  if (__any_sync(0xffffffffu, mx >= lim))
 #pragma unroll
   for (int e = 0; e < E; e++)
     asm("{\n\t.reg .pred p;\n\tsetp.ge.f32 p, %1, %2;\n\t@p or.b32 %0, %0, %3;\n\t}" : "+r"(hits) : "f"(x[e]), "f"(lim), "r"(1u << e));
@@ -158,10 +161,19 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
   }
   __syncthreads();
   int n = count;
-  if (n > FOUND) {  // equal logits in crowds (words banned by the lowest value): those above the bound, then its first words
+  if (n > FOUND) {  // equal logits in crowds (words banned by the lowest value): the exact bound, what is above it, then its first words
+    if (tid % per == 0) part[tid / per] = __float_as_uint(best);
     __syncthreads();
     if (tid == 0) count = 0;
+    int ahead = 0;
+    for (int i = tid % per; i < parts; i += per) {
+      const float y = __uint_as_float(part[i]);
+      ahead += y > best || (y == best && i < tid / per);
+    }
+    for (int d = 1; d < per; d <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
+    if (tid % per == 0 && ahead == k - 1) bound = best;
     __syncthreads();
+    const float lim = bound;  // of fewer than k parts there are words above it
 #pragma unroll
     for (int e = 0; e < E; e++)
       if (x[e] > lim) found[atomicAdd(&count, 1)] = key_of(x[e], word(e));
@@ -191,18 +203,26 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
   for (int i = n + tid; i < k; i += T) to[i] = 0;
 }
 
-// A continuation: its total, and beam * V + word; -inf and INT_MAX for none.
+// A continuation: its total, beam, and logit with word; a total of -inf for none.  Equal totals go by beam, then by logit (which a total of
+// 64 bits may have lost) and word.
 struct Total {
   double t;
-  int at;
+  unsigned long long key;
+  int f;
 };
-__device__ __forceinline__ bool ahead_of(const Total& x, const Total& y) { return x.t > y.t || (x.t == y.t && x.at < y.at); }
+__device__ __forceinline__ bool ahead_of(const Total& x, const Total& y) {
+  return x.t > y.t || (x.t == y.t && (x.f < y.f || (x.f == y.f && x.key > y.key)));
+}
+__device__ __forceinline__ Total shfl_xor(const Total& x, int d) {
+  return {__shfl_xor_sync(0xffffffffu, x.t, d), __shfl_xor_sync(0xffffffffu, x.key, d), __shfl_xor_sync(0xffffffffu, x.f, d)};
+}
 
 // CTA = a group.  Bound: latency, of two trips to L2 and the rounds of comparisons.
 __global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
   __shared__ double sh_top[MAX_BEAMS], sh_log[MAX_BEAMS], sh_score[MAX_BEAMS];
   __shared__ double part_t[TP], found_t[CAP];
-  __shared__ int part_at[TP], found_at[CAP];
+  __shared__ unsigned long long part_key[TP], found_key[CAP];
+  __shared__ uint8_t part_f[TP], found_f[CAP];
   __shared__ uint8_t sh_done[MAX_BEAMS];
   __shared__ Total bound;
   __shared__ int count;
@@ -227,18 +247,18 @@ __global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
     }
     if (lane == 0) sh_top[f] = top, sh_log[f] = log(sum), sh_score[f] = a.scores[row0 + f], sh_done[f] = done;
   }
-  if (tid == 0) count = 0, bound = {-INFINITY, 0x7fffffff};
+  if (tid == 0) count = 0, bound = {-INFINITY, 0, MAX_BEAMS};
   __syncthreads();
-  const Total none{-INFINITY, 0x7fffffff};
+  const Total none{-INFINITY, 0, MAX_BEAMS};
   // entry j of list l: l = a chunk of a row; a finished beam's only entry stands in its first list
   auto entry = [&](int l, int j) {
     const int f = l / a.chunks;
     Total x = none;
     if (sh_done[f]) {
-      if (l % a.chunks == 0 && j == 0) x = {sh_score[f], f * a.V + a.eos};
+      if (l % a.chunks == 0 && j == 0) x = {sh_score[f], key_of(0.f, a.eos), f};
     } else {
       const unsigned long long key = a.words[(row0 * a.chunks + l) * k + j];
-      if (key) x = {sh_score[f] + (((double)key_logit(key) - sh_top[f]) - sh_log[f]), f * a.V + (int)~(uint32_t)key};
+      if (key) x = {sh_score[f] + (((double)key_logit(key) - sh_top[f]) - sh_log[f]), key, f};
     }
     return isfinite(x.t) ? x : none;
   };
@@ -255,20 +275,20 @@ __global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
       if (ahead_of(x, best)) best = x;
     }
   const Total mine = best;
-  part_t[tid] = best.t, part_at[tid] = best.at;
+  part_t[tid] = best.t, part_key[tid] = best.key, part_f[tid] = best.f;
   __syncthreads();
   {
     const int from = tid / per + tid % per * parts;  // of this thread's part, TP / per of them
-    best = {part_t[from], part_at[from]};
+    best = {part_t[from], part_key[from], part_f[from]};
     for (int d = 1; d < per; d <<= 1) {
-      const Total x{__shfl_xor_sync(0xffffffffu, best.t, d), __shfl_xor_sync(0xffffffffu, best.at, d)};
+      const Total x = shfl_xor(best, d);
       if (ahead_of(x, best)) best = x;
     }
     __syncthreads();
-    if (tid % per == 0) part_t[tid / per] = best.t, part_at[tid / per] = best.at;
+    if (tid % per == 0) part_t[tid / per] = best.t, part_key[tid / per] = best.key, part_f[tid / per] = best.f;
     __syncthreads();
     int ahead = 0;
-    for (int i = tid % per; i < parts; i += per) ahead += ahead_of({part_t[i], part_at[i]}, best);
+    for (int i = tid % per; i < parts; i += per) ahead += ahead_of({part_t[i], part_key[i], part_f[i]}, best);
     for (int d = 1; d < per; d <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
     if (tid % per == 0 && ahead == k - 1 && best.t > -INFINITY) bound = best;
   }
@@ -281,13 +301,13 @@ __global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
         const Total x = entry(r % lists, j);
         if (!reaches(x)) break;
         const int n = atomicAdd(&count, 1);
-        if (n < CAP) found_t[n] = x.t, found_at[n] = x.at;
+        if (n < CAP) found_t[n] = x.t, found_key[n] = x.key, found_f[n] = x.f;
       }
   __syncthreads();
   const int n = count;
   const long long o = (long long)blockIdx.x * k;
   auto put = [&](int j, const Total& x) {
-    const int f = x.at / a.V, v = x.at % a.V;
+    const int f = x.f, v = (int)~(uint32_t)x.key;
     a.out_scores[o + j] = (float)x.t;
     a.out_parents[o + j] = (int)row0 + f;
     a.out_tokens[o + j] = v;
@@ -301,16 +321,16 @@ __global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
   };
   if (n <= CAP) {
     for (int i = tid; i < n; i += TP) {
-      const Total x{found_t[i], found_at[i]};
+      const Total x{found_t[i], found_key[i], found_f[i]};
       int ahead = 0;
-      for (int j = 0; j < n; j++) ahead += ahead_of({found_t[j], found_at[j]}, x);
+      for (int j = 0; j < n; j++) ahead += ahead_of({found_t[j], found_key[j], found_f[j]}, x);
       if (ahead < k) put(ahead, x);
     }
     for (int j = n + tid; j < k; j += TP) put_none(j);
     return;
   }
   // far more than k reach the bound (words that stand together in a few of many lists): one by one, the best behind the last
-  Total last{INFINITY, -1};
+  Total last{INFINITY, 0, -1};
   for (int j = 0; j < k; j++) {
     best = none;
     for (int r = tid; r < runs; r += TP)
@@ -323,13 +343,13 @@ __global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
         }
       }
     for (int d = 1; d < 32; d <<= 1) {
-      const Total x{__shfl_xor_sync(0xffffffffu, best.t, d), __shfl_xor_sync(0xffffffffu, best.at, d)};
+      const Total x = shfl_xor(best, d);
       if (ahead_of(x, best)) best = x;
     }
-    if (lane == 0) part_t[warp] = best.t, part_at[warp] = best.at;
+    if (lane == 0) part_t[warp] = best.t, part_key[warp] = best.key, part_f[warp] = best.f;
     __syncthreads();
     for (int w = 0; w < TP / 32; w++) {
-      const Total x{part_t[w], part_at[w]};
+      const Total x{part_t[w], part_key[w], part_f[w]};
       if (ahead_of(x, best)) best = x;
     }
     __syncthreads();
