@@ -230,17 +230,33 @@ __global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
   const long long row0 = (long long)blockIdx.x * F;
   griddep_wait();
   griddep_launch();
+  // every list is dealt out to `deal` runs (entries j, j + deal, ..: in order too); run r is of list r % lists, thread t takes runs
+  // t, t + TP, .., and threads p, p + parts, .. are a part: the best words of one beam stand in many parts
+  const int lists = F * a.chunks, parts = k <= 16 ? 64 : k <= 32 ? 128 : 256, per = TP / parts;
+  int deal = 1;
+  while (lists * deal < 2 * TP && deal < k) deal <<= 1;
+  const int runs = lists * deal;
+  // the first entries of a thread's first runs are fetched while the sums are worked out
+  constexpr int AHEAD = 4;
+  unsigned long long head[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) {
+    const int r = tid + i * TP;
+    head[i] = r < runs && r / lists < k ? a.words[(row0 * a.chunks + r % lists) * k + r / lists] : 0;
+  }
   // ---- of each row the largest logit and the log of its sum, a warp a row
   for (int f = warp; f < F; f += TP / 32) {
     const bool done = a.done && a.done[row0 + f];
     double top = -INFINITY, sum = 0.;
     if (!done) {
       const float2* s = a.sums + (row0 + f) * a.chunks;
-      float m = -INFINITY;
-      for (int c = lane; c < a.chunks; c += 32) m = fmaxf(m, s[c].x);
+      const float2 mine = lane < a.chunks ? s[lane] : make_float2(-INFINITY, 0.f);  // of the first 32 chunks, mostly all
+      float m = mine.x;
+      for (int c = lane + 32; c < a.chunks; c += 32) m = fmaxf(m, s[c].x);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-      for (int c = lane; c < a.chunks; c += 32) sum += s[c].y == 0.f ? 0. : s[c].y * exp((double)s[c].x - m);
+      if (mine.y != 0.f) sum = mine.y * exp((double)mine.x - m);
+      for (int c = lane + 32; c < a.chunks; c += 32) sum += s[c].y == 0.f ? 0. : s[c].y * exp((double)s[c].x - m);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       top = m;
@@ -251,25 +267,26 @@ __global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
   __syncthreads();
   const Total none{-INFINITY, 0, MAX_BEAMS};
   // entry j of list l: l = a chunk of a row; a finished beam's only entry stands in its first list
-  auto entry = [&](int l, int j) {
+  auto total = [&](int l, int j, unsigned long long key) {
     const int f = l / a.chunks;
     Total x = none;
     if (sh_done[f]) {
       if (l % a.chunks == 0 && j == 0) x = {sh_score[f], key_of(0.f, a.eos), f};
     } else {
-      const unsigned long long key = a.words[(row0 * a.chunks + l) * k + j];
       if (key) x = {sh_score[f] + (((double)key_logit(key) - sh_top[f]) - sh_log[f]), key, f};
     }
     return isfinite(x.t) ? x : none;
   };
-  // every list is dealt out to `deal` runs (entries j, j + deal, ..: in order too); run r is of list r % lists, thread t takes runs
-  // t, t + TP, .., and threads p, p + parts, .. are a part: the best words of one beam stand in many parts
-  const int lists = F * a.chunks, parts = k <= 16 ? 64 : k <= 32 ? 128 : 256, per = TP / parts;
-  int deal = 1;
-  while (lists * deal < 2 * TP && deal < k) deal <<= 1;
-  const int runs = lists * deal;
+  auto entry = [&](int l, int j) { return total(l, j, a.words[(row0 * a.chunks + l) * k + j]); };
   Total best = none;
-  for (int r = tid; r < runs; r += TP)
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) {
+    const int r = tid + i * TP;
+    if (r >= runs || r / lists >= k) continue;
+    const Total x = total(r % lists, r / lists, head[i]);
+    if (ahead_of(x, best)) best = x;
+  }
+  for (int r = tid + AHEAD * TP; r < runs; r += TP)
     if (r / lists < k) {
       const Total x = entry(r % lists, r / lists);
       if (ahead_of(x, best)) best = x;
@@ -295,14 +312,24 @@ __global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
   __syncthreads();
   const Total lim = bound;  // none where fewer than k parts have a continuation
   auto reaches = [&](const Total& x) { return x.t > -INFINITY && !ahead_of(lim, x); };
-  if (reaches(mine))
-    for (int r = tid; r < runs; r += TP)
-      for (int j = r / lists; j < k; j += deal) {
-        const Total x = entry(r % lists, j);
-        if (!reaches(x)) break;
+  if (reaches(mine)) {
+    auto gather = [&](int l, int j, Total x) {  // from the run's entry j, x, on
+      while (reaches(x)) {
         const int n = atomicAdd(&count, 1);
         if (n < CAP) found_t[n] = x.t, found_key[n] = x.key, found_f[n] = x.f;
+        j += deal;
+        if (j >= k) break;
+        x = entry(l, j);
       }
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) {
+      const int r = tid + i * TP;
+      if (r < runs && r / lists < k) gather(r % lists, r / lists, total(r % lists, r / lists, head[i]));
+    }
+    for (int r = tid + AHEAD * TP; r < runs; r += TP)
+      if (r / lists < k) gather(r % lists, r / lists, entry(r % lists, r / lists));
+  }
   __syncthreads();
   const int n = count;
   const long long o = (long long)blockIdx.x * k;
@@ -323,7 +350,11 @@ __global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
     for (int i = tid; i < n; i += TP) {
       const Total x{found_t[i], found_key[i], found_f[i]};
       int ahead = 0;
-      for (int j = 0; j < n; j++) ahead += ahead_of({found_t[j], found_key[j], found_f[j]}, x);
+      for (int j = 0; j < n; j++) {
+        const double y = found_t[j];
+        if (y > x.t) ahead++;
+        else if (y == x.t) ahead += ahead_of({y, found_key[j], found_f[j]}, x);
+      }
       if (ahead < k) put(ahead, x);
     }
     for (int j = n + tid; j < k; j += TP) put_none(j);
