@@ -892,32 +892,49 @@ struct Plan {
   split::Plan s;       // of few, or of the sequences' own slots
   long long o_off, ml_off, un_off, at_off, row_off, rml_off, s_off, sun_off, bytes;  // workspace
 };
-// Rows up to which one kernel takes all; tiles up to which a CTA takes a whole item (MEASURED); tiles of own slots (times two, beside
-// the prefix's) up to which the tcgen05 kernel takes them (MEASURED)
-constexpr int FEW_TILES = 32, WHOLE_TILES = 24, OWN_TILES = 24;
+// Rules on sizes alone (capacities stand for lengths), both sides measured; the names are S x F x n, Hq / H heads x D, prefix + own slots.
+//   few      up to 32 rows on a prefix (16 of heads 128 wide): against the tcgen05 kernel 1 x 8 x 1, 8/8 x 64, 730 + 60: 7 / 34 us;
+//            1 x 32 x 1, 8/8 x 64, 8,191 + 60: 34 / 41; 1 x 4 x 1, 32/8 x 128, 131,000 + 60: 84 / 138
+//   whole    a CTA for each item, where the SMs that this leaves idle could do no more than IDLE_TILES tiles each (few: tiles of one
+//            warp, eight a CTA): it saves the parts and a kernel.  8 x 32 x 1, 8/8 x 64, 2,000 + 60 (few): 35 / 53 us, 1 x 32 x 1, 8/8 x 64,
+//            8,191 + 60 (few): 76 / 34; 8 x 8 x 16, 8/8 x 64, 730 + 32: 25 / 30; 1 x 64 x 1, 32/8 x 128, 8,191 + 60: 215 / 56
+//   own      the tcgen05 kernel takes the own slots too: where each sequence has more rows than kv8_split.cu takes, or where an item's own
+//            tiles (of a few rows each) are not many.  1 x 32 x 1, 32/8 x 128, 8,191 + 60: 34 / 40 us; 1 x 64 x 1, 32/8 x 128, 8,191 + 60:
+//            43 / 56; 1 x 64 x 1, 32/8 x 128, 2,000 + 500: 75 / 53; 1 x 40 x 1, 2/2 x 64, 100 + 10: 42 / 14
+//   alt      ALT: up to 128 rows (1 x 32 x 1, 32/8 x 128, 131,000 + 60: 132 / 173 us), and of more where that is little work, whose items
+//            otherwise leave SMs idle: 1 x 16 x 32, 32/32 x 64, 730 + 0: 22 / 37; 1 x 32 x 32, the same: 42 / 35; 1 x 8 x 256, 32/8 x 128,
+//            6,001 + 511: 402 / 311
+constexpr int IDLE_TILES = 24, IDLE_FEW = 80, MOST_TILES = 256, OWN_TILES = 64, ALT_TILES = 24;
 static int few_rows(int D) { return D == 64 ? split::FEW_ROWS : 16; }
+static bool leave_idle(long long items, long long tiles, long long idle, int sms) {
+  return tiles <= MOST_TILES && ((items + sms - 1) / sms * sms - items) * tiles <= idle * sms;
+}
 
 static Plan make_plan(int S, int B, int n, int Hq, int H, int D, int Cp, int C, int sms) {
   Plan x{};
   const int F = B / S, G = Hq / H;
-  const long long all = (long long)F * n * G;
+  const long long all = (long long)F * n * G, SH = (long long)S * H;
   auto up = [](long long v) { return (v + 255) / 256 * 256; };
   x.few = all <= few_rows(D);
   if (x.few) {
     const int kt = split::keys_per_tile(D);
-    x.s = split::make_plan(S, F * n, Hq, H, D, Cp, false, sms, Cp / kt + (long long)F * (C / kt), 2LL * S * H >= sms ? 4 * FEW_TILES : FEW_TILES);
+    const long long tiles = Cp / kt + (long long)F * (C / kt);
+    x.s = split::make_plan(S, F * n, Hq, H, D, Cp, false, sms, tiles, leave_idle(SH, tiles, IDLE_FEW, sms) ? MOST_TILES : 0);
     x.sun_off = x.s.full_off;
     x.bytes = x.sun_off + (x.s.whole ? 0 : up(x.s.ctas * 16LL));
     return x;
   }
-  x.alt = all <= 128;
+  // own tiles of an item of so many rows: of the sequences that have rows in it
+  auto own_of = [&](int rows) {
+    const long long seqs = (long long)n * G >= rows ? 2 : rows / ((long long)n * G) + 2;
+    return (seqs < F ? seqs : F) * (C / BLK);
+  };
+  auto tiles_of = [&](int rows) { return Cp / BLK + (x.own ? own_of(rows) : 0); };
+  x.own = (long long)n * G > split::FEW_ROWS || own_of(256) <= OWN_TILES || own_of(256) <= Cp / BLK;
+  x.alt = all <= 128 || SH * ((all + 127) / 128) * tiles_of(128) <= (long long)ALT_TILES * sms;
   const int rows = x.alt ? 128 : 256;
   x.items = (int)((all + rows - 1) / rows), x.ctas = sms < MAX_CTAS ? sms : MAX_CTAS;
-  // sequences with rows in an item, and their tiles
-  const long long seqs = (long long)n * G >= rows ? 2 : rows / ((long long)n * G) + 2, own = (seqs < F ? seqs : F) * (C / BLK);
-  x.own = (long long)n * G > split::FEW_ROWS || own <= OWN_TILES || own <= Cp / BLK / 2;
-  const long long tiles = Cp / BLK + (x.own ? own : 0);
-  x.whole = tiles <= WHOLE_TILES || (tiles <= 4 * WHOLE_TILES && 2LL * S * H * x.items >= sms);
+  x.whole = leave_idle(SH * x.items, tiles_of(rows), IDLE_TILES, sms);
   x.ml_off = x.whole ? 0 : up(2LL * x.ctas * rows * D * 4);
   x.un_off = x.ml_off + (x.whole ? 0 : up(2LL * x.ctas * rows * 8));
   x.at_off = x.un_off + (x.whole ? 0 : up(x.ctas * 16LL));

@@ -73,7 +73,7 @@ def test_workspaces_of_empty_or_refused_problems_are_empty(L):
         assert L.vt_beam_select_ws_bytes(*a) == 0, a
 
 
-@pytest.mark.parametrize("S,F,n,Hq,H,D,Cp,C", [(8, 12, 1, 32, 32, 64, 8320, 128), (1, 4, 1, 4, 4, 64, 64, 4096), (2, 2, 2, 8, 2, 128, 512, 1024), (1, 1, 1, 1, 1, 64, 131072, 64)])
+@pytest.mark.parametrize("S,F,n,Hq,H,D,Cp,C", [(1, 12, 1, 32, 32, 64, 83200, 128), (1, 4, 1, 4, 4, 64, 64, 8192), (2, 2, 2, 8, 2, 128, 8192, 1024), (1, 1, 1, 1, 1, 64, 131072, 64)])
 def test_attn_kv8_shared_workspace_holds_the_parts_of_runs(L, S, F, n, Hq, H, D, Cp, C):
     """Few rows over more tiles than one CTA takes: two parts of 8 rows or more for each of two CTAs an SM."""
     assert L.vt_attn_kv8_shared_ws_bytes(S, S * F, n, Hq, H, D, Cp, C) >= 2 * 2 * 148 * 8 * (D * 4 + 8)
