@@ -440,7 +440,7 @@ int vt_beam_select(cudaStream_t st, const void* logits, long long ld, int f32, c
     return set_error(E_SHAPE, "%s: workspace of %lld bytes, %lld needed (16-byte aligned)", what, ws ? ws_bytes : 0LL, need);
   const beam::Plan p = beam::make_plan(S, F, V, k, sm_count());
   const long long rows = (long long)S * F, n = (long long)S * k, es = f32 ? 4 : 2;
-  if (rows > 0xffffffLL || (long long)F * V > 0x7ffffffeLL || rows * p.chunks > 0x7fffffffLL)
+  if (rows > 0xffffffLL || (long long)F * V > 0x7fff0000LL || rows * p.chunks > 0x7fffffffLL)
     return set_error(E_SHAPE, "%s: S=%d or F * V = %lld too large", what, S, (long long)F * V);
   const struct { const void* p; long long n; } in[] = {{logits, ((rows - 1) * ld + V) * es}, {scores, rows * 4}, {done, done ? rows : 0}, {ws, need}},
       outs[] = {{out_scores, n * 4}, {out_parents, n * 4}, {out_tokens, n * 4}, {out_done, n}};

@@ -580,8 +580,12 @@ def kv8_evict(cache, weights, lens, keep, recent, dst, dst_weights, dst_lens, in
 
 
 @functools.lru_cache(maxsize=1024)
-def _shared_ws_bytes(dev, *sizes):
-    return lib().vt_attn_kv8_shared_ws_bytes(*sizes)
+def _ws_bytes(fn, dev, *sizes):
+    """A workspace's size, which goes by the device's number of SMs too."""
+    if dev < 0 or dev == torch.cuda.current_device():
+        return getattr(lib(), fn)(*sizes)
+    with torch.cuda.device(dev):
+        return getattr(lib(), fn)(*sizes)
 
 
 def attn_kv8_shared_workspace(S, B, n, Hq, H, D, Cp, C, device):
@@ -609,7 +613,7 @@ def attn_kv8_shared(q, prefix, plens, cache, lens, out=None, counts=None, scale=
             out.get_device() != dev or sq[3] != 1 or so[2] != 1:
         _kv8_fail(what, f"q {tuple(q.shape)}, out {tuple(out.shape)} for a cache of B={B} H={H} D={D} (bf16, contiguous rows)")
     if ws is None:
-        nb = _shared_ws_bytes(dev, S, B, n, Hq, H, D, Cp, C)
+        nb = _ws_bytes("vt_attn_kv8_shared_ws_bytes", dev, S, B, n, Hq, H, D, Cp, C)
         if nb:  # held until the call is on the stream; its memory is reused on this stream only
             ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
         wp = ws.data_ptr() if nb else None
@@ -680,11 +684,6 @@ class Beams(NamedTuple):
     done: torch.Tensor
 
 
-@functools.lru_cache(maxsize=1024)
-def _beam_ws_bytes(dev, *sizes):
-    return lib().vt_beam_select_ws_bytes(*sizes)
-
-
 def beam_select(logits, scores, beams, k=None, eos=-1, done=None, out=None, ws=None):
     """vt_beam_select: of each group of `beams` rows of logits [S beams, V] (bf16 or fp32, any row pitch) the k (default beams)
     continuations with the largest scores [S beams] + log softmax(logits), the lowest beam * V + word first where totals are equal.
@@ -706,7 +705,7 @@ def beam_select(logits, scores, beams, k=None, eos=-1, done=None, out=None, ws=N
     else:
         to = [_kv8_vec(what, name, x, (S, k), d, dev) for name, x, d in zip(Beams._fields, out, (f32, i32, i32, flag))]
     if ws is None:
-        nb = _beam_ws_bytes(dev, S, beams, V, k)
+        nb = _ws_bytes("vt_beam_select_ws_bytes", dev, S, beams, V, k)
         ws = torch.empty(nb, dtype=torch.uint8, device=device)  # held until the call is on the stream; its memory is reused on this stream only
     elif ws.get_device() != dev or not ws.is_contiguous():
         _kv8_fail(what, "the workspace must be contiguous on the tensors' device")
