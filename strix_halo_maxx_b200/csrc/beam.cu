@@ -14,6 +14,9 @@ namespace vt {
 namespace beam {
 
 constexpr int MAX_BEAMS = 64, MAX_K = 128, T = 256, TP = 512;  // threads of a CTA of the two kernels
+// Words of a thread: with 8 or 16 for calls of few rows, to fill the GPU, their lists cost the second kernel more (32 x 8 rows of 51,200 bf16:
+// 24 us with 32, 29 with 16, 37 with 8; 4 x 8 rows: 14, 17, 21; 1 x 4 rows fp32: 8.7, 9.1, 8.8).
+constexpr int E = 32;
 constexpr int CAP = 2048;                            // totals that beam_pick_kernel gathers; beyond, one by one
 
 struct Args {
@@ -30,7 +33,7 @@ struct Args {
 };
 
 // Parts of a chunk whose maxima are compared, T / parts threads each: 2 k or more.  The best k of 2 k parts leave about 1.4 k words to
-// gather, and as many comparisons as parts squared (MEASURED3).
+// gather, and there are as many comparisons as parts squared (16 x 32 rows of 100,003 fp32, k = 32: 69 us, with 4 k parts 75).
 __host__ __device__ inline int parts_of(int k) { return k <= 16 ? 32 : k <= 32 ? 64 : k <= 64 ? 128 : 256; }
 
 // Numbers in the order of floats (zeros of both signs are one), and back.
@@ -49,7 +52,7 @@ __device__ __forceinline__ float load_word(const Word* p) {
   else return bf2f(__ldg(p));
 }
 // Words v0 + (r T + thread) VEC ..; -inf behind the row's end.
-template <typename Word, int VEC, int E>
+template <typename Word, int VEC>
 __device__ __forceinline__ void load_chunk(const Word* row, int v0, int V, float (&x)[E]) {
   const Word* p = row + v0 + (int)threadIdx.x * VEC;
   const bool whole = v0 + T * E <= V;
@@ -74,8 +77,9 @@ __device__ __forceinline__ void load_chunk(const Word* row, int v0, int V, float
   }
 }
 
-// CTA = T E words of a row.  Bound: issue slots and DRAM with many rows (MEASURED), the latency of one chunk with few.
-template <typename Word, int VEC, int E>
+// CTA = T E words of a row.  Bound with many rows: a chunk's rounds of barriers, of which four CTAs an SM hide part (16 x 32 rows of 100,003
+// fp32: 53 us, 3.9 TB/s; 57 % of the cycles issue, 20 instructions a word), with few the latency of one chunk.
+template <typename Word, int VEC>
 __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
   constexpr int FOUND = T * E / 2;  // words above the bound are of at most k of 2 k parts or more
   __shared__ float sh_max[T / 32], sh_sum[T / 32];
@@ -91,7 +95,7 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
   if (a.done && a.done[row]) return;  // its words are not looked at
   float x[E];
   const Word* words = static_cast<const Word*>(a.logits) + row * a.ld;
-  load_chunk<Word, VEC, E>(words, v0, a.V, x);
+  load_chunk<Word, VEC>(words, v0, a.V, x);
   auto word = [&](int e) { return v0 + ((e / VEC) * T + tid) * VEC + e % VEC; };
   // ---- the largest logit of the thread, its part and the chunk
   float mx = x[0];
@@ -217,7 +221,7 @@ __device__ __forceinline__ Total shfl_xor(const Total& x, int d) {
   return {__shfl_xor_sync(0xffffffffu, x.t, d), __shfl_xor_sync(0xffffffffu, x.key, d), __shfl_xor_sync(0xffffffffu, x.f, d)};
 }
 
-// CTA = a group.  Bound: latency, of two trips to L2 and the rounds of comparisons.
+// CTA = a group.  Bound: latency, of two trips to L2 and the rounds of comparisons (1 x 4 rows: 4 us of 8.7, 16 x 32 rows of 13 chunks: 15 of 69).
 __global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
   __shared__ double sh_top[MAX_BEAMS], sh_log[MAX_BEAMS], sh_score[MAX_BEAMS];
   __shared__ double part_t[TP], found_t[CAP];
@@ -390,26 +394,16 @@ __global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
 }
 
 struct Plan {
-  int e, chunks;  // words of a thread, chunks of a row
+  int chunks;  // of a row
   long long words_off, bytes;
 };
-// Large chunks (32 words a thread) cost less in lists for the second kernel, small ones fill the GPU with few rows (MEASURED2).
-static Plan make_plan(int S, int F, int V, int k, int sms) {
+static Plan make_plan(int S, int F, int V, int k) {
   Plan p;
   const long long rows = (long long)S * F;
-  for (p.e = 32; p.e > 8; p.e >>= 1)
-    if (rows * ((V + T * p.e - 1) / (T * p.e)) >= 2LL * sms) break;
-  p.chunks = (int)(((long long)V + T * p.e - 1) / (T * p.e));
+  p.chunks = (int)(((long long)V + T * E - 1) / (T * E));
   p.words_off = (rows * p.chunks * 8 + 255) / 256 * 256;
   p.bytes = p.words_off + rows * p.chunks * k * 8;
   return p;
-}
-
-template <typename Word, int VEC>
-static void launch_words(cudaStream_t st, const Args& a, const Plan& p, unsigned ctas) {
-  if (p.e == 32) launch_k(beam_words_kernel<Word, VEC, 32>, ctas, T, 0, st, a);
-  else if (p.e == 16) launch_k(beam_words_kernel<Word, VEC, 16>, ctas, T, 0, st, a);
-  else launch_k(beam_words_kernel<Word, VEC, 8>, ctas, T, 0, st, a);
 }
 
 }  // namespace beam
@@ -420,7 +414,7 @@ extern "C" {
 long long vt_beam_select_ws_bytes(int S, int F, int V, int k) {
   using namespace vt;
   if (S <= 0 || F <= 0 || F > beam::MAX_BEAMS || V <= 0 || k <= 0 || k > beam::MAX_K) return 0;
-  return beam::make_plan(S, F, V, k, sm_count()).bytes;
+  return beam::make_plan(S, F, V, k).bytes;
 }
 
 int vt_beam_select(cudaStream_t st, const void* logits, long long ld, int f32, const float* scores, const uint8_t* done, int S, int F,
@@ -438,7 +432,7 @@ int vt_beam_select(cudaStream_t st, const void* logits, long long ld, int f32, c
   const long long need = vt_beam_select_ws_bytes(S, F, V, k);
   if (!ws || !aligned16(ws) || ws_bytes < need)
     return set_error(E_SHAPE, "%s: workspace of %lld bytes, %lld needed (16-byte aligned)", what, ws ? ws_bytes : 0LL, need);
-  const beam::Plan p = beam::make_plan(S, F, V, k, sm_count());
+  const beam::Plan p = beam::make_plan(S, F, V, k);
   const long long rows = (long long)S * F, n = (long long)S * k, es = f32 ? 4 : 2;
   if (rows > 0xffffffLL || (long long)F * V > 0x7fff0000LL || rows * p.chunks > 0x7fffffffLL)
     return set_error(E_SHAPE, "%s: S=%d or F * V = %lld too large", what, S, (long long)F * V);
@@ -452,8 +446,8 @@ int vt_beam_select(cudaStream_t st, const void* logits, long long ld, int f32, c
   // rows that do not all begin on 16 bytes are read a word at a time: the words of a chunk must not depend on where its row begins
   const bool wide = aligned16(logits) && (rows == 1 || ld * es % 16 == 0);
   const unsigned ctas = (unsigned)(rows * p.chunks);
-  if (f32) wide ? beam::launch_words<float, 4>(st, a, p, ctas) : beam::launch_words<float, 1>(st, a, p, ctas);
-  else wide ? beam::launch_words<uint16_t, 8>(st, a, p, ctas) : beam::launch_words<uint16_t, 1>(st, a, p, ctas);
+  if (f32) launch_k(wide ? beam::beam_words_kernel<float, 4> : beam::beam_words_kernel<float, 1>, ctas, beam::T, 0, st, a);
+  else launch_k(wide ? beam::beam_words_kernel<uint16_t, 8> : beam::beam_words_kernel<uint16_t, 1>, ctas, beam::T, 0, st, a);
   launch_k(beam::beam_pick_kernel, S, beam::TP, 0, st, a);
   return check_launch(what);
 }

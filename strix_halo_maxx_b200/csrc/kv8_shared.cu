@@ -11,7 +11,12 @@
 // nothing.  An item is ROWS of them; its tiles of 64 keys are the prefix's, then those of each sequence that has rows in it, in order.
 //   two M tiles of 128 rows  share every converted tile; own tiles that concern the rows of one M tile are passed over by the other;
 //   ALT, up to 128 rows      both M tiles hold the same rows and take the key tiles in turn, so that two are in flight all the same; in
-//                            the end each pair of threads puts its row's two halves together (MEASURED).
+//                            the end each pair of threads puts its row's two halves together.
+// 8 x 256 tokens (some fewer), 32/8 heads x 128, over 6,001 + 511 slots, 202 GFLOP: 290 us, 697 TFLOP/s, a tile in 1.6 us; 16 x 1 over
+// 131,007 + 65, 271 MB: 136 us, two tiles in 1.8 us.  What bounds a tile is the chain of its scores through TMEM, exponentials and P, about
+// 1,400 cycles of a thread's issue and latencies, beside the operands' way through shared memory: without converting anything these two take
+// 255 and 111 us; exponentials by a polynomial on the FMA pipe instead of the MUFU, for a fifth of them, 305 and 144.  A call of few tiles:
+// launch, lists and shares (3.5 us), the first codes and q (2 to 4), the first tile's cold instructions (2 to 4).
 // Items' tiles form one list cut into equal runs, one for each SM; what spans CTAs leaves parts for attn_kv8_shared_join_kernel.
 #include "vt_common.cuh"
 #include "vt_host.h"
@@ -273,8 +278,8 @@ struct Tile {
 };
 
 // Warps 0-3, 4-7: softmax of M tile 0 / 1, thread = row; 8-11: codes -> operands; 12, 13: MMAs of M tile 0 / 1; 15: works out the CTA's
-// shares of items, for all (each warp for itself took 6 us before the first tile); 14: brings in codes and scales, `raw` tiles ahead (with the converters' registers as the only stage, one tile ahead, 16 rows x 4 heads over 131,007 slots
-// took 131 us).
+// shares of items, for all (each warp for itself took 6 us before the first tile); 14: brings in codes and scales,
+// `raw` tiles ahead (without that stage, from memory into the converters' registers, the 8 x 256 tokens above take 321 us).
 template <int D, bool ALT>
 __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __grid_constant__ Args a) {
   using L = Smem<D, ALT>;
