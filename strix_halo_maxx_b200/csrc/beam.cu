@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
         if (__all_sync(0xffffffffu, v >= min(a.V, v0 + T * E))) break;
       }
     }
-    n = k;
+    n = max(n, k);  // few parts may hold more than k words above it
     __syncthreads();
   }
   unsigned long long* to = a.words + (long long)blockIdx.x * k;

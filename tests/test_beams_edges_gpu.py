@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 from strix_halo_maxx_b200 import ops
 from strix_halo_maxx_b200._lib import device_status
 from oracle import beam_ref as R
-from test_beams_gpu import DEV, BF, as_np, check_shared, filled, i32, np_, up64
+from test_beams_gpu import DEV, BF, as_np, check_select, check_shared, filled, i32, np_, up64
 
 
 @pytest.fixture(autouse=True)
@@ -160,3 +160,19 @@ def test_two_steps_in_one_graph_share_a_workspace():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(want, [t for b in got for t in b] + outs))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, BF])
+@pytest.mark.parametrize("F,k", [(1, 1), (2, 4), (3, 16), (1, 33), (2, 128)])
+@pytest.mark.parametrize("allowed", [1, 40, 150, 3000])
+def test_beam_select_few_words_allowed_that_stand_together(dt, F, k, allowed):
+    """All words but a few runs of neighbours at one value: more words than k above it, in fewer parts of a chunk than k."""
+    V = 20000
+    g = torch.Generator(DEV).manual_seed(allowed + k)
+    for base in (torch.finfo(dt).min, -1e4, 0.0):
+        x = torch.full((F, V), base, device=DEV, dtype=dt)
+        for f in range(F):
+            for v0 in (f * 5, 8192 + 4093, 16384):
+                x[f, v0:v0 + allowed] = (torch.rand(allowed, device=DEV, generator=g) * 9 + 1).to(dt)
+        scores = torch.linspace(0, -1, F, device=DEV)
+        check_select(x, scores, F, k, -1, None, ops.beam_select(x, scores, F, k=k))
