@@ -187,7 +187,7 @@ extern "C" int vt_kv8_reorder(cudaStream_t st, int8_t* kc, int8_t* vc, float* ks
   if (layers == 0 || B == 0) return OK;
   if (Bs == 0) return set_error(E_SHAPE, "%s: no sequence to take", what);
   if (!parents || !lens) return set_error(E_SHAPE, "%s: null pointer", what);
-  if ((long long)layers * H * (Bs > B ? Bs : B) > (1LL << 26) || (long long)(C > dst_C && !in_place ? C : dst_C) * D > 0x40000000LL)
+  if ((long long)layers * H * (Bs > B ? Bs : B) > (1LL << 26) || (long long)(in_place || C > dst_C ? C : dst_C) * D > 0x40000000LL)
     return set_error(E_SHAPE, "%s: layers * B * H or C too large", what);
   const long long n = (long long)layers * Bs * H, nd = (long long)layers * B * H;
   const struct { const void* p; long long n; } src[] = {{kc, n * C * D}, {vc, n * C * D}, {ks, n * C / 16}, {vs, n * C / 16}, {parents, B * 4LL}, {lens, Bs * 4LL}},

@@ -60,7 +60,7 @@ def _reorder(L, layers=1, Bs=4, C=64, dst=None, Cd=64, B=4, beams=2, H=2, D=64, 
     (dict(beams=0), -2, b"beams=0"), (dict(beams=3), -2, b"beams=3"), (dict(beams=65, B=65, Bs=65), -2, b"beams=65"), (dict(Bs=8), -2, b"divide"), (dict(parents=None), -2, b"null"),
     (dict(lens=None), -2, b"null"), (dict(base=None), -2, b"null"), (dict(dst=M), -2, b"overlaps"), (dict(dst=M + (1 << 20)), -2, b"overlaps"), (dict(new=8192), -2, b"overlaps"),
     (dict(new=4096 + 12), -2, b"overlaps"), (dict(new=M + 64), -2, b"overlaps"), (dict(dst=M + (1 << 25), new=8196), -2, b"overlaps"), (dict(layers=1 << 16, B=1 << 15, Bs=1 << 15), -2, b"too large"),
-    (dict(layers=1 << 20, B=64, Bs=64), -2, b"too large"), (dict(dst=M + (1 << 25), Bs=0), -2, b"no sequence"), (dict(layers=0), 0, None), (dict(B=0, Bs=0), 0, None), (dict(B=0, dst=M + (1 << 25)), 0, None)])
+    (dict(layers=1 << 20, B=64, Bs=64), -2, b"too large"), (dict(C=1 << 25, Cd=0), -2, b"too large"), (dict(dst=M + (1 << 25), Bs=0), -2, b"no sequence"), (dict(layers=0), 0, None), (dict(B=0, Bs=0), 0, None), (dict(B=0, dst=M + (1 << 25)), 0, None)])
 def test_kv8_reorder_refuses_on_the_host(L, kw, rc, word):
     assert _reorder(L, **kw) == rc
     assert word is None or word in L.vt_last_error_string(), L.vt_last_error_string()
