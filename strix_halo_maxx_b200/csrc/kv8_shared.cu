@@ -896,6 +896,15 @@ struct Plan {
   int items, ctas;
   split::Plan s;       // of few, or of the sequences' own slots
   long long o_off, ml_off, un_off, at_off, row_off, rml_off, s_off, sun_off, bytes;  // workspace
+  static long long up(long long v) { return (v + 255) / 256 * 256; }
+  // Lays out what runs of items of so many rows leave for the join; its bytes.
+  long long run_bytes(int rows, int D, int sms) {
+    ctas = sms < MAX_CTAS ? sms : MAX_CTAS;
+    ml_off = up(2LL * ctas * rows * D * 4);
+    un_off = ml_off + up(2LL * ctas * rows * 8);
+    at_off = un_off + up(ctas * 16LL);
+    return at_off + up((long long)ctas * rows * 4);
+  }
 };
 // Rules on sizes alone (capacities stand for lengths), both sides measured; the names are S x F x n, Hq / H heads x D, prefix + own slots.
 //   few      up to 32 rows on a prefix (16 of heads 128 wide): against the tcgen05 kernel 1 x 8 x 1, 8/8 x 64, 730 + 60: 7 / 34 us;
@@ -919,14 +928,13 @@ static Plan make_plan(int S, int B, int n, int Hq, int H, int D, int Cp, int C, 
   Plan x{};
   const int F = B / S, G = Hq / H;
   const long long all = (long long)F * n * G, SH = (long long)S * H;
-  auto up = [](long long v) { return (v + 255) / 256 * 256; };
   x.few = all <= few_rows(D);
   if (x.few) {
     const int kt = split::keys_per_tile(D);
     const long long tiles = Cp / kt + (long long)F * (C / kt);
     x.s = split::make_plan(S, F * n, Hq, H, D, Cp, false, sms, tiles, leave_idle(SH, tiles, IDLE_FEW, sms) ? MOST_TILES : 0);
     x.sun_off = x.s.full_off;
-    x.bytes = x.sun_off + (x.s.whole ? 0 : up(x.s.ctas * 16LL));
+    x.bytes = x.sun_off + (x.s.whole ? 0 : Plan::up(x.s.ctas * 16LL));
     return x;
   }
   // own tiles of an item of so many rows: of the sequences that have rows in it
@@ -938,15 +946,13 @@ static Plan make_plan(int S, int B, int n, int Hq, int H, int D, int Cp, int C, 
   x.own = (long long)n * G > split::FEW_ROWS || own_of(256) <= OWN_TILES || own_of(256) <= Cp / BLK;
   x.alt = all <= 128 || SH * ((all + 127) / 128) * tiles_of(128) <= (long long)ALT_TILES * sms;
   const int rows = x.alt ? 128 : 256;
-  x.items = (int)((all + rows - 1) / rows), x.ctas = sms < MAX_CTAS ? sms : MAX_CTAS;
+  x.items = (int)((all + rows - 1) / rows);
   x.whole = leave_idle(SH * x.items, tiles_of(rows), IDLE_TILES, sms);
-  x.ml_off = x.whole ? 0 : up(2LL * x.ctas * rows * D * 4);
-  x.un_off = x.ml_off + (x.whole ? 0 : up(2LL * x.ctas * rows * 8));
-  x.at_off = x.un_off + (x.whole ? 0 : up(x.ctas * 16LL));
-  x.row_off = x.at_off + (x.whole ? 0 : up((long long)x.ctas * rows * 4));
-  x.rml_off = x.row_off + (x.own ? 0 : up((long long)B * n * Hq * D * 4));
-  x.s_off = x.bytes = x.rml_off + (x.own ? 0 : up((long long)B * n * Hq * 8));
-  if (!x.own) x.s = split::make_plan(B, n, Hq, H, D, C, false, sms), x.sun_off = x.s_off + x.s.full_off, x.bytes = x.sun_off + (x.s.whole ? 0 : up(x.s.ctas * 16LL));
+  const long long runs = x.run_bytes(rows, D, sms);
+  x.row_off = x.whole ? 0 : runs;
+  x.rml_off = x.row_off + (x.own ? 0 : Plan::up((long long)B * n * Hq * D * 4));
+  x.s_off = x.bytes = x.rml_off + (x.own ? 0 : Plan::up((long long)B * n * Hq * 8));
+  if (!x.own) x.s = split::make_plan(B, n, Hq, H, D, C, false, sms), x.sun_off = x.s_off + x.s.full_off, x.bytes = x.sun_off + (x.s.whole ? 0 : Plan::up(x.s.ctas * 16LL));
   return x;
 }
 
@@ -962,11 +968,13 @@ long long vt_attn_kv8_shared_ws_bytes(int S, int B, int n, int Hq, int H, int D,
   // what n tokens need, and any fewer that may follow with the same workspace: a plan for few rows needs most at its largest n
   const int sms = vt::sm_count();
   long long most = 0;
-  for (int m = n; m > 0; m = m > 64 ? (m + 1) / 2 : m - 1) {
+  for (int m = n < 64 ? n : 64; m > 0; m--) {
     const long long x = shared::make_plan(S, B, m, Hq, H, D, Cp, C, sms).bytes;
     if (x > most) most = x;
   }
-  return most;
+  // longer calls take own slots too, and so need parts and rows' places at most: those of runs of 256 rows an item
+  const long long runs = shared::Plan().run_bytes(256, D, sms);
+  return n > 64 && runs > most ? runs : most;
 }
 
 int vt_attn_kv8_shared(cudaStream_t st, const uint16_t* q, long long sq_b, long long sq_t, long long sq_h, const int8_t* pk,

@@ -133,3 +133,10 @@ def test_oracle_reorder_goes_round():
     for i in range(3):
         now, lens = R.reorder(now, [1, 2, 0], [50] * 3, 3)
         assert all(np.array_equal(a, b) for a, b in zip(now, c)) == (i == 2) and lens.tolist() == [50] * 3
+
+
+@pytest.mark.parametrize("S,F,Hq,H,D,Cp,C", [(1, 4, 32, 32, 64, 768, 64), (1, 1, 32, 8, 128, 6016, 512), (4, 3, 8, 8, 64, 1024, 128), (2, 8, 32, 8, 128, 8192, 1024), (9, 1, 16, 16, 64, 2048, 64),
+                                              (8, 3, 8, 1, 64, 768, 640), (16, 1, 16, 2, 128, 2048, 64), (1, 3, 128, 32, 64, 704, 448)])
+def test_attn_kv8_shared_workspace_is_enough_for_fewer_tokens(L, S, F, Hq, H, D, Cp, C):
+    need = [L.vt_attn_kv8_shared_ws_bytes(S, S * F, n, Hq, H, D, Cp, C) for n in range(1, 700)]
+    assert need == sorted(need)
