@@ -132,8 +132,6 @@ __device__ __forceinline__ int prefix_len(const int* plens, int s, int Cp, bool 
 }
 // Row groups of gr rows that a sequence's new tokens fill (rg of the plan at most).
 __device__ __forceinline__ int row_groups(const Args& a, const Seq& s, int gr) { return (s.cnt * a.G + gr - 1) / gr; }
-// First tile of each sequence in the list of all tiles, pre[0 .. B]; a sequence's tiles are those of its (head, row group)
-// items one after another.  Every CTA computes it for itself.
 // list[0 .. n] becomes the sums before each of its n numbers; count(i) gives them, each thread takes some that follow one another.
 template <typename Count>
 __device__ __forceinline__ void sums_before(int* list, int n, int* warp_sum, const Count& count) {
@@ -163,6 +161,8 @@ __device__ __forceinline__ void sums_before(int* list, int n, int* warp_sum, con
   if (tid == nth - 1) list[n] = at;
   __syncthreads();
 }
+// First tile of each sequence in the list of all tiles, pre[0 .. B]; a sequence's tiles are those of its (head, row group)
+// items one after another.  Every CTA computes it for itself.
 template <int MODE = PLAIN>
 __device__ __forceinline__ void tile_list(const Args& a, int kt, int gr, int* pre, int* warp_sum, int* own = nullptr) {
   const bool record = blockIdx.x == 0;  // lengths of those without work are looked at here only

@@ -59,6 +59,8 @@ class TextDecoder:
             raise ValueError(f"questions={questions}, beams={beams} (at most 64), steps={steps}: need kv8, and steps with beams")
         if beams and "lm_w" not in weights:
             raise ValueError("beams need the whole lm head: weights lm_w [vocab, dim] and lm_b")
+        if beams and weights["lm_w"].shape[0] > weights["wte"].shape[0]:  # a chosen word is the next step's input
+            raise ValueError(f"an lm head of {weights['lm_w'].shape[0]} words, embeddings of {weights['wte'].shape[0]}")
         self.cfg = cfg
         self.use_graphs = graphs
         self.int8 = int8
@@ -310,7 +312,8 @@ class TextDecoder:
     def query_many(self, ids, last):
         """Up to `questions` questions about the image at once: ids [k, q_len] int64 and last [k] (ints or int64) as query() takes
         them -> yes / no logits [k, n_yn] fp32, equal to query()'s up to the rounding of the keys' blocks (a question's keys share no
-        block with the image's here).  The static buffers and the graph are those of all `questions`; fewer leave the rest idle."""
+        block with the image's here).  A `last` outside the question is refused where it is on the host, and cut off where it is on the
+        device.  The static buffers and the graph are those of all `questions`; fewer leave the rest idle."""
         cfg, m = self.cfg, self.many
         if m is None or ids.dim() != 2 or ids.shape[1] != cfg.q_len or not 0 < ids.shape[0] <= m.B or len(last) != ids.shape[0]:
             raise ValueError(f"query_many: ids {tuple(ids.shape)} for {0 if m is None else m.B} questions of {cfg.q_len} tokens")
@@ -318,7 +321,7 @@ class TextDecoder:
         last = torch.as_tensor(last)
         if last.device.type == "cpu" and not bool(((last >= 0) & (last < cfg.q_len)).all()):
             raise ValueError("query_many: last lies outside the question")
-        last = last.to(device=self.dev, dtype=torch.int64)
+        last = last.to(device=self.dev, dtype=torch.int64).clamp(0, cfg.q_len - 1)
         m.ids.view(m.B, -1)[:k].copy_(ids)
         m.counts.zero_()
         m.counts[:k].copy_(last + 1)

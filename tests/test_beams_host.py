@@ -140,3 +140,9 @@ def test_oracle_reorder_goes_round():
 def test_attn_kv8_shared_workspace_is_enough_for_fewer_tokens(L, S, F, Hq, H, D, Cp, C):
     need = [L.vt_attn_kv8_shared_ws_bytes(S, S * F, n, Hq, H, D, Cp, C) for n in range(1, 700)]
     assert need == sorted(need)
+
+
+def test_an_lm_head_with_words_that_have_no_embedding_is_refused():
+    from strix_halo_maxx_b200.text import TextDecoder
+    with pytest.raises(ValueError, match="embeddings of 80"):
+        TextDecoder({"lm_w": torch.zeros(90, 8), "wte": torch.zeros(80, 8)}, device="cpu", kv8=True, beams=2, steps=2)

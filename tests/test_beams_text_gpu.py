@@ -146,3 +146,14 @@ def test_many_answers_are_refused_where_they_make_no_sense():
                  lambda: dec.query_many(ids[:2, :8].to(DEV), last[:2]), lambda: dec.answer(ids[0].to(DEV), 3)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_query_many_cuts_off_last_on_the_device():
+    W, _ = model()
+    emb, bos, _, _ = wg.text_inputs(TEXT, seed=5)
+    dec = TextDecoder(W, TEXT, device=DEV, kv8=True, questions=2)
+    dec.encode(torch.from_numpy(emb).to(DEV), bos)
+    ids, _ = questions(2, 1)
+    want = dec.query_many(ids.to(DEV), [0, TEXT.q_len - 1]).clone()
+    got = dec.query_many(ids.to(DEV), torch.tensor([-5, TEXT.q_len + 1000], device=DEV))
+    assert torch.equal(got, want)
