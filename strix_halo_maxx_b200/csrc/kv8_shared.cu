@@ -373,13 +373,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
         }
         __syncwarp();
       };
-      const bool q_here = ALT ? nt > 0 : g.of(t).act;
+      const bool q_here = ALT || g.of(t).act;
+      // each q is waited for in turn, without tiles here too: else the next one's phase would be taken for the one before it
+      if (q_here) ok = wait(&q_full[ALT ? 0 : t], sq & 1);
       if (!g.of(t).act) {
         pass(g.ta, g.tb);
       } else {
         int j = tile_from<ALT>(g, t, g.ta);
         pass(g.ta, j);
-        ok = ok && wait(&q_full[ALT ? 0 : t], sq & 1);
         issue_s(j, js & 1);
         bool first = true;
         while (j < g.tb && ok) {

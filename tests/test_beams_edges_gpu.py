@@ -176,3 +176,18 @@ def test_beam_select_few_words_allowed_that_stand_together(dt, F, k, allowed):
                 x[f, v0:v0 + allowed] = (torch.rand(allowed, device=DEV, generator=g) * 9 + 1).to(dt)
         scores = torch.linspace(0, -1, F, device=DEV)
         check_select(x, scores, F, k, -1, None, ops.beam_select(x, scores, F, k=k))
+
+
+@pytest.mark.parametrize("S,F,n,Hq,H,D,plens", [(3, 4, 5, 24, 3, 64, [1500, 0, 1]), (5, 4, 5, 24, 3, 64, [1500, 0, 64, 65, 1]), (3, 20, 4, 8, 2, 128, [1100, 0, 2])])
+def test_attn_kv8_shared_shares_of_one_tile_that_follow_one_another(S, F, n, Hq, H, D, plens):
+    """Items of few tiles behind the last tile of the item before: one half of a CTA has nothing in a share, and all of the next."""
+    B = S * F
+    q = (torch.randn(B, n, Hq, D, device=DEV, generator=torch.Generator(DEV).manual_seed(B)) * 1.5).to(BF)
+    for r in range(20):
+        lens = [(b * 7 + r) % 3 % 2 for b in range(B)]
+        prefix, cache = filled((S,), H, 1536, D, r), filled((B,), H, 64, D, r + 100)
+        out = ops.attn_kv8_shared(q, prefix, i32(plens), cache, i32(lens))
+        ro, mag = R.attention_shared(np_(q.float()), as_np(prefix), plens, as_np(cache), lens)
+        # as for all shapes, and 2^-32 of a row's largest product with a V scale (0.03 at most) for each term of 127 below 2^-21 of it
+        bound = np.abs(ro) * 2.0 ** -8 + mag * (2.0 ** -11 + 2.0 ** -12) + 2.0 ** -32 * 0.03 * 127 * (max(plens) + n + 1)
+        assert (np.abs(np_(out.float()) - ro) <= bound * (1 + 2.0 ** -7)).all(), r
