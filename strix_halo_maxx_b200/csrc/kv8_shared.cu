@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
   const Lists l{lists, lists + B + 1, lists + 2 * B + 1, lists + 3 * B + 2, lists + 3 * B + a.S + 3};
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
-      mbar_init(&q_full[i], ALT ? 8 : 4);  // ALT: one q, which all eight warps bring in
+      mbar_init(&q_full[i], ALT ? 8 : 4);  // of M tile i; ALT: of every other share, whose q all eight warps bring in
       mbar_init(&o_full[i], 1), mbar_init(&o_empty[i], ALT ? 8 : 4), mbar_init(&pv_done[i], 1), mbar_init(&drain[i], 1);
       mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 15);
     }
@@ -374,8 +374,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
         __syncwarp();
       };
       const bool q_here = ALT || g.of(t).act;
-      // each q is waited for in turn, without tiles here too: else the next one's phase would be taken for the one before it
-      if (q_here) ok = wait(&q_full[ALT ? 0 : t], sq & 1);
+      // each q is waited for in turn, without tiles here too: else the next one's phase would be taken for the one before it.  ALT: this
+      // warp's lag is bounded by the shares alone, two of them, so their q's have a barrier each
+      if (q_here) ok = wait(&q_full[ALT ? i & 1 : t], (ALT ? i >> 1 : sq) & 1);
       if (!g.of(t).act) {
         pass(g.ta, g.tb);
       } else {
@@ -561,7 +562,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_shared_tc_kernel(const __
       asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async_smem();
       __syncwarp();
-      mbar_arrive_if(&q_full[ALT ? 0 : t], lane == 0);
+      mbar_arrive_if(&q_full[ALT ? i & 1 : t], lane == 0);
     };
     ok = take(0);
     if (ok && segs[0].tb > segs[0].ta) load_q(0);
