@@ -381,9 +381,10 @@ long long vt_beam_select_ws_bytes(int S, int F, int V, int k);
  * beams' rows s F + f, out_tokens the words, out_done whether they are finished (word eos, or a finished beam).  eos < 0: no word
  * ends an answer (done must then be NULL).  Totals that are not finite (banned words, beams with a score of -inf, rows with a NaN, +inf
  * or nothing but -inf) are no continuations; where fewer than k are left, entry j has score -inf, word -1, row s F + j mod F
- * and counts as finished.  Sums are fp32 within at most 64 words and 64-bit beyond, totals 64-bit, rounded once to fp32;
- * where totals of one beam are equal in 64 bits though its logits differ, the larger logit comes first.  Outputs must
- * not overlap inputs.  ws: vt_beam_select_ws_bytes bytes, 16-byte aligned, one call at a time.
+ * and counts as finished.  exp(-d), d the distance to the largest of 8,192 logits, is within (1 + d) 2^-22 of its value; sums
+ * are fp32 within at most 64 words and 64-bit beyond, totals 64-bit, rounded once to fp32; where totals of one beam are equal
+ * in 64 bits though its logits differ, the larger logit comes first.  Outputs must not overlap inputs.  ws:
+ * vt_beam_select_ws_bytes bytes, 16-byte aligned, one call at a time.
  * Replaces: nothing in the reference, which answers yes or no (md2fast.py:210-212). */
 int vt_beam_select(cudaStream_t stream, const void* logits, long long ld, int f32, const float* scores, const uint8_t* done, int S,
                    int F, int V, int k, int eos, float* out_scores, int* out_parents, int* out_tokens, uint8_t* out_done, void* ws,

@@ -28,7 +28,7 @@ struct Args {
   float* out_scores;
   int *out_parents, *out_tokens;
   uint8_t* out_done;
-  float2* sums;              // [rows][chunks] largest logit, sum of exponentials of the differences to it
+  double2* sums;             // [rows][chunks] largest logit, sum of exponentials of the differences to it
   unsigned long long* words; // [rows][chunks][k] (logit, place), best first; 0: none
 };
 
@@ -82,7 +82,8 @@ __device__ __forceinline__ void load_chunk(const Word* row, int v0, int V, float
 template <typename Word, int VEC>
 __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
   constexpr int FOUND = T * E / 2;  // words above the bound are of at most k of 2 k parts or more
-  __shared__ float sh_max[T / 32], sh_sum[T / 32];
+  __shared__ float sh_max[T / 32];
+  __shared__ double sh_sum[T / 32];
   __shared__ __align__(16) uint32_t part[T];
   __shared__ unsigned long long found[FOUND];
   __shared__ float bound;
@@ -127,7 +128,8 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
     for (int d = 1; d < per; d <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
     if (tid % per == 0 && ahead == k - 1 && best > -INFINITY) bound = unordered(mine & ~number);  // -inf where fewer than k parts have a word
   }
-  // ---- sum of exponentials; a chunk of -inf adds nothing, a NaN or +inf makes it NaN
+  // ---- sum of exponentials: fp32 within the 64 words of two lanes, 64 bits from there on (a sum in fp32 throughout lost what many unlikely
+  // words add to a likely one).  A chunk of -inf adds nothing, a NaN or +inf makes it NaN
   {
     const float ref = top == -INFINITY ? 0.f : top;
     const unsigned long long ref2 = f2_pack(-ref, -ref), log2e = f2_pack(1.4426950408889634f, 1.4426950408889634f);
@@ -141,9 +143,10 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
     float s, s_odd;
     f2_unpack(s2, s, s_odd);
     s += s_odd;
+    double sum = s + __shfl_xor_sync(0xffffffffu, s, 16);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    if (lane == 0) sh_sum[warp] = s;
+    for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) sh_sum[warp] = sum;
   }
   __syncthreads();
   // ---- gather the words that reach the bound.  They are few: the others' only cost is a bit
@@ -158,10 +161,10 @@ __global__ void __launch_bounds__(T) beam_words_kernel(Args a) {
     if (n < FOUND) found[n] = key_of(load_word(words + v), v);
   }
   if (tid == 0) {
-    float s = 0.f;
+    double s = 0.;
 #pragma unroll
     for (int w = 0; w < T / 32; w++) s += sh_sum[w];
-    a.sums[blockIdx.x] = make_float2(top, s);
+    a.sums[blockIdx.x] = make_double2(top, s);
   }
   __syncthreads();
   int n = count;
@@ -253,14 +256,14 @@ __global__ void __launch_bounds__(TP) beam_pick_kernel(Args a) {
     const bool done = a.done && a.done[row0 + f];
     double top = -INFINITY, sum = 0.;
     if (!done) {
-      const float2* s = a.sums + (row0 + f) * a.chunks;
-      const float2 mine = lane < a.chunks ? s[lane] : make_float2(-INFINITY, 0.f);  // of the first 32 chunks, mostly all
-      float m = mine.x;
-      for (int c = lane + 32; c < a.chunks; c += 32) m = fmaxf(m, s[c].x);
+      const double2* s = a.sums + (row0 + f) * a.chunks;
+      const double2 mine = lane < a.chunks ? s[lane] : make_double2(-INFINITY, 0.);  // of the first 32 chunks, mostly all
+      float m = (float)mine.x;
+      for (int c = lane + 32; c < a.chunks; c += 32) m = fmaxf(m, (float)s[c].x);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-      if (mine.y != 0.f) sum = mine.y * exp((double)mine.x - m);
-      for (int c = lane + 32; c < a.chunks; c += 32) sum += s[c].y == 0.f ? 0. : s[c].y * exp((double)s[c].x - m);
+      if (mine.y != 0.) sum = mine.y * exp(mine.x - m);
+      for (int c = lane + 32; c < a.chunks; c += 32) sum += s[c].y == 0. ? 0. : s[c].y * exp(s[c].x - m);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       top = m;
@@ -401,7 +404,7 @@ static Plan make_plan(int S, int F, int V, int k) {
   Plan p;
   const long long rows = (long long)S * F;
   p.chunks = (int)(((long long)V + T * E - 1) / (T * E));
-  p.words_off = (rows * p.chunks * 8 + 255) / 256 * 256;
+  p.words_off = (rows * p.chunks * 16 + 255) / 256 * 256;
   p.bytes = p.words_off + rows * p.chunks * k * 8;
   return p;
 }
@@ -441,7 +444,7 @@ int vt_beam_select(cudaStream_t st, const void* logits, long long ld, int f32, c
   for (const auto& x : in)
     for (const auto& y : outs)
       if (x.n && kv8::overlap(x.p, x.n, y.p, y.n)) return set_error(E_SHAPE, "%s: an output overlaps an input", what);
-  beam::Args a{logits, ld, scores, done, F, V, k, eos, p.chunks, out_scores, out_parents, out_tokens, out_done, (float2*)ws,
+  beam::Args a{logits, ld, scores, done, F, V, k, eos, p.chunks, out_scores, out_parents, out_tokens, out_done, (double2*)ws,
                (unsigned long long*)((char*)ws + p.words_off)};
   // rows that do not all begin on 16 bytes are read a word at a time: the words of a chunk must not depend on where its row begins
   const bool wide = aligned16(logits) && (rows == 1 || ld * es % 16 == 0);
