@@ -160,7 +160,7 @@ class TextDecoder:
         F, V = m.B, W["lm_w"].shape[0]
         self.lm_w, self.lm_ld = _dev_mat(W["lm_w"], dev)
         self.lm_b = _dev_vec(W["lm_b"], dev)
-        m.logits = torch.zeros(F, V, dtype=F32, device=dev)
+        m.logits = torch.zeros(F, ops._pad8(V), dtype=F32, device=dev)[:, :V]  # the GEMM's rows begin on 32 bytes
         m.best = ops.Beams(*(torch.zeros(1, F, dtype=d, device=dev) for d in (F32, torch.int32, torch.int32, torch.bool)))
         m.ws_select = torch.empty(ops.lib().vt_beam_select_ws_bytes(1, F, V, F), dtype=torch.uint8, device=dev)
         m.first = torch.full((F,), -float("inf"), dtype=F32, device=dev)  # a search begins with one beam
