@@ -225,8 +225,11 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
   __shared__ __align__(8) uint64_t full[WARPS * ST];
   __shared__ float sh_m[WARPS][GR], sh_l[WARPS][GR], sh_lse[WHOLE ? GR : 1];
   __shared__ int sh_cnt[MODE == SHARED ? 32 : 1];  // rows of the sequences on a prefix
-  __shared__ int own[MODE == SHARED && !WHOLE ? MAXB + 1 : 1];
   __shared__ int sh_abort;
+  // two CTAs an SM, which the number of runs counts on (228 KB, of which each CTA costs 1 more)
+  static_assert(WHOLE || 2 * ((sizeof(pre) + sizeof(warp_sum) + sizeof(full) + sizeof(sh_m) + sizeof(sh_l) + sizeof(sh_lse) + sizeof(sh_cnt) + sizeof(sh_abort) + 1023) / 1024 * 1024 +
+                              WARPS * RING + 1024) <= 228 * 1024);
+  static_assert((MAXB + 1) * sizeof(int) <= RING);
   volatile int* abort_flag = &sh_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = sm + warp * RING;
@@ -244,7 +247,11 @@ __global__ void __launch_bounds__((WHOLE ? WHOLE_WARPS : WARPS) * 32, WHOLE ? 1 
   if (WHOLE) {
     __syncthreads();
   } else {
-    tile_list<MODE>(a, KT, GR, pre, warp_sum, own);  // its barriers also publish the mbarriers
+    tile_list<MODE>(a, KT, GR, pre, warp_sum, reinterpret_cast<int*>(sm));  // its barriers also publish the mbarriers
+    if constexpr (MODE == SHARED) {  // it had a list in the rings (8 KB of its own cost 32 rows the second CTA): that comes before the copies into them
+      fence_proxy_async_smem();
+      __syncthreads();
+    }
     total = pre[a.B];
     run = run_of(total, a.ctas);
     u_begin = (long long)blockIdx.x * run;
