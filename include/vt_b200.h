@@ -348,10 +348,11 @@ long long vt_attn_kv8_shared_ws_bytes(int S, int B, int n, int Hq, int H, int D,
  * and slots 0 .. lens[b] + i of its own cache; softmax(scale q k^T) v over both, out bf16 at out + b*so_b + i*so_t + hq*so_h (not
  * over q).  Rows behind counts[b] are left as they were.  A prefix is read once for all of its sequences.  Lengths from 0 on;
  * what does not fit in its cache is cut off and recorded in the status word (bit 9).
- * Scores, maxima, sums and O are fp32; q and the probabilities are rounded as vt_attn_kv8 says of few rows or of many: of few where all
- * rows on a prefix are (B / S) n Hq / H <= 32 (16 for D = 128), and for the own slots of sequences with n Hq / H <= 32 rows, in most sizes;
- * of many otherwise.  V scales of 2^-100 .. 2^100 (smaller ones may count as zero), those of one head of a prefix or cache within 2^64 of one
- * another.  ws: vt_attn_kv8_shared_ws_bytes bytes, 16-byte aligned, one call at a time.  The same results every time.
+ * Scores, maxima, sums and O are fp32; q and the probabilities are rounded as vt_attn_kv8 says of few rows or of many.  With R = n Hq / H
+ * rows of a sequence on a kv head: of few where (B / S) R <= 32 (16 for D = 128), and, over the own slots alone, where R <= 32 and
+ * min(B / S, 256 / R + 2) C is above both 4,096 and Cp; of many otherwise.  V scales of 2^-100 .. 2^100 (smaller ones may count
+ * as zero), those of one head of a prefix or cache within 2^64 of one another.  ws: vt_attn_kv8_shared_ws_bytes bytes, 16-byte
+ * aligned, one call at a time.  The same results every time.
  * Replaces: nothing in the reference, which asks one question of an image at a time (FastMD2._query, md2fast.py:208-212). */
 int vt_attn_kv8_shared(cudaStream_t stream, const uint16_t* q, long long sq_b, long long sq_t, long long sq_h, const int8_t* pk,
                        const int8_t* pv, const float* pks, const float* pvs, int Cp, const int* plens, int S, const int8_t* kc,

@@ -7,8 +7,8 @@ namespace kv8 {
 namespace reorder {
 
 constexpr int MAX_BEAMS = 64, THREADS = 128;
-// Bytes of the sources that are brought in together, of one of them at most.  In the order of the cases above: 16 KB and 8 KB 286, 94, 6.7 us;
-// 8 and 8 KB 286, 93, 8.8; 32 and 16 KB 294, 103, 8.4.
+// Bytes of the sources that are brought in together, of one of them at most.  Of the three calls that are named at the kernel (a served batch's
+// beams, a fork, few beams): 16 KB and 8 KB 286, 94, 6.7 us; 8 and 8 KB 286, 93, 8.8; 32 and 16 KB 294, 103, 8.4.
 constexpr int STAGE = 16384, MAX_CHUNK = 8192;
 constexpr long long kDrainCycles = 200000000LL;
 

@@ -913,7 +913,8 @@ struct Plan {
 //            1 x 32 x 1, 8/8 x 64, 8,191 + 60: 25 / 44; 1 x 4 x 1, 32/8 x 128, 131,000 + 60: 83 / 138
 //   whole    a CTA for each item, where the SMs that this leaves idle could do no more than IDLE_TILES tiles each (few: tiles of one
 //            warp, eight a CTA): it saves the parts and a kernel.  8 x 32 x 1, 8/8 x 64, 2,000 + 60 (few): 35 / 38 us, 1 x 32 x 1, 8/8 x 64,
-//            8,191 + 60 (few): 76 / 25; near where the rule changes 32 rows lose by it (1 x 24 x 1, 8/8 x 64, 1,500 + 60: 27 / 18); 8 x 8 x 16, 8/8 x 64, 730 + 32: 25 / 30; 1 x 64 x 1, 32/8 x 128, 8,191 + 60: 215 / 56
+//            8,191 + 60 (few): 76 / 25; near where the rule changes 32 rows lose by it (1 x 24 x 1, 8/8 x 64,
+//            1,500 + 60: 27 / 18); 8 x 8 x 16, 8/8 x 64, 730 + 32: 25 / 30; 1 x 64 x 1, 32/8 x 128, 8,191 + 60: 215 / 56
 //   own      the tcgen05 kernel takes the own slots too: where each sequence has more rows than kv8_split.cu takes, or where an item's own
 //            tiles (of a few rows each) are not many.  1 x 32 x 1, 32/8 x 128, 8,191 + 60: 34 / 40 us; 1 x 64 x 1, 32/8 x 128, 8,191 + 60:
 //            43 / 56; 1 x 64 x 1, 32/8 x 128, 2,000 + 500: 75 / 53; 1 x 40 x 1, 2/2 x 64, 100 + 10: 42 / 14
