@@ -2,7 +2,7 @@
 
 One nvcc invocation over csrc/vt_b200.cu (which includes every kernel file), static cudart, no libcuda
 link (cuTensorMapEncodeTiled is fetched through cudaGetDriverEntryPoint), so the .so only needs a
-driver on the GPU box.
+driver where it runs.
 """
 import os
 import shutil

@@ -12,7 +12,7 @@
 //   two M tiles of 128 rows  share every converted tile; own tiles that concern the rows of one M tile are passed over by the other;
 //   ALT, up to 128 rows      both M tiles hold the same rows and take the key tiles in turn, so that two are in flight all the same; in
 //                            the end each pair of threads puts its row's two halves together.
-// 8 x 256 tokens (some fewer), 32/8 heads x 128, over 6,001 + 511 slots, 202 GFLOP: 290 us, 697 TFLOP/s, a tile in 1.6 us; 16 x 1 over
+// 8 x 256 tokens (some fewer), 32/8 heads x 128, over 6,001 + 511 slots, 202 GFLOP: 294 us, 688 TFLOP/s, a tile in 1.6 us; 16 x 1 over
 // 131,007 + 65, 271 MB: 136 us, two tiles in 1.8 us.  What bounds a tile is the chain of its scores through TMEM, exponentials and P, about
 // 1,400 cycles of a thread's issue and latencies, beside the operands' way through shared memory: without converting anything these two take
 // 255 and 111 us; exponentials by a polynomial on the FMA pipe instead of the MUFU, for a fifth of them, 305 and 144.  A call of few tiles:
